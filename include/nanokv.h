@@ -606,6 +606,78 @@ int nkv_norm_gemv_silu_mul(const uint16_t* gate_up_weight, const uint16_t* x, co
                            const uint16_t* norm_weight, float eps, uint16_t* y, uint16_t* residual_out,
                            int intermediate, int k, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 8-bit projections of the decoder (no reference counterpart: its linears,
+ * nanovllm/layers/linear.py, are bf16).  A row y[n] is held as int8 codes
+ * and one fp32 scale: with a = max |y|,
+ *   q = rne(y * 127 / a), s = a / 127, y ~ q * s.
+ * A row with a < 2^-119 is zero (s = 0, q = 0); one with a NaN or an infinity
+ * has s = NaN and q = 0, so that what is computed from it is NaN.  A weight
+ * [n][k] is held the same way, one scale an output channel.  Products are
+ * summed in 32-bit integers (exact) and scaled in fp32:
+ *   Y[m][c] = (sum_k x.q[m][k] w.q[c][k]) * x.s[m] * w.s[c] (+ bias[c]).
+ * bf16 tensors, dense rows unless said; matrices of rows 16-byte aligned; row
+ * lengths (n of rows, k of products) are multiples of 16; outputs overlap no
+ * input and not each other.  Each call is one launch on `stream`.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * Rows of x (x_stride elements apart, a multiple of 8) -> codes q [rows][n]
+ * and scale [rows].  n: at most 32768.
+ */
+int nkv_quantize_q8(const uint16_t* x, int64_t x_stride, int8_t* q, float* scale, int rows, int n, void* stream);
+
+/* out [rows][n] = bf16(q * scale). */
+int nkv_dequantize_q8(const int8_t* q, const float* scale, uint16_t* out, int rows, int n, void* stream);
+
+/*
+ * nkv_rmsnorm's norm (optionally after a residual add), its output as codes
+ * and scales and not rounded before: t = x (+ residual) in fp32;
+ * residual_out = bf16(t) (if non-NULL; it may be x or residual itself); the
+ * row t * rsqrt(mean(t^2) + eps) * weight is quantised.  A row whose largest
+ * |t * weight| is below 2^-119 is zero too; one whose sum of squares passes
+ * fp32's range is NaN.  n: at most 32768.
+ */
+int nkv_rmsnorm_q8(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, float eps, int8_t* q,
+                   float* scale, uint16_t* residual_out, int rows, int n, void* stream);
+
+/*
+ * y [m][n] (bf16) = the product above of x [m][k] and weight [n][k], plus bias
+ * [n] (bf16) if non-NULL.  k: at most 131056 (the exact sum's range).
+ */
+int nkv_linear_q8(const int8_t* weight, const float* w_scale, const int8_t* x, const float* x_scale,
+                  const uint16_t* bias, uint16_t* y, int m, int n, int k, void* stream);
+
+/*
+ * The product with gate_up_weight [2 intermediate][k] (gate rows, then up
+ * rows) and SiLU-and-mul in fp32: y [m][intermediate] = bf16(g / (1 + e^-g) * u).
+ */
+int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const int8_t* x, const float* x_scale,
+                           uint16_t* y, int m, int intermediate, int k, void* stream);
+
+/*
+ * nkv_quantize_q8 of 1 <= m <= 4 dense bf16 rows x [m][k] followed by the
+ * product, in one launch (decode steps): the results of the two calls bit for
+ * bit.  m * k: at most 49152; k: at most 32768.
+ */
+int nkv_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* bias, uint16_t* y,
+                int m, int n, int k, void* stream);
+int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y, int m,
+                         int intermediate, int k, void* stream);
+
+/*
+ * nkv_rmsnorm_q8 of 1 <= m <= 4 rows followed by the product, in one launch:
+ * the results of the two calls up to the fp32 order of the sum of squares.
+ * residual_out (or NULL) overlaps no input here: every workgroup reads the
+ * rows while one writes it.  Sizes as nkv_gemv_q8.
+ */
+int nkv_norm_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* residual,
+                     const uint16_t* norm_weight, float eps, const uint16_t* bias, uint16_t* y,
+                     uint16_t* residual_out, int m, int n, int k, void* stream);
+int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x,
+                              const uint16_t* residual, const uint16_t* norm_weight, float eps, uint16_t* y,
+                              uint16_t* residual_out, int m, int intermediate, int k, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

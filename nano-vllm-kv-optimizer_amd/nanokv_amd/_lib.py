@@ -80,6 +80,15 @@ SIGNATURES = {
     "nkv_gemv_silu_mul": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "nkv_norm_gemv": (_I, [_P, _P, _P, _P, _F, _P, _P, _I, _I, _P]),
     "nkv_norm_gemv_silu_mul": (_I, [_P, _P, _P, _P, _F, _P, _P, _I, _I, _P]),
+    "nkv_quantize_q8": (_I, [_P, _I64, _P, _P, _I, _I, _P]),
+    "nkv_dequantize_q8": (_I, [_P, _P, _P, _I, _I, _P]),
+    "nkv_rmsnorm_q8": (_I, [_P, _P, _P, _F, _P, _P, _P, _I, _I, _P]),
+    "nkv_linear_q8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_linear_silu_mul_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_gemv_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_norm_gemv_q8": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_norm_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _I, _I, _I, _P]),
     "nkv_decode_step_ring": (_I, [_SP, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P, _F, _I, _P, _P, _P,
                                   _P, _P]),
     "nkv_prefill_attend": (_I, [_SP, _I, _I, _P, _I64, _I, _P, _P, _I64, _P, _I64, _I, _P, _I64,
