@@ -656,27 +656,26 @@ int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, c
                            uint16_t* y, int m, int intermediate, int k, void* stream);
 
 /*
- * nkv_quantize_q8 of 1 <= m <= 4 dense bf16 rows x [m][k] followed by the
- * product, in one launch (decode steps): the results of the two calls bit for
- * bit.  m * k: at most 49152; k: at most 32768.
+ * nkv_quantize_q8 of one row x [k] followed by the product, in one launch
+ * (decode steps): the results of the two calls bit for bit.  k: at most 12288.
  */
 int nkv_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* bias, uint16_t* y,
-                int m, int n, int k, void* stream);
-int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y, int m,
+                int n, int k, void* stream);
+int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y,
                          int intermediate, int k, void* stream);
 
 /*
- * nkv_rmsnorm_q8 of 1 <= m <= 4 rows followed by the product, in one launch:
- * the results of the two calls up to the fp32 order of the sum of squares.
+ * nkv_rmsnorm_q8 of one row followed by the product, in one launch: the
+ * results of the two calls up to the fp32 order of the sum of squares.
  * residual_out (or NULL) overlaps no input here: every workgroup reads the
- * rows while one writes it.  Sizes as nkv_gemv_q8.
+ * row while one writes it.  k: at most 12288.
  */
 int nkv_norm_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* residual,
                      const uint16_t* norm_weight, float eps, const uint16_t* bias, uint16_t* y,
-                     uint16_t* residual_out, int m, int n, int k, void* stream);
+                     uint16_t* residual_out, int n, int k, void* stream);
 int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x,
                               const uint16_t* residual, const uint16_t* norm_weight, float eps, uint16_t* y,
-                              uint16_t* residual_out, int m, int intermediate, int k, void* stream);
+                              uint16_t* residual_out, int intermediate, int k, void* stream);
 
 #ifdef __cplusplus
 }

@@ -155,7 +155,9 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* __restric
 }
 
 // SiLU(g) * u in fp32.
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.442695041f)) * u;
+}
 
 // A product's sum in fp32, scaled by token and channel: every kernel rounds alike.
 __device__ __forceinline__ float scaled(int acc, float sx, float sw, float bias) {
@@ -172,38 +174,327 @@ struct Product {
   int m, n, k;
 };
 
-// A wavefront owns 16 channels x 16 rows and reads its operands from memory.
-template <bool SILU>
-__global__ __launch_bounds__(256) void product_kernel(const Product p) {
+// Products stage rows in pieces of 128 codes, one 128-byte LDS row each.
+constexpr int kTileK = 128;
+constexpr int kRsrcWord3 = 0x00020000;   // raw buffer, 32-bit data format
+// LDS row r's 16-byte piece c lies at piece c ^ swizzle(r): the 16 lanes that
+// are served together (of 16 rows, at c or, for lanes 16 on, at c ^ 1) hit
+// the 16 pieces of 256 bytes.
+__device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
+
+// Workgroup barrier behind this wavefront's LDS operations; its loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);                  // lgkmcnt(0)
+  asm volatile("s_barrier" ::: "memory");
+}
+
+// Few rows (16 NB a workgroup): the product is bound by reading the weight once.
+// A workgroup owns 16 channels (SILU: and their up channels); its wavefronts
+// take 128-code pieces of k in turn, each on its own: whole 128-byte lines into
+// registers, kDeep pieces in flight, turned through the wavefront's own LDS rows
+// into the matrix instruction's operands (no barrier), and the partial sums are
+// joined through LDS at the end: exact, being integers.
+constexpr int kFewWaves = 4;
+constexpr int few_bytes(int tiles) { return tiles * kFewWaves * 16 * kTileK; }
+template <int NB, bool SILU>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
+  constexpr int kHalves = SILU ? 2 : 1, kTiles = kHalves + NB;   // 16-row tiles of a piece: channels, then rows
+  constexpr int kDeep = kTiles <= 3 ? 5 : kTiles <= 5 ? 4 : 3;
+  extern __shared__ __align__(128) char s_few[];       // [wave][kTiles][16 rows][128]; then the partial sums
+  constexpr int waves = kFewWaves;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x & (kWave - 1);
-  const int c0 = blockIdx.x * 64 + static_cast<int>(threadIdx.x / kWave) * 16;
-  const int m0 = blockIdx.y * 16;
-  if (c0 >= p.n) return;
   const int r = lane & 15, g = lane >> 4;
-  const int8_t* wr = p.w + static_cast<int64_t>(min(c0 + r, p.n - 1)) * p.k;
-  const int8_t* ur = wr + static_cast<int64_t>(p.n) * p.k;   // SILU: the up row
-  const int8_t* xr = p.x + static_cast<int64_t>(min(m0 + r, p.m - 1)) * p.k;
-  i32x4 acc = {0, 0, 0, 0}, up = {0, 0, 0, 0};
-  for (int k = 16 * g; k < p.k + 16 * g; k += 64) {
-    i32x4 a = {0, 0, 0, 0}, b = a, u = a;
-    if (k < p.k) {
-      a = *reinterpret_cast<const i32x4*>(wr + k);
-      b = *reinterpret_cast<const i32x4*>(xr + k);
-      if constexpr (SILU) u = *reinterpret_cast<const i32x4*>(ur + k);
-    }
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0);
-    if constexpr (SILU) up = __builtin_amdgcn_mfma_i32_16x16x64_i8(u, b, up, 0, 0, 0);
-  }
-  const int m = m0 + r;
-  if (m >= p.m) return;
-  const float sx = p.sx[m];
+  const int c0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * NB;
+  // lane u fetches 16 bytes, piece u & 7 of row u >> 3, of each 8-row half of a tile; past a
+  // matrix's or a row's end the loads give zeros
+  const int sub = lane >> 3, kc = 16 * (lane & 7);
+  const int voff = sub * p.k + kc;
+  __amdgpu_buffer_rsrc_t rs[kHalves + 1];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int c = c0 + 4 * g + e;
-    if (c >= p.n) break;
-    float v = scaled(acc[e], sx, p.sw[c], p.bias ? bf16_to_f32(p.bias[c]) : 0.0f);
-    if constexpr (SILU) v = silu_mul(v, scaled(up[e], sx, p.sw[p.n + c], 0.0f));
-    p.y[static_cast<int64_t>(m) * p.n + c] = f32_to_bf16(v);
+  for (int h = 0; h < kHalves; ++h)
+    rs[h] = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.w + (static_cast<int64_t>(h) * p.n + c0) * p.k), 0,
+                                              min(p.n - c0, 16) * p.k, kRsrcWord3);
+  rs[kHalves] = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.x + static_cast<int64_t>(m0) * p.k), 0,
+                                                  min(p.m - m0, 16 * NB) * p.k, kRsrcWord3);
+  char* mine_lds = s_few + wave * kTiles * 16 * kTileK;
+  const int put_at = sub * kTileK + 16 * ((lane & 7) ^ swizzle(sub));       // (row 8 + sub: 8 rows on, its swizzle ^ 4)
+  const int get_at = r * kTileK + 16 * (g ^ swizzle(r));
+  i32x4 acc[kHalves][NB];
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[h][j] = i32x4{0, 0, 0, 0};
+  i32x4 st[kDeep][kTiles][2];
+  auto fetch = [&](int d, int q) {
+    const bool in_row = kTileK * q + kc < p.k;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int off = voff + ((t < kHalves ? 0 : 16 * (t - kHalves)) + 8 * e) * p.k + kTileK * q;
+        st[d][t][e] = __builtin_bit_cast(
+            i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs[min(t, kHalves)], in_row ? off : 0x7fffffff, 0, 0));
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto products = [&](int d) {
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<i32x4*>(mine_lds + (16 * t + 8 * e) * kTileK + (put_at ^ (64 * e))) = st[d][t][e];
+    wave_lds_sync();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      i32x4 f[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) f[t] = *reinterpret_cast<const i32x4*>(mine_lds + 16 * t * kTileK + (get_at ^ (64 * e)));
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[h][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h], f[kHalves + j], acc[h][j], 0, 0, 0);
+    }
+    wave_lds_sync();
+  };
+  const int pieces = (p.k + kTileK - 1) / kTileK;
+  const int mine = (pieces - wave + waves - 1) / waves;   // pieces wave, wave + waves, ...
+  // (fetches past the last piece read no row; made without a branch, so that the waits stay exact)
+#pragma unroll
+  for (int d = 0; d < kDeep; ++d) fetch(d, wave + d * waves);
+  int i = 0;
+  for (; i + kDeep < mine; i += kDeep)
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      products(d);
+      fetch(d, wave + (i + d + kDeep) * waves);
+    }
+#pragma unroll
+  for (int d = 0; d < kDeep; ++d)
+    if (i + d < mine) products(d);
+  // the joined sums: [wave][kHalves NB][lane]
+  i32x4* s_part = reinterpret_cast<i32x4*>(s_few);
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) s_part[((wave * kHalves + h) * NB + j) * kWave + lane] = acc[h][j];
+  __syncthreads();
+  for (int j = wave; j < NB; j += waves) {
+    i32x4 sum[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      sum[h] = s_part[(h * NB + j) * kWave + lane];
+      for (int v = 1; v < waves; ++v) sum[h] += s_part[((v * kHalves + h) * NB + j) * kWave + lane];
+    }
+    const int m = m0 + 16 * j + r;
+    if (m >= p.m) continue;
+    const float sx = p.sx[m];
+    uint16_t* y = p.y + static_cast<int64_t>(m) * p.n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = c0 + 4 * g + e;
+      if (c >= p.n) break;
+      float v = scaled(sum[0][e], sx, p.sw[c], p.bias ? bf16_to_f32(p.bias[c]) : 0.0f);
+      if constexpr (SILU) v = silu_mul(v, scaled(sum[kHalves - 1][e], sx, p.sw[p.n + c], 0.0f));
+      y[c] = f32_to_bf16(v);
+    }
+  }
+}
+
+// Tiles of 32 NA channels (SILU: 16 NA gate channels and their up channels) x
+// 16 NB WM rows, one a workgroup of 2 x WM wavefronts (channels x rows); a
+// wavefront owns NA x NB products of 16 x 16.
+// LDS rows of a stage (weight rows, then x rows), rounded up to whole rounds of copies
+constexpr int tile_rows(int na, int nb, int wm) { return (32 * na + 16 * nb * wm + 16 * wm - 1) / (16 * wm) * (16 * wm); }
+
+template <int NA, int NB, int WM, int DEPTH, bool SILU>
+__global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt, int nt) {
+  extern __shared__ __align__(128) char s_tile[];
+  constexpr int kTileM = 16 * NB * WM, kWaves = 2 * WM;
+  __shared__ __align__(16) float s_scale[32 * NA], s_bias[SILU ? 4 : 32 * NA], s_x[kTileM];
+  constexpr int kStage = tile_rows(NA, NB, WM) * kTileK;
+  constexpr int kCopies = tile_rows(NA, NB, WM) / (8 * kWaves);   // 8-row pieces a wavefront copies
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kWave - 1);
+  // tiles: a run of them per XCD, 8 row tiles by all channel tiles at a time
+  int t;
+  {
+    const int total = mt * nt, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const int per = total >> 3, more = total & 7;
+    t = xcd * per + min(xcd, more) + at;
+  }
+  const int band = t / (8 * nt), in = t - band * 8 * nt;
+  const int rows_of_band = min(8, mt - band * 8);
+  const int m0 = (band * 8 + in % rows_of_band) * kTileM;
+  const int c0 = (in / rows_of_band) * (SILU ? 16 : 32) * NA;
+
+  const int cn = min(p.n - c0, (SILU ? 16 : 32) * NA), mn = min(p.m - m0, kTileM);
+
+  // A wavefront's share of a stage: 8-row pieces wave, wave + kWaves, ..., lane u with
+  // 16 bytes of row u >> 3.  They go through registers: loaded a stage ahead of
+  // the step that puts them into LDS.  (Copies straight into LDS reach 61 B/ns
+  // a CU, loads into registers 89: two 256-row tiles a stage want 64.)
+  const int sub = lane >> 3;
+  const int kc = 16 * (lane & 7);
+  const int voff = sub * p.k + kc;
+  const int lds_at = sub * kTileK + 16 * ((lane & 7) ^ swizzle(8 * wave + sub));   // (kWaves groups on: the same swizzle)
+  i32x4 st[DEPTH][kCopies];
+  auto fetch = [&](int set, int s, int i) {
+    int row = 8 * (wave + kWaves * i);                 // of the stage (rows past its last: zeros)
+    const int8_t* base = p.w + static_cast<int64_t>(c0) * p.k;
+    int rows = cn;
+    if (row >= 32 * NA) {
+      row -= 32 * NA;
+      base = p.x + static_cast<int64_t>(m0) * p.k;
+      rows = mn;
+    } else if constexpr (SILU) {                       // of a wavefront's 16 NA rows half are gate rows, half up rows
+      constexpr int half = 8 * NA;
+      if ((row / half) & 1) base += static_cast<int64_t>(p.n) * p.k;
+      row = (row / (2 * half)) * half + row % half;
+    }
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, rows * p.k, kRsrcWord3);
+    const int off = kc < p.k - s * kTileK ? voff + row * p.k + s * kTileK : 0x7fffffff;   // past the row's end: zeros
+    st[set][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+  };
+  auto put = [&](int set, int buf, int i) {
+    const int row = 8 * (wave + kWaves * i);
+    *reinterpret_cast<i32x4*>(s_tile + buf + row * kTileK + lds_at) = st[set][i];
+  };
+
+  // the scales of the tile's weight rows and x rows, and its bias
+  for (int row = threadIdx.x; row < 32 * NA; row += 64 * kWaves) {
+    const int64_t up = SILU && (row / (8 * NA)) & 1 ? p.n : 0;
+    const int c = c0 + min(SILU ? (row / (16 * NA)) * 8 * NA + row % (8 * NA) : row, cn - 1);
+    s_scale[row] = p.sw[up + c];
+    if constexpr (!SILU) s_bias[row] = p.bias ? bf16_to_f32(p.bias[c]) : 0.0f;
+  }
+  for (int row = threadIdx.x; row < kTileM; row += 64 * kWaves) s_x[row] = p.sx[m0 + min(row, mn - 1)];
+
+  const int wc = wave & 1, wm = wave >> 1;
+  const int r = lane & 15, g = lane >> 4;
+  const int at = r * kTileK + 16 * (g ^ swizzle(r));
+  i32x4 acc[NA][NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+
+  // A stage is 2 NA steps of NB products, step i with weight fragment i % NA of
+  // the k half i / NA.  Fragments are read kAhead steps ahead (a ring of
+  // registers).  Meanwhile the next stage goes into the other buffer, and the
+  // one after it into the registers.  Before the last kAhead steps a wavefront has
+  // read all of its stage and written its share of the next: behind the one
+  // barrier there the next stage's first fragments are read under these steps.
+  constexpr int kSteps = 2 * NA, kRing = NA % 2 == 0 ? 4 : 5, kAhead = NA > 2 ? kRing - 1 : 2;
+  static_assert(kSteps % kRing == 0 && NB <= NA && NB + kAhead <= kSteps, "");
+  i32x4 a[kRing], b[2][NB];
+  const char* base_a = s_tile + wc * 16 * NA * kTileK;
+  const char* base_b = s_tile + (32 * NA + wm * 16 * NB) * kTileK;
+  auto read_a = [&](int buf, int i) {
+    a[i % kRing] = *reinterpret_cast<const i32x4*>(base_a + buf + (i % NA) * 16 * kTileK + (at ^ (64 * (i / NA))));
+  };
+  auto read_b = [&](int buf, int ks, int j) {
+    b[ks][j] = *reinterpret_cast<const i32x4*>(base_b + buf + j * 16 * kTileK + (at ^ (64 * ks)));
+  };
+  auto products = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      acc[i % NA][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i % kRing], b[i / NA][j], acc[i % NA][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  const int stages = (p.k + kTileK - 1) / kTileK;
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) fetch(0, 0, i);
+#pragma unroll
+  for (int d = 1; d < DEPTH; ++d)
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) fetch(d, d, i);
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    put(0, 0, i);
+    fetch(0, DEPTH, i);
+  }
+  lds_barrier();
+#pragma unroll
+  for (int j = 0; j < NB; ++j) read_b(0, 0, j);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) read_a(0, i);
+  auto stage = [&](int s, int set) {                   // set: registers that hold stage s + 1
+    const int buf = (s & 1) * kStage, next = kStage - buf;
+#pragma unroll
+    for (int i = 0; i < kSteps - kAhead; ++i) {
+      read_a(buf, i + kAhead);
+      if (i < NB) read_b(buf, 1, i);
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c)
+        if (c * (kSteps - kAhead) / kCopies == i) {
+          put(set, next, c);
+          fetch(set, s + 1 + DEPTH, c);
+        }
+      products(i);
+    }
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    // (past the last stage these read what lies in the other buffer, and nothing uses it)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) read_b(next, 0, j);
+#pragma unroll
+    for (int i = kSteps - kAhead; i < kSteps; ++i) {
+      read_a(next, i + kAhead - kSteps);
+      products(i);
+    }
+  };
+  for (int s = 0; s < stages; s += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (d > 0 && s + d >= stages) break;
+      stage(s + d, (d + 1) % DEPTH);
+    }
+  }
+
+  constexpr int kOut = SILU ? NA / 2 : NA;             // channel groups of 16 that are written
+  const float4* my_scale = reinterpret_cast<const float4*>(s_scale + wc * 16 * NA + 4 * g);
+  const float4* my_bias = reinterpret_cast<const float4*>(s_bias + wc * 16 * NA + 4 * g);
+  float4 sw[NA], sb[SILU ? 1 : NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    sw[i] = my_scale[4 * i];
+    if constexpr (!SILU) sb[i] = my_bias[4 * i];
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int mj = (wm * NB + j) * 16 + r;
+    if (mj >= mn) continue;
+    const float sx = s_x[mj];
+    uint16_t* y = p.y + static_cast<int64_t>(m0 + mj) * p.n;
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      const int c = c0 + (wc * kOut + i) * 16 + 4 * g;
+      const float ws[4] = {sw[i].x, sw[i].y, sw[i].z, sw[i].w};
+      float v[4];
+      if constexpr (SILU) {
+        const float4 u4 = sw[NA / 2 + i];
+        const float us[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = silu_mul(scaled(acc[i][j][e], sx, ws[e], 0.0f), scaled(acc[NA / 2 + i][j][e], sx, us[e], 0.0f));
+      } else {
+        const float bs[4] = {sb[i].x, sb[i].y, sb[i].z, sb[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = scaled(acc[i][j][e], sx, ws[e], bs[e]);
+      }
+      const uint2 o = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+      if ((p.n & 3) == 0) {                            // (then rows of y are 8-byte aligned, and c + 4 <= n or c >= n)
+        if (c < p.n) *reinterpret_cast<uint2*>(y + c) = o;
+      } else {
+        if (c < p.n) y[c] = static_cast<uint16_t>(o.x);
+        if (c + 1 < p.n) y[c + 1] = static_cast<uint16_t>(o.x >> 16);
+        if (c + 2 < p.n) y[c + 2] = static_cast<uint16_t>(o.y);
+        if (c + 3 < p.n) y[c + 3] = static_cast<uint16_t>(o.y >> 16);
+      }
+    }
   }
 }
 
@@ -213,14 +504,30 @@ __device__ __forceinline__ int dot16(const i32x4& a, const i32x4& b, int acc) {
   return acc;
 }
 
-// The same product for 1-4 rows that are still bf16, with the rows' norm
-// (NORM) and quantisation in the same launch: every workgroup quantises the rows
-// into LDS, then each of its wavefronts takes channel pairs (SILU: a gate
-// channel and its up channel), lanes along k.
+// Sum of x over the wavefront, in every lane, without the LDS pipeline.
+__device__ __forceinline__ int wave_sum(int x) {
+#define NKV_ROR_ADD(n) x += __builtin_amdgcn_update_dpp(0, x, 0x120 + n, 0xf, 0xf, true)
+  NKV_ROR_ADD(8);
+  NKV_ROR_ADD(4);
+  NKV_ROR_ADD(2);
+  NKV_ROR_ADD(1);
+#undef NKV_ROR_ADD
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = static_cast<int>(a[0]) + static_cast<int>(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return static_cast<int>(b[0]) + static_cast<int>(b[1]);
+}
+
+// The same product for one row that is still bf16 (a decode token), with its norm
+// (NORM) and quantisation in the same launch.  Resident workgroups (one round)
+// take two channels a wavefront at a time -- consecutive ones (long rows: one), or
+// with SILU a gate channel and its up channel -- lanes along k, the weight rows'
+// NCH = ceil(k / 1024) 16-byte chunks a lane in flight at once.  Each workgroup quantises the row
+// for itself while its first weights are in flight.
 struct Token {
   const int8_t* w;
   const float* sw;
-  const uint16_t* x;      // [m][k] bf16
+  const uint16_t* x;      // [k] bf16
   const uint16_t* res;    // NORM: residual added first, or null
   const uint16_t* nw;     // NORM: norm weight
   const uint16_t* bias;
@@ -229,109 +536,121 @@ struct Token {
   float eps;
   int n, k;
 };
-constexpr int kTokenThreads = 256;
-constexpr int kTokenWaves = kTokenThreads / kWave;
+constexpr int kTokenWaves = 4;
+constexpr int kTokenThreads = kTokenWaves * kWave;
+constexpr int kTokenMaxK = 12288;
+constexpr int token_rows(int nch, bool silu) { return silu || nch <= 4 ? 2 : 1; }
+// resident wavefronts per SIMD the kernel is built for and launched with
+constexpr int token_waves(int nch, bool silu) { return nch <= 6 ? 4 : silu ? (nch <= 8 ? 3 : 2) : nch <= 8 ? 4 : 3; }
 
-template <int MR, bool NORM, bool SILU>
-__global__ __launch_bounds__(kTokenThreads) void token_kernel(const Token p) {
-  extern __shared__ uint4 s_codes[];     // [MR][k / 16]
-  __shared__ float s_sum[kTokenWaves][MR];
-  __shared__ uint32_t s_top[kTokenWaves][MR];
+template <int NCH, bool NORM, bool SILU>
+__global__ __launch_bounds__(kTokenThreads, token_waves(NCH, SILU)) void token_kernel(const Token p) {
+  constexpr int R = token_rows(NCH, SILU);
+  constexpr int XC = (NCH * 1024 + 8 * kTokenThreads - 1) / (8 * kTokenThreads);   // 8-element chunks of x a thread
+  __shared__ i32x4 s_codes[NCH * kWave];
+  __shared__ float s_sum[kTokenWaves];
+  __shared__ uint32_t s_top[kTokenWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x & (kWave - 1);
-  const int nc = p.k >> 3;
-  float ss[MR];
-  uint32_t top[MR];
-  auto load = [&](int m, int c, float (&v)[8], bool first) {
-    const int64_t at = static_cast<int64_t>(m) * nc + c;
-    unpack8(reinterpret_cast<const uint4*>(p.x)[at], v);
+  const int nc = p.k >> 3, nq = p.k >> 4;
+
+  uint4 xv[XC], rv[XC], nv[XC];
+#pragma unroll
+  for (int j = 0; j < XC; ++j) {
+    const int c = min(static_cast<int>(threadIdx.x) + j * kTokenThreads, nc - 1);   // past the row: its last, not used
+    xv[j] = reinterpret_cast<const uint4*>(p.x)[c];
     if constexpr (NORM) {
-      if (p.res) {
-        float r[8];
-        unpack8(reinterpret_cast<const uint4*>(p.res)[at], r);
+      if (p.res) rv[j] = reinterpret_cast<const uint4*>(p.res)[c];
+      nv[j] = reinterpret_cast<const uint4*>(p.nw)[c];
+    }
+  }
+  const int units = SILU ? p.n : (p.n + R - 1) / R;
+  const int stride = gridDim.x * kTokenWaves;
+  int u = static_cast<int>(blockIdx.x) * kTokenWaves + wave;
+  i32x4 b[R][NCH];
+  auto load = [&](int unit) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += r[e];
-      }
-      if (first && p.res_out && blockIdx.x == 0) reinterpret_cast<uint4*>(p.res_out)[at] = pack8(v);
-      if (first)
+    for (int j = 0; j < R; ++j) {
+      const int row = SILU ? unit + j * p.n : min(R * unit + j, p.n - 1);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<int8_t*>(p.w + static_cast<int64_t>(row) * p.k), 0, p.k, kRsrcWord3);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss[m] += v[e] * v[e];
-      float wf[8];
-      unpack8(reinterpret_cast<const uint4*>(p.nw)[c], wf);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= wf[e];
+      for (int i = 0; i < NCH; ++i)                    // past the row: zeros
+        b[j][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * lane + 1024 * i, 0, 0));
     }
   };
-#pragma unroll
-  for (int m = 0; m < MR; ++m) {
-    ss[m] = 0.0f;
-    top[m] = 0;
-    for (int c = threadIdx.x; c < nc; c += kTokenThreads) {
-      float v[8];
-      load(m, c, v, true);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top[m] = max(top[m], mag(v[e]));
-    }
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) {
-      ss[m] += __shfl_xor(ss[m], o);
-      top[m] = max(top[m], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[m]), o)));
-    }
-    if (lane == 0) s_sum[wave][m] = ss[m], s_top[wave][m] = top[m];
-  }
-  __syncthreads();
-  float sx[MR];
-#pragma unroll
-  for (int m = 0; m < MR; ++m) {
-    float sum = 0.0f;
-    uint32_t all = 0;
-#pragma unroll
-    for (int i = 0; i < kTokenWaves; ++i) sum += s_sum[i][m], all = max(all, s_top[i][m]);
-    const RowScale rs = NORM ? norm_row_scale(all, sum, p.k, p.eps) : row_scale(all);
-    sx[m] = rs.scale;
-    for (int c = threadIdx.x; c < nc; c += kTokenThreads) {
-      float v[8];
-      load(m, c, v, false);
-      reinterpret_cast<uint2*>(s_codes)[m * nc + c] =
-          make_uint2(codes4(v[0], v[1], v[2], v[3], rs.inv), codes4(v[4], v[5], v[6], v[7], rs.inv));
-    }
-  }
-  __syncthreads();
+  load(min(u, units - 1));
 
-  const int nq = p.k >> 4;
-  const i32x4* xv = reinterpret_cast<const i32x4*>(s_codes);
-  const int units = SILU ? p.n : (p.n + 1) >> 1;
-  for (int u = blockIdx.x * kTokenWaves + wave; u < units; u += gridDim.x * kTokenWaves) {
-    const i32x4* w0 = reinterpret_cast<const i32x4*>(p.w + static_cast<int64_t>(SILU ? u : 2 * u) * p.k);
-    const i32x4* w1 = reinterpret_cast<const i32x4*>(p.w + static_cast<int64_t>(SILU ? u + p.n : min(2 * u + 1, p.n - 1)) * p.k);
-    int acc[MR][2] = {};
-    for (int c = lane; c < nq; c += kWave) {
-      const i32x4 a = w0[c], b = w1[c];
+  // the row: its scale, and its codes into LDS, with zeros behind them
+  float v[XC][8];
+  float ss = 0.0f;
+  uint32_t top = 0;
 #pragma unroll
-      for (int m = 0; m < MR; ++m) {
-        const i32x4 xm = xv[m * nq + c];
-        acc[m][0] = dot16(a, xm, acc[m][0]);
-        acc[m][1] = dot16(b, xm, acc[m][1]);
+  for (int j = 0; j < XC; ++j) {
+    const int c = threadIdx.x + j * kTokenThreads;
+    unpack8(xv[j], v[j]);
+    if constexpr (NORM) {
+      float wf[8];
+      unpack8(nv[j], wf);
+      if (p.res) {
+        float t[8];
+        unpack8(rv[j], t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] += t[e];
+      }
+      if (p.res_out && blockIdx.x == 0 && c < nc) reinterpret_cast<uint4*>(p.res_out)[c] = pack8(v[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (c < nc) ss += v[j][e] * v[j][e];
+        v[j][e] *= wf[e];
       }
     }
 #pragma unroll
-    for (int m = 0; m < MR; ++m)
+    for (int e = 0; e < 8; ++e) top = max(top, mag(v[j][e]));
+  }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    ss += __shfl_xor(ss, o);
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
+  }
+  if (lane == 0) s_sum[wave] = ss, s_top[wave] = top;
+  lds_barrier();
+  ss = 0.0f;
+  top = 0;
 #pragma unroll
-        for (int o = kWave / 2; o > 0; o >>= 1) acc[m][j] += __shfl_xor(acc[m][j], o);
+  for (int i = 0; i < kTokenWaves; ++i) ss += s_sum[i], top = max(top, s_top[i]);
+  const RowScale rs = NORM ? norm_row_scale(top, ss, p.k, p.eps) : row_scale(top);
+#pragma unroll
+  for (int j = 0; j < XC; ++j) {
+    const int c = threadIdx.x + j * kTokenThreads;
+    if (XC * kTokenThreads == NCH * kWave * 2 || c < NCH * kWave * 2)
+      reinterpret_cast<uint2*>(s_codes)[c] =
+          c < nc ? make_uint2(codes4(v[j][0], v[j][1], v[j][2], v[j][3], rs.inv), codes4(v[j][4], v[j][5], v[j][6], v[j][7], rs.inv))
+                 : make_uint2(0u, 0u);
+  }
+  lds_barrier();
+  while (u < units) {
+    int acc[R] = {};
+    if constexpr (NCH > 4) asm volatile("" ::: "memory");   // (a long row's codes are read again, not held in registers)
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const i32x4 x = s_codes[i * kWave + lane];
+#pragma unroll
+      for (int j = 0; j < R; ++j) acc[j] = dot16(b[j][i], x, acc[j]);
+    }
+    const int now = u;
+    u += stride;
+    if (u < units) load(u);
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[j] = wave_sum(acc[j]);
     if (lane != 0) continue;
+    if constexpr (SILU) {
+      p.y[now] = f32_to_bf16(silu_mul(scaled(acc[0], rs.scale, p.sw[now], 0.0f), scaled(acc[R - 1], rs.scale, p.sw[p.n + now], 0.0f)));
+    } else {
 #pragma unroll
-    for (int m = 0; m < MR; ++m) {
-      uint16_t* y = p.y + static_cast<int64_t>(m) * p.n;
-      if constexpr (SILU) {
-        y[u] = f32_to_bf16(silu_mul(scaled(acc[m][0], sx[m], p.sw[u], 0.0f), scaled(acc[m][1], sx[m], p.sw[p.n + u], 0.0f)));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int c = 2 * u + j;
-          if (c < p.n) y[c] = f32_to_bf16(scaled(acc[m][j], sx[m], p.sw[c], p.bias ? bf16_to_f32(p.bias[c]) : 0.0f));
-        }
+      for (int j = 0; j < R; ++j) {
+        const int c = R * now + j;
+        if (c < p.n) p.y[c] = f32_to_bf16(scaled(acc[j], rs.scale, p.sw[c], p.bias ? bf16_to_f32(p.bias[c]) : 0.0f));
       }
     }
   }
@@ -355,28 +674,101 @@ void launch_rows(const uint16_t* x, int64_t x_stride, const uint16_t* res, const
   else go(rows_q8_kernel<1024, NORM>, 1024);
 }
 
-template <bool SILU>
-void launch_product(const Product& p, hipStream_t s) {
-  hipLaunchKernelGGL(product_kernel<SILU>, dim3((p.n + 63) / 64, (p.m + 15) / 16), dim3(256), 0, s, p);
+template <int NB, bool SILU>
+int launch_few(const Product& p, hipStream_t s) {
+  const int mt = (p.m + 16 * NB - 1) / (16 * NB);
+  hipLaunchKernelGGL((few_kernel<NB, SILU>), dim3((p.n + 15) / 16, mt), dim3(64 * kFewWaves), few_bytes(NB + (SILU ? 2 : 1)),
+                     s, p);
+  return NKV_OK;
 }
 
-template <bool NORM, bool SILU>
-void launch_token(const Token& p, int m, hipStream_t s) {
-  const int cus = device_cus();
-  const int units = SILU ? p.n : (p.n + 1) / 2;
-  auto go = [&](auto kern) {
-    const int grid = std::min(4 * (cus > 0 ? cus : 256), (units + kTokenWaves - 1) / kTokenWaves);
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(kTokenThreads), m * p.k, s, p);
-  };
-  switch (m) {
-    case 1: go(token_kernel<1, NORM, SILU>); break;
-    case 2: go(token_kernel<2, NORM, SILU>); break;
-    case 3: go(token_kernel<3, NORM, SILU>); break;
-    default: go(token_kernel<4, NORM, SILU>); break;
+template <int NA, int NB, int WM, int DEPTH, bool SILU>
+int launch_tile(const Product& p, hipStream_t s) {
+  constexpr int kLds = 2 * tile_rows(NA, NB, WM) * kTileK;
+  const auto kern = tile_kernel<NA, NB, WM, DEPTH, SILU>;
+  if (kLds > 65536) {   // beyond the default limit of a launch (per device, so asked each time: it is a table lookup)
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      set_error("nkv_linear_q8: %d bytes of LDS refused: %s", kLds, hipGetErrorString(e));
+      return NKV_ERR_HIP;
+    }
+  }
+  constexpr int kM = 16 * NB * WM, kN = (SILU ? 16 : 32) * NA;
+  const int mt = (p.m + kM - 1) / kM, nt = (p.n + kN - 1) / kN;
+  hipLaunchKernelGGL(kern, dim3(mt * nt), dim3(128 * WM), kLds, s, p, mt, nt);
+  return NKV_OK;
+}
+
+// Which kernel a product takes.  Few rows and few enough 16-channel groups for
+// one round of workgroups, or at most 16 rows: the one that splits k over
+// wavefronts.  Otherwise the tile whose busiest CU is done first: ceil(tiles /
+// CUs) tiles of the shape's time for a stage of 128 codes (us, plus what one
+// tile alone waits), as measured at 20-76 stages and 65-4096 rows.  Larger
+// tiles do more products a byte (2.4 PFLOP/s at 256 x 256, 1.9 at 128 x 128 on
+// 8192^3), smaller ones leave fewer CUs idle.
+struct Shape {
+  int channels, rows;   // (SILU: half as many channels of y)
+  float us, wait_us;
+};
+constexpr Shape kShapes[] = {{256, 256, 1.35f, 0.0f}, {192, 256, 1.20f, 0.0f}, {160, 256, 1.00f, 0.0f},
+                             {128, 256, 0.88f, 0.0f}, {128, 128, 0.58f, 0.0f}, {128, 64, 0.40f, 0.06f},
+                             {64, 64, 0.25f, 0.12f},  {64, 32, 0.22f, 0.07f}};
+
+template <bool SILU>
+int launch_product(const Product& p, hipStream_t s) {
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  if (p.m <= 16) return launch_few<1, SILU>(p, s);
+  if (p.m <= 64 && (p.n + 15) / 16 <= cus) {
+    if (p.m <= 32) return launch_few<2, SILU>(p, s);
+    if (p.m <= 48) return launch_few<3, SILU>(p, s);
+    return launch_few<4, SILU>(p, s);
+  }
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < static_cast<int>(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
+    const Shape& sh = kShapes[i];
+    if (SILU && sh.channels == 160) continue;          // (an odd number of 16-channel groups a wavefront)
+    const int ch = SILU ? sh.channels / 2 : sh.channels;
+    const int64_t tiles = static_cast<int64_t>((p.n + ch - 1) / ch) * ((p.m + sh.rows - 1) / sh.rows);
+    const float us = static_cast<float>((tiles + cus - 1) / cus) * sh.us + sh.wait_us;
+    if (i == 0 || us < least) best = i, least = us;
+  }
+  switch (best) {
+    case 0: return launch_tile<8, 4, 4, 1, SILU>(p, s);
+    case 1: return launch_tile<6, 4, 4, 1, SILU>(p, s);
+    case 2:
+      if constexpr (!SILU) return launch_tile<5, 4, 4, 1, SILU>(p, s);
+      return NKV_ERR_UNSUPPORTED;                      // (never chosen)
+    case 3: return launch_tile<4, 4, 4, 1, SILU>(p, s);
+    case 4: return launch_tile<4, 2, 4, 1, SILU>(p, s);
+    case 5: return launch_tile<4, 2, 2, 2, SILU>(p, s);
+    case 6: return launch_tile<2, 2, 2, 4, SILU>(p, s);
+    default: return launch_tile<2, 1, 2, 4, SILU>(p, s);
   }
 }
 
-constexpr int kTokenCodes = 49152;   // m * k of a token launch: its rows' codes lie in LDS
+template <int NCH, bool NORM, bool SILU>
+void launch_token(const Token& p, hipStream_t s) {
+  const int cus = device_cus() > 0 ? device_cus() : 256;
+  constexpr int R = token_rows(NCH, SILU);
+  const int units = SILU ? p.n : (p.n + R - 1) / R;
+  const int grid = std::min(token_waves(NCH, SILU) * cus, (units + kTokenWaves - 1) / kTokenWaves);   // waves per SIMD = workgroups per CU
+  hipLaunchKernelGGL((token_kernel<NCH, NORM, SILU>), dim3(grid), dim3(kTokenThreads), 0, s, p);
+}
+
+template <bool NORM, bool SILU>
+void launch_token(const Token& p, hipStream_t s) {
+  const int nch = (p.k + 1023) / 1024;
+  if (nch <= 1) launch_token<1, NORM, SILU>(p, s);
+  else if (nch <= 2) launch_token<2, NORM, SILU>(p, s);
+  else if (nch <= 3) launch_token<3, NORM, SILU>(p, s);
+  else if (nch <= 4) launch_token<4, NORM, SILU>(p, s);
+  else if (nch <= 6) launch_token<6, NORM, SILU>(p, s);
+  else if (nch <= 8) launch_token<8, NORM, SILU>(p, s);
+  else if (nch <= 10) launch_token<10, NORM, SILU>(p, s);
+  else launch_token<12, NORM, SILU>(p, s);
+}
 
 int check_rows(const char* who, const void* x, const int8_t* q, const float* scale, int rows, int n) {
   NKV_CHECK_ARG(x != nullptr && q != nullptr && scale != nullptr, "%s: every pointer must be non-NULL", who);
@@ -391,7 +783,10 @@ int check_product(const char* who, const Product& p, int outputs_per_channel) {
                 "%s: weight, w_scale, x, x_scale and y must be non-NULL", who);
   NKV_CHECK_ARG(p.m >= 1 && p.n >= 1 && p.k >= 16 && p.k % 16 == 0 && p.k <= kMaxDepth,
                 "%s: m and n >= 1 and k a multiple of 16 in [16, %d] (got %d, %d, %d)", who, kMaxDepth, p.m, p.n, p.k);
-  NKV_CHECK_ARG(p.n <= INT32_MAX / 2 - 512 && p.m <= INT32_MAX - 512, "%s: m or n too large (got %d, %d)", who, p.m, p.n);
+  // one workgroup a tile: at least 64 x 32 outputs each, or 16 channels of at most 64 rows
+  NKV_CHECK_ARG(p.n <= INT32_MAX / 2 - 512 && p.m <= INT32_MAX - 512 &&
+                    static_cast<int64_t>((p.n + 31) / 32) * ((p.m + 31) / 32) <= INT32_MAX,
+                "%s: m or n too large (got %d, %d)", who, p.m, p.n);
   NKV_CHECK_ARG(aligned16(p.w) && aligned16(p.x), "%s: weight and x must be 16-byte aligned", who);
   const int64_t out = 2 * static_cast<int64_t>(p.m) * p.n, channels = static_cast<int64_t>(p.n) * outputs_per_channel;
   NKV_CHECK_ARG(apart(p.y, out, p.w, channels * p.k) && apart(p.y, out, p.sw, 4 * channels) &&
@@ -402,31 +797,29 @@ int check_product(const char* who, const Product& p, int outputs_per_channel) {
 }
 
 template <bool NORM, bool SILU>
-int token(const char* who, const Token& p, int m, void* stream) {
+int token(const char* who, const Token& p, void* stream) {
   NKV_CHECK_ARG(p.w != nullptr && p.sw != nullptr && p.x != nullptr && p.y != nullptr && (!NORM || p.nw != nullptr),
                 "%s: weight, w_scale, x%s and y must be non-NULL", who, NORM ? ", norm_weight" : "");
-  NKV_CHECK_ARG(m >= 1 && m <= 4, "%s: m must be in [1, 4] (got %d)", who, m);
-  NKV_CHECK_ARG(p.n >= 1 && p.n <= INT32_MAX / 2 - 512 && p.k >= 16 && p.k % 16 == 0 && p.k <= kMaxRow,
-                "%s: n >= 1 and k a multiple of 16 in [16, %d] (got %d, %d)", who, kMaxRow, p.n, p.k);
-  NKV_CHECK_ARG(m * p.k <= kTokenCodes, "%s: m * k must be at most %d (got %d * %d)", who, kTokenCodes, m, p.k);
+  NKV_CHECK_ARG(p.n >= 1 && p.n <= INT32_MAX / 2 - 512 && p.k >= 16 && p.k % 16 == 0 && p.k <= kTokenMaxK,
+                "%s: n >= 1 and k a multiple of 16 in [16, %d] (got %d, %d)", who, kTokenMaxK, p.n, p.k);
   NKV_CHECK_ARG(aligned16(p.w) && aligned16(p.x) && (!p.res || aligned16(p.res)) && (!p.nw || aligned16(p.nw)) &&
                     (!p.res_out || aligned16(p.res_out)),
-                "%s: weight, the rows, norm_weight and residual_out must be 16-byte aligned", who);
-  // every workgroup reads the rows, norm_weight and its scales while others write y and one writes residual_out
-  const int64_t row = 2 * static_cast<int64_t>(p.k), rows = m * row, out = 2 * static_cast<int64_t>(m) * p.n;
+                "%s: weight, x, residual, norm_weight and residual_out must be 16-byte aligned", who);
+  // every workgroup reads the row, norm_weight and its scales while others write y and one writes residual_out
+  const int64_t row = 2 * static_cast<int64_t>(p.k), out = 2 * static_cast<int64_t>(p.n);
   const int64_t channels = static_cast<int64_t>(p.n) * (SILU ? 2 : 1);
   struct Out {
     const char* name;
     const void* at;
     int64_t bytes;
   };
-  for (const Out& o : {Out{"y", p.y, out}, Out{"residual_out", p.res_out, rows}})
-    NKV_CHECK_ARG(apart(o.at, o.bytes, p.x, rows) && apart(o.at, o.bytes, p.res, rows) && apart(o.at, o.bytes, p.nw, row) &&
+  for (const Out& o : {Out{"y", p.y, out}, Out{"residual_out", p.res_out, row}})
+    NKV_CHECK_ARG(apart(o.at, o.bytes, p.x, row) && apart(o.at, o.bytes, p.res, row) && apart(o.at, o.bytes, p.nw, row) &&
                       apart(o.at, o.bytes, p.w, channels * p.k) && apart(o.at, o.bytes, p.sw, 4 * channels) &&
                       apart(o.at, o.bytes, p.bias, 2 * channels),
                   "%s: %s must not overlap an input", who, o.name);
-  NKV_CHECK_ARG(apart(p.y, out, p.res_out, rows), "%s: y must not overlap residual_out", who);
-  launch_token<NORM, SILU>(p, m, reinterpret_cast<hipStream_t>(stream));
+  NKV_CHECK_ARG(apart(p.y, out, p.res_out, row), "%s: y must not overlap residual_out", who);
+  launch_token<NORM, SILU>(p, reinterpret_cast<hipStream_t>(stream));
   return launch_status(who);
 }
 
@@ -486,8 +879,8 @@ extern "C" int nkv_linear_q8(const int8_t* weight, const float* w_scale, const i
   const Product p{weight, w_scale, x, x_scale, bias, y, m, n, k};
   const int rc = check_product("nkv_linear_q8", p, 1);
   if (rc != NKV_OK) return rc;
-  launch_product<false>(p, reinterpret_cast<hipStream_t>(stream));
-  return launch_status("nkv_linear_q8");
+  const int launched = launch_product<false>(p, reinterpret_cast<hipStream_t>(stream));
+  return launched != NKV_OK ? launched : launch_status("nkv_linear_q8");
 }
 
 extern "C" int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const int8_t* x,
@@ -495,33 +888,32 @@ extern "C" int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float*
   const Product p{gate_up_weight, w_scale, x, x_scale, nullptr, y, m, intermediate, k};
   const int rc = check_product("nkv_linear_silu_mul_q8", p, 2);
   if (rc != NKV_OK) return rc;
-  launch_product<true>(p, reinterpret_cast<hipStream_t>(stream));
-  return launch_status("nkv_linear_silu_mul_q8");
+  const int launched = launch_product<true>(p, reinterpret_cast<hipStream_t>(stream));
+  return launched != NKV_OK ? launched : launch_status("nkv_linear_silu_mul_q8");
 }
 
 extern "C" int nkv_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* bias, uint16_t* y,
-                           int m, int n, int k, void* stream) {
-  return token<false, false>("nkv_gemv_q8", Token{weight, w_scale, x, nullptr, nullptr, bias, y, nullptr, 0.0f, n, k}, m, stream);
+                           int n, int k, void* stream) {
+  return token<false, false>("nkv_gemv_q8", Token{weight, w_scale, x, nullptr, nullptr, bias, y, nullptr, 0.0f, n, k}, stream);
 }
 
-extern "C" int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y, int m,
+extern "C" int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y,
                                     int intermediate, int k, void* stream) {
   return token<false, true>("nkv_gemv_silu_mul_q8",
-                            Token{gate_up_weight, w_scale, x, nullptr, nullptr, nullptr, y, nullptr, 0.0f, intermediate, k}, m,
-                            stream);
+                            Token{gate_up_weight, w_scale, x, nullptr, nullptr, nullptr, y, nullptr, 0.0f, intermediate, k}, stream);
 }
 
 extern "C" int nkv_norm_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* residual,
                                 const uint16_t* norm_weight, float eps, const uint16_t* bias, uint16_t* y,
-                                uint16_t* residual_out, int m, int n, int k, void* stream) {
+                                uint16_t* residual_out, int n, int k, void* stream) {
   return token<true, false>("nkv_norm_gemv_q8",
-                            Token{weight, w_scale, x, residual, norm_weight, bias, y, residual_out, eps, n, k}, m, stream);
+                            Token{weight, w_scale, x, residual, norm_weight, bias, y, residual_out, eps, n, k}, stream);
 }
 
 extern "C" int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x,
                                          const uint16_t* residual, const uint16_t* norm_weight, float eps, uint16_t* y,
-                                         uint16_t* residual_out, int m, int intermediate, int k, void* stream) {
+                                         uint16_t* residual_out, int intermediate, int k, void* stream) {
   return token<true, true>("nkv_norm_gemv_silu_mul_q8",
                            Token{gate_up_weight, w_scale, x, residual, norm_weight, nullptr, y, residual_out, eps, intermediate, k},
-                           m, stream);
+                           stream);
 }

@@ -13,8 +13,8 @@ an infinity has the scale NaN and the codes 0, so what is computed from it is
 NaN.
 
 On the GPU the operands are bf16 and the work is this library's kernels (no
-fallback: the library must load); 1-4 rows (decode steps) take the row's norm
-and quantisation inside the product's launch.  CPU tensors take the formulas,
+fallback: the library must load); one row (a decode token) takes its norm and
+quantisation inside the product's launch.  CPU tensors take the formulas,
 which the tests of the modules' routing run on.  Inference only: nothing here
 has a gradient, and inputs that ask for one are refused.
 """
@@ -29,9 +29,7 @@ from . import _lib
 from .store import current_stream_ptr
 
 TINY = 2.0 ** -119       # rows whose largest magnitude is below are zero
-MAX_ROW = 32768          # longest row that is quantised on the GPU
-TOKEN_ROWS = 4           # rows a product quantises in its own launch, ...
-TOKEN_CODES = 49152      # ... of at most so many elements together
+TOKEN_ROW = 12288        # longest row that a product quantises in its own launch
 
 
 class Q8(NamedTuple):
@@ -221,10 +219,10 @@ def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
     if m == 0 or n == 0:
         return y
     if not isinstance(x, Q8):
-        if m <= TOKEN_ROWS and m * k <= TOKEN_CODES and k <= MAX_ROW:
+        if m == 1 and k <= TOKEN_ROW:
             x = _rows(x, who)
             _call("gemv_silu_mul_q8" if silu_mul else "gemv_q8", x.get_device(), weight.q.data_ptr(),
-                  weight.scale.data_ptr(), x.data_ptr(), *b, y.data_ptr(), m, n, k)
+                  weight.scale.data_ptr(), x.data_ptr(), *b, y.data_ptr(), n, k)
             return y
         x = quantize_q8(x)
     x = _dense(x)
@@ -248,7 +246,7 @@ def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool
     k = x.shape[-1] if x.dim() else 0
     _check_weight(weight, k, x.device, who, silu_mul)
     m = x.numel() // k
-    if not (x.is_cuda and 1 <= m <= TOKEN_ROWS and m * k <= TOKEN_CODES and k <= MAX_ROW) or not weight.q.shape[0]:
+    if not (x.is_cuda and m == 1 and k <= TOKEN_ROW and weight.q.shape[0]):
         t, res_out = rmsnorm_q8(x, norm_weight, eps, residual)
         return _linear(t, weight, bias, silu_mul, who), res_out
     weight = _dense(weight)
@@ -266,7 +264,7 @@ def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool
     has = residual is not None
     _call("norm_gemv_silu_mul_q8" if silu_mul else "norm_gemv_q8", x.get_device(), weight.q.data_ptr(),
           weight.scale.data_ptr(), x.data_ptr(), residual.data_ptr() if has else None, norm_weight.data_ptr(),
-          float(eps), *b, y.data_ptr(), res_out.data_ptr() if has else None, m, n, k)
+          float(eps), *b, y.data_ptr(), res_out.data_ptr() if has else None, n, k)
     return y, res_out
 
 

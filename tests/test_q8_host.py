@@ -94,15 +94,15 @@ def _product(name, m=8, n=64, k=128, **moved):
     return lib.nkv_linear_silu_mul_q8(p["w"], p["sw"], p["x"], p["sx"], p["y"], m, n, k, None)
 
 
-def _token(name, m=2, n=64, k=128, **moved):
+def _token(name, n=64, k=128, **moved):
     p, lib = _p(**moved), _lib.load()
     if name == "nkv_gemv_q8":
-        return lib.nkv_gemv_q8(p["w"], p["sw"], p["x"], p["b"], p["y"], m, n, k, None)
+        return lib.nkv_gemv_q8(p["w"], p["sw"], p["x"], p["b"], p["y"], n, k, None)
     if name == "nkv_gemv_silu_mul_q8":
-        return lib.nkv_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["y"], m, n, k, None)
+        return lib.nkv_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["y"], n, k, None)
     if name == "nkv_norm_gemv_q8":
-        return lib.nkv_norm_gemv_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["b"], p["y"], p["ro"], m, n, k, None)
-    return lib.nkv_norm_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["y"], p["ro"], m, n, k, None)
+        return lib.nkv_norm_gemv_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["b"], p["y"], p["ro"], n, k, None)
+    return lib.nkv_norm_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["y"], p["ro"], n, k, None)
 
 
 @pytest.mark.parametrize("name", ["nkv_linear_q8", "nkv_linear_silu_mul_q8"])
@@ -119,12 +119,12 @@ def test_products_refuse_bad_arguments(name):
 @pytest.mark.parametrize("name", ["nkv_gemv_q8", "nkv_gemv_silu_mul_q8", "nkv_norm_gemv_q8", "nkv_norm_gemv_silu_mul_q8"])
 def test_token_products_refuse_bad_arguments(name):
     norm = "norm" in name
-    for bad in [dict(m=0), dict(m=5), dict(n=0), dict(k=0), dict(k=24), dict(k=32784), dict(m=4, k=12304), dict(w=8),
+    for bad in [dict(n=0), dict(k=0), dict(k=24), dict(k=12304), dict(n=2 ** 31 - 1), dict(w=8),
                 dict(x=4104), dict(w=0), dict(sw=0), dict(x=0), dict(y=0)] + norm * [dict(nw=0), dict(nw=8), dict(res=24),
                                                                                      dict(ro=8)]:
         assert _token(name, **bad) == _lib.NKV_ERR_ARG, bad
-    row = 2 * 2 * 128
-    for out, size in [("y", 2 * 2 * 64)] + norm * [("ro", row)]:
+    row = 2 * 128
+    for out, size in [("y", 2 * 64)] + norm * [("ro", row)]:
         for what, length in [("w", 64 * 128), ("sw", 4 * 64), ("x", row)] + norm * [("res", row), ("nw", 256)]:
             for where in (AT[what], AT[what] + length - 16, AT[what] - size + 16):
                 assert _token(name, **{out: where}) == _lib.NKV_ERR_ARG and b"overlap" in _lib.load().nkv_last_error()
