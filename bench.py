@@ -314,7 +314,7 @@ def bench_model(args, dev):
     launches (not the batched 36-layer launches of the decode line)."""
     import torch
 
-    from nanokv_amd.qwen3 import Qwen3Config, Qwen3ForCausalLM, init_random_
+    from nanokv_amd.qwen3 import Qwen3Config, Qwen3ForCausalLM, init_random_, quantize_linears_
     from nanokv_amd.sparse import M12Config
 
     T = args.context
@@ -330,6 +330,9 @@ def bench_model(args, dev):
     finally:
         torch.set_default_dtype(prev)
     init_random_(model, args.seed)
+    params = sum(p.numel() for p in model.parameters())
+    if args.weights == "int8":
+        quantize_linears_(model)
     model.attach(m12, dev)
     prompt = torch.randint(0, cfg.vocab_size, (T,), device=dev,
                            generator=torch.Generator(device=dev).manual_seed(args.seed))
@@ -362,7 +365,6 @@ def bench_model(args, dev):
     eager_ms, eager_host = run(model.decode, max(4, args.steps // 4))
     run(model.decode_graph, args.warmup + 2)   # eager device-ring step, capture, replays
     tpot, host_ms = run(model.decode_graph, args.steps)
-    params = sum(p.numel() for p in model.parameters())
     return {
         "metric": MODEL_METRIC,
         "value": round(1e3 / tpot, 2),
@@ -374,7 +376,7 @@ def bench_model(args, dev):
         "higher_is_better": True,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": "bf16",
+        "dtype": "bf16" if args.weights == "bf16" else "bf16, projections and LM head int8 x int8",
         "data": "synthetic (random N(0, 0.02) weights, seeded random prompt tokens, greedy decode)",
         "config": {
             "workload": (f"Qwen3-4B architecture ({args.layers} layers, {params / 1e9:.2f} B parameters), "
@@ -382,7 +384,7 @@ def bench_model(args, dev):
                          f"sparse attention top-{args.top_k} + sink {m12.sink_tokens} + recent "
                          f"{m12.recent_tokens}, {args.kv_format} history"),
             "layers": args.layers, "context": T, "chunk": args.chunk, "top_k": args.top_k,
-            "kv_format": args.kv_format,
+            "kv_format": args.kv_format, "weights": args.weights,
         },
         "tpot_ms": round(tpot, 4),
         "host_enqueue_ms_per_token": round(host_ms, 4),
@@ -543,6 +545,8 @@ def main():
                          "lossless speculative verify (use --context 16384), or whole-model "
                          "Qwen3-4B decode (tokens/s = 1 / TPOT)")
     ap.add_argument("--chunk", type=int, default=4096, help="prefill chunk length")
+    ap.add_argument("--weights", choices=["bf16", "int8"], default="bf16",
+                    help="model: the projections' and the LM head's weights (int8: nanokv_amd.q8)")
     ap.add_argument("--prefill-selection", choices=["chunk", "tile"], default="chunk",
                     help="prefill: one selection per chunk (the reference's routing) or per 64-query tile")
     ap.add_argument("--copy-probe-mib", type=int, default=0,

@@ -66,21 +66,31 @@ def _silu_mul_formula(x: Q8, weight: Q8) -> torch.Tensor:
 
 
 # -- operands --------------------------------------------------------------------
+# A token's call is bound by the host (about 4 us of launch, 1.3 us an allocation),
+# so the checks ask each tensor for little, and devices are compared as numbers.
+_I8, _F32, _BF16 = torch.int8, torch.float32, torch.bfloat16
+_ENTRY: dict = {}        # the library's functions by name, once it is loaded
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or current_stream_ptr
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(name: str, device: int, *args) -> None:
-    """nkv_<name>(*args, stream): the tensors' device is made current for the launch."""
-    fn = getattr(_lib.load(), "nkv_" + name)
-    if device == torch.cuda.current_device():
-        rc = fn(*args, current_stream_ptr())
+    """nkv_<name>(*args, stream) on the tensors' device, which is made current for the launch."""
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(_lib.load(), "nkv_" + name)
+    if device == _current_device():
+        rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, current_stream_ptr())
+            rc = fn(*args, _raw_stream(device))
     if rc:
         _lib.check(rc, name)
 
 
 def _rows(x: torch.Tensor, who: str, what: str = "x") -> torch.Tensor:
     """x as dense bf16 rows on a 16-byte boundary (copied if it is neither)."""
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not _BF16:
         raise ValueError(f"{who}: {what} must be bfloat16 on the GPU (got {x.dtype})")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{who}: {what} asks for a gradient, and the 8-bit operators have none")
@@ -89,30 +99,32 @@ def _rows(x: torch.Tensor, who: str, what: str = "x") -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _vector(t: torch.Tensor, n: int, device: torch.device, who: str, what: str) -> torch.Tensor:
-    if t.dim() != 1 or t.shape[0] != n or t.device != device:
-        raise ValueError(f"{who}: {what} must be a [{n}] tensor on {device} (got {tuple(t.shape)} on {t.device})")
+def _vector(t: torch.Tensor, n: int, device: int, who: str, what: str) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != n or t.get_device() != device:
+        raise ValueError(f"{who}: {what} must be a [{n}] tensor on x's device (got {tuple(t.shape)} on {t.device})")
     return _rows(t, who, what)
 
 
 def _like(t: torch.Tensor, x: torch.Tensor, who: str, what: str) -> torch.Tensor:
-    if t.shape != x.shape or t.device != x.device:
+    if t.shape != x.shape or t.get_device() != x.get_device():
         raise ValueError(f"{who}: {what} must be like x, {tuple(x.shape)} on {x.device} "
                          f"(got {tuple(t.shape)} on {t.device})")
     return _rows(t, who, what)
 
 
-def _check_width(n: int, who: str) -> None:
+def _width(x: torch.Tensor, who: str) -> int:
+    n = x.shape[-1] if x.dim() else 0
     if n < 16 or n % 16:
         raise ValueError(f"{who}: the last dimension must be a positive multiple of 16 (got {n})")
+    return n
 
 
 def _check_q8(t: Q8, who: str, what: str) -> None:
     q, scale = t
-    if q.dtype != torch.int8 or scale.dtype != torch.float32 or q.dim() < 1 or scale.shape != q.shape[:-1]:
+    if q.dtype is not _I8 or scale.dtype is not _F32 or q.dim() < 1 or scale.shape != q.shape[:-1]:
         raise ValueError(f"{who}: {what} must hold int8 codes [..., n] and float32 scales [...] "
                          f"(got {q.dtype} {tuple(q.shape)}, {scale.dtype} {tuple(scale.shape)})")
-    if q.device != scale.device:
+    if q.get_device() != scale.get_device():
         raise ValueError(f"{who}: {what}'s codes and scales must be on one device")
 
 
@@ -123,14 +135,22 @@ def _dense(t: Q8) -> Q8:
     return Q8(q, scale if scale.is_contiguous() else scale.contiguous())
 
 
-def _check_weight(weight: Q8, k: int, device: torch.device, who: str, halves: bool = False) -> None:
-    _check_q8(weight, who, "weight")
-    q = weight.q
-    if q.dim() != 2 or q.shape[1] != k or q.device != device:
-        raise ValueError(f"{who}: weight must be [n, {k}] on {device} (got {tuple(q.shape)} on {q.device})")
-    if halves and q.shape[0] % 2:
-        raise ValueError(f"{who}: the gate|up weight needs an even number of rows")
-    _check_width(k, who)
+def _weight(weight: Q8, k: int, device: int, who: str, halves: bool) -> tuple:
+    """(codes [n, k], scales [n], channels of y) of a weight on `device` (a number, -1: CPU), dense on the GPU."""
+    q, scale = weight
+    if (q.dtype is not _I8 or scale.dtype is not _F32 or q.dim() != 2 or scale.dim() != 1 or q.size(1) != k
+            or scale.size(0) != q.size(0) or q.get_device() != device or scale.get_device() != device):
+        raise ValueError(f"{who}: weight must hold int8 codes [n, {k}] and float32 scales [n] on x's device "
+                         f"(got {q.dtype} {tuple(q.shape)} on {q.device}, {scale.dtype} {tuple(scale.shape)} on "
+                         f"{scale.device})")
+    n = q.size(0)
+    if halves:
+        if n % 2:
+            raise ValueError(f"{who}: the gate|up weight needs an even number of rows")
+        n //= 2
+    if device >= 0 and not (q.is_contiguous() and scale.is_contiguous() and q.data_ptr() % 16 == 0):
+        q, scale = _dense(Q8(q, scale))
+    return q, scale, n
 
 
 # -- operators ---------------------------------------------------------------------
@@ -139,96 +159,114 @@ def quantize_q8(x: torch.Tensor) -> Q8:
 
     2-D rows may lie apart (a column range of a wider matrix, on 16-byte
     boundaries) and are read in place."""
-    if x.dim() < 1:
-        raise ValueError("quantize_q8: x needs at least one dimension")
-    n = x.shape[-1]
-    _check_width(n, "quantize_q8")
+    n = _width(x, "quantize_q8")
     if not x.is_cuda:
         return _quantize_formula(x.float())
-    stride = n
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) > n and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 \
-            and x.dtype == torch.bfloat16 and not x.requires_grad:
-        stride = x.stride(0)
-    else:
-        x = _rows(x, "quantize_q8")
-    out = Q8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-             torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device))
-    rows = out.scale.numel()
+    x, stride = _strided(x, n, "quantize_q8")
+    out = Q8(torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[:-1], dtype=_F32, device=x.device))
+    rows = x.numel() // n
     if rows:
         _call("quantize_q8", x.get_device(), x.data_ptr(), stride, out.q.data_ptr(), out.scale.data_ptr(), rows, n)
     return out
 
 
+def _strided(x: torch.Tensor, n: int, who: str) -> tuple:
+    """(x, elements from row to row): 2-D bf16 rows that lie apart stay where they are."""
+    if (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) > n and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
+            and x.dtype is _BF16 and not x.requires_grad):
+        return x, x.stride(0)
+    return _rows(x, who), n
+
+
 def dequantize_q8(t: Q8) -> torch.Tensor:
     """bf16(q * scale)."""
     _check_q8(t, "dequantize_q8", "t")
-    n = t.q.shape[-1]
-    _check_width(n, "dequantize_q8")
+    n = _width(t.q, "dequantize_q8")
     if not t.q.is_cuda:
-        return (t.q.float() * t.scale.unsqueeze(-1)).to(torch.bfloat16)
-    t = _dense(t)
-    out = torch.empty(t.q.shape, dtype=torch.bfloat16, device=t.q.device)
-    if out.numel():
-        _call("dequantize_q8", out.get_device(), t.q.data_ptr(), t.scale.data_ptr(), out.data_ptr(), t.scale.numel(), n)
+        return (t.q.float() * t.scale.unsqueeze(-1)).to(_BF16)
+    q, scale = _dense(t)
+    out = torch.empty(q.shape, dtype=_BF16, device=q.device)
+    rows = out.numel() // n
+    if rows:
+        _call("dequantize_q8", out.get_device(), q.data_ptr(), scale.data_ptr(), out.data_ptr(), rows, n)
     return out
+
+
+def _norm(x, weight, eps, residual, q: int, scale: int, rows: int, n: int, who: str, what: str):
+    """nkv_rmsnorm_q8 of checked dense rows x into the addresses q and scale; the new residual."""
+    device = x.get_device()
+    weight = _vector(weight, n, device, who, what)
+    res_out = x
+    if residual is not None:
+        residual = _like(residual, x, who, "residual")
+        res_out = torch.empty_like(x)
+    if rows:
+        has = residual is not None
+        _call("rmsnorm_q8", device, x.data_ptr(), residual.data_ptr() if has else None, weight.data_ptr(), float(eps),
+              q, scale, res_out.data_ptr() if has else None, rows, n)
+    return res_out
 
 
 def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None):
     """RMSNorm of x (+ residual) over the last dim, held in 8 bits: (Q8, the new
     residual bf16(x + residual), or x itself without one)."""
-    n = x.shape[-1] if x.dim() else 0
-    _check_width(n, "rmsnorm_q8")
+    n = _width(x, "rmsnorm_q8")
     if not x.is_cuda:
         return _norm_formula(x, weight, eps, residual)
     x = _rows(x, "rmsnorm_q8")
-    weight = _vector(weight, n, x.device, "rmsnorm_q8", "weight")
-    out = Q8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-             torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device))
-    res_out = x
-    if residual is not None:
-        residual = _like(residual, x, "rmsnorm_q8", "residual")
-        res_out = torch.empty_like(x)
-    rows = out.scale.numel()
-    if rows:
-        _call("rmsnorm_q8", x.get_device(), x.data_ptr(), residual.data_ptr() if residual is not None else None,
-              weight.data_ptr(), float(eps), out.q.data_ptr(), out.scale.data_ptr(),
-              res_out.data_ptr() if residual is not None else None, rows, n)
-    return out, res_out
+    out = Q8(torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[:-1], dtype=_F32, device=x.device))
+    return out, _norm(x, weight, eps, residual, out.q.data_ptr(), out.scale.data_ptr(), x.numel() // n, n, "rmsnorm_q8",
+                      "weight")
+
+
+def _product(q: int, scale: int, shape, device: torch.device, m: int, k: int, weight: tuple, bias, silu_mul: bool):
+    """The product of m > 0 rows of codes at the addresses q and scale; y [*shape[:-1], n]."""
+    wq, ws, n = weight
+    y = torch.empty((*shape[:-1], n), dtype=_BF16, device=device)
+    if n:
+        b = () if silu_mul else (bias.data_ptr() if bias is not None else None,)
+        _call("linear_silu_mul_q8" if silu_mul else "linear_q8", y.get_device(), wq.data_ptr(), ws.data_ptr(), q, scale,
+              *b, y.data_ptr(), m, n, k)
+    return y
 
 
 def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
-    q = x.q if isinstance(x, Q8) else x
-    if isinstance(x, Q8):
+    held = isinstance(x, Q8)
+    if held:
         _check_q8(x, who, "x")
-    if q.dim() < 1:
-        raise ValueError(f"{who}: x needs at least one dimension")
-    k = q.shape[-1]
-    _check_weight(weight, k, q.device, who, silu_mul)
-    n = weight.q.shape[0] // (2 if silu_mul else 1)
-    if not q.is_cuda:
-        t = x if isinstance(x, Q8) else quantize_q8(x)
+    q = x.q if held else x
+    k = _width(q, who)
+    device = q.get_device()
+    w = _weight(weight, k, device, who, silu_mul)
+    if device < 0:
+        t = x if held else quantize_q8(x)
         y = _silu_mul_formula(t, weight) if silu_mul else _product_formula(t, weight, bias)
-        return y.to(torch.bfloat16 if isinstance(x, Q8) else x.dtype)
-    weight = _dense(weight)
+        return y.to(_BF16 if held else x.dtype)
+    n = w[2]
     if bias is not None:
-        bias = _vector(bias, n, q.device, who, "bias")
-    b = () if silu_mul else (bias.data_ptr() if bias is not None else None,)
-    name = "linear_silu_mul_q8" if silu_mul else "linear_q8"
-    y = torch.empty(*q.shape[:-1], n, dtype=torch.bfloat16, device=q.device)
+        bias = _vector(bias, n, device, who, "bias")
     m = q.numel() // k
-    if m == 0 or n == 0:
+    if held:
+        x = _dense(x)
+        if m:
+            return _product(x.q.data_ptr(), x.scale.data_ptr(), q.shape, q.device, m, k, w, bias, silu_mul)
+    elif m == 1 and k <= TOKEN_ROW and n:
+        x = _rows(x, who)
+        y = torch.empty((*x.shape[:-1], n), dtype=_BF16, device=x.device)
+        if silu_mul:
+            _call("gemv_silu_mul_q8", device, w[0].data_ptr(), w[1].data_ptr(), x.data_ptr(), y.data_ptr(), n, k)
+        else:
+            _call("gemv_q8", device, w[0].data_ptr(), w[1].data_ptr(), x.data_ptr(),
+                  bias.data_ptr() if bias is not None else None, y.data_ptr(), n, k)
         return y
-    if not isinstance(x, Q8):
-        if m == 1 and k <= TOKEN_ROW:
-            x = _rows(x, who)
-            _call("gemv_silu_mul_q8" if silu_mul else "gemv_q8", x.get_device(), weight.q.data_ptr(),
-                  weight.scale.data_ptr(), x.data_ptr(), *b, y.data_ptr(), n, k)
-            return y
-        x = quantize_q8(x)
-    x = _dense(x)
-    _call(name, y.get_device(), weight.q.data_ptr(), weight.scale.data_ptr(), x.q.data_ptr(), x.scale.data_ptr(), *b,
-          y.data_ptr(), m, n, k)
-    return y
+    else:
+        x, stride = _strided(x, k, who)
+        if m:
+            codes = torch.empty(m * (k + 4), dtype=_I8, device=x.device)    # the codes, then their scales
+            at = codes.data_ptr()
+            _call("quantize_q8", device, x.data_ptr(), stride, at, at + m * k, m, k)
+            return _product(at, at + m * k, x.shape, x.device, m, k, w, bias, silu_mul)
+    return torch.empty((*q.shape[:-1], n), dtype=_BF16, device=q.device)
 
 
 def linear_q8(x, weight: Q8, bias: torch.Tensor | None = None) -> torch.Tensor:
@@ -243,28 +281,36 @@ def linear_silu_mul_q8(x, gate_up_weight: Q8) -> torch.Tensor:
 
 
 def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool, who: str):
-    k = x.shape[-1] if x.dim() else 0
-    _check_weight(weight, k, x.device, who, silu_mul)
-    m = x.numel() // k
-    if not (x.is_cuda and m == 1 and k <= TOKEN_ROW and weight.q.shape[0]):
-        t, res_out = rmsnorm_q8(x, norm_weight, eps, residual)
-        return _linear(t, weight, bias, silu_mul, who), res_out
-    weight = _dense(weight)
+    k = _width(x, who)
+    device = x.get_device()
+    w = _weight(weight, k, device, who, silu_mul)
+    if device < 0:
+        t, res_out = _norm_formula(x, norm_weight, eps, residual)
+        y = _silu_mul_formula(t, weight) if silu_mul else _product_formula(t, weight, bias)
+        return y.to(x.dtype), res_out
+    n = w[2]
     x = _rows(x, who)
-    norm_weight = _vector(norm_weight, k, x.device, who, "norm_weight")
-    n = weight.q.shape[0] // (2 if silu_mul else 1)
+    if bias is not None:
+        bias = _vector(bias, n, device, who, "bias")
+    m = x.numel() // k
+    if m != 1 or k > TOKEN_ROW or not n:
+        codes = torch.empty(m * (k + 4), dtype=_I8, device=x.device)        # the codes, then their scales
+        at = codes.data_ptr()
+        res_out = _norm(x, norm_weight, eps, residual, at, at + m * k, m, k, who, "norm_weight")
+        if m == 0:
+            return torch.empty((*x.shape[:-1], n), dtype=_BF16, device=x.device), res_out
+        return _product(at, at + m * k, x.shape, x.device, m, k, w, bias, silu_mul), res_out
+    norm_weight = _vector(norm_weight, k, device, who, "norm_weight")
     res_out = x
-    if residual is not None:
+    has = residual is not None
+    if has:
         residual = _like(residual, x, who, "residual")
         res_out = torch.empty_like(x)
-    if bias is not None:
-        bias = _vector(bias, n, x.device, who, "bias")
+    y = torch.empty((*x.shape[:-1], n), dtype=_BF16, device=x.device)
     b = () if silu_mul else (bias.data_ptr() if bias is not None else None,)
-    y = torch.empty(*x.shape[:-1], n, dtype=torch.bfloat16, device=x.device)
-    has = residual is not None
-    _call("norm_gemv_silu_mul_q8" if silu_mul else "norm_gemv_q8", x.get_device(), weight.q.data_ptr(),
-          weight.scale.data_ptr(), x.data_ptr(), residual.data_ptr() if has else None, norm_weight.data_ptr(),
-          float(eps), *b, y.data_ptr(), res_out.data_ptr() if has else None, n, k)
+    _call("norm_gemv_silu_mul_q8" if silu_mul else "norm_gemv_q8", device, w[0].data_ptr(), w[1].data_ptr(),
+          x.data_ptr(), residual.data_ptr() if has else None, norm_weight.data_ptr(), float(eps), *b, y.data_ptr(),
+          res_out.data_ptr() if has else None, n, k)
     return y, res_out
 
 

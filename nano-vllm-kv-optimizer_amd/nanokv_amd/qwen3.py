@@ -19,7 +19,10 @@ library's kernels, routed by the per-step context.  On the GPU the
 elementwise chains are this library's fused kernels (nkv_rmsnorm,
 nkv_qk_norm_rope, nkv_silu_mul: one launch each, same rounding points) and
 the decode-step projections its HBM-bound GEMV (nkv_gemv); the tensor-op
-formulas below are the CPU path of the same modules.
+formulas below are the CPU path of the same modules.  ``quantize_linears_``
+(``from_pretrained(weights="int8")``) turns the projections and the LM head
+into 8-bit ones (``nanokv_amd.q8``): half the weight bytes of a token, integer
+products for a prompt.
 
 Weights come from a local checkpoint directory (config.json + *.safetensors
 with the Hugging Face Qwen3 parameter names, packed into the fused
@@ -44,6 +47,7 @@ from torch import nn
 
 from . import _lib
 from .attention import Attention, attach_m12_runtimes, set_context
+from .q8 import Q8, linear_q8, linear_silu_mul_q8, norm_linear_q8, norm_linear_silu_mul_q8, quantize_q8
 from .sparse.m12_runtime import M12Config
 from .store import _ptr, _stream
 
@@ -201,6 +205,46 @@ class Linear(nn.Linear):
         if self.bias is None and _gemv_ok(x, self.weight):
             return gemv_dev(x, self.weight)
         return F.linear(x, self.weight, self.bias)
+
+
+class Q8Linear(nn.Module):
+    """A projection whose weight is held in 8 bits with a scale an output channel
+    and whose inputs are quantised row by row (``nanokv_amd.q8.linear_q8``).
+
+    ``weight`` [n, k]: k a multiple of 16, finite.  The codes and scales are buffers
+    (``weight_q8``, ``weight_scale``), the scales fp32 whatever the model is cast to."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None):
+        super().__init__()
+        if weight.dim() != 2:
+            raise ValueError(f"Q8Linear: weight must be [n, k] (got {tuple(weight.shape)})")
+        q, scale = quantize_q8(weight.detach())
+        if not bool(scale.isfinite().all()):
+            raise ValueError("Q8Linear: the weight holds NaN or infinite values")
+        self.out_features, self.in_features = weight.shape
+        self.register_buffer("weight_q8", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:      # a cast of the model: moved, not rounded
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
+    @property
+    def weight(self) -> Q8:
+        return Q8(self.weight_q8, self.weight_scale)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear_q8(x, self.weight, self.bias)
+
+
+def _norm_q8(norm: nn.Module, proj: nn.Module) -> bool:
+    """Whether norm followed by proj may run as one norm_linear_q8 (or its gated
+    form): this file's modules without hooks."""
+    return _own(norm, RMSNorm) and _own(proj, Q8Linear) and not nn.modules.module._has_any_global_hook()
 
 
 def silu_mul_dev(gate_up: torch.Tensor) -> torch.Tensor:
@@ -416,6 +460,8 @@ class Qwen3MLP(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         proj = self.gate_up_proj
+        if _own(proj, Q8Linear) and proj.bias is None:
+            return self.down_proj(linear_silu_mul_q8(x, proj.weight))
         if (_own(proj, Linear) and proj.bias is None and _gemv_ok(x, proj.weight)
                 and proj.weight.shape[0] % 2 == 0):
             return self.down_proj(gemv_silu_mul_dev(x, proj.weight))   # one launch for both
@@ -442,6 +488,10 @@ class Qwen3DecoderLayer(nn.Module):
         if fused:
             qkv, residual = norm_gemv_dev(h, residual, *fused)
             h = attn.attend(positions, qkv)
+        elif _own(attn, Qwen3Attention) and _norm_q8(norm, attn.qkv_proj):
+            proj = attn.qkv_proj
+            qkv, residual = norm_linear_q8(h, norm.weight, norm.eps, proj.weight, residual, proj.bias)
+            h = attn.attend(positions, qkv)
         else:
             h, residual = (norm(h), h) if residual is None else norm(h, residual)
             h = attn(positions, h)
@@ -450,11 +500,14 @@ class Qwen3DecoderLayer(nn.Module):
         if fused and fused[2].shape[0] % 2 == 0:
             h, residual = norm_gemv_dev(h, residual, *fused, silu_mul=True)
             return mlp.down_proj(h), residual
+        if _own(mlp, Qwen3MLP) and _norm_q8(norm, mlp.gate_up_proj) and mlp.gate_up_proj.bias is None:
+            h, residual = norm_linear_silu_mul_q8(h, norm.weight, norm.eps, mlp.gate_up_proj.weight, residual)
+            return mlp.down_proj(h), residual
         h, residual = norm(h, residual)
         return mlp(h), residual
 
 
-_FORWARDS.update((c, c.forward) for c in (Linear, RMSNorm, RotaryEmbedding, Qwen3Attention, Qwen3MLP))
+_FORWARDS.update((c, c.forward) for c in (Linear, Q8Linear, RMSNorm, RotaryEmbedding, Qwen3Attention, Qwen3MLP))
 
 
 class Qwen3Model(nn.Module):
@@ -490,6 +543,7 @@ class Qwen3ForCausalLM(nn.Module):
             self.lm_head_weight = self.model.embed_tokens.weight
         else:
             self.lm_head_weight = nn.Parameter(torch.empty(cfg.vocab_size, cfg.hidden_size))
+        self.lm_head_q8 = None   # the head in 8 bits (quantize_linears_)
         self.requires_grad_(False)   # inference only
         self.runtimes = []
         self._graph = None       # captured decode step (decode_graph)
@@ -500,6 +554,8 @@ class Qwen3ForCausalLM(nn.Module):
         return self.model(input_ids, positions)
 
     def compute_logits(self, h: torch.Tensor) -> torch.Tensor:
+        if self.lm_head_q8 is not None:
+            return self.lm_head_q8(h)
         if _gemv_ok(h, self.lm_head_weight):
             return gemv_dev(h, self.lm_head_weight)
         return F.linear(h, self.lm_head_weight)
@@ -618,6 +674,40 @@ class Qwen3ForCausalLM(nn.Module):
 
 
 # -- weights -------------------------------------------------------------------
+def _check_not_quantized(model: nn.Module, what: str) -> None:
+    if any(isinstance(m, Q8Linear) for m in model.modules()):
+        raise ValueError(f"{what}: the model's projections are in 8 bits already (quantize_linears_ comes last)")
+
+
+@torch.no_grad()
+def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
+    """Replace every projection of `model` (this file's Linear) by a Q8Linear of its
+    weights, and with `lm_head` add the LM head in 8 bits (the embedding it may be
+    tied to stays); returns the number of weights quantised.
+
+    After loading the weights and moving the model to its device.  Projections
+    that were replaced or hooked before stay as they are.  A weight that cannot be held
+    in 8 bits (rows that are not a multiple of 16, NaN, infinities) raises ValueError."""
+    found = [(name, m) for name, m in model.named_modules() if _own(m, Linear)]
+    made = {}
+    for name, m in found:
+        try:
+            made[name] = Q8Linear(m.weight, m.bias)
+        except ValueError as e:
+            raise ValueError(f"quantize_linears_: {name}: {e}") from None
+    head = None
+    if lm_head and isinstance(model, Qwen3ForCausalLM):
+        head = Q8Linear(model.lm_head_weight)
+    for name, new in made.items():
+        parent, _, leaf = name.rpartition(".")
+        setattr(model.get_submodule(parent), leaf, new.train(model.training))
+    if isinstance(model, Qwen3ForCausalLM):
+        model.release_graph()
+        if head is not None:
+            model.lm_head_q8 = head
+    return len(made) + (head is not None)
+
+
 def _packed_target(model: Qwen3ForCausalLM, name: str):
     """(parameter, row offset) for a Hugging Face name that lands in a fused
     projection (q/k/v -> qkv_proj, gate/up -> gate_up_proj), else None."""
@@ -638,6 +728,7 @@ def load_checkpoint(model: Qwen3ForCausalLM, path: str) -> int:
     names and shape mismatches raise."""
     from safetensors import safe_open
 
+    _check_not_quantized(model, "load_checkpoint")
     files = sorted(glob.glob(os.path.join(path, "*.safetensors")))
     if not files:
         raise FileNotFoundError(f"no *.safetensors under {path}")
@@ -666,6 +757,7 @@ def load_checkpoint(model: Qwen3ForCausalLM, path: str) -> int:
 def init_random_(model: Qwen3ForCausalLM, seed: int = 0, std: float = 0.02) -> None:
     """N(0, std) matrices and embeddings, unit norms, zero biases (for
     measurement without a checkpoint)."""
+    _check_not_quantized(model, "init_random_")
     g = None
     for name, p in model.named_parameters():
         if g is None or g.device != p.device:
@@ -679,8 +771,13 @@ def init_random_(model: Qwen3ForCausalLM, seed: int = 0, std: float = 0.02) -> N
 
 
 def from_pretrained(path: str, m12: M12Config | None = None, device="cuda",
-                    dtype=torch.bfloat16) -> Qwen3ForCausalLM:
-    """Build from a local checkpoint directory and attach the sparse runtimes."""
+                    dtype=torch.bfloat16, weights: str = "bf16") -> Qwen3ForCausalLM:
+    """Build from a local checkpoint directory and attach the sparse runtimes.
+
+    weights="int8" holds the projections and the LM head in 8 bits
+    (quantize_linears_)."""
+    if weights not in ("bf16", "int8"):
+        raise ValueError(f"weights must be 'bf16' or 'int8' (got {weights!r})")
     cfg = Qwen3Config.from_dir(path)
     m12 = m12 or M12Config(num_heads=cfg.num_attention_heads, num_kv_heads=cfg.num_key_value_heads,
                            head_dim=cfg.head_dim)
@@ -692,9 +789,11 @@ def from_pretrained(path: str, m12: M12Config | None = None, device="cuda",
         torch.set_default_dtype(prev)
     load_checkpoint(model, path)
     model.to(device=device, dtype=dtype)
+    if weights == "int8":
+        quantize_linears_(model)
     model.attach(m12, device)
     return model
 
 
-__all__ = ["Qwen3Config", "Qwen3ForCausalLM", "RMSNorm", "RotaryEmbedding", "from_pretrained",
-           "init_random_", "load_checkpoint"]
+__all__ = ["Q8Linear", "Qwen3Config", "Qwen3ForCausalLM", "RMSNorm", "RotaryEmbedding", "from_pretrained",
+           "init_random_", "load_checkpoint", "quantize_linears_"]
