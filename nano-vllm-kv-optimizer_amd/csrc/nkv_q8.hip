@@ -68,27 +68,33 @@ __device__ __forceinline__ RowScale norm_row_scale(uint32_t top, float ss, int n
   return rs;
 }
 
-// One workgroup of THREADS a row; NCH 8-element chunks a thread.
-constexpr int kRowChunks = 4;
-template <int THREADS, bool NORM>
-__global__ __launch_bounds__(THREADS) void rows_q8_kernel(const uint16_t* __restrict__ x, int64_t x_stride,
-                                                          const uint16_t* __restrict__ res,
-                                                          const uint16_t* __restrict__ w, float eps,
-                                                          int8_t* __restrict__ q, float* __restrict__ scale,
-                                                          uint16_t* __restrict__ res_out, int n) {
-  __shared__ float s_sum[THREADS / kWave];
-  __shared__ uint32_t s_top[THREADS / kWave];
-  const int64_t row = blockIdx.x;
+// WPR wavefronts a row, NCH 8-element chunks a lane, held in registers between the
+// pass that finds the row's peak (and sum of squares) and the one that writes its
+// codes: every byte is moved once.  Short rows of many take a wavefront each
+// (no barrier), others a workgroup.
+constexpr int row_threads(int wpr) { return kWave * (wpr == 1 ? 4 : wpr); }
+template <int WPR, int NCH, bool NORM>
+__global__ __launch_bounds__(row_threads(WPR)) void rows_q8_kernel(const uint16_t* __restrict__ x, int64_t x_stride,
+                                                                   const uint16_t* __restrict__ res,
+                                                                   const uint16_t* __restrict__ w, float eps,
+                                                                   int8_t* __restrict__ q, float* __restrict__ scale,
+                                                                   uint16_t* __restrict__ res_out, int rows, int n) {
+  constexpr int kRows = row_threads(WPR) / (WPR * kWave), kLanes = WPR * kWave;
+  __shared__ float s_sum[WPR];
+  __shared__ uint32_t s_top[WPR];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (kRows > 1 ? threadIdx.x / kLanes : 0);
+  if (kRows > 1 && row >= rows) return;                // (no barrier follows)
+  const int t = kRows > 1 ? threadIdx.x % kLanes : threadIdx.x;
   const int nc = n >> 3;
   const uint4* xr = reinterpret_cast<const uint4*>(x + row * x_stride);
   const uint4* rr = NORM && res ? reinterpret_cast<const uint4*>(res + row * n) : nullptr;
   uint4* ro = NORM && res_out ? reinterpret_cast<uint4*>(res_out + row * n) : nullptr;
-  float v[kRowChunks][8];
+  float v[NCH][8];
   float ss = 0.0f;
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < kRowChunks; ++j) {
-    const int c = threadIdx.x + j * THREADS;
+  for (int j = 0; j < NCH; ++j) {
+    const int c = t + j * kLanes;
     if (c < nc) {
       unpack8(xr[c], v[j]);
       if constexpr (NORM) {
@@ -116,24 +122,24 @@ __global__ __launch_bounds__(THREADS) void rows_q8_kernel(const uint16_t* __rest
     ss += __shfl_xor(ss, o);
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
   }
-  if constexpr (THREADS > kWave) {
+  if constexpr (WPR > 1) {
     const int wave = threadIdx.x / kWave;
     if ((threadIdx.x & (kWave - 1)) == 0) s_sum[wave] = ss, s_top[wave] = top;
     __syncthreads();
     ss = 0.0f;
     top = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / kWave; ++i) ss += s_sum[i], top = max(top, s_top[i]);
+    for (int i = 0; i < WPR; ++i) ss += s_sum[i], top = max(top, s_top[i]);
   }
   const RowScale rs = NORM ? norm_row_scale(top, ss, n, eps) : row_scale(top);
   uint2* qr = reinterpret_cast<uint2*>(q + row * n);
 #pragma unroll
-  for (int j = 0; j < kRowChunks; ++j) {
-    const int c = threadIdx.x + j * THREADS;
+  for (int j = 0; j < NCH; ++j) {
+    const int c = t + j * kLanes;
     if (c < nc)
       qr[c] = make_uint2(codes4(v[j][0], v[j][1], v[j][2], v[j][3], rs.inv), codes4(v[j][4], v[j][5], v[j][6], v[j][7], rs.inv));
   }
-  if (threadIdx.x == 0) scale[row] = rs.scale;
+  if (t == 0) scale[row] = rs.scale;
 }
 
 // One thread per 16 codes.
@@ -667,11 +673,20 @@ bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
 template <bool NORM>
 void launch_rows(const uint16_t* x, int64_t x_stride, const uint16_t* res, const uint16_t* w, float eps, int8_t* q,
                  float* scale, uint16_t* res_out, int rows, int n, hipStream_t s) {
-  auto go = [&](auto kern, int threads) {
-    hipLaunchKernelGGL(kern, dim3(rows), dim3(threads), 0, s, x, x_stride, res, w, eps, q, scale, res_out, n);
+  auto go = [&](auto kern, int wpr) {
+    const int per = wpr == 1 ? 4 : 1;
+    hipLaunchKernelGGL(kern, dim3((rows + per - 1) / per), dim3(row_threads(wpr)), 0, s, x, x_stride, res, w, eps, q, scale, res_out,
+                       rows, n);
   };
-  if (n <= 256 * kRowChunks * 8) go(rows_q8_kernel<256, NORM>, 256);
-  else go(rows_q8_kernel<1024, NORM>, 1024);
+  if (n <= 512) go(rows_q8_kernel<1, 1, NORM>, 1);
+  else if (n <= 1024) go(rows_q8_kernel<2, 1, NORM>, 2);
+  else if (n <= 2048) go(rows_q8_kernel<4, 1, NORM>, 4);
+  else if (n <= 2560) go(rows_q8_kernel<5, 1, NORM>, 5);
+  else if (n <= 4096) go(rows_q8_kernel<8, 1, NORM>, 8);
+  else if (n <= 8192) go(rows_q8_kernel<8, 2, NORM>, 8);
+  else if (n <= 12288) go(rows_q8_kernel<8, 3, NORM>, 8);
+  else if (n <= 16384) go(rows_q8_kernel<8, 4, NORM>, 8);
+  else go(rows_q8_kernel<16, 4, NORM>, 16);
 }
 
 template <int NB, bool SILU>
