@@ -644,16 +644,23 @@ int nkv_rmsnorm_q8(const uint16_t* x, const uint16_t* residual, const uint16_t* 
 /*
  * y [m][n] (bf16) = the product above of x [m][k] and weight [n][k], plus bias
  * [n] (bf16) if non-NULL.  k: at most 131056 (the exact sum's range).
+ * workspace: nkv_linear_q8_workspace(m, n, k, 0) int32, 16-byte aligned (a long
+ * k of few tiles is cut over workgroups, whose sums a second launch joins: the
+ * same bits); NULL where that is 0.  Calls that share one must not overlap.
  */
 int nkv_linear_q8(const int8_t* weight, const float* w_scale, const int8_t* x, const float* x_scale,
-                  const uint16_t* bias, uint16_t* y, int m, int n, int k, void* stream);
+                  const uint16_t* bias, uint16_t* y, int m, int n, int k, int32_t* workspace, void* stream);
 
 /*
  * The product with gate_up_weight [2 intermediate][k] (gate rows, then up
  * rows) and SiLU-and-mul in fp32: y [m][intermediate] = bf16(g / (1 + e^-g) * u).
+ * workspace: nkv_linear_q8_workspace(m, intermediate, k, 1) int32, as above.
  */
 int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const int8_t* x, const float* x_scale,
-                           uint16_t* y, int m, int intermediate, int k, void* stream);
+                           uint16_t* y, int m, int intermediate, int k, int32_t* workspace, void* stream);
+
+/* int32 values of workspace a product of these sizes needs on the current device (gated: with SiLU-and-mul). */
+int64_t nkv_linear_q8_workspace(int m, int n, int k, int gated);
 
 /*
  * nkv_quantize_q8 of one row x [k] followed by the product, in one launch

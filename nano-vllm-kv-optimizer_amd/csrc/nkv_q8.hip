@@ -314,8 +314,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
 // LDS rows of a stage (weight rows, then x rows), rounded up to whole rounds of copies
 constexpr int tile_rows(int na, int nb, int wm) { return (32 * na + 16 * nb * wm + 16 * wm - 1) / (16 * wm) * (16 * wm); }
 
-template <int NA, int NB, int WM, int DEPTH, bool SILU>
-__global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt, int nt) {
+// With PART, gridDim.y workgroups share a tile, each a run of its stages, and the
+// sums go to part[blockIdx.y][m][n] for join_kernel.
+template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false>
+__global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt, int nt, bool wide, int* part) {
+  static_assert(!(SILU && PART), "");
   extern __shared__ __align__(128) char s_tile[];
   constexpr int kTileM = 16 * NB * WM, kWaves = 2 * WM;
   __shared__ __align__(16) float s_scale[32 * NA], s_bias[SILU ? 4 : 32 * NA], s_x[kTileM];
@@ -336,6 +339,10 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
   const int c0 = (in / rows_of_band) * (SILU ? 16 : 32) * NA;
 
   const int cn = min(p.n - c0, (SILU ? 16 : 32) * NA), mn = min(p.m - m0, kTileM);
+
+  const int all = (p.k + kTileK - 1) / kTileK;
+  const int first = PART ? static_cast<int>(static_cast<int64_t>(all) * blockIdx.y / gridDim.y) : 0;
+  const int stages = PART ? static_cast<int>(static_cast<int64_t>(all) * (blockIdx.y + 1) / gridDim.y) - first : all;
 
   // A wavefront's share of a stage: 8-row pieces wave, wave + kWaves, ..., lane u with
   // 16 bytes of row u >> 3.  They go through registers: loaded a stage ahead of
@@ -360,7 +367,8 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
       row = (row / (2 * half)) * half + row % half;
     }
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, rows * p.k, kRsrcWord3);
-    const int off = kc < p.k - s * kTileK ? voff + row * p.k + s * kTileK : 0x7fffffff;   // past the row's end: zeros
+    const int kb = (first + s) * kTileK;
+    const int off = kc < p.k - kb ? voff + row * p.k + kb : 0x7fffffff;   // past the row's end: zeros
     st[set][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
   };
   auto put = [&](int set, int buf, int i) {
@@ -369,13 +377,13 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
   };
 
   // the scales of the tile's weight rows and x rows, and its bias
-  for (int row = threadIdx.x; row < 32 * NA; row += 64 * kWaves) {
+  for (int row = threadIdx.x; !PART && row < 32 * NA; row += 64 * kWaves) {
     const int64_t up = SILU && (row / (8 * NA)) & 1 ? p.n : 0;
     const int c = c0 + min(SILU ? (row / (16 * NA)) * 8 * NA + row % (8 * NA) : row, cn - 1);
     s_scale[row] = p.sw[up + c];
     if constexpr (!SILU) s_bias[row] = p.bias ? bf16_to_f32(p.bias[c]) : 0.0f;
   }
-  for (int row = threadIdx.x; row < kTileM; row += 64 * kWaves) s_x[row] = p.sx[m0 + min(row, mn - 1)];
+  for (int row = threadIdx.x; !PART && row < kTileM; row += 64 * kWaves) s_x[row] = p.sx[m0 + min(row, mn - 1)];
 
   const int wc = wave & 1, wm = wave >> 1;
   const int r = lane & 15, g = lane >> 4;
@@ -410,7 +418,6 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  const int stages = (p.k + kTileK - 1) / kTileK;
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) fetch(0, 0, i);
 #pragma unroll
@@ -460,6 +467,27 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
     }
   }
 
+  if constexpr (PART) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int mj = (wm * NB + j) * 16 + r;
+      if (mj >= mn) continue;
+      int* o = part + (static_cast<int64_t>(blockIdx.y) * p.m + m0 + mj) * p.n;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int c = c0 + (wc * NA + i) * 16 + 4 * g;
+        if (wide) {
+          if (c < p.n) *reinterpret_cast<i32x4*>(o + c) = acc[i][j];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < p.n) o[c + e] = acc[i][j][e];
+        }
+      }
+    }
+    return;
+  }
+
   constexpr int kOut = SILU ? NA / 2 : NA;             // channel groups of 16 that are written
   const float4* my_scale = reinterpret_cast<const float4*>(s_scale + wc * 16 * NA + 4 * g);
   const float4* my_bias = reinterpret_cast<const float4*>(s_bias + wc * 16 * NA + 4 * g);
@@ -492,7 +520,7 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
         for (int e = 0; e < 4; ++e) v[e] = scaled(acc[i][j][e], sx, ws[e], bs[e]);
       }
       const uint2 o = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-      if ((p.n & 3) == 0) {                            // (then rows of y are 8-byte aligned, and c + 4 <= n or c >= n)
+      if (wide) {                                      // (rows of y are 8-byte aligned, and c + 4 <= n or c >= n)
         if (c < p.n) *reinterpret_cast<uint2*>(y + c) = o;
       } else {
         if (c < p.n) y[c] = static_cast<uint16_t>(o.x);
@@ -501,6 +529,41 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
         if (c + 3 < p.n) y[c + 3] = static_cast<uint16_t>(o.y >> 16);
       }
     }
+  }
+}
+
+// The sums of a product whose k was cut over `parts` workgroups, joined: y of
+// channels c .. c + V - 1 of a row a thread.  part: [parts][m][n], with SILU [parts]
+// [m][2 n] (gate, then up).
+template <int V, bool SILU>
+__global__ __launch_bounds__(256) void join_kernel(const Product p, const int* __restrict__ part, int parts) {
+  const int width = SILU ? 2 * p.n : p.n;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int per = (p.n + V - 1) / V;
+  const int64_t m = i / per;
+  if (m >= p.m) return;
+  const int c = static_cast<int>(i - m * per) * V;
+  const int* at = part + m * width + c;
+  const int64_t stride = static_cast<int64_t>(p.m) * width;
+  int sum[SILU ? 2 : 1][V] = {};
+  for (int s = 0; s < parts; ++s, at += stride)
+#pragma unroll
+    for (int h = 0; h < (SILU ? 2 : 1); ++h) {
+      if constexpr (V == 4) {
+        const i32x4 v = *reinterpret_cast<const i32x4*>(at + h * p.n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[h][e] += v[e];
+      } else {
+        sum[h][0] += at[h * p.n];
+      }
+    }
+  const float sx = p.sx[m];
+  uint16_t* y = p.y + m * p.n + c;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    float v = scaled(sum[0][e], sx, p.sw[c + e], p.bias ? bf16_to_f32(p.bias[c + e]) : 0.0f);
+    if constexpr (SILU) v = silu_mul(v, scaled(sum[SILU ? 1 : 0][e], sx, p.sw[p.n + c + e], 0.0f));
+    y[e] = f32_to_bf16(v);
   }
 }
 
@@ -697,10 +760,10 @@ int launch_few(const Product& p, hipStream_t s) {
   return NKV_OK;
 }
 
-template <int NA, int NB, int WM, int DEPTH, bool SILU>
-int launch_tile(const Product& p, hipStream_t s) {
+template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false>
+int launch_tile(const Product& p, hipStream_t s, int parts = 1, int* part = nullptr) {
   constexpr int kLds = 2 * tile_rows(NA, NB, WM) * kTileK;
-  const auto kern = tile_kernel<NA, NB, WM, DEPTH, SILU>;
+  const auto kern = tile_kernel<NA, NB, WM, DEPTH, SILU, PART>;
   if (kLds > 65536) {   // beyond the default limit of a launch (per device, so asked each time: it is a table lookup)
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) {
@@ -711,17 +774,20 @@ int launch_tile(const Product& p, hipStream_t s) {
   }
   constexpr int kM = 16 * NB * WM, kN = (SILU ? 16 : 32) * NA;
   const int mt = (p.m + kM - 1) / kM, nt = (p.n + kN - 1) / kN;
-  hipLaunchKernelGGL(kern, dim3(mt * nt), dim3(128 * WM), kLds, s, p, mt, nt);
+  const bool wide = p.n % 4 == 0 && (PART || reinterpret_cast<uintptr_t>(p.y) % 8 == 0);
+  hipLaunchKernelGGL(kern, dim3(mt * nt, parts), dim3(128 * WM), kLds, s, p, mt, nt, wide, part);
   return NKV_OK;
 }
 
-// Which kernel a product takes.  Few rows and few enough 16-channel groups for
-// one round of workgroups, or at most 16 rows: the one that splits k over
+// How a product runs.  Few rows and few enough 16-channel groups for one round
+// of workgroups, or at most 32 rows (us, few-row kernel / tiles, 40 rows: 4096 x
+// 4096 8.9 / 12.9, 6144 x 2560 10.7 / 10.3): the kernel that cuts k over
 // wavefronts.  Otherwise the tile whose busiest CU is done first: ceil(tiles /
 // CUs) tiles of the shape's time for a stage of 128 codes (us, plus what one
 // tile alone waits), as measured at 20-76 stages and 65-4096 rows.  Larger
-// tiles do more products a byte (2.4 PFLOP/s at 256 x 256, 1.9 at 128 x 128 on
-// 8192^3), smaller ones leave fewer CUs idle.
+// tiles do more products a byte (2.5 PFLOP/s at 256 x 256, 1.9 at 128 x 128 on
+// 8192^3), smaller ones leave fewer CUs idle.  A long k of few tiles is cut over
+// workgroups where that gains more than joining the sums costs.
 struct Shape {
   int channels, rows;   // (SILU: half as many channels of y)
   float us, wait_us;
@@ -729,27 +795,63 @@ struct Shape {
 constexpr Shape kShapes[] = {{256, 256, 1.35f, 0.0f}, {192, 256, 1.20f, 0.0f}, {160, 256, 1.00f, 0.0f},
                              {128, 256, 0.88f, 0.0f}, {128, 128, 0.58f, 0.0f}, {128, 64, 0.40f, 0.06f},
                              {64, 64, 0.25f, 0.12f},  {64, 32, 0.22f, 0.07f}};
-
-template <bool SILU>
-int launch_product(const Product& p, hipStream_t s) {
+constexpr int kParted = 4;            // the shape of products whose k is cut
+constexpr int kMaxParts = 8;
+struct Plan {
+  int few;      // 16-row tiles of the few-row kernel, or 0
+  int shape;    // kShapes
+  int parts;    // workgroups a tile
+};
+Plan plan_product(int m, int n, int k, bool silu) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  if (p.m <= 16) return launch_few<1, SILU>(p, s);
-  if (p.m <= 64 && (p.n + 15) / 16 <= cus) {
-    if (p.m <= 32) return launch_few<2, SILU>(p, s);
-    if (p.m <= 48) return launch_few<3, SILU>(p, s);
-    return launch_few<4, SILU>(p, s);
-  }
+  if (m <= 32 || (m <= 64 && (n + 15) / 16 <= cus)) return {std::min(4, (m + 15) / 16), 0, 1};
+  const int stages = (k + kTileK - 1) / kTileK;
+  auto tiles = [&](const Shape& sh, int channels) {
+    return static_cast<int64_t>((channels + sh.channels - 1) / sh.channels) * ((m + sh.rows - 1) / sh.rows);
+  };
+  const int64_t channels = silu ? 2 * static_cast<int64_t>(n) : n;
   int best = 0;
   float least = 0.0f;
   for (int i = 0; i < static_cast<int>(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
     const Shape& sh = kShapes[i];
-    if (SILU && sh.channels == 160) continue;          // (an odd number of 16-channel groups a wavefront)
-    const int ch = SILU ? sh.channels / 2 : sh.channels;
-    const int64_t tiles = static_cast<int64_t>((p.n + ch - 1) / ch) * ((p.m + sh.rows - 1) / sh.rows);
-    const float us = static_cast<float>((tiles + cus - 1) / cus) * sh.us + sh.wait_us;
+    if (silu && sh.channels == 160) continue;          // (an odd number of 16-channel groups a wavefront)
+    const float us = static_cast<float>(stages) * (static_cast<float>((tiles(sh, channels) + cus - 1) / cus) * sh.us + sh.wait_us);
     if (i == 0 || us < least) best = i, least = us;
   }
-  switch (best) {
+  Plan plan{0, best, 1};
+  for (int parts = 2; parts <= kMaxParts && stages >= 8 * parts; ++parts) {
+    const Shape& sh = kShapes[kParted];
+    // the join: a launch behind the tiles' last stores, and every sum written and read once at 4 TB/s
+    // (us, cut / whole: 65 x 9728 -> 2560 17.3 / 24.2, 301 23.4 / 30.3, 512 28.8 / 41.6; 200 x 4096 -> 2560 15.9 / 11.5)
+    const float join = 7.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(channels) * 8.0f / 4.0e6f;
+    const float us = static_cast<float>((stages + parts - 1) / parts) * static_cast<float>((tiles(sh, channels) * parts + cus - 1) / cus) * sh.us + join;
+    if (us < least) least = us, plan = {0, kParted, parts};
+  }
+  return plan;
+}
+
+template <bool SILU>
+int launch_product(const Product& p, int* workspace, hipStream_t s) {
+  const Plan plan = plan_product(p.m, p.n, p.k, SILU);
+  switch (plan.few) {
+    case 0: break;
+    case 1: return launch_few<1, SILU>(p, s);
+    case 2: return launch_few<2, SILU>(p, s);
+    case 3: return launch_few<3, SILU>(p, s);
+    default: return launch_few<4, SILU>(p, s);
+  }
+  if (plan.parts > 1) {
+    Product q = p;                                     // (gate and up rows are one matrix here)
+    if (SILU) q.n = 2 * p.n;
+    const int rc = launch_tile<4, 2, 4, 1, false, true>(q, s, plan.parts, workspace);
+    if (rc != NKV_OK) return rc;
+    const int v = p.n % 4 == 0 ? 4 : 1;
+    const unsigned grid = static_cast<unsigned>((static_cast<int64_t>((p.n + v - 1) / v) * p.m + 255) / 256);
+    if (v == 4) hipLaunchKernelGGL((join_kernel<4, SILU>), dim3(grid), dim3(256), 0, s, p, workspace, plan.parts);
+    else hipLaunchKernelGGL((join_kernel<1, SILU>), dim3(grid), dim3(256), 0, s, p, workspace, plan.parts);
+    return NKV_OK;
+  }
+  switch (plan.shape) {
     case 0: return launch_tile<8, 4, 4, 1, SILU>(p, s);
     case 1: return launch_tile<6, 4, 4, 1, SILU>(p, s);
     case 2:
@@ -761,6 +863,11 @@ int launch_product(const Product& p, hipStream_t s) {
     case 6: return launch_tile<2, 2, 2, 4, SILU>(p, s);
     default: return launch_tile<2, 1, 2, 4, SILU>(p, s);
   }
+}
+
+int64_t workspace_ints(int m, int n, int k, bool silu) {
+  const Plan plan = plan_product(m, n, k, silu);
+  return plan.parts > 1 ? static_cast<int64_t>(plan.parts) * m * n * (silu ? 2 : 1) : 0;
 }
 
 template <int NCH, bool NORM, bool SILU>
@@ -793,7 +900,7 @@ int check_rows(const char* who, const void* x, const int8_t* q, const float* sca
   return NKV_OK;
 }
 
-int check_product(const char* who, const Product& p, int outputs_per_channel) {
+int check_product(const char* who, const Product& p, int outputs_per_channel, const int* workspace) {
   NKV_CHECK_ARG(p.w != nullptr && p.sw != nullptr && p.x != nullptr && p.sx != nullptr && p.y != nullptr,
                 "%s: weight, w_scale, x, x_scale and y must be non-NULL", who);
   NKV_CHECK_ARG(p.m >= 1 && p.n >= 1 && p.k >= 16 && p.k % 16 == 0 && p.k <= kMaxDepth,
@@ -808,6 +915,13 @@ int check_product(const char* who, const Product& p, int outputs_per_channel) {
                     apart(p.y, out, p.x, static_cast<int64_t>(p.m) * p.k) && apart(p.y, out, p.sx, 4 * static_cast<int64_t>(p.m)) &&
                     apart(p.y, out, p.bias, 2 * channels),
                 "%s: y must not overlap an input", who);
+  const int64_t ws = 4 * workspace_ints(p.m, p.n, p.k, outputs_per_channel == 2);
+  NKV_CHECK_ARG(ws == 0 || (workspace != nullptr && aligned16(workspace)),
+                "%s: this product needs a 16-byte aligned workspace of %lld bytes", who, static_cast<long long>(ws));
+  NKV_CHECK_ARG(ws == 0 || (apart(workspace, ws, p.y, out) && apart(workspace, ws, p.w, channels * p.k) &&
+                            apart(workspace, ws, p.sw, 4 * channels) && apart(workspace, ws, p.x, static_cast<int64_t>(p.m) * p.k) &&
+                            apart(workspace, ws, p.sx, 4 * static_cast<int64_t>(p.m)) && apart(workspace, ws, p.bias, 2 * channels)),
+                "%s: the workspace must not overlap an input or y", who);
   return NKV_OK;
 }
 
@@ -889,21 +1003,28 @@ extern "C" int nkv_rmsnorm_q8(const uint16_t* x, const uint16_t* residual, const
   return launch_status("nkv_rmsnorm_q8");
 }
 
+extern "C" int64_t nkv_linear_q8_workspace(int m, int n, int k, int gated) {
+  if (m < 1 || n < 1 || k < 16 || n > INT32_MAX / 2 - 512) return 0;
+  return workspace_ints(m, n, k, gated != 0);
+}
+
 extern "C" int nkv_linear_q8(const int8_t* weight, const float* w_scale, const int8_t* x, const float* x_scale,
-                             const uint16_t* bias, uint16_t* y, int m, int n, int k, void* stream) {
+                             const uint16_t* bias, uint16_t* y, int m, int n, int k, int32_t* workspace,
+                             void* stream) {
   const Product p{weight, w_scale, x, x_scale, bias, y, m, n, k};
-  const int rc = check_product("nkv_linear_q8", p, 1);
+  const int rc = check_product("nkv_linear_q8", p, 1, workspace);
   if (rc != NKV_OK) return rc;
-  const int launched = launch_product<false>(p, reinterpret_cast<hipStream_t>(stream));
+  const int launched = launch_product<false>(p, workspace, reinterpret_cast<hipStream_t>(stream));
   return launched != NKV_OK ? launched : launch_status("nkv_linear_q8");
 }
 
 extern "C" int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const int8_t* x,
-                                      const float* x_scale, uint16_t* y, int m, int intermediate, int k, void* stream) {
+                                      const float* x_scale, uint16_t* y, int m, int intermediate, int k, int32_t* workspace,
+                                      void* stream) {
   const Product p{gate_up_weight, w_scale, x, x_scale, nullptr, y, m, intermediate, k};
-  const int rc = check_product("nkv_linear_silu_mul_q8", p, 2);
+  const int rc = check_product("nkv_linear_silu_mul_q8", p, 2, workspace);
   if (rc != NKV_OK) return rc;
-  const int launched = launch_product<true>(p, reinterpret_cast<hipStream_t>(stream));
+  const int launched = launch_product<true>(p, workspace, reinterpret_cast<hipStream_t>(stream));
   return launched != NKV_OK ? launched : launch_status("nkv_linear_silu_mul_q8");
 }
 

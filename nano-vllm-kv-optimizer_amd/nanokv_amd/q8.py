@@ -29,6 +29,7 @@ from . import _lib
 from .store import current_stream_ptr
 
 TINY = 2.0 ** -119       # rows whose largest magnitude is below are zero
+SPLIT_ROWS = 32          # products of more rows may need a workspace
 TOKEN_ROW = 12288        # longest row that a product quantises in its own launch
 
 
@@ -225,9 +226,25 @@ def _product(q: int, scale: int, shape, device: torch.device, m: int, k: int, we
     y = torch.empty((*shape[:-1], n), dtype=_BF16, device=device)
     if n:
         b = () if silu_mul else (bias.data_ptr() if bias is not None else None,)
-        _call("linear_silu_mul_q8" if silu_mul else "linear_q8", y.get_device(), wq.data_ptr(), ws.data_ptr(), q, scale,
-              *b, y.data_ptr(), m, n, k)
+        device = y.get_device()
+        sums = None              # of a k that is cut over workgroups (dropped behind the launch: the stream orders its reuse)
+        if m > SPLIT_ROWS:
+            need = _workspace(device, m, n, k, silu_mul)
+            if need:
+                sums = torch.empty(need, dtype=torch.int32, device=y.device)
+        _call("linear_silu_mul_q8" if silu_mul else "linear_q8", device, wq.data_ptr(), ws.data_ptr(), q, scale,
+              *b, y.data_ptr(), m, n, k, sums.data_ptr() if sums is not None else None)
     return y
+
+
+def _workspace(device: int, m: int, n: int, k: int, silu_mul: bool) -> int:
+    fn = _ENTRY.get("workspace")
+    if fn is None:
+        fn = _ENTRY["workspace"] = _lib.load().nkv_linear_q8_workspace
+    if device == _current_device():
+        return fn(m, n, k, silu_mul)
+    with torch.cuda.device(device):
+        return fn(m, n, k, silu_mul)
 
 
 def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:

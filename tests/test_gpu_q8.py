@@ -186,7 +186,7 @@ def test_strided_and_unaligned_rows():
 SHAPES = [(1, 1, 16), (1, 7, 48), (2, 33, 64), (3, 1000, 2560), (5, 17, 80), (6, 2560, 9728), (15, 100, 144),
           (16, 64, 128), (17, 65, 1040), (31, 129, 2576), (33, 96, 208), (48, 200, 512), (49, 2560, 1024), (63, 255, 272),
           (64, 256, 256), (65, 257, 4096), (100, 1, 2560), (128, 128, 128), (129, 130, 16), (200, 384, 32), (255, 511, 112),
-          (257, 300, 640), (513, 6144, 384), (1000, 77, 1000 // 16 * 16), (1025, 1283, 336)]
+          (257, 300, 640), (513, 6144, 384), (1000, 77, 1000 // 16 * 16), (1025, 1283, 336), (70, 130, 9728), (99, 257, 12304), (300, 101, 2064), (130, 640, 16400)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -304,14 +304,21 @@ def test_rows_behind_the_last_are_left_as_they_were():
     lib = _lib.load()
     stream = torch.cuda.current_stream().cuda_stream
     p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
-    for m, n, k in ((1, 3, 64), (5, 33, 48), (37, 129, 256), (70, 65, 128), (300, 300, 144)):
+    sums = []
+
+    def ws(*size):
+        sums.append(torch.full((lib.nkv_linear_q8_workspace(*size) + 64,), 5, dtype=torch.int32, device="cuda"))
+        return p(sums[-1])
+
+    for m, n, k in ((1, 3, 64), (5, 33, 48), (37, 129, 256), (70, 65, 128), (300, 300, 144), (70, 130, 9728)):
         x, w = _codes(m, k, seed=m), _codes(2 * n, k, seed=n)
         y = torch.full((m * n + 512,), 7.0, dtype=torch.bfloat16, device="cuda")
-        assert lib.nkv_linear_q8(p(w.q), p(w.scale), p(x.q), p(x.scale), None, p(y), m, n, k, stream) == 0
+        assert lib.nkv_linear_q8(p(w.q), p(w.scale), p(x.q), p(x.scale), None, p(y), m, n, k, ws(m, n, k, 0), stream) == 0
         assert bool((y[m * n:] == 7).all())
         y.fill_(7.0)
-        assert lib.nkv_linear_silu_mul_q8(p(w.q), p(w.scale), p(x.q), p(x.scale), p(y), m, n, k, stream) == 0
+        assert lib.nkv_linear_silu_mul_q8(p(w.q), p(w.scale), p(x.q), p(x.scale), p(y), m, n, k, ws(m, n, k, 1), stream) == 0
         assert bool((y[m * n:] == 7).all())
+        assert all(bool((t[-64:] == 5).all()) for t in sums)
         q = torch.full((m * k + 512,), 9, dtype=torch.int8, device="cuda")
         s = torch.full((m + 64,), 9.0, device="cuda")
         assert lib.nkv_quantize_q8(p(_hidden(m, k, 1)), k, p(q), p(s), m, k, stream) == 0

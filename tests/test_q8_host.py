@@ -80,7 +80,7 @@ def test_shapes_and_refusals():
 
 # -- the C entry points (addresses are never dereferenced) ------------------------
 AT = {"w": 1 << 24, "sw": 1 << 25, "x": 4096, "sx": 1 << 26, "res": 1 << 16, "nw": 1 << 17, "b": 1 << 18, "y": 1 << 27,
-      "ro": 1 << 28, "q": 1 << 29, "s": 1 << 30}
+      "ro": 1 << 28, "q": 1 << 29, "s": 1 << 30, "ws": 1 << 34}
 
 
 def _p(**moved):
@@ -90,8 +90,8 @@ def _p(**moved):
 def _product(name, m=8, n=64, k=128, **moved):
     p, lib = _p(**moved), _lib.load()
     if name == "nkv_linear_q8":
-        return lib.nkv_linear_q8(p["w"], p["sw"], p["x"], p["sx"], p["b"], p["y"], m, n, k, None)
-    return lib.nkv_linear_silu_mul_q8(p["w"], p["sw"], p["x"], p["sx"], p["y"], m, n, k, None)
+        return lib.nkv_linear_q8(p["w"], p["sw"], p["x"], p["sx"], p["b"], p["y"], m, n, k, p["ws"], None)
+    return lib.nkv_linear_silu_mul_q8(p["w"], p["sw"], p["x"], p["sx"], p["y"], m, n, k, p["ws"], None)
 
 
 def _token(name, n=64, k=128, **moved):
