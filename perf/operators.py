@@ -177,13 +177,18 @@ def _plain(s):
     return {"y": h, "residual": res}
 
 
-def _own(s):
-    op, x, res = s["op"], s["x"], s["residual"]
-    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    package = os.path.join(root, "nano-vllm-kv-optimizer_amd")
+def _framework():
+    """nanokv_amd.q8, imported once as a program does, not in every pass."""
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "nano-vllm-kv-optimizer_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
     from nanokv_amd import q8
+    return q8
+
+
+def _own(s):
+    op, x, res = s["op"], s["x"], s["residual"]
+    q8 = sys.modules.get("nanokv_amd.q8") or _framework()
     if op == "quant":
         t = q8.quantize_q8(x)
         return {"values": q8.dequantize_q8(t), "scale": t.scale}
