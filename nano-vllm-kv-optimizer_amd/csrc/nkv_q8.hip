@@ -70,15 +70,19 @@ __device__ __forceinline__ RowScale norm_row_scale(uint32_t top, float ss, int n
 
 // WPR wavefronts a row, NCH 8-element chunks a lane, held in registers between the
 // pass that finds the row's peak (and sum of squares) and the one that writes its
-// codes: every byte is moved once.  Short rows of many take a wavefront each
-// (no barrier), others a workgroup.
+// codes: every byte is moved once.  Bound by HBM for many rows (quantise 4096 x
+// 9728 22.1 us, 5.4 TB/s; norm with residual 50.9 us, 5.5 TB/s; a large copy runs at
+// 5.1), by the launch for few (1 x 2560 2.5 and 3.2 us in a captured chain).  Rows
+// of up to 512 take a wavefront each, no barrier (4096 x 512 5.0 -> 3.9 us, 16384
+// x 128 12 -> 5.8); longer ones as many wavefronts as leave no lane idle (a fixed
+// four: 1 x 2560 3.0 us, 4096 x 9728 26.5).  (x, res and res_out may be one buffer.)
 constexpr int row_threads(int wpr) { return kWave * (wpr == 1 ? 4 : wpr); }
 template <int WPR, int NCH, bool NORM>
-__global__ __launch_bounds__(row_threads(WPR)) void rows_q8_kernel(const uint16_t* __restrict__ x, int64_t x_stride,
-                                                                   const uint16_t* __restrict__ res,
-                                                                   const uint16_t* __restrict__ w, float eps,
-                                                                   int8_t* __restrict__ q, float* __restrict__ scale,
-                                                                   uint16_t* __restrict__ res_out, int rows, int n) {
+__global__ __launch_bounds__(row_threads(WPR)) void rows_q8_kernel(const uint16_t* x, int64_t x_stride,
+                                                                   const uint16_t* res, const uint16_t* __restrict__ w,
+                                                                   float eps, int8_t* __restrict__ q,
+                                                                   float* __restrict__ scale, uint16_t* res_out,
+                                                                   int rows, int n) {
   constexpr int kRows = row_threads(WPR) / (WPR * kWave), kLanes = WPR * kWave;
   __shared__ float s_sum[WPR];
   __shared__ uint32_t s_top[WPR];
@@ -142,7 +146,7 @@ __global__ __launch_bounds__(row_threads(WPR)) void rows_q8_kernel(const uint16_
   if (t == 0) scale[row] = rs.scale;
 }
 
-// One thread per 16 codes.
+// One thread per 16 codes (4096 x 9728: 23.6 us, 5.1 TB/s).
 __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale,
                                                          uint16_t* __restrict__ out, int64_t chunks, int n) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -160,7 +164,10 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* __restric
   }
 }
 
-// SiLU(g) * u in fp32.
+// SiLU(g) * u in fp32.  The hardware's exp2 and reciprocal (1 ulp each; the argument's
+// rounding makes it |g| 2^-24 relative, far below the output's 2^-8): with
+// expf and a division the epilogue of a 256 x 256 tile cost a tenth of the product
+// (gate|up of 4096 rows 236 -> 207 us).
 __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.442695041f)) * u;
 }
@@ -199,7 +206,13 @@ __device__ __forceinline__ void lds_barrier() {
 // take 128-code pieces of k in turn, each on its own: whole 128-byte lines into
 // registers, kDeep pieces in flight, turned through the wavefront's own LDS rows
 // into the matrix instruction's operands (no barrier), and the partial sums are
-// joined through LDS at the end: exact, being integers.
+// joined through LDS at the end: exact, being integers.  In a captured chain over
+// cold weights (us): 6 x 2560 -> 6144 6.1, 6 x 9728 -> 2560 8.4 (3.0 TB/s), gate|up of
+// 6 rows 12.9 (3.9 TB/s), 37 x 9728 -> 2560 13.3, where reading the rows, once a
+// workgroup, counts as much as the weight.  Operands read straight from memory as
+// the matrix instruction wants them (64 bytes of 16 rows a load) took 11.5, 16.8 and 20.9
+// for the last three; refills under a branch made the compiler wait for every
+// load (8.4 -> 15.1); 8 wavefronts a workgroup: gate|up 15.8.
 constexpr int kFewWaves = 4;
 constexpr int few_bytes(int tiles) { return tiles * kFewWaves * 16 * kTileK; }
 template <int NB, bool SILU>
@@ -311,6 +324,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
 // Tiles of 32 NA channels (SILU: 16 NA gate channels and their up channels) x
 // 16 NB WM rows, one a workgroup of 2 x WM wavefronts (channels x rows); a
 // wavefront owns NA x NB products of 16 x 16.
+//
+// 8192^3: 447 us, 2.46 PFLOP/s (a library's int8 product 2.09); a 4096-token chunk:
+// 4096 -> 2560 46 us (1.87), 9728 -> 2560 96 (2.13), gate|up with SiLU 192 (2.12).
+// The large ones are bound by the chip's power: the clock falls to 1.9-2.06 GHz, and
+// matrix instructions on registers alone reach 3.2-3.5 PFLOP/s there.  8192^3 with
+// parts taken out (us, timing copies): no loads 364, no LDS writes 396, no LDS reads 347,
+// neither loads nor writes 337, against 420-447.  Measured on the way (8192^3): LDS
+// rows that conflict two ways and direct copies into LDS 516; fragments read ahead
+// 485; copies through registers 480; scales from LDS in the epilogue 447.  No gain:
+// 128 x 128 a wavefront with one a SIMD (686), fragments read further ahead, two
+// stages in registers, one workgroup a CU taking tile after tile with the next
+// one's loads under the epilogue (480), wave priorities.
+//
 // LDS rows of a stage (weight rows, then x rows), rounded up to whole rounds of copies
 constexpr int tile_rows(int na, int nb, int wm) { return (32 * na + 16 * nb * wm + 16 * wm - 1) / (16 * wm) * (16 * wm); }
 
@@ -567,6 +593,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Product p, const int* _
   }
 }
 
+// Sum of the products of 16 codes, added to acc.
 __device__ __forceinline__ int dot16(const i32x4& a, const i32x4& b, int acc) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_sdot4(a[e], b[e], acc, false);

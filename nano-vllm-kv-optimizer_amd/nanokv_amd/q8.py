@@ -51,8 +51,16 @@ def _quantize_formula(y: torch.Tensor) -> Q8:
 
 def _norm_formula(x, weight, eps, residual):
     t = x.float() if residual is None else x.float() + residual.float()
-    y = t * torch.rsqrt(t.pow(2).mean(dim=-1, keepdim=True) + eps) * weight.float()
-    return _quantize_formula(y), x if residual is None else t.to(x.dtype)
+    mean = t.pow(2).mean(dim=-1)
+    r = torch.rsqrt(mean + eps)
+    codes = _quantize_formula(t * weight.float())       # (they do not depend on r)
+    top = (t * weight.float()).abs().amax(dim=-1) * r
+    zero = (codes.scale == 0) | (top < TINY)
+    odd = ~(mean.isfinite() & top.isfinite())           # NaN where the squares pass fp32's range too
+    scale = torch.where(zero, torch.zeros_like(top), top / 127.0)
+    q = torch.where((zero | odd).unsqueeze(-1), torch.zeros_like(codes.q), codes.q)
+    return (Q8(q, torch.where(odd, torch.full_like(top, float("nan")), scale)),
+            x if residual is None else t.to(x.dtype))
 
 
 def _product_formula(x: Q8, weight: Q8, bias=None) -> torch.Tensor:

@@ -159,6 +159,40 @@ def test_norm_of_rows_without_a_finite_peak(rows):
             assert row not in nan + zero or bool((t.q[j] == 0).all())
 
 
+@pytest.mark.parametrize("rows,n", [(5, 256), (3, 2560), (2, 9728)])
+def test_residual_out_may_be_an_input(rows, n):
+    import ctypes
+
+    from nanokv_amd import _lib
+    from nanokv_amd.q8 import rmsnorm_q8
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    wn = (1 + 0.2 * torch.randn(n, generator=_gen(n), device="cuda")).bfloat16()
+    x, res = _hidden(rows, n, 1), _hidden(rows, n, 2)
+    want, out = rmsnorm_q8(x, wn, 1e-6, res)
+    for into in (0, 1):
+        ins = [x.clone(), res.clone()]
+        q, s = torch.empty_like(want.q), torch.empty_like(want.scale)
+        _lib.check(_lib.load().nkv_rmsnorm_q8(p(ins[0]), p(ins[1]), p(wn), 1e-6, p(q), p(s), p(ins[into]), rows, n,
+                                              torch.cuda.current_stream().cuda_stream), "rmsnorm_q8")
+        assert torch.equal(q, want.q) and torch.equal(s, want.scale) and torch.equal(ins[into], out)
+
+
+def test_an_output_off_its_eight_bytes():
+    """y two bytes into an allocation: the wide stores are not taken."""
+    import ctypes
+
+    from nanokv_amd import _lib
+    lib = _lib.load()
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    for m, n, k in ((1, 64, 64), (20, 64, 64), (300, 640, 128), (70, 256, 9728)):
+        x, w = _codes(m, k, seed=m), _codes(n, k, seed=n)
+        ws = torch.empty(max(4, lib.nkv_linear_q8_workspace(m, n, k, 0)), dtype=torch.int32, device="cuda")
+        y = torch.empty(m * n + 1, dtype=torch.bfloat16, device="cuda")[1:]
+        assert lib.nkv_linear_q8(p(w.q), p(w.scale), p(x.q), p(x.scale), None, p(y), m, n, k, p(ws),
+                                 torch.cuda.current_stream().cuda_stream) == 0
+        _check_product(y.view(m, n), x, w)
+
+
 def test_strided_and_unaligned_rows():
     from nanokv_amd.q8 import linear_q8, quantize_q8, rmsnorm_q8
     wide = _hidden(33, 1024, 3)
@@ -243,6 +277,25 @@ def test_norm_then_product(m, n, k, with_residual):
     y, got = norm_linear_silu_mul_q8(x, wn, 1e-6, w, res)
     assert torch.equal(got, want)
     _check_gated(y, t, w, 2.0 ** -9)              # |gate| < 500 times the scale's 2^-18
+
+
+def test_a_cut_k_gives_the_same_bits():
+    """Sums joined from several workgroups are the sums: rows of a call that is cut
+    against the same rows in calls that are not."""
+    from nanokv_amd import _lib
+    from nanokv_amd.q8 import Q8, linear_q8, linear_silu_mul_q8
+    need = _lib.load().nkv_linear_q8_workspace
+    for m, n, k in ((70, 130, 9728), (99, 257, 12304), (130, 640, 16400)):
+        assert need(m, n, k, 0) and need(m, n, k, 1) and not need(16, n, k, 0)
+        x, w = _codes(m, k, seed=m), _codes(2 * n, k, seed=n)
+        x = Q8(x.q, x.scale * (20 / k ** 0.5))
+        half = Q8(w.q[:n], w.scale[:n])
+        bias = torch.randn(n, generator=_gen(n), device="cuda").bfloat16()
+        whole, gated = linear_q8(x, half, bias), linear_silu_mul_q8(x, w)
+        for i in range(0, m, 16):
+            part = Q8(x.q[i:i + 16], x.scale[i:i + 16])
+            assert torch.equal(whole[i:i + 16], linear_q8(part, half, bias))
+            assert torch.equal(gated[i:i + 16], linear_silu_mul_q8(part, w))
 
 
 def test_longest_sums_are_exact():
@@ -336,10 +389,11 @@ def _mlp(x, res, wn, gate_up, down):
     return linear_q8(linear_silu_mul_q8(t, gate_up), down), res
 
 
-@pytest.mark.parametrize("m", [1, 6, 77, 300])
-def test_a_captured_mlp_replays_with_new_rows(m):
+# (3000 rows: tiles of more than 64 KiB of LDS; 70 rows of 9728: sums in a workspace)
+@pytest.mark.parametrize("m,k,inter", [(1, 512, 1040), (6, 512, 1040), (77, 512, 1040), (300, 512, 1040), (3000, 512, 1040),
+                                       (70, 512, 9728)])
+def test_a_captured_mlp_replays_with_new_rows(m, k, inter):
     from nanokv_amd.q8 import norm_linear_silu_mul_q8, linear_q8
-    k, inter = 512, 1040
     wn = torch.ones(k, dtype=torch.bfloat16, device="cuda")
     gate_up, down = _codes(2 * inter, k, seed=1), _codes(k, inter, seed=2)
     gate_up = type(gate_up)(gate_up.q, gate_up.scale * 0.01)

@@ -61,6 +61,17 @@ def test_norm_by_its_definition():
         assert torch.equal(norm_linear_silu_mul_q8(x, wn, 1e-6, w, res)[0], linear_silu_mul_q8(t, w))
 
 
+def test_norm_of_rows_without_a_finite_peak():
+    x = torch.ones(5, 32)
+    x[0] = 0
+    x[1, 3] = float("nan")
+    x[2, 4] = -float("inf")
+    x[3] = 2.0 ** 70                  # its squares pass fp32's range
+    x[4] = 2.0 ** -121
+    t, _ = rmsnorm_q8(x, torch.ones(32), 1e-6)
+    assert (t.scale[[0, 4]] == 0).all() and t.scale[1:4].isnan().all() and not t.q.any()
+
+
 def test_shapes_and_refusals():
     x, w = _rows(6, 32, 1), quantize_q8(_rows(8, 32, 2))
     assert linear_q8(x.view(2, 3, 32), w).shape == (2, 3, 8) and linear_q8(x[0], w).shape == (8,)
@@ -111,6 +122,12 @@ def test_products_refuse_bad_arguments(name):
                 dict(x=4100), dict(w=0), dict(sw=0), dict(x=0), dict(sx=0), dict(y=0)):
         assert _product(name, **bad) == _lib.NKV_ERR_ARG, bad
     out = 2 * 8 * 64
+    lib = _lib.load()
+    for bad in (dict(ws=0), dict(ws=AT["ws"] + 4), dict(ws=AT["y"] - 64), dict(ws=AT["w"]), dict(ws=AT["x"] + 512)):
+        size = dict(m=70, n=256, k=9728)
+        if lib.nkv_linear_q8_workspace(70, 256, 9728, name != "nkv_linear_q8"):
+            assert _product(name, **size, **bad) == _lib.NKV_ERR_ARG, bad
+            assert b"workspace" in lib.nkv_last_error()
     for what, size in (("w", 64 * 128), ("sw", 4 * 64), ("x", 8 * 128), ("sx", 4 * 8)):
         for where in (AT[what], AT[what] + size - 2, AT[what] - out + 2):
             assert _product(name, y=where) == _lib.NKV_ERR_ARG and b"overlap" in _lib.load().nkv_last_error()
@@ -130,6 +147,15 @@ def test_token_products_refuse_bad_arguments(name):
                 assert _token(name, **{out: where}) == _lib.NKV_ERR_ARG and b"overlap" in _lib.load().nkv_last_error()
     if norm:
         assert _token(name, y=AT["ro"] + 16) == _lib.NKV_ERR_ARG
+
+
+def test_workspace_sizes():
+    need = _lib.load().nkv_linear_q8_workspace
+    assert need(1, 2560, 9728, 0) == need(32, 2560, 9728, 1) == 0          # few rows: cut inside a workgroup
+    assert need(4096, 2560, 4096, 0) == need(1000, 6144, 2560, 0) == 0     # tiles enough
+    parts, rest = divmod(need(70, 130, 9728, 1), 70 * 2 * 130)
+    assert parts >= 2 and rest == 0
+    assert need(0, 8, 16, 0) == need(8, 0, 16, 0) == need(8, 8, 0, 0) == need(-1, -1, -1, 1) == 0
 
 
 def test_rows_refuse_bad_arguments():
