@@ -36,12 +36,15 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // the infinities and NaN on top.
 __device__ __forceinline__ uint32_t mag(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-// 4 codes: rne(v * inv) for |v * inv| <= 127.5, in the low byte of the sum with
-// 1.5 * 2^23 (one fma, its rounding to nearest even); NaN gives 0.
+// 4 codes: rne(fl(v * inv)) for |v * inv| <= 127.5, in the low byte of the sum with
+// 1.5 * 2^23 (whose rounding is to nearest even); NaN gives 0.  The product is
+// rounded before (no fma): where v is a simple fraction of the row's peak, v * 127 /
+// peak lies half way between two codes, and the error of inv must not decide.
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+#pragma clang fp contract(off)
   constexpr float kMagic = 12582912.0f;
-  const uint32_t x = __float_as_uint(__builtin_fmaf(a, inv, kMagic)), y = __float_as_uint(__builtin_fmaf(b, inv, kMagic));
-  const uint32_t z = __float_as_uint(__builtin_fmaf(c, inv, kMagic)), w = __float_as_uint(__builtin_fmaf(d, inv, kMagic));
+  const uint32_t x = __float_as_uint(a * inv + kMagic), y = __float_as_uint(b * inv + kMagic);
+  const uint32_t z = __float_as_uint(c * inv + kMagic), w = __float_as_uint(d * inv + kMagic);
   return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
 }
 
@@ -768,11 +771,15 @@ void launch_rows(const uint16_t* x, int64_t x_stride, const uint16_t* res, const
     hipLaunchKernelGGL(kern, dim3((rows + per - 1) / per), dim3(row_threads(wpr)), 0, s, x, x_stride, res, w, eps, q, scale, res_out,
                        rows, n);
   };
+  // many rows: half the wavefronts a row, two chunks in flight a lane (us, 4096 rows of 2560: 16.4
+  // against 17.2 with a norm, 8.7 / 9.6 without; of 4096: 22.6 / 24.0, 11.6 / 12.6); few: one chunk
+  // a lane (1 x 2560: 3.2 against 3.5 and 2.5 / 3.0)
+  const bool many = rows >= 1024;
   if (n <= 512) go(rows_q8_kernel<1, 1, NORM>, 1);
-  else if (n <= 1024) go(rows_q8_kernel<2, 1, NORM>, 2);
-  else if (n <= 2048) go(rows_q8_kernel<4, 1, NORM>, 4);
-  else if (n <= 2560) go(rows_q8_kernel<5, 1, NORM>, 5);
-  else if (n <= 4096) go(rows_q8_kernel<8, 1, NORM>, 8);
+  else if (n <= 1024) many ? go(rows_q8_kernel<1, 2, NORM>, 1) : go(rows_q8_kernel<2, 1, NORM>, 2);
+  else if (n <= 2048) many ? go(rows_q8_kernel<2, 2, NORM>, 2) : go(rows_q8_kernel<4, 1, NORM>, 4);
+  else if (n <= 2560) many ? go(rows_q8_kernel<3, 2, NORM>, 3) : go(rows_q8_kernel<5, 1, NORM>, 5);
+  else if (n <= 4096) many ? go(rows_q8_kernel<4, 2, NORM>, 4) : go(rows_q8_kernel<8, 1, NORM>, 8);
   else if (n <= 8192) go(rows_q8_kernel<8, 2, NORM>, 8);
   else if (n <= 12288) go(rows_q8_kernel<8, 3, NORM>, 8);
   else if (n <= 16384) go(rows_q8_kernel<8, 4, NORM>, 8);

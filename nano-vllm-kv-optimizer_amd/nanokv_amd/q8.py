@@ -108,6 +108,11 @@ def _rows(x: torch.Tensor, who: str, what: str = "x") -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+def _fine(t: torch.Tensor) -> bool:
+    """What _rows returns as it is."""
+    return t.dtype is _BF16 and not t.requires_grad and t.is_contiguous() and t.data_ptr() % 16 == 0
+
+
 def _vector(t: torch.Tensor, n: int, device: int, who: str, what: str) -> torch.Tensor:
     if t.dim() != 1 or t.shape[0] != n or t.get_device() != device:
         raise ValueError(f"{who}: {what} must be a [{n}] tensor on x's device (got {tuple(t.shape)} on {t.device})")
@@ -171,12 +176,15 @@ def quantize_q8(x: torch.Tensor) -> Q8:
     n = _width(x, "quantize_q8")
     if not x.is_cuda:
         return _quantize_formula(x.float())
-    x, stride = _strided(x, n, "quantize_q8")
-    out = Q8(torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[:-1], dtype=_F32, device=x.device))
+    stride = n
+    if not _fine(x):
+        x, stride = _strided(x, n, "quantize_q8")
+    shape, device = x.shape, x.device
+    q, scale = torch.empty(shape, dtype=_I8, device=device), torch.empty(shape[:-1], dtype=_F32, device=device)
     rows = x.numel() // n
     if rows:
-        _call("quantize_q8", x.get_device(), x.data_ptr(), stride, out.q.data_ptr(), out.scale.data_ptr(), rows, n)
-    return out
+        _call("quantize_q8", x.get_device(), x.data_ptr(), stride, q.data_ptr(), scale.data_ptr(), rows, n)
+    return Q8(q, scale)
 
 
 def _strided(x: torch.Tensor, n: int, who: str) -> tuple:
@@ -193,7 +201,9 @@ def dequantize_q8(t: Q8) -> torch.Tensor:
     n = _width(t.q, "dequantize_q8")
     if not t.q.is_cuda:
         return (t.q.float() * t.scale.unsqueeze(-1)).to(_BF16)
-    q, scale = _dense(t)
+    q, scale = t
+    if not (q.is_contiguous() and scale.is_contiguous() and q.data_ptr() % 16 == 0):
+        q, scale = _dense(t)
     out = torch.empty(q.shape, dtype=_BF16, device=q.device)
     rows = out.numel() // n
     if rows:
@@ -204,15 +214,18 @@ def dequantize_q8(t: Q8) -> torch.Tensor:
 def _norm(x, weight, eps, residual, q: int, scale: int, rows: int, n: int, who: str, what: str):
     """nkv_rmsnorm_q8 of checked dense rows x into the addresses q and scale; the new residual."""
     device = x.get_device()
-    weight = _vector(weight, n, device, who, what)
-    res_out = x
-    if residual is not None:
+    if weight.get_device() != device or weight.shape != (n,) or not _fine(weight):
+        weight = _vector(weight, n, device, who, what)
+    if residual is None:
+        if rows:
+            _call("rmsnorm_q8", device, x.data_ptr(), None, weight.data_ptr(), float(eps), q, scale, None, rows, n)
+        return x
+    if residual.get_device() != device or residual.shape != x.shape or not _fine(residual):
         residual = _like(residual, x, who, "residual")
-        res_out = torch.empty_like(x)
+    res_out = torch.empty_like(x)
     if rows:
-        has = residual is not None
-        _call("rmsnorm_q8", device, x.data_ptr(), residual.data_ptr() if has else None, weight.data_ptr(), float(eps),
-              q, scale, res_out.data_ptr() if has else None, rows, n)
+        _call("rmsnorm_q8", device, x.data_ptr(), residual.data_ptr(), weight.data_ptr(), float(eps), q, scale,
+              res_out.data_ptr(), rows, n)
     return res_out
 
 
@@ -222,10 +235,12 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torc
     n = _width(x, "rmsnorm_q8")
     if not x.is_cuda:
         return _norm_formula(x, weight, eps, residual)
-    x = _rows(x, "rmsnorm_q8")
-    out = Q8(torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[:-1], dtype=_F32, device=x.device))
-    return out, _norm(x, weight, eps, residual, out.q.data_ptr(), out.scale.data_ptr(), x.numel() // n, n, "rmsnorm_q8",
-                      "weight")
+    if not _fine(x):
+        x = _rows(x, "rmsnorm_q8")
+    shape, device = x.shape, x.device
+    q, scale = torch.empty(shape, dtype=_I8, device=device), torch.empty(shape[:-1], dtype=_F32, device=device)
+    res_out = _norm(x, weight, eps, residual, q.data_ptr(), scale.data_ptr(), x.numel() // n, n, "rmsnorm_q8", "weight")
+    return Q8(q, scale), res_out
 
 
 def _product(q: int, scale: int, shape, device: torch.device, m: int, k: int, weight: tuple, bias, silu_mul: bool):
@@ -276,7 +291,8 @@ def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
         if m:
             return _product(x.q.data_ptr(), x.scale.data_ptr(), q.shape, q.device, m, k, w, bias, silu_mul)
     elif m == 1 and k <= TOKEN_ROW and n:
-        x = _rows(x, who)
+        if not _fine(x):
+            x = _rows(x, who)
         y = torch.empty((*x.shape[:-1], n), dtype=_BF16, device=x.device)
         if silu_mul:
             _call("gemv_silu_mul_q8", device, w[0].data_ptr(), w[1].data_ptr(), x.data_ptr(), y.data_ptr(), n, k)
@@ -285,7 +301,9 @@ def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
                   bias.data_ptr() if bias is not None else None, y.data_ptr(), n, k)
         return y
     else:
-        x, stride = _strided(x, k, who)
+        stride = k
+        if not _fine(x):
+            x, stride = _strided(x, k, who)
         if m:
             codes = torch.empty(m * (k + 4), dtype=_I8, device=x.device)    # the codes, then their scales
             at = codes.data_ptr()

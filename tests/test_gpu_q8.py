@@ -2,7 +2,7 @@
 
 Tolerances, with u = 2^-24 the half step of fp32:
 * a row's scale is one division: off by u relative; its codes are the nearest
-  integer of y * inv with inv off by u relative, so within 1/2 + 127 u < 1/2 + 2^-16
+  integer of y * inv, inv and the product off by u relative each, so within 1/2 + 2 * 127 u < 1/2 + 2^-16
   of y * 127 / a.
 * behind a norm, t = x + r and t * w are rounded once each: codes within
   1/2 + 127 * 4 u + ... < 1/2 + 2^-14; the sum of n <= 32768 squares is a chain of
@@ -75,7 +75,8 @@ def _check_gated(y, x, w, extra=0.0):
 
 # -- rows ------------------------------------------------------------------------
 @pytest.mark.parametrize("rows,n", [(1, 16), (3, 32), (2, 512), (5, 528), (1, 2560), (257, 2560), (7, 8192), (3, 8208),
-                                    (1, 9728), (1030, 9728), (2, 32768), (4099, 128)])
+                                    (1, 9728), (1030, 9728), (2, 32768), (4099, 128), (1025, 1008), (1024, 2048),
+                                    (1500, 2544), (1100, 4096), (2, 12288), (2, 16384), (3, 1024), (3, 4080)])
 def test_quantize_and_read_back(rows, n):
     from nanokv_amd.q8 import dequantize_q8, quantize_q8
     x = _hidden(rows, n, rows + n)
@@ -91,7 +92,8 @@ def test_quantize_and_read_back(rows, n):
 
 @pytest.mark.parametrize("with_residual", [False, True])
 @pytest.mark.parametrize("rows,n", [(1, 16), (3, 48), (2, 512), (5, 528), (1, 2560), (300, 2560), (7, 8192), (3, 8208),
-                                    (2, 32768), (4099, 128)])
+                                    (2, 32768), (4099, 128), (1025, 1008), (1024, 2048), (1500, 2544), (1100, 4096),
+                                    (2, 12288), (2, 16384), (3, 1024), (3, 4080)])
 def test_rmsnorm(rows, n, with_residual):
     from nanokv_amd.q8 import rmsnorm_q8
     x, w = _hidden(rows, n, rows + n), (1 + 0.2 * torch.randn(n, generator=_gen(n), device="cuda")).bfloat16()
