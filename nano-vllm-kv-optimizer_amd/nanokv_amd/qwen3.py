@@ -235,10 +235,11 @@ class Q8Linear(nn.Module):
 
     @property
     def weight(self) -> Q8:
-        return Q8(self.weight_q8, self.weight_scale)
+        held = self._buffers         # (an attribute of a module costs about 0.4 us)
+        return Q8(held["weight_q8"], held["weight_scale"])
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return linear_q8(x, self.weight, self.bias)
+        return linear_q8(x, self.weight, self._buffers["bias"])
 
 
 def _norm_q8(norm: nn.Module, proj: nn.Module) -> bool:
