@@ -345,15 +345,22 @@ constexpr int tile_rows(int na, int nb, int wm) { return (32 * na + 16 * nb * wm
 
 // With PART, gridDim.y workgroups share a tile, each a run of its stages, and the
 // sums go to part[blockIdx.y][m][n] for join_kernel.
-template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false>
-__global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt, int nt, bool wide, int* part) {
-  static_assert(!(SILU && PART), "");
-  extern __shared__ __align__(128) char s_tile[];
+// With KS = 2 a workgroup has two groups of wavefronts, which take the stages in turn,
+// each in buffers of its own, and add their sums through LDS at the end: for the
+// small tiles, whose one wavefront a SIMD waits for LDS between products (us, KS = 1 / 2:
+// 200 x 2560 -> 6144 14.8 / 13.3, 200 x 4096 -> 2560 11.8 / 10.1, 65 x 4096 -> 2560 11.1 / 9.2;
+// fragments read a whole stage ahead instead: no gain.  128 x 128 18.2 / 17.5).
+template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false, int KS = 1>
+__global__ __launch_bounds__(128 * WM * KS) void tile_kernel(const Product p, int mt, int nt, bool wide, int* part) {
+  static_assert(!(SILU && PART) && !(PART && KS > 1) && (KS == 1 || (KS == 2 && NB % 2 == 0)), "");
+  extern __shared__ __align__(128) char s_lds[];
   constexpr int kTileM = 16 * NB * WM, kWaves = 2 * WM;
   __shared__ __align__(16) float s_scale[32 * NA], s_bias[SILU ? 4 : 32 * NA], s_x[kTileM];
   constexpr int kStage = tile_rows(NA, NB, WM) * kTileK;
   constexpr int kCopies = tile_rows(NA, NB, WM) / (8 * kWaves);   // 8-row pieces a wavefront copies
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % kWaves;
+  const int group = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / kWaves : 0;
+  char* s_tile = s_lds + group * 2 * kStage;
   const int lane = threadIdx.x & (kWave - 1);
   // tiles: a run of them per XCD, 8 row tiles by all channel tiles at a time
   int t;
@@ -371,7 +378,7 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
 
   const int all = (p.k + kTileK - 1) / kTileK;
   const int first = PART ? static_cast<int>(static_cast<int64_t>(all) * blockIdx.y / gridDim.y) : 0;
-  const int stages = PART ? static_cast<int>(static_cast<int64_t>(all) * (blockIdx.y + 1) / gridDim.y) - first : all;
+  const int stages = PART ? static_cast<int>(static_cast<int64_t>(all) * (blockIdx.y + 1) / gridDim.y) - first : (all + KS - 1) / KS;
 
   // A wavefront's share of a stage: 8-row pieces wave, wave + kWaves, ..., lane u with
   // 16 bytes of row u >> 3.  They go through registers: loaded a stage ahead of
@@ -396,7 +403,7 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
       row = (row / (2 * half)) * half + row % half;
     }
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, rows * p.k, kRsrcWord3);
-    const int kb = (first + s) * kTileK;
+    const int kb = (KS > 1 ? s * KS + group : first + s) * kTileK;
     const int off = kc < p.k - kb ? voff + row * p.k + kb : 0x7fffffff;   // past the row's end: zeros
     st[set][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
   };
@@ -406,13 +413,13 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
   };
 
   // the scales of the tile's weight rows and x rows, and its bias
-  for (int row = threadIdx.x; !PART && row < 32 * NA; row += 64 * kWaves) {
+  for (int row = threadIdx.x; !PART && row < 32 * NA; row += 64 * kWaves * KS) {
     const int64_t up = SILU && (row / (8 * NA)) & 1 ? p.n : 0;
     const int c = c0 + min(SILU ? (row / (16 * NA)) * 8 * NA + row % (8 * NA) : row, cn - 1);
     s_scale[row] = p.sw[up + c];
     if constexpr (!SILU) s_bias[row] = p.bias ? bf16_to_f32(p.bias[c]) : 0.0f;
   }
-  for (int row = threadIdx.x; !PART && row < kTileM; row += 64 * kWaves) s_x[row] = p.sx[m0 + min(row, mn - 1)];
+  for (int row = threadIdx.x; !PART && row < kTileM; row += 64 * kWaves * KS) s_x[row] = p.sx[m0 + min(row, mn - 1)];
 
   const int wc = wave & 1, wm = wave >> 1;
   const int r = lane & 15, g = lane >> 4;
@@ -517,6 +524,26 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
     return;
   }
 
+  // the groups' sums: each finishes half of the row tiles
+  auto mine = [&](int j) { return KS == 1 || j / (NB / KS) == group; };
+  if constexpr (KS > 1) {
+    static_assert(2 * kWaves * NA * NB * kWave * 16 / KS <= 2 * KS * kStage, "");
+    i32x4* s_join = reinterpret_cast<i32x4*>(s_lds) + wave * NA * (NB / KS) * kWave + lane;
+    constexpr int kGroup = kWaves * NA * (NB / KS) * kWave;
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (!mine(j))
+#pragma unroll
+        for (int i = 0; i < NA; ++i) s_join[(1 - group) * kGroup + (i * (NB / KS) + j % (NB / KS)) * kWave] = acc[i][j];
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (mine(j))
+#pragma unroll
+        for (int i = 0; i < NA; ++i) acc[i][j] += s_join[group * kGroup + (i * (NB / KS) + j % (NB / KS)) * kWave];
+  }
+
   constexpr int kOut = SILU ? NA / 2 : NA;             // channel groups of 16 that are written
   const float4* my_scale = reinterpret_cast<const float4*>(s_scale + wc * 16 * NA + 4 * g);
   const float4* my_bias = reinterpret_cast<const float4*>(s_bias + wc * 16 * NA + 4 * g);
@@ -529,7 +556,7 @@ __global__ __launch_bounds__(128 * WM) void tile_kernel(const Product p, int mt,
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int mj = (wm * NB + j) * 16 + r;
-    if (mj >= mn) continue;
+    if (!mine(j) || mj >= mn) continue;
     const float sx = s_x[mj];
     uint16_t* y = p.y + static_cast<int64_t>(m0 + mj) * p.n;
 #pragma unroll
@@ -766,10 +793,14 @@ bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
 template <bool NORM>
 void launch_rows(const uint16_t* x, int64_t x_stride, const uint16_t* res, const uint16_t* w, float eps, int8_t* q,
                  float* scale, uint16_t* res_out, int rows, int n, hipStream_t s) {
+  // (a launch holds less than 2^32 threads: 2^21 rows of at most 1024)
   auto go = [&](auto kern, int wpr) {
     const int per = wpr == 1 ? 4 : 1;
-    hipLaunchKernelGGL(kern, dim3((rows + per - 1) / per), dim3(row_threads(wpr)), 0, s, x, x_stride, res, w, eps, q, scale, res_out,
-                       rows, n);
+    for (int64_t at = 0; at < rows; at += 1 << 21) {
+      const int some = static_cast<int>(std::min<int64_t>(rows - at, 1 << 21));
+      hipLaunchKernelGGL(kern, dim3((some + per - 1) / per), dim3(row_threads(wpr)), 0, s, x + at * x_stride, x_stride,
+                         res ? res + at * n : nullptr, w, eps, q + at * n, scale + at, res_out ? res_out + at * n : nullptr, some, n);
+    }
   };
   // many rows: half the wavefronts a row, two chunks in flight a lane (us, 4096 rows of 2560: 16.4
   // against 17.2 with a norm, 8.7 / 9.6 without; of 4096: 22.6 / 24.0, 11.6 / 12.6); few: one chunk
@@ -794,10 +825,10 @@ int launch_few(const Product& p, hipStream_t s) {
   return NKV_OK;
 }
 
-template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false>
+template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false, int KS = 1>
 int launch_tile(const Product& p, hipStream_t s, int parts = 1, int* part = nullptr) {
-  constexpr int kLds = 2 * tile_rows(NA, NB, WM) * kTileK;
-  const auto kern = tile_kernel<NA, NB, WM, DEPTH, SILU, PART>;
+  constexpr int kLds = 2 * KS * tile_rows(NA, NB, WM) * kTileK;
+  const auto kern = tile_kernel<NA, NB, WM, DEPTH, SILU, PART, KS>;
   if (kLds > 65536) {   // beyond the default limit of a launch (per device, so asked each time: it is a table lookup)
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) {
@@ -809,13 +840,13 @@ int launch_tile(const Product& p, hipStream_t s, int parts = 1, int* part = null
   constexpr int kM = 16 * NB * WM, kN = (SILU ? 16 : 32) * NA;
   const int mt = (p.m + kM - 1) / kM, nt = (p.n + kN - 1) / kN;
   const bool wide = p.n % 4 == 0 && (PART || reinterpret_cast<uintptr_t>(p.y) % 8 == 0);
-  hipLaunchKernelGGL(kern, dim3(mt * nt, parts), dim3(128 * WM), kLds, s, p, mt, nt, wide, part);
+  hipLaunchKernelGGL(kern, dim3(mt * nt, parts), dim3(128 * WM * KS), kLds, s, p, mt, nt, wide, part);
   return NKV_OK;
 }
 
 // How a product runs.  Few rows and few enough 16-channel groups for one round
-// of workgroups, or at most 32 rows (us, few-row kernel / tiles, 40 rows: 4096 x
-// 4096 8.9 / 12.9, 6144 x 2560 10.7 / 10.3): the kernel that cuts k over
+// of workgroups, or at most 32 rows (us, few-row kernel / tiles: 48 x 4096 -> 4096
+// 9.1 / 11.1, 33 x 2560 -> 6144 9.7 / 8.7): the kernel that cuts k over
 // wavefronts.  Otherwise the tile whose busiest CU is done first: ceil(tiles /
 // CUs) tiles of the shape's time for a stage of 128 codes (us, plus what one
 // tile alone waits), as measured at 20-76 stages and 65-4096 rows.  Larger
@@ -827,8 +858,8 @@ struct Shape {
   float us, wait_us;
 };
 constexpr Shape kShapes[] = {{256, 256, 1.35f, 0.0f}, {192, 256, 1.20f, 0.0f}, {160, 256, 1.00f, 0.0f},
-                             {128, 256, 0.88f, 0.0f}, {128, 128, 0.58f, 0.0f}, {128, 64, 0.40f, 0.06f},
-                             {64, 64, 0.25f, 0.12f},  {64, 32, 0.22f, 0.07f}};
+                             {128, 256, 0.88f, 0.0f}, {128, 128, 0.58f, 0.0f}, {128, 64, 0.40f, 0.0f},
+                             {64, 64, 0.19f, 0.04f},  {64, 32, 0.13f, 0.06f}};
 constexpr int kParted = 4;            // the shape of products whose k is cut
 constexpr int kMaxParts = 8;
 struct Plan {
@@ -855,9 +886,9 @@ Plan plan_product(int m, int n, int k, bool silu) {
   Plan plan{0, best, 1};
   for (int parts = 2; parts <= kMaxParts && stages >= 8 * parts; ++parts) {
     const Shape& sh = kShapes[kParted];
-    // the join: a launch behind the tiles' last stores, and every sum written and read once at 4 TB/s
-    // (us, cut / whole: 65 x 9728 -> 2560 17.3 / 24.2, 301 23.4 / 30.3, 512 28.8 / 41.6; 200 x 4096 -> 2560 15.9 / 11.5)
-    const float join = 7.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(channels) * 8.0f / 4.0e6f;
+    // the join: a launch behind the tiles' last stores, and every sum written and read once at 6 TB/s
+    // (us, cut / whole: 65 x 9728 -> 2560 17.1 / 19.4, 128 19.1 / 21.0, 512 28.8 / 35.2; 200 x 4096 -> 2560 15.9 / 10.1)
+    const float join = 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(channels) * 8.0f / 6.0e6f;
     const float us = static_cast<float>((stages + parts - 1) / parts) * static_cast<float>((tiles(sh, channels) * parts + cus - 1) / cus) * sh.us + join;
     if (us < least) least = us, plan = {0, kParted, parts};
   }
@@ -893,9 +924,9 @@ int launch_product(const Product& p, int* workspace, hipStream_t s) {
       return NKV_ERR_UNSUPPORTED;                      // (never chosen)
     case 3: return launch_tile<4, 4, 4, 1, SILU>(p, s);
     case 4: return launch_tile<4, 2, 4, 1, SILU>(p, s);
-    case 5: return launch_tile<4, 2, 2, 2, SILU>(p, s);
-    case 6: return launch_tile<2, 2, 2, 4, SILU>(p, s);
-    default: return launch_tile<2, 1, 2, 4, SILU>(p, s);
+    case 5: return launch_tile<4, 2, 2, 2, SILU, false, 2>(p, s);
+    case 6: return launch_tile<2, 2, 2, 4, SILU, false, 2>(p, s);
+    default: return launch_tile<2, 2, 1, 4, SILU, false, 2>(p, s);
   }
 }
 
@@ -1010,7 +1041,7 @@ extern "C" int nkv_dequantize_q8(const int8_t* q, const float* scale, uint16_t* 
                 rows, n);
   NKV_CHECK_ARG(aligned16(q) && aligned16(out), "nkv_dequantize_q8: q and out must be 16-byte aligned");
   const int64_t codes = static_cast<int64_t>(rows) * n, chunks = codes / 16;
-  NKV_CHECK_ARG(chunks <= INT64_C(256) * INT32_MAX, "nkv_dequantize_q8: too many elements");
+  NKV_CHECK_ARG(chunks <= INT64_C(256) * ((1 << 24) - 1), "nkv_dequantize_q8: at most 2^36 - 2^12 elements (a launch's threads)");
   NKV_CHECK_ARG(apart(out, 2 * codes, q, codes) && apart(out, 2 * codes, scale, 4 * static_cast<int64_t>(rows)),
                 "nkv_dequantize_q8: out must not overlap an input");
   hipLaunchKernelGGL(dequantize_kernel, dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0,
@@ -1038,7 +1069,7 @@ extern "C" int nkv_rmsnorm_q8(const uint16_t* x, const uint16_t* residual, const
 }
 
 extern "C" int64_t nkv_linear_q8_workspace(int m, int n, int k, int gated) {
-  if (m < 1 || n < 1 || k < 16 || n > INT32_MAX / 2 - 512) return 0;
+  if (m < 1 || n < 1 || k < 16 || m > INT32_MAX - 512 || n > INT32_MAX / 2 - 512 || k > kMaxDepth) return 0;
   return workspace_ints(m, n, k, gated != 0);
 }
 

@@ -336,6 +336,22 @@ def test_offsets_past_32_bits():
     _check_product(linear_q8(x, Q8(w.q[-3:], w.scale[-3:]))[-9:], Q8(w.q[-9:], w.scale[-9:]), Q8(w.q[-3:], w.scale[-3:]))
 
 
+def test_more_rows_than_one_launch_takes():
+    from nanokv_amd.q8 import dequantize_q8, quantize_q8, rmsnorm_q8
+    rows = 2**21 + 5
+    x = _hidden(rows, 32, 6)
+    wn = torch.ones(32, dtype=torch.bfloat16, device="cuda")
+    t, (h, res) = quantize_q8(x), rmsnorm_q8(x, wn, 1e-6, x)
+    wide = quantize_q8(x[:, :16])                  # rows that lie apart
+    for at in (slice(0, 9), slice(2**21 - 4, rows)):
+        a, (b, r) = quantize_q8(x[at].contiguous()), rmsnorm_q8(x[at].contiguous(), wn, 1e-6, x[at].contiguous())
+        assert torch.equal(t.q[at], a.q) and torch.equal(t.scale[at], a.scale) and torch.equal(res[at], r)
+        assert torch.equal(h.q[at], b.q) and torch.equal(h.scale[at], b.scale)
+        c = quantize_q8(x[at, :16].contiguous())
+        assert torch.equal(wide.q[at], c.q) and torch.equal(wide.scale[at], c.scale)
+        assert torch.equal(dequantize_q8(t)[at], dequantize_q8(a))
+
+
 def test_no_rows_and_no_channels():
     from nanokv_amd.q8 import (dequantize_q8, linear_q8, linear_silu_mul_q8, norm_linear_q8, quantize_q8, rmsnorm_q8)
     x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")

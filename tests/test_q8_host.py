@@ -156,6 +156,8 @@ def test_workspace_sizes():
     parts, rest = divmod(need(70, 130, 9728, 1), 70 * 2 * 130)
     assert parts >= 2 and rest == 0
     assert need(0, 8, 16, 0) == need(8, 0, 16, 0) == need(8, 8, 0, 0) == need(-1, -1, -1, 1) == 0
+    top = 2**31 - 1                                                        # what the products refuse needs none
+    assert need(top, 8, 16, 0) == need(8, top, 16, 1) == need(70, 130, top, 0) == need(top, top, top, 1) == 0
 
 
 def test_rows_refuse_bad_arguments():
@@ -176,6 +178,7 @@ def test_rows_refuse_bad_arguments():
     for fn in (quantize, norm, back):
         for bad in (dict(rows=0), dict(rows=-1), dict(n=0), dict(n=8), dict(n=72), dict(q=8), dict(q=0), dict(s=0)):
             assert fn(**bad) == _lib.NKV_ERR_ARG, (fn.__name__, bad)
+    assert back(rows=2**31 - 1, n=64) == _lib.NKV_ERR_ARG
     for bad in (dict(n=32784, stride=32784), dict(x=0), dict(x=4104), dict(stride=56), dict(stride=68), dict(q=AT["x"] + 16),
                 dict(s=AT["x"] + 16), dict(s=AT["q"] + 16), dict(q=AT["x"] + 2 * (3 * 128 + 64) - 16, stride=128)):
         assert quantize(**bad) == _lib.NKV_ERR_ARG, bad
