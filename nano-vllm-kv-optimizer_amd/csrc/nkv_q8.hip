@@ -352,7 +352,7 @@ constexpr int tile_rows(int na, int nb, int wm) { return (32 * na + 16 * nb * wm
 // fragments read a whole stage ahead instead: no gain.  128 x 128 18.2 / 17.5).
 template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false, int KS = 1>
 __global__ __launch_bounds__(128 * WM * KS) void tile_kernel(const Product p, int mt, int nt, bool wide, int* part) {
-  static_assert(!(SILU && PART) && !(PART && KS > 1) && (KS == 1 || (KS == 2 && NB % 2 == 0)), "");
+  static_assert(!(SILU && PART) && (KS == 1 || (KS == 2 && NB % 2 == 0)), "");
   extern __shared__ __align__(128) char s_lds[];
   constexpr int kTileM = 16 * NB * WM, kWaves = 2 * WM;
   __shared__ __align__(16) float s_scale[32 * NA], s_bias[SILU ? 4 : 32 * NA], s_x[kTileM];
@@ -378,7 +378,8 @@ __global__ __launch_bounds__(128 * WM * KS) void tile_kernel(const Product p, in
 
   const int all = (p.k + kTileK - 1) / kTileK;
   const int first = PART ? static_cast<int>(static_cast<int64_t>(all) * blockIdx.y / gridDim.y) : 0;
-  const int stages = PART ? static_cast<int>(static_cast<int64_t>(all) * (blockIdx.y + 1) / gridDim.y) - first : (all + KS - 1) / KS;
+  const int end = PART ? static_cast<int>(static_cast<int64_t>(all) * (blockIdx.y + 1) / gridDim.y) : all;
+  const int stages = (end - first + KS - 1) / KS;      // of a group (KS = 2: the other's last one may be empty)
 
   // A wavefront's share of a stage: 8-row pieces wave, wave + kWaves, ..., lane u with
   // 16 bytes of row u >> 3.  They go through registers: loaded a stage ahead of
@@ -403,8 +404,9 @@ __global__ __launch_bounds__(128 * WM * KS) void tile_kernel(const Product p, in
       row = (row / (2 * half)) * half + row % half;
     }
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(base), 0, rows * p.k, kRsrcWord3);
-    const int kb = (KS > 1 ? s * KS + group : first + s) * kTileK;
-    const int off = kc < p.k - kb ? voff + row * p.k + kb : 0x7fffffff;   // past the row's end: zeros
+    const int kb = (first + s * KS + group) * kTileK;
+    const int past = PART && KS > 1 ? min(p.k, end * kTileK) : p.k;       // past the row's (or run's) end: zeros
+    const int off = kc < past - kb ? voff + row * p.k + kb : 0x7fffffff;
     st[set][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
   };
   auto put = [&](int set, int buf, int i) {
@@ -503,27 +505,6 @@ __global__ __launch_bounds__(128 * WM * KS) void tile_kernel(const Product p, in
     }
   }
 
-  if constexpr (PART) {
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int mj = (wm * NB + j) * 16 + r;
-      if (mj >= mn) continue;
-      int* o = part + (static_cast<int64_t>(blockIdx.y) * p.m + m0 + mj) * p.n;
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const int c = c0 + (wc * NA + i) * 16 + 4 * g;
-        if (wide) {
-          if (c < p.n) *reinterpret_cast<i32x4*>(o + c) = acc[i][j];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < p.n) o[c + e] = acc[i][j][e];
-        }
-      }
-    }
-    return;
-  }
-
   // the groups' sums: each finishes half of the row tiles
   auto mine = [&](int j) { return KS == 1 || j / (NB / KS) == group; };
   if constexpr (KS > 1) {
@@ -542,6 +523,27 @@ __global__ __launch_bounds__(128 * WM * KS) void tile_kernel(const Product p, in
       if (mine(j))
 #pragma unroll
         for (int i = 0; i < NA; ++i) acc[i][j] += s_join[group * kGroup + (i * (NB / KS) + j % (NB / KS)) * kWave];
+  }
+
+  if constexpr (PART) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int mj = (wm * NB + j) * 16 + r;
+      if (!mine(j) || mj >= mn) continue;
+      int* o = part + (static_cast<int64_t>(blockIdx.y) * p.m + m0 + mj) * p.n;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int c = c0 + (wc * NA + i) * 16 + 4 * g;
+        if (wide) {
+          if (c < p.n) *reinterpret_cast<i32x4*>(o + c) = acc[i][j];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < p.n) o[c + e] = acc[i][j][e];
+        }
+      }
+    }
+    return;
   }
 
   constexpr int kOut = SILU ? NA / 2 : NA;             // channel groups of 16 that are written
@@ -844,10 +846,10 @@ int launch_tile(const Product& p, hipStream_t s, int parts = 1, int* part = null
   return NKV_OK;
 }
 
-// How a product runs.  Few rows and few enough 16-channel groups for one round
-// of workgroups, or at most 32 rows (us, few-row kernel / tiles: 48 x 4096 -> 4096
-// 9.1 / 11.1, 33 x 2560 -> 6144 9.7 / 8.7): the kernel that cuts k over
-// wavefronts.  Otherwise the tile whose busiest CU is done first: ceil(tiles /
+// How a product runs.  Few rows, few enough 16-channel groups for one round of
+// workgroups and a k that is not too long for one, or at most 32 rows (us, few-row
+// kernel / tiles: 48 x 4096 -> 4096 9.1 / 11.1, 33 x 2560 -> 6144 9.7 / 8.7, 37 x 9728 ->
+// 2560 13.4 / 13.7, 64 16.8 / 14.8): the kernel that cuts k over wavefronts.  Otherwise the tile whose busiest CU is done first: ceil(tiles /
 // CUs) tiles of the shape's time for a stage of 128 codes (us, plus what one
 // tile alone waits), as measured at 20-76 stages and 65-4096 rows.  Larger
 // tiles do more products a byte (2.5 PFLOP/s at 256 x 256, 1.9 at 128 x 128 on
@@ -860,7 +862,7 @@ struct Shape {
 constexpr Shape kShapes[] = {{256, 256, 1.35f, 0.0f}, {192, 256, 1.20f, 0.0f}, {160, 256, 1.00f, 0.0f},
                              {128, 256, 0.88f, 0.0f}, {128, 128, 0.58f, 0.0f}, {128, 64, 0.40f, 0.0f},
                              {64, 64, 0.19f, 0.04f},  {64, 32, 0.13f, 0.06f}};
-constexpr int kParted = 4;            // the shape of products whose k is cut
+constexpr int kParted[] = {4, 6};     // the shapes of products whose k is cut
 constexpr int kMaxParts = 8;
 struct Plan {
   int few;      // 16-row tiles of the few-row kernel, or 0
@@ -869,8 +871,8 @@ struct Plan {
 };
 Plan plan_product(int m, int n, int k, bool silu) {
   const int cus = device_cus() > 0 ? device_cus() : 256;
-  if (m <= 32 || (m <= 64 && (n + 15) / 16 <= cus)) return {std::min(4, (m + 15) / 16), 0, 1};
   const int stages = (k + kTileK - 1) / kTileK;
+  if (m <= 32 || (m <= 64 && (n + 15) / 16 <= cus && m * stages <= 4000)) return {std::min(4, (m + 15) / 16), 0, 1};
   auto tiles = [&](const Shape& sh, int channels) {
     return static_cast<int64_t>((channels + sh.channels - 1) / sh.channels) * ((m + sh.rows - 1) / sh.rows);
   };
@@ -884,14 +886,17 @@ Plan plan_product(int m, int n, int k, bool silu) {
     if (i == 0 || us < least) best = i, least = us;
   }
   Plan plan{0, best, 1};
-  for (int parts = 2; parts <= kMaxParts && stages >= 8 * parts; ++parts) {
-    const Shape& sh = kShapes[kParted];
-    // the join: a launch behind the tiles' last stores, and every sum written and read once at 6 TB/s
-    // (us, cut / whole: 65 x 9728 -> 2560 17.1 / 19.4, 128 19.1 / 21.0, 512 28.8 / 35.2; 200 x 4096 -> 2560 15.9 / 10.1)
-    const float join = 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(channels) * 8.0f / 6.0e6f;
-    const float us = static_cast<float>((stages + parts - 1) / parts) * static_cast<float>((tiles(sh, channels) * parts + cus - 1) / cus) * sh.us + join;
-    if (us < least) least = us, plan = {0, kParted, parts};
-  }
+  for (const int i : kParted)
+    for (int parts = 2; parts <= kMaxParts && stages >= 8 * parts; ++parts) {
+      const Shape& sh = kShapes[i];
+      // the join: a launch behind the tiles' last stores, and every sum written and read once at 6 TB/s
+      // (us, cut / whole: 65 x 9728 -> 2560 14.9 / 19.4, 128 17.0 / 21.0, 512 28.8 / 35.2; 200 x 4096 -> 2560
+      // 14.2 / 9.8.  128 x 128 tiles alone: 65 rows 17.1, 128 19.5)
+      const float join = 3.0f + static_cast<float>(parts) * static_cast<float>(m) * static_cast<float>(channels) * 8.0f / 6.0e6f;
+      const float us = static_cast<float>((stages + parts - 1) / parts) *
+                           (static_cast<float>((tiles(sh, channels) * parts + cus - 1) / cus) * sh.us + sh.wait_us) + join;
+      if (us < least) least = us, plan = {0, i, parts};
+    }
   return plan;
 }
 
@@ -908,7 +913,8 @@ int launch_product(const Product& p, int* workspace, hipStream_t s) {
   if (plan.parts > 1) {
     Product q = p;                                     // (gate and up rows are one matrix here)
     if (SILU) q.n = 2 * p.n;
-    const int rc = launch_tile<4, 2, 4, 1, false, true>(q, s, plan.parts, workspace);
+    const int rc = plan.shape == kParted[0] ? launch_tile<4, 2, 4, 1, false, true>(q, s, plan.parts, workspace)
+                                            : launch_tile<2, 2, 2, 4, false, true, 2>(q, s, plan.parts, workspace);
     if (rc != NKV_OK) return rc;
     const int v = p.n % 4 == 0 ? 4 : 1;
     const unsigned grid = static_cast<unsigned>((static_cast<int64_t>((p.n + v - 1) / v) * p.m + 255) / 256);

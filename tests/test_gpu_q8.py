@@ -287,7 +287,7 @@ def test_a_cut_k_gives_the_same_bits():
     from nanokv_amd import _lib
     from nanokv_amd.q8 import Q8, linear_q8, linear_silu_mul_q8
     need = _lib.load().nkv_linear_q8_workspace
-    for m, n, k in ((70, 130, 9728), (99, 257, 12304), (130, 640, 16400)):
+    for m, n, k in ((70, 130, 9728), (99, 257, 12304), (130, 640, 16400), (47, 2560, 12304), (64, 301, 16400), (400, 640, 9744)):
         assert need(m, n, k, 0) and need(m, n, k, 1) and not need(16, n, k, 0)
         x, w = _codes(m, k, seed=m), _codes(2 * n, k, seed=n)
         x = Q8(x.q, x.scale * (20 / k ** 0.5))
