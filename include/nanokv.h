@@ -663,26 +663,28 @@ int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, c
 int64_t nkv_linear_q8_workspace(int m, int n, int k, int gated);
 
 /*
- * nkv_quantize_q8 of one row x [k] followed by the product, in one launch
- * (decode steps): the results of the two calls bit for bit.  k: at most 12288.
+ * nkv_quantize_q8 of a few rows x [m][k] (m: at most 8) followed by the product, in
+ * one launch (decode and draft steps): the results of the two calls bit for bit.
+ * k: at most 12288 for one row, 4096 for more.  Every 16 channels of y quantise the
+ * rows for themselves, so many channels of several rows are better off with two.
  */
 int nkv_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* bias, uint16_t* y,
-                int n, int k, void* stream);
-int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y,
+                int m, int n, int k, void* stream);
+int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y, int m,
                          int intermediate, int k, void* stream);
 
 /*
- * nkv_rmsnorm_q8 of one row followed by the product, in one launch: the
+ * nkv_rmsnorm_q8 of a few rows followed by the product, in one launch: the
  * results of the two calls up to the fp32 order of the sum of squares.
  * residual_out (or NULL) overlaps no input here: every workgroup reads the
- * row while one writes it.  k: at most 12288.
+ * rows while one writes it.  m and k: as above.
  */
 int nkv_norm_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* residual,
                      const uint16_t* norm_weight, float eps, const uint16_t* bias, uint16_t* y,
-                     uint16_t* residual_out, int n, int k, void* stream);
+                     uint16_t* residual_out, int m, int n, int k, void* stream);
 int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x,
                               const uint16_t* residual, const uint16_t* norm_weight, float eps, uint16_t* y,
-                              uint16_t* residual_out, int intermediate, int k, void* stream);
+                              uint16_t* residual_out, int m, int intermediate, int k, void* stream);
 
 #ifdef __cplusplus
 }

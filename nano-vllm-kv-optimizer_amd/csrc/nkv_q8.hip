@@ -216,11 +216,30 @@ __device__ __forceinline__ void lds_barrier() {
 // the matrix instruction wants them (64 bytes of 16 rows a load) took 11.5, 16.8 and 20.9
 // for the last three; refills under a branch made the compiler wait for every
 // load (8.4 -> 15.1); 8 wavefronts a workgroup: gate|up 15.8.
+//
+// NCH > 0: up to 8 rows that are still bf16 (p.x and p.sx are not read), of up to
+// 512 NCH elements: every workgroup normalises (NORM) and quantises them itself, a
+// wavefront one or two rows, while its first weights are in flight, and keeps their codes
+// in LDS, in pieces like the weight's.  In a captured chain (us, with the rows' own launch
+// before the product / in one): 4 x 2560 -> 6144 with a norm 8.8 / 7.8, 4 x 4096 -> 2560 7.4 / 5.9,
+// 4 x 1024 -> 1024 5.3 / 3.6, gate|up of 9728 for 6 rows 15.4 / 14.7, with a norm 15.7 / 16.9 (what every
+// workgroup does again).  All first weights fetched before a norm spilled registers
+// (gate|up for 4 rows 18.0 against 15.2).
 constexpr int kFewWaves = 4;
+constexpr int kDraftRows = 2 * kFewWaves;
+constexpr int kDraftMaxK = 4096;
 constexpr int few_bytes(int tiles) { return tiles * kFewWaves * 16 * kTileK; }
-template <int NB, bool SILU>
-__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
-  constexpr int kHalves = SILU ? 2 : 1, kTiles = kHalves + NB;   // 16-row tiles of a piece: channels, then rows
+struct Rows {
+  const uint16_t* x;      // [m][k] bf16
+  const uint16_t* res;    // NORM: residual added first, or null
+  const uint16_t* nw;     // NORM: norm weight
+  uint16_t* res_out;      // NORM: bf16(x + res), or null
+  float eps;
+};
+template <int NB, bool SILU, int NCH = 0, bool NORM = false>
+__global__ __launch_bounds__(64 * kFewWaves, NCH == 0 ? 1 : NCH <= 5 ? 3 : 2) void few_kernel(const Product p, const Rows in) {
+  static_assert(NCH == 0 || NB == 1, "");
+  constexpr int kHalves = SILU ? 2 : 1, kTiles = kHalves + (NCH ? 0 : NB);   // 16-row tiles of a piece: channels, then rows
   constexpr int kDeep = kTiles <= 3 ? 5 : kTiles <= 5 ? 4 : 3;
   extern __shared__ __align__(128) char s_few[];       // [wave][kTiles][16 rows][128]; then the partial sums
   constexpr int waves = kFewWaves;
@@ -237,8 +256,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
   for (int h = 0; h < kHalves; ++h)
     rs[h] = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.w + (static_cast<int64_t>(h) * p.n + c0) * p.k), 0,
                                               min(p.n - c0, 16) * p.k, kRsrcWord3);
-  rs[kHalves] = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.x + static_cast<int64_t>(m0) * p.k), 0,
-                                                  min(p.m - m0, 16 * NB) * p.k, kRsrcWord3);
+  if constexpr (NCH == 0)
+    rs[kHalves] = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.x + static_cast<int64_t>(m0) * p.k), 0,
+                                                    min(p.m - m0, 16 * NB) * p.k, kRsrcWord3);
   char* mine_lds = s_few + wave * kTiles * 16 * kTileK;
   const int put_at = sub * kTileK + 16 * ((lane & 7) ^ swizzle(sub));       // (row 8 + sub: 8 rows on, its swizzle ^ 4)
   const int get_at = r * kTileK + 16 * (g ^ swizzle(r));
@@ -260,7 +280,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
       }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto products = [&](int d) {
+  // NCH: the rows' codes, [piece][8 rows][128] (columns 8 on of a product repeat the first 8 and are not used)
+  __shared__ __align__(128) char s_rows[NCH ? 512 * NCH * kDraftRows : 16];
+  __shared__ float s_row_scale[kDraftRows];
+  const int row_at = (r & 7) * kTileK + 16 * (g ^ swizzle(r & 7));
+  auto products = [&](int d, int q) {
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -269,9 +293,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
     wave_lds_sync();
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      i32x4 f[kTiles];
+      i32x4 f[kHalves + NB];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) f[t] = *reinterpret_cast<const i32x4*>(mine_lds + 16 * t * kTileK + (get_at ^ (64 * e)));
+      if constexpr (NCH > 0) f[kHalves] = *reinterpret_cast<const i32x4*>(s_rows + q * kDraftRows * kTileK + (row_at ^ (64 * e)));
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
 #pragma unroll
@@ -282,18 +307,102 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
   const int pieces = (p.k + kTileK - 1) / kTileK;
   const int mine = (pieces - wave + waves - 1) / waves;   // pieces wave, wave + waves, ...
   // (fetches past the last piece read no row; made without a branch, so that the waits stay exact)
+  if constexpr (NCH == 0) {
 #pragma unroll
-  for (int d = 0; d < kDeep; ++d) fetch(d, wave + d * waves);
+    for (int d = 0; d < kDeep; ++d) fetch(d, wave + d * waves);
+  } else {
+    constexpr int kNorm = NORM ? NCH : 1;
+    const int nc = p.k >> 3;
+    constexpr int kShare = NORM ? (NCH + waves - 1) / waves : 1;
+    static_assert(kShare <= 2, "");
+    uint4 xv[2][NCH], rv[2][kNorm], nv0, nv1;
+    __shared__ uint4 s_nw[NORM ? kWave * waves * kShare : 1];
+    if constexpr (NORM) {                              // (past the row: its last, not used)
+      nv0 = reinterpret_cast<const uint4*>(in.nw)[min(static_cast<int>(threadIdx.x), nc - 1)];
+      if constexpr (kShare > 1) nv1 = reinterpret_cast<const uint4*>(in.nw)[min(static_cast<int>(threadIdx.x) + kWave * waves, nc - 1)];
+    }
+    const uint16_t* res = in.res ? in.res : in.x;      // (without one: loaded, not added)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t row = min(wave + waves * h, p.m - 1);
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        const int64_t c = row * nc + min(lane + kWave * j, nc - 1);
+        xv[h][j] = reinterpret_cast<const uint4*>(in.x)[c];
+        if constexpr (NORM) rv[h][j] = reinterpret_cast<const uint4*>(res)[c];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // (the rest behind the first row, whose registers they take)
+    constexpr int kFirst = NORM ? (SILU ? 1 : 2) : kDeep;
+#pragma unroll
+    for (int d = 0; d < kFirst; ++d) fetch(d, wave + d * waves);
+    if constexpr (NORM) {
+      s_nw[threadIdx.x] = nv0;
+      if constexpr (kShare > 1) s_nw[threadIdx.x + kWave * waves] = nv1;
+      lds_barrier();
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = wave + waves * h;
+      if (h == 1) {
+#pragma unroll
+        for (int d = kFirst; d < kDeep; ++d) fetch(d, wave + d * waves);
+      }
+      if (row >= p.m) continue;
+      float v[NCH][8], ss = 0.0f;
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        const int c = lane + kWave * j;
+        unpack8(xv[h][j], v[j]);
+        if constexpr (NORM) {
+          if (in.res) {
+            float t[8];
+            unpack8(rv[h][j], t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] += t[e];
+          }
+          if (in.res_out && blockIdx.x == 0 && c < nc)
+            reinterpret_cast<uint4*>(in.res_out)[static_cast<int64_t>(row) * nc + c] = pack8(v[j]);
+          float wf[8];
+          unpack8(s_nw[c], wf);                        // (past the row: its last)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (c < nc) ss += v[j][e] * v[j][e];
+            v[j][e] *= wf[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, mag(v[j][e]));
+      }
+#pragma unroll
+      for (int o = kWave / 2; o > 0; o >>= 1) {
+        if constexpr (NORM) ss += __shfl_xor(ss, o);
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
+      }
+      const RowScale sc = NORM ? norm_row_scale(top, ss, p.k, in.eps) : row_scale(top);
+      if (lane == 0) s_row_scale[row] = sc.scale;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        const int c = lane + kWave * j;                // 8 codes: half of 16-byte unit (c / 2) % 8 of piece c / 16
+        if (c < nc)
+          *reinterpret_cast<uint2*>(s_rows + (c >> 4) * kDraftRows * kTileK + row * kTileK + 16 * (((c >> 1) & 7) ^ swizzle(row)) + 8 * (c & 1)) =
+              make_uint2(codes4(v[j][0], v[j][1], v[j][2], v[j][3], sc.inv), codes4(v[j][4], v[j][5], v[j][6], v[j][7], sc.inv));
+      }
+    }
+    lds_barrier();
+  }
   int i = 0;
   for (; i + kDeep < mine; i += kDeep)
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      products(d);
+      products(d, wave + (i + d) * waves);
       fetch(d, wave + (i + d + kDeep) * waves);
     }
 #pragma unroll
   for (int d = 0; d < kDeep; ++d)
-    if (i + d < mine) products(d);
+    if (i + d < mine) products(d, wave + (i + d) * waves);
   // the joined sums: [wave][kHalves NB][lane]
   i32x4* s_part = reinterpret_cast<i32x4*>(s_few);
   __syncthreads();
@@ -311,7 +420,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const Product p) {
     }
     const int m = m0 + 16 * j + r;
     if (m >= p.m) continue;
-    const float sx = p.sx[m];
+    const float sx = NCH ? s_row_scale[m & (kDraftRows - 1)] : p.sx[m];
     uint16_t* y = p.y + static_cast<int64_t>(m) * p.n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -823,8 +932,13 @@ template <int NB, bool SILU>
 int launch_few(const Product& p, hipStream_t s) {
   const int mt = (p.m + 16 * NB - 1) / (16 * NB);
   hipLaunchKernelGGL((few_kernel<NB, SILU>), dim3((p.n + 15) / 16, mt), dim3(64 * kFewWaves), few_bytes(NB + (SILU ? 2 : 1)),
-                     s, p);
+                     s, p, Rows{});
   return NKV_OK;
+}
+
+template <int NCH, bool NORM, bool SILU>
+void launch_draft(const Product& p, const Rows& in, hipStream_t s) {
+  hipLaunchKernelGGL((few_kernel<1, SILU, NCH, NORM>), dim3((p.n + 15) / 16), dim3(64 * kFewWaves), few_bytes(SILU ? 2 : 1), s, p, in);
 }
 
 template <int NA, int NB, int WM, int DEPTH, bool SILU, bool PART = false, int KS = 1>
@@ -997,29 +1111,40 @@ int check_product(const char* who, const Product& p, int outputs_per_channel, co
 }
 
 template <bool NORM, bool SILU>
-int token(const char* who, const Token& p, void* stream) {
+int token(const char* who, const Token& p, int m, void* stream) {
   NKV_CHECK_ARG(p.w != nullptr && p.sw != nullptr && p.x != nullptr && p.y != nullptr && (!NORM || p.nw != nullptr),
                 "%s: weight, w_scale, x%s and y must be non-NULL", who, NORM ? ", norm_weight" : "");
-  NKV_CHECK_ARG(p.n >= 1 && p.n <= INT32_MAX / 2 - 512 && p.k >= 16 && p.k % 16 == 0 && p.k <= kTokenMaxK,
-                "%s: n >= 1 and k a multiple of 16 in [16, %d] (got %d, %d)", who, kTokenMaxK, p.n, p.k);
+  NKV_CHECK_ARG(m >= 1 && m <= kDraftRows && p.n >= 1 && p.n <= INT32_MAX / 2 - 512 && p.k >= 16 && p.k % 16 == 0 &&
+                    p.k <= (m == 1 ? kTokenMaxK : kDraftMaxK),
+                "%s: 1 <= m <= %d, n >= 1 and k a multiple of 16 in [16, %d], with one row [16, %d] (got %d, %d, %d)", who,
+                kDraftRows, kDraftMaxK, kTokenMaxK, m, p.n, p.k);
   NKV_CHECK_ARG(aligned16(p.w) && aligned16(p.x) && (!p.res || aligned16(p.res)) && (!p.nw || aligned16(p.nw)) &&
                     (!p.res_out || aligned16(p.res_out)),
                 "%s: weight, x, residual, norm_weight and residual_out must be 16-byte aligned", who);
-  // every workgroup reads the row, norm_weight and its scales while others write y and one writes residual_out
-  const int64_t row = 2 * static_cast<int64_t>(p.k), out = 2 * static_cast<int64_t>(p.n);
+  // every workgroup reads the rows, norm_weight and its scales while others write y and one writes residual_out
+  const int64_t rows = 2 * static_cast<int64_t>(m) * p.k, out = 2 * static_cast<int64_t>(m) * p.n, vec = 2 * static_cast<int64_t>(p.k);
   const int64_t channels = static_cast<int64_t>(p.n) * (SILU ? 2 : 1);
   struct Out {
     const char* name;
     const void* at;
     int64_t bytes;
   };
-  for (const Out& o : {Out{"y", p.y, out}, Out{"residual_out", p.res_out, row}})
-    NKV_CHECK_ARG(apart(o.at, o.bytes, p.x, row) && apart(o.at, o.bytes, p.res, row) && apart(o.at, o.bytes, p.nw, row) &&
+  for (const Out& o : {Out{"y", p.y, out}, Out{"residual_out", p.res_out, rows}})
+    NKV_CHECK_ARG(apart(o.at, o.bytes, p.x, rows) && apart(o.at, o.bytes, p.res, rows) && apart(o.at, o.bytes, p.nw, vec) &&
                       apart(o.at, o.bytes, p.w, channels * p.k) && apart(o.at, o.bytes, p.sw, 4 * channels) &&
                       apart(o.at, o.bytes, p.bias, 2 * channels),
                   "%s: %s must not overlap an input", who, o.name);
-  NKV_CHECK_ARG(apart(p.y, out, p.res_out, row), "%s: y must not overlap residual_out", who);
-  launch_token<NORM, SILU>(p, reinterpret_cast<hipStream_t>(stream));
+  NKV_CHECK_ARG(apart(p.y, out, p.res_out, rows), "%s: y must not overlap residual_out", who);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (m == 1) {
+    launch_token<NORM, SILU>(p, s);
+  } else {
+    const Product q{p.w, p.sw, nullptr, nullptr, p.bias, p.y, m, p.n, p.k};
+    const Rows in{p.x, p.res, p.nw, p.res_out, p.eps};
+    if (p.k <= 1024) launch_draft<2, NORM, SILU>(q, in, s);
+    else if (p.k <= 2560) launch_draft<5, NORM, SILU>(q, in, s);
+    else launch_draft<8, NORM, SILU>(q, in, s);
+  }
   return launch_status(who);
 }
 
@@ -1100,27 +1225,27 @@ extern "C" int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float*
 }
 
 extern "C" int nkv_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* bias, uint16_t* y,
-                           int n, int k, void* stream) {
-  return token<false, false>("nkv_gemv_q8", Token{weight, w_scale, x, nullptr, nullptr, bias, y, nullptr, 0.0f, n, k}, stream);
+                           int m, int n, int k, void* stream) {
+  return token<false, false>("nkv_gemv_q8", Token{weight, w_scale, x, nullptr, nullptr, bias, y, nullptr, 0.0f, n, k}, m, stream);
 }
 
-extern "C" int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y,
+extern "C" int nkv_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x, uint16_t* y, int m,
                                     int intermediate, int k, void* stream) {
   return token<false, true>("nkv_gemv_silu_mul_q8",
-                            Token{gate_up_weight, w_scale, x, nullptr, nullptr, nullptr, y, nullptr, 0.0f, intermediate, k}, stream);
+                            Token{gate_up_weight, w_scale, x, nullptr, nullptr, nullptr, y, nullptr, 0.0f, intermediate, k}, m, stream);
 }
 
 extern "C" int nkv_norm_gemv_q8(const int8_t* weight, const float* w_scale, const uint16_t* x, const uint16_t* residual,
                                 const uint16_t* norm_weight, float eps, const uint16_t* bias, uint16_t* y,
-                                uint16_t* residual_out, int n, int k, void* stream) {
+                                uint16_t* residual_out, int m, int n, int k, void* stream) {
   return token<true, false>("nkv_norm_gemv_q8",
-                            Token{weight, w_scale, x, residual, norm_weight, bias, y, residual_out, eps, n, k}, stream);
+                            Token{weight, w_scale, x, residual, norm_weight, bias, y, residual_out, eps, n, k}, m, stream);
 }
 
 extern "C" int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, const uint16_t* x,
                                          const uint16_t* residual, const uint16_t* norm_weight, float eps, uint16_t* y,
-                                         uint16_t* residual_out, int intermediate, int k, void* stream) {
+                                         uint16_t* residual_out, int m, int intermediate, int k, void* stream) {
   return token<true, true>("nkv_norm_gemv_silu_mul_q8",
-                           Token{gate_up_weight, w_scale, x, residual, norm_weight, nullptr, y, residual_out, eps, intermediate, k},
+                           Token{gate_up_weight, w_scale, x, residual, norm_weight, nullptr, y, residual_out, eps, intermediate, k}, m,
                            stream);
 }

@@ -86,10 +86,10 @@ SIGNATURES = {
     "nkv_linear_q8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "nkv_linear_q8_workspace": (_I64, [_I, _I, _I, _I]),
     "nkv_linear_silu_mul_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
-    "nkv_gemv_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _P]),
-    "nkv_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _I, _I, _P]),
-    "nkv_norm_gemv_q8": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _P, _I, _I, _P]),
-    "nkv_norm_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _I, _I, _P]),
+    "nkv_gemv_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_norm_gemv_q8": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _P, _I, _I, _I, _P]),
+    "nkv_norm_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _I, _I, _I, _P]),
     "nkv_decode_step_ring": (_I, [_SP, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P, _F, _I, _P, _P, _P,
                                   _P, _P]),
     "nkv_prefill_attend": (_I, [_SP, _I, _I, _P, _I64, _I, _P, _P, _I64, _P, _I64, _I, _P, _I64,

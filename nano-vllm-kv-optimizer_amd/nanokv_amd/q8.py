@@ -13,8 +13,9 @@ an infinity has the scale NaN and the codes 0, so what is computed from it is
 NaN.
 
 On the GPU the operands are bf16 and the work is this library's kernels (no
-fallback: the library must load); one row (a decode token) takes its norm and
-quantisation inside the product's launch.  CPU tensors take the formulas,
+fallback: the library must load); one row (a decode token) and up to 8 (a draft,
+not too many channels) take their norm and quantisation inside the product's
+launch.  CPU tensors take the formulas,
 which the tests of the modules' routing run on.  Inference only: nothing here
 has a gradient, and inputs that ask for one are refused.
 """
@@ -30,7 +31,8 @@ from .store import current_stream_ptr
 
 TINY = 2.0 ** -119       # rows whose largest magnitude is below are zero
 SPLIT_ROWS = 32          # products of more rows may need a workspace
-TOKEN_ROW = 12288        # longest row that a product quantises in its own launch
+TOKEN_ROW = 12288        # longest row that a product quantises in its own launch: one,
+DRAFT_ROWS, DRAFT_ROW = 8, 4096          # or each of several
 
 
 class Q8(NamedTuple):
@@ -176,6 +178,20 @@ def _weight(weight: Q8, k: int, device: int, who: str, halves: bool) -> tuple:
     return q, scale, n
 
 
+def _one_launch(m: int, n: int, k: int, norm: bool) -> bool:
+    """Whether m rows take their norm and quantisation inside the product's launch.
+
+    Several rows (one or two a wavefront) are quantised again by every workgroup,
+    16 channels each, while its first weights are on their way: more of that, or a
+    norm with its residual, takes longer than a launch of the rows' own (us, two launches /
+    one: 2 to 4 x 4096 -> 2560 7.4 / 5.9, gate|up of 9728 for 6 rows 15.4 / 14.7, 6 x 2560 -> 24576
+    15.9 / 16.9; with a norm 4 x 2560 -> 6144 8.8 / 7.8, gate|up of 9728 for 4 rows 15.6 / 15.2,
+    for 6 15.7 / 16.9).  Eagerly a launch and its buffer are 5 us of host time too."""
+    if m == 1:
+        return k <= TOKEN_ROW and n > 0
+    return 0 < m <= DRAFT_ROWS and k <= DRAFT_ROW and 0 < (m + 3) // 4 * n * k <= (1 << 25 if norm else 1 << 26)
+
+
 # -- operators ---------------------------------------------------------------------
 def quantize_q8(x: torch.Tensor) -> Q8:
     """x [..., n] (n a multiple of 16) as int8 codes and a scale a row.
@@ -299,15 +315,15 @@ def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
         x = _dense(x)
         if m:
             return _product(x.q.data_ptr(), x.scale.data_ptr(), q.shape, q.device, m, k, w, bias, silu_mul)
-    elif m == 1 and k <= TOKEN_ROW and n:
+    elif _one_launch(m, n, k, False):
         if not _fine(x):
             x = _rows(x, who)
         y = _empty((*x.shape[:-1], n), _BF16, x.device)
         if silu_mul:
-            _call("gemv_silu_mul_q8", device, w[0].data_ptr(), w[1].data_ptr(), x.data_ptr(), y.data_ptr(), n, k)
+            _call("gemv_silu_mul_q8", device, w[0].data_ptr(), w[1].data_ptr(), x.data_ptr(), y.data_ptr(), m, n, k)
         else:
             _call("gemv_q8", device, w[0].data_ptr(), w[1].data_ptr(), x.data_ptr(),
-                  bias.data_ptr() if bias is not None else None, y.data_ptr(), n, k)
+                  bias.data_ptr() if bias is not None else None, y.data_ptr(), m, n, k)
         return y
     else:
         stride = k
@@ -345,7 +361,7 @@ def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool
     if bias is not None:
         bias = _vector(bias, n, device, who, "bias")
     m = x.numel() // k
-    if m != 1 or k > TOKEN_ROW or not n:
+    if not _one_launch(m, n, k, True):
         codes = torch.empty(m * (k + 4), dtype=_I8, device=x.device)        # the codes, then their scales
         at = codes.data_ptr()
         res_out = _norm(x, norm_weight, eps, residual, at, at + m * k, m, k, who, "norm_weight")
@@ -362,7 +378,7 @@ def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool
     b = () if silu_mul else (bias.data_ptr() if bias is not None else None,)
     _call("norm_gemv_silu_mul_q8" if silu_mul else "norm_gemv_q8", device, w[0].data_ptr(), w[1].data_ptr(),
           x.data_ptr(), residual.data_ptr() if has else None, norm_weight.data_ptr(), float(eps), *b, y.data_ptr(),
-          res_out.data_ptr() if has else None, n, k)
+          res_out.data_ptr() if has else None, m, n, k)
     return y, res_out
 
 

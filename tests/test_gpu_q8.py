@@ -142,9 +142,12 @@ def test_rows_without_a_finite_peak(n):
         y = linear_q8(x[i:i + 1], w)
         assert bool(y.isnan().all()) if i in nan else bool(y.isfinite().all())
         assert i not in zero or bool((y == 0).all())
+    for i in (0, 1, 5):                           # drafts of 8 and of 4
+        part = x[i:i + 8] if i < 2 else x[i:]
+        assert torch.equal(linear_q8(part, w).nan_to_num(7.0), linear_q8(t, w)[i:i + part.shape[0]].nan_to_num(7.0))
 
 
-@pytest.mark.parametrize("rows", [1, 4, 9])
+@pytest.mark.parametrize("rows", [1, 4, 8, 9])
 def test_norm_of_rows_without_a_finite_peak(rows):
     from nanokv_amd.q8 import norm_linear_q8, rmsnorm_q8
     x, nan, zero = _odd_rows(2560)
@@ -244,8 +247,9 @@ def test_gated_product(m, n, k):
     _check_gated(y, x, w)
 
 
-@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 40])
-@pytest.mark.parametrize("n,k", [(1, 16), (31, 496), (514, 1040), (2560, 4096), (130, 9728), (5, 12288)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 6, 7, 8, 9, 40])
+@pytest.mark.parametrize("n,k", [(1, 16), (31, 496), (17, 1024), (514, 1040), (100, 2560), (31, 2576), (2560, 4096), (7, 4112),
+                                 (130, 9728), (5, 12288), (8200, 144)])
 def test_bf16_rows_are_quantised_then_multiplied(m, n, k):
     """One launch or two: the same bits."""
     from nanokv_amd.q8 import linear_q8, linear_silu_mul_q8, quantize_q8
@@ -262,7 +266,8 @@ def test_bf16_rows_are_quantised_then_multiplied(m, n, k):
 
 @pytest.mark.parametrize("with_residual", [False, True])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 3000, 2560), (2, 31, 496), (3, 514, 1040), (4, 77, 4096),
-                                   (1, 10, 12288), (5, 60, 2560), (70, 60, 528)])
+                                   (1, 10, 12288), (5, 60, 2560), (70, 60, 528), (8, 40, 16), (2, 9728, 2560), (6, 9728, 2560),
+                                   (7, 33, 2576), (8, 12300, 144), (8, 1000, 1024), (2, 16, 4112), (9, 16, 2560)])
 def test_norm_then_product(m, n, k, with_residual):
     from nanokv_amd.q8 import norm_linear_q8, norm_linear_silu_mul_q8, rmsnorm_q8
     x, w = _hidden(m, k, m + n + k), _codes(2 * n, k, seed=n)
@@ -381,7 +386,7 @@ def test_rows_behind_the_last_are_left_as_they_were():
         sums.append(torch.full((lib.nkv_linear_q8_workspace(*size) + 64,), 5, dtype=torch.int32, device="cuda"))
         return p(sums[-1])
 
-    for m, n, k in ((1, 3, 64), (5, 33, 48), (37, 129, 256), (70, 65, 128), (300, 300, 144), (70, 130, 9728)):
+    for m, n, k in ((1, 3, 64), (5, 33, 48), (3, 17, 2560), (8, 100, 4096), (37, 129, 256), (70, 65, 128), (300, 300, 144), (70, 130, 9728)):
         x, w = _codes(m, k, seed=m), _codes(2 * n, k, seed=n)
         y = torch.full((m * n + 512,), 7.0, dtype=torch.bfloat16, device="cuda")
         assert lib.nkv_linear_q8(p(w.q), p(w.scale), p(x.q), p(x.scale), None, p(y), m, n, k, ws(m, n, k, 0), stream) == 0
@@ -394,10 +399,16 @@ def test_rows_behind_the_last_are_left_as_they_were():
         s = torch.full((m + 64,), 9.0, device="cuda")
         assert lib.nkv_quantize_q8(p(_hidden(m, k, 1)), k, p(q), p(s), m, k, stream) == 0
         assert bool((q[m * k:] == 9).all()) and bool((s[m:] == 9).all())
-        if m == 1:
+        if m <= 8:
             y.fill_(7.0)
-            assert lib.nkv_gemv_q8(p(w.q), p(w.scale), p(_hidden(m, k, 1)), None, p(y), n, k, stream) == 0
-            assert bool((y[m * n:] == 7).all())
+            assert lib.nkv_gemv_q8(p(w.q), p(w.scale), p(_hidden(m, k, 1)), None, p(y), m, n, k, stream) == 0
+            assert bool((y[m * n:] == 7).all()) and bool((y[:m * n] != 7).any())
+            y.fill_(7.0)
+            ro = torch.full((m * k + 512,), 9.0, dtype=torch.bfloat16, device="cuda")
+            rows, wn = _hidden(m, k, 1), torch.ones(k, dtype=torch.bfloat16, device="cuda")
+            assert lib.nkv_norm_gemv_silu_mul_q8(p(w.q), p(w.scale), p(rows), None, p(wn), 1e-6, p(y), p(ro), m, n, k, stream) == 0
+            assert bool((y[m * n:] == 7).all()) and bool((ro[m * k:] == 9).all())
+            assert torch.equal(ro[:m * k].view(m, k), rows)    # without a residual: x
 
 
 # -- together -----------------------------------------------------------------------

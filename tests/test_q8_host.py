@@ -105,15 +105,15 @@ def _product(name, m=8, n=64, k=128, **moved):
     return lib.nkv_linear_silu_mul_q8(p["w"], p["sw"], p["x"], p["sx"], p["y"], m, n, k, p["ws"], None)
 
 
-def _token(name, n=64, k=128, **moved):
+def _token(name, m=1, n=64, k=128, **moved):
     p, lib = _p(**moved), _lib.load()
     if name == "nkv_gemv_q8":
-        return lib.nkv_gemv_q8(p["w"], p["sw"], p["x"], p["b"], p["y"], n, k, None)
+        return lib.nkv_gemv_q8(p["w"], p["sw"], p["x"], p["b"], p["y"], m, n, k, None)
     if name == "nkv_gemv_silu_mul_q8":
-        return lib.nkv_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["y"], n, k, None)
+        return lib.nkv_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["y"], m, n, k, None)
     if name == "nkv_norm_gemv_q8":
-        return lib.nkv_norm_gemv_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["b"], p["y"], p["ro"], n, k, None)
-    return lib.nkv_norm_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["y"], p["ro"], n, k, None)
+        return lib.nkv_norm_gemv_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["b"], p["y"], p["ro"], m, n, k, None)
+    return lib.nkv_norm_gemv_silu_mul_q8(p["w"], p["sw"], p["x"], p["res"], p["nw"], 1e-6, p["y"], p["ro"], m, n, k, None)
 
 
 @pytest.mark.parametrize("name", ["nkv_linear_q8", "nkv_linear_silu_mul_q8"])
@@ -140,6 +140,10 @@ def test_token_products_refuse_bad_arguments(name):
                 dict(x=4104), dict(w=0), dict(sw=0), dict(x=0), dict(y=0)] + norm * [dict(nw=0), dict(nw=8), dict(res=24),
                                                                                      dict(ro=8)]:
         assert _token(name, **bad) == _lib.NKV_ERR_ARG, bad
+    for bad in (dict(m=0), dict(m=-1), dict(m=9), dict(m=2, k=4112), dict(m=8, k=12288)):
+        assert _token(name, **bad) == _lib.NKV_ERR_ARG, bad
+    for out, where in [("y", AT["x"] + 2 * 8 * 128 - 16)] + norm * [("ro", AT["res"] - 2 * 8 * 128 + 16), ("y", AT["ro"] + 2 * 7 * 128)]:
+        assert _token(name, m=8, **{out: where}) == _lib.NKV_ERR_ARG and b"overlap" in _lib.load().nkv_last_error()
     row = 2 * 128
     for out, size in [("y", 2 * 64)] + norm * [("ro", row)]:
         for what, length in [("w", 64 * 128), ("sw", 4 * 64), ("x", row)] + norm * [("res", row), ("nw", 256)]:
