@@ -321,17 +321,19 @@ __global__ __launch_bounds__(64 * kFewWaves, NCH == 0 ? 1 : NCH <= 5 ? 3 : 2) vo
       nv0 = reinterpret_cast<const uint4*>(in.nw)[min(static_cast<int>(threadIdx.x), nc - 1)];
       if constexpr (kShare > 1) nv1 = reinterpret_cast<const uint4*>(in.nw)[min(static_cast<int>(threadIdx.x) + kWave * waves, nc - 1)];
     }
-    const uint16_t* res = in.res ? in.res : in.x;      // (without one: loaded, not added)
+    // past the row, past the last row, and without a residual: zeros, and nothing is read
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(in.x), 0, 2 * p.m * p.k, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(NORM ? in.res : in.x), 0,
+                                                                        NORM && in.res ? 2 * p.m * p.k : 0, kRsrcWord3);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t row = min(wave + waves * h, p.m - 1);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
-        const int64_t c = row * nc + min(lane + kWave * j, nc - 1);
-        xv[h][j] = reinterpret_cast<const uint4*>(in.x)[c];
-        if constexpr (NORM) rv[h][j] = reinterpret_cast<const uint4*>(res)[c];
+        const int c = lane + kWave * j;
+        const int off = c < nc ? 2 * (wave + waves * h) * p.k + 16 * c : 0x7fffffff;
+        xv[h][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+        if constexpr (NORM) rv[h][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rr, off, 0, 0));
       }
-    }
     __builtin_amdgcn_sched_barrier(0);
     // (the rest behind the first row, whose registers they take)
     constexpr int kFirst = NORM ? (SILU ? 1 : 2) : kDeep;
