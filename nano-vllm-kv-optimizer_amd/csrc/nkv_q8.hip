@@ -36,15 +36,18 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // the infinities and NaN on top.
 __device__ __forceinline__ uint32_t mag(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-// 4 codes: rne(fl(v * inv)) for |v * inv| <= 127.5, in the low byte of the sum with
-// 1.5 * 2^23 (whose rounding is to nearest even); NaN gives 0.  The product is
-// rounded before (no fma): where v is a simple fraction of the row's peak, v * 127 /
-// peak lies half way between two codes, and the error of inv must not decide.
+// 4 codes.  v * inv is off by less than 127 * 2^-23 < 2^-16 (inv and the product are rounded
+// once each, no fma).  bf16 v and peak put v * 127 / peak half way between two codes or more than
+// 2^-16 off (all pairs of mantissas were tried), so the product is rounded to 2^-15 first --
+// the sum with 1.5 * 2^8, whose last bit that is -- which makes a half way one exact again:
+// the codes are rne(v * 127 / peak) itself.  (Rounded at once, 14 of the 254 half way pairs
+// of mantissas went to the other code.)
+// Then the low byte of a sum in [2^23, 2^24), rounded to nearest even; NaN gives 0.
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
 #pragma clang fp contract(off)
-  constexpr float kMagic = 12582912.0f;
-  const uint32_t x = __float_as_uint(a * inv + kMagic), y = __float_as_uint(b * inv + kMagic);
-  const uint32_t z = __float_as_uint(c * inv + kMagic), w = __float_as_uint(d * inv + kMagic);
+  constexpr float kSnap = 384.0f, kMagic = 12582912.0f - kSnap;
+  const uint32_t x = __float_as_uint((a * inv + kSnap) + kMagic), y = __float_as_uint((b * inv + kSnap) + kMagic);
+  const uint32_t z = __float_as_uint((c * inv + kSnap) + kMagic), w = __float_as_uint((d * inv + kSnap) + kMagic);
   return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
 }
 

@@ -42,12 +42,18 @@ class Q8(NamedTuple):
 
 
 # -- formulas (CPU tensors) ----------------------------------------------------
+SNAP, MAGIC = 1.5 * 2.0 ** 8, 1.5 * 2.0 ** 23    # sums with them are rounded to 2^-15, to whole numbers
+
+
 def _quantize_formula(y: torch.Tensor) -> Q8:
     top = y.abs().amax(dim=-1)      # (NaN where the row holds one)
     zero, odd = top < TINY, ~top.isfinite()
     none = torch.zeros_like(top)
-    inv = torch.where(zero | odd, none, 127.0 / top)
-    q = torch.where(odd.unsqueeze(-1), none.unsqueeze(-1), torch.round(y * inv.unsqueeze(-1))).to(torch.int8)
+    # the kernels' roundings, so their bits: a true division (127.0 / top is a reciprocal and
+    # a product), and y * inv to 2^-15 before whole numbers, which makes ties exact
+    inv = torch.where(zero | odd, none, torch.full_like(top, 127.0) / top)
+    code = ((y * inv.unsqueeze(-1) + SNAP) + (MAGIC - SNAP)) - MAGIC
+    q = torch.where(odd.unsqueeze(-1), none.unsqueeze(-1), code).to(torch.int8)
     return Q8(q, torch.where(odd, torch.full_like(top, float("nan")), torch.where(zero, none, top / 127.0)))
 
 
