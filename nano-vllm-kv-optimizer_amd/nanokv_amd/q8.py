@@ -17,7 +17,8 @@ fallback: the library must load); one row (a decode token) and up to 8 (a draft,
 not too many channels) take their norm and quantisation inside the product's
 launch.  CPU tensors take the formulas,
 which the tests of the modules' routing run on.  Inference only: nothing here
-has a gradient, and inputs that ask for one are refused.
+has a gradient, and operands that ask for one (``requires_grad`` with gradients
+enabled, or a forward-mode tangent) are refused on either.
 """
 
 from __future__ import annotations
@@ -25,6 +26,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .store import current_stream_ptr
@@ -88,6 +90,7 @@ def _silu_mul_formula(x: Q8, weight: Q8) -> torch.Tensor:
 _I8, _F32, _BF16 = torch.int8, torch.float32, torch.bfloat16
 _ENTRY: dict = {}        # the library's functions by name, once it is loaded
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or current_stream_ptr
+_grad_enabled = torch.is_grad_enabled
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -114,12 +117,22 @@ def _call(name: str, device: int, *args) -> None:
         _lib.check(rc, name)
 
 
+def _no_gradients(who: str, *operands) -> None:
+    asks = False
+    if _grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                asks = True
+    if forward_ad._current_level >= 0:       # inside a dual_level
+        asks = asks or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands)
+    if asks:
+        raise ValueError(f"{who}: an operand asks for a gradient, and the 8-bit operators have none")
+
+
 def _rows(x: torch.Tensor, who: str, what: str = "x") -> torch.Tensor:
     """x as dense bf16 rows on a 16-byte boundary (copied if it is neither)."""
     if x.dtype is not _BF16:
         raise ValueError(f"{who}: {what} must be bfloat16 on the GPU (got {x.dtype})")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{who}: {what} asks for a gradient, and the 8-bit operators have none")
     if not x.is_contiguous():
         x = x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
@@ -127,7 +140,7 @@ def _rows(x: torch.Tensor, who: str, what: str = "x") -> torch.Tensor:
 
 def _fine(t: torch.Tensor) -> bool:
     """What _rows returns as it is."""
-    return t.dtype is _BF16 and not t.requires_grad and t.is_contiguous() and t.data_ptr() % 16 == 0
+    return t.dtype is _BF16 and t.is_contiguous() and t.data_ptr() % 16 == 0
 
 
 def _vector(t: torch.Tensor, n: int, device: int, who: str, what: str) -> torch.Tensor:
@@ -205,6 +218,7 @@ def quantize_q8(x: torch.Tensor) -> Q8:
     2-D rows may lie apart (a column range of a wider matrix, on 16-byte
     boundaries) and are read in place."""
     n = _width(x, "quantize_q8")
+    _no_gradients("quantize_q8", x)
     if not x.is_cuda:
         return _quantize_formula(x.float())
     stride = n
@@ -221,7 +235,7 @@ def quantize_q8(x: torch.Tensor) -> Q8:
 def _strided(x: torch.Tensor, n: int, who: str) -> tuple:
     """(x, elements from row to row): 2-D bf16 rows that lie apart stay where they are."""
     if (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) > n and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
-            and x.dtype is _BF16 and not x.requires_grad):
+            and x.dtype is _BF16):
         return x, x.stride(0)
     return _rows(x, who), n
 
@@ -230,6 +244,7 @@ def dequantize_q8(t: Q8) -> torch.Tensor:
     """bf16(q * scale)."""
     _check_q8(t, "dequantize_q8", "t")
     n = _width(t.q, "dequantize_q8")
+    _no_gradients("dequantize_q8", t.scale)
     if not t.q.is_cuda:
         return (t.q.float() * t.scale.unsqueeze(-1)).to(_BF16)
     q, scale = t
@@ -264,6 +279,7 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torc
     """RMSNorm of x (+ residual) over the last dim, held in 8 bits: (Q8, the new
     residual bf16(x + residual), or x itself without one)."""
     n = _width(x, "rmsnorm_q8")
+    _no_gradients("rmsnorm_q8", x, weight, residual)
     if not x.is_cuda:
         return _norm_formula(x, weight, eps, residual)
     if not _fine(x):
@@ -307,6 +323,7 @@ def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
         _check_q8(x, who, "x")
     q = x.q if held else x
     k = _width(q, who)
+    _no_gradients(who, x.scale if held else x, weight[1], bias)
     device = q.get_device()
     w = _weight(weight, k, device, who, silu_mul)
     if device < 0:
@@ -356,6 +373,7 @@ def linear_silu_mul_q8(x, gate_up_weight: Q8) -> torch.Tensor:
 
 def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool, who: str):
     k = _width(x, who)
+    _no_gradients(who, x, norm_weight, weight[1], residual, bias)
     device = x.get_device()
     w = _weight(weight, k, device, who, silu_mul)
     if device < 0:

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests.test_q8_edges import every_value_and_peak
+from tests.test_q8_edges import check_gradients_are_refused, every_value_and_peak
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,7 @@ def test_codes_behind_a_norm_are_the_cpu_forms():
             assert torch.equal(a.q.cpu(), b.q)
             # a sum of n squares, 43 roundings at most here and a library's order there, under a root
             assert bool(((a.scale.cpu() - b.scale).abs() <= 2.0 ** -17 * b.scale).all())
+
+
+def test_operands_that_ask_for_a_gradient_are_refused():
+    check_gradients_are_refused("cuda")

@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from nanokv_amd.q8 import quantize_q8
+from nanokv_amd.q8 import (Q8, dequantize_q8, linear_q8, linear_silu_mul_q8, norm_linear_q8, norm_linear_silu_mul_q8,
+                           quantize_q8, rmsnorm_q8)
 
 
 # -- the code of every bf16 value under every bf16 peak ------------------------------
@@ -34,3 +35,48 @@ def test_codes_are_the_nearest_with_ties_to_even():
     assert torch.equal(quantize_q8(x).q.long(), codes)
     big = quantize_q8(x * 2.0 ** 100)
     assert torch.equal(big.q.long(), codes)
+
+
+# -- gradients -----------------------------------------------------------------------
+def gradient_calls(device="cpu"):
+    """(name, call, the operands it takes) with every operand that a gradient could be asked of."""
+    g = torch.Generator().manual_seed(1)
+    x, r = (torch.randn(3, 32, generator=g).bfloat16().to(device) for _ in range(2))
+    wn, b = torch.ones(32, device=device).bfloat16(), torch.zeros(8, device=device).bfloat16()
+    w, t = quantize_q8(torch.randn(8, 32, generator=g).bfloat16().to(device)), quantize_q8(x)
+    return [("quantize", lambda x: quantize_q8(x), (x,)),
+            ("dequantize", lambda s: dequantize_q8(Q8(t.q, s)), (t.scale,)),
+            ("rmsnorm", lambda x, wn, r: rmsnorm_q8(x, wn, 1e-6, r), (x, wn, r)),
+            ("linear", lambda x, s, b: linear_q8(x, Q8(w.q, s), b), (x, w.scale, b)),
+            ("linear of codes", lambda xs, s, b: linear_q8(Q8(t.q, xs), Q8(w.q, s), b), (t.scale, w.scale, b)),
+            ("gated", lambda x, s: linear_silu_mul_q8(x, Q8(w.q, s)), (x, w.scale)),
+            ("norm, linear", lambda x, wn, s, r, b: norm_linear_q8(x, wn, 1e-6, Q8(w.q, s), r, b), (x, wn, w.scale, r, b)),
+            ("norm, gated", lambda x, wn, s, r: norm_linear_silu_mul_q8(x, wn, 1e-6, Q8(w.q, s), r), (x, wn, w.scale, r))]
+
+
+def check_gradients_are_refused(device):
+    from torch.autograd import forward_ad
+    for name, call, operands in gradient_calls(device):
+        call(*operands)
+        for i, t in enumerate(operands):
+            asks = t.clone().requires_grad_()
+            args = [asks if j == i else o for j, o in enumerate(operands)]
+            with pytest.raises(ValueError, match="gradient"):
+                call(*args)
+                pytest.fail(f"{name}: operand {i}")
+            for off in (torch.no_grad, torch.inference_mode):      # (nothing is asked there)
+                with off():
+                    call(*args)
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(ValueError, match="gradient"):
+                    call(*[dual if j == i else o for j, o in enumerate(operands)])
+                call(*operands)
+
+
+def test_operands_that_ask_for_a_gradient_are_refused():
+    check_gradients_are_refused("cpu")
+    w = quantize_q8(torch.randn(8, 32))
+    for transform in (torch.func.grad, lambda f: lambda x: torch.func.jvp(f, (x,), (x,))):
+        with pytest.raises(ValueError, match="gradient"):
+            transform(lambda x: linear_q8(x, w).sum())(torch.randn(3, 32))
