@@ -146,14 +146,22 @@ def _fine(t: torch.Tensor) -> bool:
 def _vector(t: torch.Tensor, n: int, device: int, who: str, what: str) -> torch.Tensor:
     if t.dim() != 1 or t.shape[0] != n or t.get_device() != device:
         raise ValueError(f"{who}: {what} must be a [{n}] tensor on x's device (got {tuple(t.shape)} on {t.device})")
-    return _rows(t, who, what)
+    return _rows(t, who, what) if device >= 0 else t
 
 
 def _like(t: torch.Tensor, x: torch.Tensor, who: str, what: str) -> torch.Tensor:
     if t.shape != x.shape or t.get_device() != x.get_device():
         raise ValueError(f"{who}: {what} must be like x, {tuple(x.shape)} on {x.device} "
                          f"(got {tuple(t.shape)} on {t.device})")
-    return _rows(t, who, what)
+    return _rows(t, who, what) if t.is_cuda else t
+
+
+def _norm_checked(x, weight, eps, residual, who: str, what: str):
+    """_norm_formula of operands that the kernels would take (none is broadcast)."""
+    _vector(weight, x.shape[-1], x.get_device(), who, what)
+    if residual is not None:
+        _like(residual, x, who, "residual")
+    return _norm_formula(x, weight, eps, residual)
 
 
 def _width(x: torch.Tensor, who: str) -> int:
@@ -281,7 +289,7 @@ def rmsnorm_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torc
     n = _width(x, "rmsnorm_q8")
     _no_gradients("rmsnorm_q8", x, weight, residual)
     if not x.is_cuda:
-        return _norm_formula(x, weight, eps, residual)
+        return _norm_checked(x, weight, eps, residual, "rmsnorm_q8", "weight")
     if not _fine(x):
         x = _rows(x, "rmsnorm_q8")
     shape, device = x.shape, x.device
@@ -326,13 +334,13 @@ def _linear(x, weight: Q8, bias, silu_mul: bool, who: str) -> torch.Tensor:
     _no_gradients(who, x.scale if held else x, weight[1], bias)
     device = q.get_device()
     w = _weight(weight, k, device, who, silu_mul)
+    n = w[2]
+    if bias is not None:
+        bias = _vector(bias, n, device, who, "bias")
     if device < 0:
         t = x if held else quantize_q8(x)
         y = _silu_mul_formula(t, weight) if silu_mul else _product_formula(t, weight, bias)
         return y.to(_BF16 if held else x.dtype)
-    n = w[2]
-    if bias is not None:
-        bias = _vector(bias, n, device, who, "bias")
     m = q.numel() // k
     if held:
         x = _dense(x)
@@ -376,14 +384,14 @@ def _norm_linear(x, norm_weight, eps, weight: Q8, residual, bias, silu_mul: bool
     _no_gradients(who, x, norm_weight, weight[1], residual, bias)
     device = x.get_device()
     w = _weight(weight, k, device, who, silu_mul)
-    if device < 0:
-        t, res_out = _norm_formula(x, norm_weight, eps, residual)
-        y = _silu_mul_formula(t, weight) if silu_mul else _product_formula(t, weight, bias)
-        return y.to(x.dtype), res_out
     n = w[2]
-    x = _rows(x, who)
     if bias is not None:
         bias = _vector(bias, n, device, who, "bias")
+    if device < 0:
+        t, res_out = _norm_checked(x, norm_weight, eps, residual, who, "norm_weight")
+        y = _silu_mul_formula(t, weight) if silu_mul else _product_formula(t, weight, bias)
+        return y.to(x.dtype), res_out
+    x = _rows(x, who)
     m = x.numel() // k
     if not _one_launch(m, n, k, True):
         codes = torch.empty(m * (k + 4), dtype=_I8, device=x.device)        # the codes, then their scales

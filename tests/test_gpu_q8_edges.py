@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests.test_q8_edges import check_gradients_are_refused, every_value_and_peak
+from tests.test_q8_edges import check_gradients_are_refused, check_nothing_is_broadcast, every_value_and_peak
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,7 @@ def test_codes_behind_a_norm_are_the_cpu_forms():
 
 def test_operands_that_ask_for_a_gradient_are_refused():
     check_gradients_are_refused("cuda")
+
+
+def test_nothing_is_broadcast():
+    check_nothing_is_broadcast("cuda")

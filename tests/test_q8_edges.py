@@ -80,3 +80,31 @@ def test_operands_that_ask_for_a_gradient_are_refused():
     for transform in (torch.func.grad, lambda f: lambda x: torch.func.jvp(f, (x,), (x,))):
         with pytest.raises(ValueError, match="gradient"):
             transform(lambda x: linear_q8(x, w).sum())(torch.randn(3, 32))
+
+
+# -- operands ------------------------------------------------------------------------
+def check_nothing_is_broadcast(device):
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(3, 32, generator=g).bfloat16().to(device)
+    w = quantize_q8(torch.randn(8, 32, generator=g).bfloat16().to(device))
+    one, wn = torch.ones(1, device=device).bfloat16(), torch.ones(32, device=device).bfloat16()
+    for rows in (x, x[:1], quantize_q8(x)):
+        for bias in (one, one[0], one.expand(3, 1), torch.zeros(3, 8, device=device).bfloat16(), one.expand(4)):
+            with pytest.raises(ValueError, match="bias"):
+                linear_q8(rows, w, bias)
+            if not isinstance(rows, Q8):
+                with pytest.raises(ValueError, match="bias"):
+                    norm_linear_q8(rows, wn, 1e-6, w, None, bias)
+    for norm in (lambda wn, r: rmsnorm_q8(x, wn, 1e-6, r), lambda wn, r: norm_linear_q8(x, wn, 1e-6, w, r),
+                 lambda wn, r: norm_linear_silu_mul_q8(x, wn, 1e-6, w, r)):
+        norm(wn, x)
+        for bad in (one, one[0], wn.expand(3, 32), wn[:16]):
+            with pytest.raises(ValueError, match="weight"):
+                norm(bad, None)
+        for bad in (x[:1], x[0], x[:, :1], x.view(3, 1, 32), x.view(1, 3, 32)):
+            with pytest.raises(ValueError, match="residual"):
+                norm(wn, bad)
+
+
+def test_nothing_is_broadcast():
+    check_nothing_is_broadcast("cpu")
