@@ -35,6 +35,7 @@ TINY = 2.0 ** -119       # rows whose largest magnitude is below are zero
 SPLIT_ROWS = 32          # products of more rows may need a workspace
 TOKEN_ROW = 12288        # longest row that a product quantises in its own launch: one,
 DRAFT_ROWS, DRAFT_ROW = 8, 4096          # or each of several
+INT_MAX = 2 ** 31 - 1    # the library's sizes are C ints
 
 
 class Q8(NamedTuple):
@@ -168,6 +169,8 @@ def _width(x: torch.Tensor, who: str) -> int:
     n = x.shape[-1] if x.dim() else 0
     if n < 16 or n % 16:
         raise ValueError(f"{who}: the last dimension must be a positive multiple of 16 (got {n})")
+    if x.numel() > INT_MAX and max(n, x.numel() // n) > INT_MAX:       # (as C ints they would wrap)
+        raise ValueError(f"{who}: at most {INT_MAX} rows and elements a row (got {x.numel() // n} rows of {n})")
     return n
 
 
@@ -196,6 +199,8 @@ def _weight(weight: Q8, k: int, device: int, who: str, halves: bool) -> tuple:
                          f"(got {q.dtype} {tuple(q.shape)} on {q.device}, {scale.dtype} {tuple(scale.shape)} on "
                          f"{scale.device})")
     n = q.size(0)
+    if n > INT_MAX:
+        raise ValueError(f"{who}: the weight has at most {INT_MAX} rows (got {n})")
     if halves:
         if n % 2:
             raise ValueError(f"{who}: the gate|up weight needs an even number of rows")

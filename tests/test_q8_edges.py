@@ -108,3 +108,28 @@ def check_nothing_is_broadcast(device):
 
 def test_nothing_is_broadcast():
     check_nothing_is_broadcast("cpu")
+
+
+def test_sizes_that_no_c_int_holds_are_refused():
+    """ctypes would hand the low 32 bits on: 2^32 + 1 rows would be one."""
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    def codes(n, k):
+        return Q8(empty(n, k, dtype=torch.int8), empty(n, dtype=torch.float32))
+
+    wn = empty(16)
+    for rows in (2 ** 31, 2 ** 32 + 1):
+        for call in (lambda: quantize_q8(empty(rows, 16)), lambda: dequantize_q8(codes(rows, 16)),
+                     lambda: rmsnorm_q8(empty(rows, 16), wn, 1e-6), lambda: linear_q8(empty(rows, 16), codes(4, 16)),
+                     lambda: linear_q8(codes(rows, 16), codes(4, 16)),
+                     lambda: norm_linear_q8(empty(rows, 16), wn, 1e-6, codes(4, 16)),
+                     lambda: linear_q8(empty(2, 16), codes(rows, 16)),
+                     lambda: norm_linear_silu_mul_q8(empty(2, 16), wn, 1e-6, codes(rows, 16))):
+            with pytest.raises(ValueError, match="at most 2147483647"):
+                call()
+    k = 2 ** 32 + 16
+    for call in (lambda: quantize_q8(empty(1, k)), lambda: linear_q8(empty(2, k), codes(4, k)),
+                 lambda: rmsnorm_q8(empty(1, k), empty(k), 1e-6)):
+        with pytest.raises(ValueError, match="at most 2147483647"):
+            call()
