@@ -977,10 +977,11 @@ int launch_tile(const Product& p, hipStream_t s, int parts = 1, int* part = null
 struct Shape {
   int channels, rows;   // (SILU: half as many channels of y)
   float us, wait_us;
+  int threads;          // a workgroup
 };
-constexpr Shape kShapes[] = {{256, 256, 1.35f, 0.0f}, {192, 256, 1.20f, 0.0f}, {160, 256, 1.00f, 0.0f},
-                             {128, 256, 0.88f, 0.0f}, {128, 128, 0.58f, 0.0f}, {128, 64, 0.40f, 0.0f},
-                             {64, 64, 0.19f, 0.04f},  {64, 32, 0.13f, 0.06f}};
+constexpr Shape kShapes[] = {{256, 256, 1.35f, 0.0f, 512}, {192, 256, 1.20f, 0.0f, 512}, {160, 256, 1.00f, 0.0f, 512},
+                             {128, 256, 0.88f, 0.0f, 512}, {128, 128, 0.58f, 0.0f, 512}, {128, 64, 0.40f, 0.0f, 512},
+                             {64, 64, 0.19f, 0.04f, 512},  {64, 32, 0.13f, 0.06f, 256}};
 constexpr int kParted[] = {4, 6};     // the shapes of products whose k is cut
 constexpr int kMaxParts = 8;
 struct Plan {
@@ -1017,6 +1018,19 @@ Plan plan_product(int m, int n, int k, bool silu) {
       if (us < least) least = us, plan = {0, i, parts};
     }
   return plan;
+}
+
+// A launch holds less than 2^32 threads.
+constexpr int64_t kMaxThreads = (INT64_C(1) << 32) - 1;
+int64_t few_threads(int n) { return (static_cast<int64_t>(n) + 15) / 16 * (64 * kFewWaves); }
+// Threads of a product's largest launch.
+int64_t product_threads(int m, int n, int k, bool silu) {
+  const Plan plan = plan_product(m, n, k, silu);
+  if (plan.few) return few_threads(n);
+  const Shape& sh = kShapes[plan.shape];
+  const int64_t channels = silu ? 2 * static_cast<int64_t>(n) : n;
+  const int64_t tiles = (channels + sh.channels - 1) / sh.channels * ((static_cast<int64_t>(m) + sh.rows - 1) / sh.rows);
+  return std::max(tiles * sh.threads, plan.parts > 1 ? static_cast<int64_t>(m) * n + 255 : 0);   // (the join: at most an output each)
 }
 
 template <bool SILU>
@@ -1095,10 +1109,9 @@ int check_product(const char* who, const Product& p, int outputs_per_channel, co
                 "%s: weight, w_scale, x, x_scale and y must be non-NULL", who);
   NKV_CHECK_ARG(p.m >= 1 && p.n >= 1 && p.k >= 16 && p.k % 16 == 0 && p.k <= kMaxDepth,
                 "%s: m and n >= 1 and k a multiple of 16 in [16, %d] (got %d, %d, %d)", who, kMaxDepth, p.m, p.n, p.k);
-  // one workgroup a tile: at least 64 x 32 outputs each, or 16 channels of at most 64 rows
   NKV_CHECK_ARG(p.n <= INT32_MAX / 2 - 512 && p.m <= INT32_MAX - 512 &&
-                    static_cast<int64_t>((p.n + 31) / 32) * ((p.m + 31) / 32) <= INT32_MAX,
-                "%s: m or n too large (got %d, %d)", who, p.m, p.n);
+                    product_threads(p.m, p.n, p.k, outputs_per_channel == 2) <= kMaxThreads,
+                "%s: m or n too large for a launch (got %d, %d)", who, p.m, p.n);
   NKV_CHECK_ARG(aligned16(p.w) && aligned16(p.x), "%s: weight and x must be 16-byte aligned", who);
   const int64_t out = 2 * static_cast<int64_t>(p.m) * p.n, channels = static_cast<int64_t>(p.n) * outputs_per_channel;
   NKV_CHECK_ARG(apart(p.y, out, p.w, channels * p.k) && apart(p.y, out, p.sw, 4 * channels) &&
@@ -1123,6 +1136,7 @@ int token(const char* who, const Token& p, int m, void* stream) {
                     p.k <= (m == 1 ? kTokenMaxK : kDraftMaxK),
                 "%s: 1 <= m <= %d, n >= 1 and k a multiple of 16 in [16, %d], with one row [16, %d] (got %d, %d, %d)", who,
                 kDraftRows, kDraftMaxK, kTokenMaxK, m, p.n, p.k);
+  NKV_CHECK_ARG(m == 1 || few_threads(p.n) <= kMaxThreads, "%s: n too large for a launch (got %d)", who, p.n);
   NKV_CHECK_ARG(aligned16(p.w) && aligned16(p.x) && (!p.res || aligned16(p.res)) && (!p.nw || aligned16(p.nw)) &&
                     (!p.res_out || aligned16(p.res_out)),
                 "%s: weight, x, residual, norm_weight and residual_out must be 16-byte aligned", who);

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from nanokv_amd import _lib
 from nanokv_amd.q8 import (Q8, dequantize_q8, linear_q8, linear_silu_mul_q8, norm_linear_q8, norm_linear_silu_mul_q8,
                            quantize_q8, rmsnorm_q8)
 
@@ -133,3 +134,29 @@ def test_sizes_that_no_c_int_holds_are_refused():
                  lambda: rmsnorm_q8(empty(1, k), empty(k), 1e-6)):
         with pytest.raises(ValueError, match="at most 2147483647"):
             call()
+
+
+def test_products_that_no_launch_holds_are_refused():
+    """2^32 threads: 256 for 16 channels of few rows, 256 or 512 for a tile (addresses are never dereferenced)."""
+    lib, gap = _lib.load(), 1 << 44
+    w, sw, x, sx, y, ws = (gap * i for i in range(1, 7))
+    # (the largest sizes that fit are not called here: without a device the launch itself would fail)
+    for m, n in ((2, 2 ** 28), (32, 2 ** 28), (2 ** 29 + 2 ** 28, 8), (6 * 10 ** 8, 8), (2 ** 20, 2 ** 20)):
+        for rc in (lib.nkv_linear_q8(w, sw, x, sx, None, y, m, n, 16, ws, None),
+                   lib.nkv_linear_silu_mul_q8(w, sw, x, sx, y, m, n, 16, ws, None)):
+            assert rc == _lib.NKV_ERR_ARG and b"too large for a launch" in lib.nkv_last_error(), (m, n)
+    for m, n in ((2, 2 ** 28), (8, 2 ** 29)):
+        for rc in (lib.nkv_gemv_q8(w, sw, x, None, y, m, n, 16, None),
+                   lib.nkv_gemv_silu_mul_q8(w, sw, x, y, m, n, 16, None),
+                   lib.nkv_norm_gemv_q8(w, sw, x, None, sx, 1e-6, None, y, None, m, n, 16, None),
+                   lib.nkv_norm_gemv_silu_mul_q8(w, sw, x, None, sx, 1e-6, y, None, m, n, 16, None)):
+            assert rc == _lib.NKV_ERR_ARG and b"too large for a launch" in lib.nkv_last_error(), (m, n)
+    # what is refused for its size is refused before anything else is: a call that fits gets further
+    assert lib.nkv_linear_q8(w + 8, sw, x, sx, None, y, 32, 2 ** 28 - 16, 16, ws, None) == _lib.NKV_ERR_ARG
+    assert b"aligned" in lib.nkv_last_error()
+    assert lib.nkv_gemv_q8(w + 8, sw, x, None, y, 8, 2 ** 28 - 16, 16, None) == _lib.NKV_ERR_ARG
+    assert b"aligned" in lib.nkv_last_error()
+    assert lib.nkv_linear_q8(w + 8, sw, x, sx, None, y, 2 ** 28, 8, 16, ws, None) == _lib.NKV_ERR_ARG
+    assert b"aligned" in lib.nkv_last_error()
+    assert lib.nkv_gemv_q8(w + 8, sw, x, None, y, 1, 2 ** 29, 16, None) == _lib.NKV_ERR_ARG    # resident workgroups
+    assert b"aligned" in lib.nkv_last_error()
