@@ -550,6 +550,7 @@ class Qwen3ForCausalLM(nn.Module):
         self._graph = None       # captured decode step (decode_graph)
         self._graph_io = None    # its (token, position, logits) buffers
         self._graph_warm = False
+        self._graph_weights = 0  # _replaced when the step was first run for a graph
 
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         return self.model(input_ids, positions)
@@ -634,11 +635,13 @@ class Qwen3ForCausalLM(nn.Module):
         if not all(rt.device_ring_ready() for rt in self.runtimes):
             raise RuntimeError("decode_graph needs a full sink and recent window and the default decode "
                                "selection (use decode() until then)")
+        if self._graph_warm and self._graph_weights != _replaced:
+            self.release_graph()
         for rt in self.runtimes:
             rt.device_ring = True
         if self._graph is None:
             if not self._graph_warm:
-                self._graph_warm = True
+                self._graph_warm, self._graph_weights = True, _replaced
                 return self.decode(token, position)
             self._capture(token.device)
         tok, pos, logits = self._graph_io
@@ -675,6 +678,9 @@ class Qwen3ForCausalLM(nn.Module):
 
 
 # -- weights -------------------------------------------------------------------
+_replaced = 0    # how often quantize_linears_ replaced weights: captured steps of before read freed memory
+
+
 def _check_not_quantized(model: nn.Module, what: str) -> None:
     if any(isinstance(m, Q8Linear) for m in model.modules()):
         raise ValueError(f"{what}: the model's projections are in 8 bits already (quantize_linears_ comes last)")
@@ -686,9 +692,11 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
     weights, and with `lm_head` add the LM head in 8 bits (the embedding it may be
     tied to stays); returns the number of weights quantised.
 
-    After loading the weights and moving the model to its device.  Projections
+    After loading the weights and moving the model to its device; a captured decode
+    step is captured anew, whatever part of its model is given here.  Projections
     that were replaced or hooked before stay as they are.  A weight that cannot be held
     in 8 bits (rows that are not a multiple of 16, NaN, infinities) raises ValueError."""
+    global _replaced
     found = [(name, m) for name, m in model.named_modules() if _own(m, Linear)]
     made = {}
     for name, m in found:
@@ -699,6 +707,7 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
     head = None
     if lm_head and isinstance(model, Qwen3ForCausalLM):
         head = Q8Linear(model.lm_head_weight)
+    _replaced += bool(made)
     for name, new in made.items():
         parent, _, leaf = name.rpartition(".")
         setattr(model.get_submodule(parent), leaf, new.train(model.training))

@@ -1,0 +1,84 @@
+"""quantize_linears_ at its edges, on CPU tensors: captured steps, the untied head,
+hooks, shared projections."""
+
+import pytest
+import torch
+
+from nanokv_amd import qwen3
+from tests.test_qwen3_q8_modules import _forward, _model
+
+
+class _Graph:
+    """Stands for a captured step."""
+
+    def __init__(self):
+        self.replays = 0
+
+    def replay(self):
+        self.replays += 1
+
+
+class _Runtime:
+    """Stands for a layer's runtime in steady decode."""
+    device_ring = False
+
+    def device_ring_ready(self):
+        return True
+
+    def ring_replayed(self):
+        pass
+
+
+def _captured(model, monkeypatch):
+    """A model whose decode_graph() captures and replays _Graphs and steps eagerly into `steps`."""
+    model.runtimes = [_Runtime()]
+    steps, graphs = [], []
+    monkeypatch.setattr(model, "decode", lambda token, position: steps.append(position), raising=False)
+
+    def capture(graph):
+        graphs.append(graph())
+        return graphs[-1]
+
+    class Capturing:
+        def __init__(self, *a):
+            pass
+
+        __enter__ = __exit__ = lambda self, *a: None
+
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: capture(_Graph))
+    monkeypatch.setattr(torch.cuda, "graph", Capturing)
+    monkeypatch.setattr(_Runtime, "decode_state", lambda self: None, raising=False)
+    monkeypatch.setattr(_Runtime, "restore_decode_state", lambda self, st: None, raising=False)
+    monkeypatch.setattr(qwen3, "set_context", lambda *a, **k: None)
+    return steps, graphs
+
+
+@pytest.mark.parametrize("part", [lambda m: m, lambda m: m.model, lambda m: m.model.layers[1],
+                                  lambda m: m.model.layers[0].mlp])
+def test_a_captured_step_does_not_outlive_its_weights(part, monkeypatch):
+    """Whatever part of the model is quantised: the replay would read weights that were freed."""
+    model = _model()
+    steps, graphs = _captured(model, monkeypatch)
+    tok = torch.tensor([3])
+    for position in range(3):
+        model.decode_graph(tok, position)
+    assert steps == [0] and len(graphs) == 1 and graphs[0].replays == 2
+    qwen3.quantize_linears_(part(model))
+    for position in range(3, 6):                  # an eager step, a capture, a replay
+        model.decode_graph(tok, position)
+    assert steps == [0, 3] and len(graphs) == 2 and [g.replays for g in graphs] == [2, 2]
+    assert model.runtimes[0].device_ring
+    other = _model()                              # nothing of this model is replaced: nothing is captured again
+    model.decode_graph(tok, 6)
+    assert len(graphs) == 2 and graphs[1].replays == 3 and other._graph is None
+
+
+def test_weights_replaced_before_the_capture(monkeypatch):
+    """The eager step in front of a capture is run again with the new weights."""
+    model = _model()
+    steps, graphs = _captured(model, monkeypatch)
+    model.decode_graph(torch.tensor([3]), 0)
+    qwen3.quantize_linears_(model.model)
+    for position in range(1, 4):
+        model.decode_graph(torch.tensor([3]), position)
+    assert steps == [0, 1] and len(graphs) == 1 and graphs[0].replays == 2
