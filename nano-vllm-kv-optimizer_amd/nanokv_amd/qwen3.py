@@ -689,8 +689,9 @@ def _check_not_quantized(model: nn.Module, what: str) -> None:
 @torch.no_grad()
 def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
     """Replace every projection of `model` (this file's Linear) by a Q8Linear of its
-    weights, and with `lm_head` add the LM head in 8 bits (the embedding it may be
-    tied to stays); returns the number of weights quantised.
+    weights, and with `lm_head` add the LM head in 8 bits: the embedding it may be
+    tied to stays, a weight of its own is dropped (lm_head_weight is None then).
+    Returns the number of weights quantised; what is in 8 bits already stays as it is.
 
     After loading the weights and moving the model to its device; a captured decode
     step is captured anew, whatever part of its model is given here.  Projections
@@ -705,7 +706,7 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
         except ValueError as e:
             raise ValueError(f"quantize_linears_: {name}: {e}") from None
     head = None
-    if lm_head and isinstance(model, Qwen3ForCausalLM):
+    if lm_head and isinstance(model, Qwen3ForCausalLM) and model.lm_head_q8 is None:
         head = Q8Linear(model.lm_head_weight)
     _replaced += bool(made)
     for name, new in made.items():
@@ -715,6 +716,8 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
         model.release_graph()
         if head is not None:
             model.lm_head_q8 = head
+            if model.lm_head_weight is not model.model.embed_tokens.weight:
+                model.lm_head_weight = None
     return len(made) + (head is not None)
 
 

@@ -82,3 +82,34 @@ def test_weights_replaced_before_the_capture(monkeypatch):
     for position in range(1, 4):
         model.decode_graph(torch.tensor([3]), position)
     assert steps == [0, 1] and len(graphs) == 1 and graphs[0].replays == 2
+
+
+@pytest.mark.parametrize("tie", [True, False])
+def test_an_untied_head_is_held_once(tie):
+    model = _model(tie=tie)
+    n = 2 * 4 + 1
+    head, embed = model.lm_head_weight, model.model.embed_tokens.weight
+    assert qwen3.quantize_linears_(model) == n
+    assert model.model.embed_tokens.weight is embed
+    if tie:
+        assert model.lm_head_weight is embed
+    else:
+        assert model.lm_head_weight is None and not any(p is head for p in model.parameters())
+        assert "lm_head_weight" not in model.state_dict()
+    want, held = _forward(model), model.lm_head_q8
+    assert qwen3.quantize_linears_(model) == 0 and model.lm_head_q8 is held     # nothing is quantised again
+    assert torch.equal(_forward(model), want)
+    other = _model(tie=tie)
+    with torch.no_grad():
+        other.model.embed_tokens.weight.mul_(0.5)
+    qwen3.quantize_linears_(other)
+    other.load_state_dict(model.state_dict())
+    assert torch.equal(_forward(other), want)
+    model.to(torch.float32).to(torch.bfloat16)
+    assert torch.equal(_forward(model), want)
+
+
+def test_the_head_can_follow_the_projections():
+    model = _model(tie=False)
+    assert qwen3.quantize_linears_(model, lm_head=False) == 8 and model.lm_head_weight is not None
+    assert qwen3.quantize_linears_(model) == 1 and model.lm_head_weight is None
