@@ -461,7 +461,7 @@ class Qwen3MLP(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         proj = self.gate_up_proj
-        if _own(proj, Q8Linear) and proj.bias is None:
+        if _own(proj, Q8Linear) and proj.bias is None and not nn.modules.module._has_any_global_hook():
             return self.down_proj(linear_silu_mul_q8(x, proj.weight))
         if (_own(proj, Linear) and proj.bias is None and _gemv_ok(x, proj.weight)
                 and proj.weight.shape[0] % 2 == 0):

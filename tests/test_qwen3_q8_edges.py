@@ -3,6 +3,7 @@ hooks, shared projections."""
 
 import pytest
 import torch
+from torch import nn
 
 from nanokv_amd import qwen3
 from tests.test_qwen3_q8_modules import _forward, _model
@@ -113,3 +114,25 @@ def test_the_head_can_follow_the_projections():
     model = _model(tie=False)
     assert qwen3.quantize_linears_(model, lm_head=False) == 8 and model.lm_head_weight is not None
     assert qwen3.quantize_linears_(model) == 1 and model.lm_head_weight is None
+
+
+def test_global_hooks_see_every_projection():
+    layer = _model().model.layers[0]
+    qwen3.quantize_linears_(layer)
+    h, res = torch.randn(2, 256).bfloat16(), torch.randn(2, 256).bfloat16()
+    seen = []
+    hook = nn.modules.module.register_module_forward_hook(lambda m, i, o: seen.append(m))
+    try:
+        alone = layer.mlp(h)
+        assert seen == [layer.mlp.gate_up_proj, layer.mlp.down_proj, layer.mlp]
+        seen.clear()
+        hooked = layer(torch.arange(2), h, res)
+    finally:
+        hook.remove()
+    attn, mlp = layer.self_attn, layer.mlp
+    assert [m for m in seen if isinstance(m, qwen3.Q8Linear)] == [attn.qkv_proj, attn.o_proj, mlp.gate_up_proj, mlp.down_proj]
+    # the fused forms round less on the way: the norm's output (2^-8) and SiLU's factors are not rounded to
+    # bf16 there, which moves values over a code's edge: a step of 1 / 127 of a row's peak (4 of its rms) in
+    # some of its values, in two products one after the other
+    for a, b in ((alone, layer.mlp(h)), (hooked[0], layer(torch.arange(2), h, res)[0])):
+        assert float((a.double() - b.double()).norm() / b.double().norm()) < 2 * 4 / 127
