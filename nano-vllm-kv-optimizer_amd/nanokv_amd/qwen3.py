@@ -698,20 +698,21 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
     that were replaced or hooked before stay as they are.  A weight that cannot be held
     in 8 bits (rows that are not a multiple of 16, NaN, infinities) raises ValueError."""
     global _replaced
-    found = [(name, m) for name, m in model.named_modules() if _own(m, Linear)]
-    made = {}
+    found = [(name, m) for name, m in model.named_modules(remove_duplicate=False) if _own(m, Linear)]
+    made = {}                # by the projection: one that several modules share stays shared
     for name, m in found:
         try:
-            made[name] = Q8Linear(m.weight, m.bias)
+            if m not in made:
+                made[m] = Q8Linear(m.weight, m.bias)
         except ValueError as e:
             raise ValueError(f"quantize_linears_: {name}: {e}") from None
     head = None
     if lm_head and isinstance(model, Qwen3ForCausalLM) and model.lm_head_q8 is None:
         head = Q8Linear(model.lm_head_weight)
     _replaced += bool(made)
-    for name, new in made.items():
+    for name, m in found:
         parent, _, leaf = name.rpartition(".")
-        setattr(model.get_submodule(parent), leaf, new.train(model.training))
+        setattr(model.get_submodule(parent), leaf, made[m].train(model.training))
     if isinstance(model, Qwen3ForCausalLM):
         model.release_graph()
         if head is not None:

@@ -136,3 +136,14 @@ def test_global_hooks_see_every_projection():
     # some of its values, in two products one after the other
     for a, b in ((alone, layer.mlp(h)), (hooked[0], layer(torch.arange(2), h, res)[0])):
         assert float((a.double() - b.double()).norm() / b.double().norm()) < 2 * 4 / 127
+
+
+def test_a_shared_projection_stays_shared():
+    model = _model()
+    a, b = (layer.mlp for layer in model.model.layers)
+    b.down_proj = a.down_proj
+    model.model.layers[1].self_attn = model.model.layers[0].self_attn
+    assert qwen3.quantize_linears_(model, lm_head=False) == 5    # q|k|v, o, down once, gate|up twice
+    assert type(a.down_proj) is qwen3.Q8Linear and b.down_proj is a.down_proj
+    assert not any(isinstance(m, nn.Linear) for m in model.modules())
+    _forward(model)
