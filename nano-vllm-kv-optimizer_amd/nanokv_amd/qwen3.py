@@ -696,8 +696,11 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
     After loading the weights and moving the model to its device; a captured decode
     step is captured anew, whatever part of its model is given here.  Projections
     that were replaced or hooked before stay as they are.  A weight that cannot be held
-    in 8 bits (rows that are not a multiple of 16, NaN, infinities) raises ValueError."""
+    in 8 bits (rows that are not a multiple of 16, NaN, infinities) raises ValueError,
+    and so does a projection by itself, which nothing holds here."""
     global _replaced
+    if _own(model, Linear):
+        raise ValueError("quantize_linears_: a projection is replaced in the module that holds it (Q8Linear(weight, bias) makes one)")
     found = [(name, m) for name, m in model.named_modules(remove_duplicate=False) if _own(m, Linear)]
     made = {}                # by the projection: one that several modules share stays shared
     for name, m in found:

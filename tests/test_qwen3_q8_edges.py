@@ -147,3 +147,10 @@ def test_a_shared_projection_stays_shared():
     assert type(a.down_proj) is qwen3.Q8Linear and b.down_proj is a.down_proj
     assert not any(isinstance(m, nn.Linear) for m in model.modules())
     _forward(model)
+
+
+def test_a_projection_by_itself_is_refused():
+    proj = qwen3.Linear(32, 16, bias=False)
+    with pytest.raises(ValueError, match="Q8Linear"):
+        qwen3.quantize_linears_(proj)
+    assert not list(proj.children())
