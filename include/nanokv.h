@@ -665,6 +665,13 @@ int nkv_linear_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale, c
 int64_t nkv_linear_q8_workspace(int m, int n, int k, int gated);
 
 /*
+ * How a product of these sizes runs on the current device (for tests and
+ * profiles): the weight rows of a workgroup's tile | its rows of x << 10 | the
+ * workgroups that k is cut over << 20, or 0 for the kernel of few rows.
+ */
+int nkv_linear_q8_tile(int m, int n, int k, int gated);
+
+/*
  * nkv_quantize_q8 of a few rows x [m][k] (m: at most 8) followed by the product, in
  * one launch (decode and draft steps): the results of the two calls bit for bit.
  * k: at most 12288 for one row, 4096 for more.  Every 16 channels of y quantise the

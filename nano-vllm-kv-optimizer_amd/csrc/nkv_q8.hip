@@ -1223,6 +1223,12 @@ extern "C" int64_t nkv_linear_q8_workspace(int m, int n, int k, int gated) {
   return workspace_ints(m, n, k, gated != 0);
 }
 
+extern "C" int nkv_linear_q8_tile(int m, int n, int k, int gated) {
+  if (m < 1 || n < 1 || k < 16 || m > INT32_MAX - 512 || n > INT32_MAX / 2 - 512 || k > kMaxDepth) return 0;
+  const Plan plan = plan_product(m, n, k, gated != 0);
+  return plan.few ? 0 : kShapes[plan.shape].channels | kShapes[plan.shape].rows << 10 | plan.parts << 20;
+}
+
 extern "C" int nkv_linear_q8(const int8_t* weight, const float* w_scale, const int8_t* x, const float* x_scale,
                              const uint16_t* bias, uint16_t* y, int m, int n, int k, int32_t* workspace,
                              void* stream) {

@@ -85,6 +85,7 @@ SIGNATURES = {
     "nkv_rmsnorm_q8": (_I, [_P, _P, _P, _F, _P, _P, _P, _I, _I, _P]),
     "nkv_linear_q8": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "nkv_linear_q8_workspace": (_I64, [_I, _I, _I, _I]),
+    "nkv_linear_q8_tile": (_I, [_I, _I, _I, _I]),
     "nkv_linear_silu_mul_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "nkv_gemv_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
     "nkv_gemv_silu_mul_q8": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),

@@ -160,3 +160,40 @@ def test_products_that_no_launch_holds_are_refused():
     assert b"aligned" in lib.nkv_last_error()
     assert lib.nkv_gemv_q8(w + 8, sw, x, None, y, 1, 2 ** 29, 16, None) == _lib.NKV_ERR_ARG    # resident workgroups
     assert b"aligned" in lib.nkv_last_error()
+
+
+# -- the tiles of products -----------------------------------------------------------
+# (m, n, gated) -> (weight rows, rows of x) of a tile: each of them, ragged on both sides
+TILES = [(2079, 5395, 0, (256, 256)), (1549, 5819, 0, (192, 256)), (1287, 5409, 0, (160, 256)), (5003, 777, 0, (128, 256)),
+         (327, 5517, 0, (128, 128)), (301, 6143, 0, (128, 64)), (5657, 133, 0, (128, 64)), (4495, 65, 0, (64, 64)),
+         (173, 1, 0, (64, 32)), (1073, 4915, 1, (256, 256)), (649, 5513, 1, (192, 256)), (323, 5511, 1, (128, 256)),
+         (143, 5453, 1, (128, 128)), (5657, 65, 1, (128, 64)), (33, 4687, 1, (64, 64)), (209, 5, 1, (64, 32))]
+# the same with a k that is cut over workgroups
+CUT_TILES = [(65, 3225, 11200, 0, (128, 128)), (87, 3, 11200, 0, (64, 64)), (65, 1365, 11200, 1, (128, 128)),
+             (163, 5, 11200, 1, (64, 64))]
+
+
+def tile_of(m, n, k, gated):
+    """(weight rows, rows of x), and the workgroups that k is cut over; (0, 0), 0: the kernel of few rows."""
+    t = _lib.load().nkv_linear_q8_tile(m, n, k, gated)
+    return (t & 1023, t >> 10 & 1023), t >> 20
+
+
+def test_every_tile_has_its_sizes():
+    """What the GPU tests go over is every tile that a product takes (a table that is tuned
+    anew says so here)."""
+    for m, n, gated, tile in TILES:
+        for k in (144, 1040):
+            assert tile_of(m, n, k, gated) == tile_of(m, (n + 3) // 4 * 4, k, gated) == (tile, 1), (m, n, k, gated)
+    for m, n, k, gated, tile in CUT_TILES:
+        assert tile_of(m, n, k, gated)[0] == tile and tile_of(m, n, k, gated)[1] > 1, (m, n, k, gated)
+    listed = ({(g, t, False) for _, _, g, t in TILES} | {(g, t, True) for _, _, _, g, t in CUT_TILES}
+              | {(g, (0, 0), False) for g in (0, 1)})
+    import random
+    rng = random.Random(5)
+    for _ in range(20000):
+        m, n = round(2 ** rng.uniform(0, 13)), round(2 ** rng.uniform(0, 15))
+        k, g = 16 * round(2 ** rng.uniform(0, 11)), rng.randint(0, 1)
+        tile, parts = tile_of(m, n, k, g)
+        assert (g, tile, parts > 1) in listed, (m, n, k, g)
+    assert tile_of(0, 8, 16, 0) == tile_of(8, 0, 16, 0) == tile_of(8, 8, 0, 1) == tile_of(100, 8, 131072, 0) == ((0, 0), 0)
