@@ -611,7 +611,7 @@ int nkv_norm_gemv_silu_mul(const uint16_t* gate_up_weight, const uint16_t* x, co
  * nanovllm/layers/linear.py, are bf16).  A row y[n] is held as int8 codes
  * and one fp32 scale: with a = max |y|,
  *   q = rne(y * 127 / a), s = a / 127, y ~ q * s
- * (exactly for bf16 rows; behind a norm a value within 2^-15 of half way
+ * (exactly for bf16 rows; behind a norm a value within 2^-14 of half way
  * between two codes may go to either).
  * A row with a < 2^-119 is zero (s = 0, q = 0); one with a NaN or an infinity
  * has s = NaN and q = 0, so that what is computed from it is NaN.  A weight

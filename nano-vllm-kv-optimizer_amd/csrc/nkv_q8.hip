@@ -36,18 +36,23 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // the infinities and NaN on top.
 __device__ __forceinline__ uint32_t mag(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-// 4 codes.  v * inv is off by less than 127 * 2^-23 < 2^-16 (inv and the product are rounded
-// once each, no fma).  bf16 v and peak put v * 127 / peak half way between two codes or more than
-// 2^-16 off (all pairs of mantissas were tried), so the product is rounded to 2^-15 first --
-// the sum with 1.5 * 2^8, whose last bit that is -- which makes a half way one exact again:
-// the codes are rne(v * 127 / peak) itself.  (Rounded at once, 14 of the 254 half way pairs
-// of mantissas went to the other code.)
-// Then the low byte of a sum in [2^23, 2^24), rounded to nearest even; NaN gives 0.
+// 4 codes: v * inv rounded to whole numbers, to nearest even, in the low byte of its sum with
+// 1.5 * 2^23; NaN gives 0.  v * inv is off by less than 127 * 2^-23 < 2^-16 (inv and the product
+// are rounded once each, no fma).  bf16 v and peak put v * 127 / peak half way between two codes or
+// more than 2^-16 off (all pairs of mantissas were tried), so with EXACT (rows that are bf16) the
+// product is rounded to 2^-15 first -- the sum with 1.5 * 2^8, whose last bit that is -- which
+// makes a half way one exact again: the codes are rne(v * 127 / peak) itself.  (Rounded at once,
+// 14 of the 254 half way pairs of mantissas went to the other code.)  Behind a norm v is fp32,
+// half way means nothing, and the step would only move small values (4096 x 2560: 140 codes
+// off the nearest against 10).
+template <bool EXACT>
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
 #pragma clang fp contract(off)
-  constexpr float kSnap = 384.0f, kMagic = 12582912.0f - kSnap;
-  const uint32_t x = __float_as_uint((a * inv + kSnap) + kMagic), y = __float_as_uint((b * inv + kSnap) + kMagic);
-  const uint32_t z = __float_as_uint((c * inv + kSnap) + kMagic), w = __float_as_uint((d * inv + kSnap) + kMagic);
+  constexpr float kSnap = EXACT ? 384.0f : 0.0f, kMagic = 12582912.0f - kSnap;
+  float p[4] = {a * inv, b * inv, c * inv, d * inv};
+  if constexpr (EXACT) p[0] += kSnap, p[1] += kSnap, p[2] += kSnap, p[3] += kSnap;
+  const uint32_t x = __float_as_uint(p[0] + kMagic), y = __float_as_uint(p[1] + kMagic);
+  const uint32_t z = __float_as_uint(p[2] + kMagic), w = __float_as_uint(p[3] + kMagic);
   return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
 }
 
@@ -147,7 +152,7 @@ __global__ __launch_bounds__(row_threads(WPR)) void rows_q8_kernel(const uint16_
   for (int j = 0; j < NCH; ++j) {
     const int c = t + j * kLanes;
     if (c < nc)
-      qr[c] = make_uint2(codes4(v[j][0], v[j][1], v[j][2], v[j][3], rs.inv), codes4(v[j][4], v[j][5], v[j][6], v[j][7], rs.inv));
+      qr[c] = make_uint2(codes4<!NORM>(v[j][0], v[j][1], v[j][2], v[j][3], rs.inv), codes4<!NORM>(v[j][4], v[j][5], v[j][6], v[j][7], rs.inv));
   }
   if (t == 0) scale[row] = rs.scale;
 }
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(64 * kFewWaves, NCH == 0 ? 1 : NCH <= 5 ? 3 : 2) vo
         const int c = lane + kWave * j;                // 8 codes: half of 16-byte unit (c / 2) % 8 of piece c / 16
         if (c < nc)
           *reinterpret_cast<uint2*>(s_rows + (c >> 4) * kDraftRows * kTileK + row * kTileK + 16 * (((c >> 1) & 7) ^ swizzle(row)) + 8 * (c & 1)) =
-              make_uint2(codes4(v[j][0], v[j][1], v[j][2], v[j][3], sc.inv), codes4(v[j][4], v[j][5], v[j][6], v[j][7], sc.inv));
+              make_uint2(codes4<!NORM>(v[j][0], v[j][1], v[j][2], v[j][3], sc.inv), codes4<!NORM>(v[j][4], v[j][5], v[j][6], v[j][7], sc.inv));
       }
     }
     lds_barrier();
@@ -867,7 +872,7 @@ __global__ __launch_bounds__(kTokenThreads, token_waves(NCH, SILU)) void token_k
     const int c = threadIdx.x + j * kTokenThreads;
     if (XC * kTokenThreads == NCH * kWave * 2 || c < NCH * kWave * 2)
       reinterpret_cast<uint2*>(s_codes)[c] =
-          c < nc ? make_uint2(codes4(v[j][0], v[j][1], v[j][2], v[j][3], rs.inv), codes4(v[j][4], v[j][5], v[j][6], v[j][7], rs.inv))
+          c < nc ? make_uint2(codes4<!NORM>(v[j][0], v[j][1], v[j][2], v[j][3], rs.inv), codes4<!NORM>(v[j][4], v[j][5], v[j][6], v[j][7], rs.inv))
                  : make_uint2(0u, 0u);
   }
   lds_barrier();

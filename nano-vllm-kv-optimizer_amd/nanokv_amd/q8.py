@@ -48,14 +48,15 @@ class Q8(NamedTuple):
 SNAP, MAGIC = 1.5 * 2.0 ** 8, 1.5 * 2.0 ** 23    # sums with them are rounded to 2^-15, to whole numbers
 
 
-def _quantize_formula(y: torch.Tensor) -> Q8:
+def _quantize_formula(y: torch.Tensor, exact: bool = True) -> Q8:
     top = y.abs().amax(dim=-1)      # (NaN where the row holds one)
     zero, odd = top < TINY, ~top.isfinite()
     none = torch.zeros_like(top)
-    # the kernels' roundings, so their bits: a true division (127.0 / top is a reciprocal and
-    # a product), and y * inv to 2^-15 before whole numbers, which makes ties exact
+    # the kernels' roundings, so their bits: a true division (127.0 / top is a reciprocal and a
+    # product), and with `exact` y * inv to 2^-15 before whole numbers, which makes ties of bf16 exact
     inv = torch.where(zero | odd, none, torch.full_like(top, 127.0) / top)
-    code = ((y * inv.unsqueeze(-1) + SNAP) + (MAGIC - SNAP)) - MAGIC
+    code = y * inv.unsqueeze(-1)
+    code = ((code + SNAP) + (MAGIC - SNAP)) - MAGIC if exact else torch.round(code)
     q = torch.where(odd.unsqueeze(-1), none.unsqueeze(-1), code).to(torch.int8)
     return Q8(q, torch.where(odd, torch.full_like(top, float("nan")), torch.where(zero, none, top / 127.0)))
 
@@ -64,7 +65,7 @@ def _norm_formula(x, weight, eps, residual):
     t = x.float() if residual is None else x.float() + residual.float()
     mean = t.pow(2).mean(dim=-1)
     r = torch.rsqrt(mean + eps)
-    codes = _quantize_formula(t * weight.float())       # (they do not depend on r)
+    codes = _quantize_formula(t * weight.float(), exact=False)      # (they do not depend on r)
     top = (t * weight.float()).abs().amax(dim=-1) * r
     zero = (codes.scale == 0) | (top < TINY)
     odd = ~(mean.isfinite() & top.isfinite())           # NaN where the squares pass fp32's range too

@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from tests.test_q8_edges import check_gradients_are_refused, check_nothing_is_broadcast, every_value_and_peak
+from tests.test_q8_edges import (check_codes_behind_a_norm, check_gradients_are_refused, check_nothing_is_broadcast,
+                                 every_value_and_peak)
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,7 @@ def test_operands_that_ask_for_a_gradient_are_refused():
 
 def test_nothing_is_broadcast():
     check_nothing_is_broadcast("cuda")
+
+
+def test_codes_behind_a_norm():
+    check_codes_behind_a_norm("cuda")

@@ -38,6 +38,24 @@ def test_codes_are_the_nearest_with_ties_to_even():
     assert torch.equal(big.q.long(), codes)
 
 
+def check_codes_behind_a_norm(device):
+    """A code is the nearest integer up to the roundings in front of it, relative to the value:
+    t * w, its peak's, 127 / a and the product with it, u = 2^-24 each; with a residual t and its
+    peak's t too.  (Not 2^-16 absolute, which moves ten times as many small values.)"""
+    g = torch.Generator(device=device).manual_seed(7)
+    x, r = (torch.randn(400, 2560, generator=g, device=device).bfloat16() for _ in range(2))
+    w = (1 + 0.2 * torch.randn(2560, generator=g, device=device)).bfloat16()
+    for res, roundings in ((None, 4), (r, 6)):
+        t, _ = rmsnorm_q8(x, w, 1e-6, res)
+        y = (x.double() if res is None else x.double() + r.double()) * w.double()
+        y *= 127 / y.abs().amax(-1, keepdim=True)
+        assert bool(((t.q.double() - y).abs() <= 0.5 + y.abs() * roundings * 2.0 ** -24 * (1 + 2.0 ** -20)).all())
+
+
+def test_codes_behind_a_norm():
+    check_codes_behind_a_norm("cpu")
+
+
 # -- gradients -----------------------------------------------------------------------
 def gradient_calls(device="cpu"):
     """(name, call, the operands it takes) with every operand that a gradient could be asked of."""
