@@ -620,7 +620,11 @@ int nkv_norm_gemv_silu_mul(const uint16_t* gate_up_weight, const uint16_t* x, co
  *   Y[m][c] = (sum_k x.q[m][k] w.q[c][k]) * x.s[m] * w.s[c] (+ bias[c]).
  * bf16 tensors, dense rows unless said; matrices of rows 16-byte aligned; row
  * lengths (n of rows, k of products) are multiples of 16; outputs overlap no
- * input and not each other.  Each call is one launch on `stream`.
+ * input (unless said) and not each other.  A call is one launch on `stream`; a product
+ * whose k is cut over workgroups (nkv_linear_q8) is two, and rows past 2^21 of
+ * nkv_quantize_q8 and nkv_rmsnorm_q8 take a launch for every 2^21.  Sizes that no
+ * launch holds (2^32 threads: from 2^28 channels of 2 to 32 rows on, about 5e8 rows of
+ * few channels) are NKV_ERR_ARG.
  * ---------------------------------------------------------------------- */
 
 /*
@@ -637,8 +641,8 @@ int nkv_dequantize_q8(const int8_t* q, const float* scale, uint16_t* out, int ro
  * and scales and not rounded before: t = x (+ residual) in fp32;
  * residual_out = bf16(t) (if non-NULL; it may be x or residual itself); the
  * row t * rsqrt(mean(t^2) + eps) * weight is quantised.  A row whose largest
- * |t * weight| is below 2^-119 is zero too; one whose sum of squares passes
- * fp32's range is NaN.  n: at most 32768.
+ * |t * weight| is below 2^-119 is zero too; one whose sum of squares or largest
+ * |t * weight| passes fp32's range is NaN.  n: at most 32768.
  */
 int nkv_rmsnorm_q8(const uint16_t* x, const uint16_t* residual, const uint16_t* weight, float eps, int8_t* q,
                    float* scale, uint16_t* residual_out, int rows, int n, void* stream);

@@ -68,7 +68,7 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {
 }
 
 // The same for a row t * r, r = rsqrt(mean(t^2) + eps), given the largest |t w|:
-// the codes do not depend on r.  NaN also where the squares pass fp32's range.
+// the codes do not depend on r.  NaN also where the squares or |t w| pass fp32's range.
 __device__ __forceinline__ RowScale norm_row_scale(uint32_t top, float ss, int n, float eps) {
   RowScale rs = row_scale(top);
   const float r = rsqrtf(ss / static_cast<float>(n) + eps);
@@ -82,11 +82,12 @@ __device__ __forceinline__ RowScale norm_row_scale(uint32_t top, float ss, int n
 // WPR wavefronts a row, NCH 8-element chunks a lane, held in registers between the
 // pass that finds the row's peak (and sum of squares) and the one that writes its
 // codes: every byte is moved once.  Bound by HBM for many rows (quantise 4096 x
-// 9728 22.1 us, 5.4 TB/s; norm with residual 50.9 us, 5.5 TB/s; a large copy runs at
+// 9728 22.1 us, 5.4 TB/s; norm with residual 50.9-56.9 us, 4.9-5.5 TB/s; a large copy runs at
 // 5.1), by the launch for few (1 x 2560 2.5 and 3.2 us in a captured chain).  Rows
 // of up to 512 take a wavefront each, no barrier (4096 x 512 5.0 -> 3.9 us, 16384
-// x 128 12 -> 5.8); longer ones as many wavefronts as leave no lane idle (a fixed
-// four: 1 x 2560 3.0 us, 4096 x 9728 26.5).  (x, res and res_out may be one buffer.)
+// x 128 12 -> 5.8); longer ones more, in the steps of launch_rows (a fixed four: 1 x
+// 2560 3.0 us, 4096 x 9728 26.5; just above a step up to half of the lanes have no
+// chunk).  (x, res and res_out may be one buffer.)
 constexpr int row_threads(int wpr) { return kWave * (wpr == 1 ? 4 : wpr); }
 template <int WPR, int NCH, bool NORM>
 __global__ __launch_bounds__(row_threads(WPR)) void rows_q8_kernel(const uint16_t* x, int64_t x_stride,
@@ -218,9 +219,10 @@ __device__ __forceinline__ void lds_barrier() {
 // registers, kDeep pieces in flight, turned through the wavefront's own LDS rows
 // into the matrix instruction's operands (no barrier), and the partial sums are
 // joined through LDS at the end: exact, being integers.  In a captured chain over
-// cold weights (us): 6 x 2560 -> 6144 6.1, 6 x 9728 -> 2560 8.4 (3.0 TB/s), gate|up of
-// 6 rows 12.9 (3.9 TB/s), 37 x 9728 -> 2560 13.3, where reading the rows, once a
-// workgroup, counts as much as the weight.  Operands read straight from memory as
+// 512 MB of weights and more (us): 6 x 2560 -> 6144 8.8, 6 x 9728 -> 2560 11.1 (2.2 TB/s), gate|up of
+// 6 rows 15.9 (3.1 TB/s), 37 x 9728 -> 2560 16.7, where reading the rows, once a
+// workgroup, counts as much as the weight.  Over 380 to 600 MB, in part from the 256 MB cache, 6.1, 8.4,
+// 12.9 and 13.3, and what was compared there: operands read straight from memory as
 // the matrix instruction wants them (64 bytes of 16 rows a load) took 11.5, 16.8 and 20.9
 // for the last three; refills under a branch made the compiler wait for every
 // load (8.4 -> 15.1); 8 wavefronts a workgroup: gate|up 15.8.
@@ -228,9 +230,9 @@ __device__ __forceinline__ void lds_barrier() {
 // NCH > 0: up to 8 rows that are still bf16 (p.x and p.sx are not read), of up to
 // 512 NCH elements: every workgroup normalises (NORM) and quantises them itself, a
 // wavefront one or two rows, while its first weights are in flight, and keeps their codes
-// in LDS, in pieces like the weight's.  In a captured chain (us, with the rows' own launch
-// before the product / in one): 4 x 2560 -> 6144 with a norm 8.8 / 7.8, 4 x 4096 -> 2560 7.4 / 5.9,
-// 4 x 1024 -> 1024 5.3 / 3.6, gate|up of 9728 for 6 rows 15.4 / 14.7, with a norm 15.7 / 16.9 (what every
+// in LDS, in pieces like the weight's.  Over cold weights (us, with the rows' own launch
+// before the product / in one): 4 x 2560 -> 6144 with a norm 9.0 / 7.9, 4 x 4096 -> 2560 8.2 / 6.5,
+// 4 x 1024 -> 1024 5.7 / 3.7, gate|up of 9728 for 6 rows 16.0 / 15.5, with a norm 16.4 / 17.4 (what every
 // workgroup does again).  All first weights fetched before a norm spilled registers
 // (gate|up for 4 rows 18.0 against 15.2).
 constexpr int kFewWaves = 4;
@@ -925,7 +927,8 @@ void launch_rows(const uint16_t* x, int64_t x_stride, const uint16_t* res, const
   };
   // many rows: half the wavefronts a row, two chunks in flight a lane (us, 4096 rows of 2560: 16.4
   // against 17.2 with a norm, 8.7 / 9.6 without; of 4096: 22.6 / 24.0, 11.6 / 12.6); few: one chunk
-  // a lane (1 x 2560: 3.2 against 3.5 and 2.5 / 3.0)
+  // a lane (1 x 2560: 3.2 against 3.5 and 2.5 / 3.0).  The steps of n: powers of two, and the widths
+  // that were measured (2560, 9728)
   const bool many = rows >= 1024;
   if (n <= 512) go(rows_q8_kernel<1, 1, NORM>, 1);
   else if (n <= 1024) many ? go(rows_q8_kernel<1, 2, NORM>, 1) : go(rows_q8_kernel<2, 1, NORM>, 2);

@@ -10,7 +10,8 @@ the RMSNorm (+ residual add) whose output is held in 8 bits; the
 
 A row whose largest magnitude is below 2^-119 is zero; one that holds a NaN or
 an infinity has the scale NaN and the codes 0, so what is computed from it is
-NaN.
+NaN.  (Behind a norm also one whose sum of squares or largest |t * weight|, before
+the root's division, passes fp32's range.)
 
 On the GPU the operands are bf16 and the work is this library's kernels (no
 fallback: the library must load); one row (a decode token) and up to 8 (a draft,
@@ -216,10 +217,10 @@ def _one_launch(m: int, n: int, k: int, norm: bool) -> bool:
 
     Several rows (one or two a wavefront) are quantised again by every workgroup,
     16 channels each, while its first weights are on their way: more of that, or a
-    norm with its residual, takes longer than a launch of the rows' own (us, two launches /
-    one: 2 to 4 x 4096 -> 2560 7.4 / 5.9, gate|up of 9728 for 6 rows 15.4 / 14.7, 6 x 2560 -> 24576
-    15.9 / 16.9; with a norm 4 x 2560 -> 6144 8.8 / 7.8, gate|up of 9728 for 4 rows 15.6 / 15.2,
-    for 6 15.7 / 16.9).  Eagerly a launch and its buffer are 5 us of host time too."""
+    norm with its residual, takes longer than a launch of the rows' own (us over cold weights,
+    two launches / one: 2 to 4 x 4096 -> 2560 8.2 / 6.5, gate|up of 9728 for 6 rows 16.0 / 15.5,
+    6 x 2560 -> 24576 17.2 / 17.9; with a norm 4 x 2560 -> 6144 9.0 / 7.9, 6 rows 9.2 / 9.4, gate|up of
+    9728 for 2 rows 16.0 / 14.2, 4 rows 16.2 / 15.7, 6 rows 16.4 / 17.4).  Eagerly a launch and its buffer are 5 us of host time too."""
     if m == 1:
         return k <= TOKEN_ROW and n > 0
     return 0 < m <= DRAFT_ROWS and k <= DRAFT_ROW and 0 < (m + 3) // 4 * n * k <= (1 << 25 if norm else 1 << 26)

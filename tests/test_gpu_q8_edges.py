@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from tests.test_q8_edges import (check_codes_behind_a_norm, check_gradients_are_refused, check_nothing_is_broadcast,
-                                 every_value_and_peak)
+from tests.test_q8_edges import (check_a_norm_past_the_range, check_codes_behind_a_norm, check_gradients_are_refused,
+                                 check_nothing_is_broadcast, every_value_and_peak)
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,7 @@ def test_nothing_is_broadcast():
 
 def test_codes_behind_a_norm():
     check_codes_behind_a_norm("cuda")
+
+
+def test_a_norm_past_the_range():
+    check_a_norm_past_the_range("cuda")

@@ -56,6 +56,20 @@ def test_codes_behind_a_norm():
     check_codes_behind_a_norm("cpu")
 
 
+def check_a_norm_past_the_range(device):
+    """|t * weight| is held in fp32 before the root's division: past its range the row is NaN."""
+    x = torch.full((2, 32), 100.0).bfloat16().to(device)
+    x[1] = 1
+    w = torch.full((32,), 2.0 ** 127).bfloat16().to(device)
+    t, _ = rmsnorm_q8(x, w, 1e-6)
+    assert bool(t.scale[0].isnan()) and not bool(t.q[0].any())
+    assert abs(float(t.scale[1]) * 127 / 2.0 ** 127 - 1) < 1e-5 and bool((t.q[1] == 127).all())
+
+
+def test_a_norm_past_the_range():
+    check_a_norm_past_the_range("cpu")
+
+
 # -- gradients -----------------------------------------------------------------------
 def gradient_calls(device="cpu"):
     """(name, call, the operands it takes) with every operand that a gradient could be asked of."""

@@ -154,3 +154,13 @@ def test_a_projection_by_itself_is_refused():
     with pytest.raises(ValueError, match="Q8Linear"):
         qwen3.quantize_linears_(proj)
     assert not list(proj.children())
+
+
+def test_weights_are_off_by_half_a_step():
+    model = _model()
+    weights = {n: m.weight.double() for n, m in model.named_modules() if isinstance(m, qwen3.Linear)}
+    qwen3.quantize_linears_(model)
+    for name, w in weights.items():
+        q, scale = model.get_submodule(name).weight
+        # the nearest code, and the scale's own rounding: 127 * 2^-24 of a step
+        assert bool(((q.double() * scale.double()[:, None] - w).abs() <= (0.5 + 127 * 2.0 ** -24) * scale.double()[:, None]).all())
