@@ -220,7 +220,8 @@ def _one_launch(m: int, n: int, k: int, norm: bool) -> bool:
     norm with its residual, takes longer than a launch of the rows' own (us over cold weights,
     two launches / one: 2 to 4 x 4096 -> 2560 8.2 / 6.5, gate|up of 9728 for 6 rows 16.0 / 15.5,
     6 x 2560 -> 24576 17.2 / 17.9; with a norm 4 x 2560 -> 6144 9.0 / 7.9, 6 rows 9.2 / 9.4, gate|up of
-    9728 for 2 rows 16.0 / 14.2, 4 rows 16.2 / 15.7, 6 rows 16.4 / 17.4).  Eagerly a launch and its buffer are 5 us of host time too."""
+    9728 for 2 rows 16.0 / 14.2, 4 rows 16.2 / 15.7, 6 rows 16.4 / 17.4).  Eagerly a launch and its
+    buffer are 5 us of host time too."""
     if m == 1:
         return k <= TOKEN_ROW and n > 0
     return 0 < m <= DRAFT_ROWS and k <= DRAFT_ROW and 0 < (m + 3) // 4 * n * k <= (1 << 25 if norm else 1 << 26)

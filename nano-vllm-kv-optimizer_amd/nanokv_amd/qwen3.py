@@ -700,7 +700,8 @@ def quantize_linears_(model: nn.Module, lm_head: bool = True) -> int:
     and so does a projection by itself, which nothing holds here."""
     global _replaced
     if _own(model, Linear):
-        raise ValueError("quantize_linears_: a projection is replaced in the module that holds it (Q8Linear(weight, bias) makes one)")
+        raise ValueError("quantize_linears_: a projection is replaced in the module that holds it "
+                         "(Q8Linear(weight, bias) makes one)")
     found = [(name, m) for name, m in model.named_modules(remove_duplicate=False) if _own(m, Linear)]
     made = {}                # by the projection: one that several modules share stays shared
     for name, m in found:
