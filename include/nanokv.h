@@ -699,6 +699,77 @@ int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale
                               const uint16_t* residual, const uint16_t* norm_weight, float eps, uint16_t* y,
                               uint16_t* residual_out, int m, int intermediate, int k, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Dense attention over a paged cache (the reference's paged path,
+ * nanovllm/layers/attention.py:12-44, :100-119, which leaves it to other
+ * libraries), and log probabilities.
+ *
+ * The cache of one layer: k, v [pages][Hkv][page_size][D], bf16, or int8 codes
+ * with k_scale, v_scale fp32 [pages][Hkv][page_size] (dense); NULL scales: bf16.
+ * page_stride, head_stride and token_stride are the elements from page to page,
+ * head to head and token to token (rows on 16-byte boundaries, at most 64 MiB
+ * from token to token), so other orders of the first three dimensions are read in place.
+ * Slot s is token s % page_size of page s / page_size.
+ * Constraints: D 64 or 128; page_size a power of two from 16 to 4096.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * Rows of heads into the cache, and the rotated queries out
+ * (store_kvcache of nanovllm/layers/attention.py:12-44 with q_norm, k_norm and
+ * rotary_emb of nanovllm/models/qwen3.py:99-110 in the same pass).
+ *
+ * Row t's queries q_rows + t q_stride [num_heads][D], keys and values likewise
+ * (of one fused projection output or apart).  Per head of q and k: x rsqrt(mean(x^2) + eps) *
+ * weight [D] (q_weight / k_weight NULL: none); then dims [0, rotary_dim) are
+ * rotated by cos/sin_table [max_position][rotary_dim / 2] at positions[t]
+ * (clamped to the table), pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+ * interleaved; fp32 throughout, rounded once.  q goes to q_out
+ * [rows][num_heads][D]; k and v to slot slots[t] (bf16, or codes
+ * rne(y 127 / a) with scale a / 127, a = max |y|; a < 2^-119: zeros; NaN or
+ * infinite rows: scale NaN).  Slots outside the cache store nothing.  The
+ * slots of one call are distinct.  num_heads 0: keys and values only.
+ * Constraints: rotary_dim a multiple of 16 up to D (0: no rotation); 16-byte
+ * aligned rows, weights and tables.
+ */
+int nkv_paged_append(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride, int64_t head_stride,
+                     int64_t token_stride, int pages, int num_kv_heads, int page_size, int head_dim,
+                     const uint16_t* q_rows, int64_t q_stride, const uint16_t* k_rows, int64_t k_stride,
+                     const uint16_t* v_rows, int64_t v_stride, int rows, int num_heads, const int32_t* slots,
+                     const int64_t* positions, const float* cos_table, const float* sin_table, int max_position,
+                     int rotary_dim, int interleaved, const uint16_t* q_weight, const uint16_t* k_weight, float eps,
+                     uint16_t* q_out, void* stream);
+
+/* Rows at slots as bf16: k_out, v_out [rows][Hkv][D] (zeros where a slot lies outside the cache). */
+int nkv_paged_read(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride, int64_t head_stride,
+                   int64_t token_stride, int pages, int num_kv_heads, int page_size, int head_dim,
+                   const int32_t* slots, int rows, uint16_t* k_out, uint16_t* v_out, void* stream);
+
+/*
+ * Rows from slots src to slots dst, as they lie in the cache, all read before any is
+ * written (an accepted path of a drafted tree closes up in place).  A pair with a slot
+ * outside the cache moves nothing; the dst of one call are distinct.
+ * workspace: nkv_paged_move_workspace(Hkv, D, int8, rows) bytes, 16-byte aligned.
+ */
+int nkv_paged_move(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride, int64_t head_stride,
+                   int64_t token_stride, int pages, int num_kv_heads, int page_size, int head_dim, const int32_t* src,
+                   const int32_t* dst, int rows, void* workspace, void* stream);
+int64_t nkv_paged_move_workspace(int num_kv_heads, int head_dim, int int8, int rows);
+
+/*
+ * Log probabilities of rows of logits [rows][vocab] (kind 0: fp32, 1: bf16, 2:
+ * fp16; row_stride elements from row to row): logprob[t] of tokens[t] (NaN for
+ * a token outside [0, vocab)), entropy[t] of the distribution, and the top most
+ * likely (top_logprobs, top_ids [rows][top]: value descending, NaN above all,
+ * ties to the lower id).  -inf logits have no probability; a row of -inf alone,
+ * or with a NaN or +inf, has NaN for all of its numbers.  fp32 throughout.
+ * workspace: nkv_token_logprobs_workspace(rows, vocab, top) floats (NULL where that is 0).
+ * Constraints: top <= min(64, vocab).
+ */
+int nkv_token_logprobs(const void* logits, int kind, int64_t row_stride, int rows, int vocab, const int64_t* tokens,
+                       int top, float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids,
+                       float* workspace, void* stream);
+int64_t nkv_token_logprobs_workspace(int rows, int vocab, int top);
+
 #ifdef __cplusplus
 }
 #endif

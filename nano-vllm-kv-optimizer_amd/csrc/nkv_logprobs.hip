@@ -1,0 +1,469 @@
+// Log probabilities of given tokens, the entropy of their distribution and its
+// most likely alternatives, from rows of logits, in one pass over each row.
+//
+// With m the row's maximum, s the sum of e^(x - m) over all elements but the
+// maximum, and w the sum of (m - x) e^(x - m):
+//   log Z = m + log1p(s),  log p(t) = (x_t - m) - log1p(s),
+//   H = log1p(s) + w / (1 + s).
+// The maximum's own term, 1, stays out of s: the sum keeps the digits that a
+// confident row's entropy and log probability are made of (1 + 1e-9 is 1).
+// Pieces (m, s, w) join exactly: with d = m1 - m2 >= 0 and r = e^-d,
+//   s = s1 + r (s2 + 1),  w = w1 + r (w2 + d (s2 + 1)).
+//
+// Work split: a wavefront takes a run of its row; its maximum is the same in
+// all lanes and moves rarely, so an element costs a subtraction, a product, an exp2, two
+// additions and the comparisons.  Alternatives: an element that beats the
+// wavefront's n-th best so far goes to its list of up to 256 in LDS; a full list is
+// cut to its best n, which raises the bar.  The bar starts at the n-th largest of
+// the lanes' maxima over the first piece, so few elements ever pass it.  Order:
+// value descending (NaN above all), index ascending.  Bound by reading the
+// logits once, or by the launches (one row).
+#include <algorithm>
+
+#include "nkv_common.h"
+
+namespace nkv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kList = 256;       // candidates a wavefront keeps at most
+constexpr int kMaxTop = 64;      // alternatives: one a lane in the final order
+constexpr int kEach = 16;        // elements a lane takes per iteration
+constexpr int kMaxSplits = 64;   // pieces of a row
+constexpr float kLog2e = 1.44269504088896340736f;
+
+enum Kind { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+struct Params {
+  const char* x;
+  int64_t stride;          // elements from row to row
+  int rows, vocab, top, splits;
+  const int64_t* tokens;
+  float* logprob;
+  float* entropy;
+  float* top_lp;           // [rows][top]
+  int64_t* top_ids;
+  float* ws;               // [rows][splits][4 + 2 top]: m, s, w, entries, then their keys and ids
+};
+
+template <int K> constexpr int kBytes = K == kF32 ? 4 : 2;
+
+template <int K>
+__device__ __forceinline__ float element(const char* row, int64_t i) {
+  if (K == kF32) return reinterpret_cast<const float*>(row)[i];
+  const uint16_t b = reinterpret_cast<const uint16_t*>(row)[i];
+  return K == kBf16 ? bf16_to_f32(b) : f16_bits_to_f32(b);
+}
+
+struct Stat { float m, s, w; };
+
+__device__ __forceinline__ float exp_neg(float y) { return __builtin_amdgcn_exp2f(y * -kLog2e); }
+
+__device__ __forceinline__ Stat join(Stat a, Stat b) {
+  if (b.m > a.m) { const Stat t = a; a = b; b = t; }
+  if (b.m == -INFINITY) return Stat{a.m, a.s + b.s, a.w + b.w};   // nothing, or a NaN that stays
+  // (past 200 r is 0; d itself, 3e38 behind rows masked with the lowest value, times a sum would be infinite)
+  const float d = fminf(a.m - b.m, 200.0f), r = exp_neg(d);
+  return Stat{a.m, a.s + r * (b.s + 1.0f), a.w + r * (b.w + d * (b.s + 1.0f))};
+}
+
+__device__ __forceinline__ int count(uint64_t mask) { return __popcll(mask); }
+__device__ __forceinline__ int below(uint64_t mask) {   // set bits under this lane's
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+
+// A wavefront's candidates: (key, id) in LDS, and the bar that a new one has to
+// beat: a larger key, or the same with a lower id.
+struct List {
+  uint32_t* keys;
+  int* ids;
+  int cnt, top;
+  uint32_t bar;
+  int bar_id;
+
+  __device__ __forceinline__ bool beats(uint32_t key, int id) const { return key > bar || (key == bar && id < bar_id); }
+
+  // The best `top` of up to four candidates a lane (an empty one has key 0,
+  // below every element's): they become the list, the last of them the bar.
+  __device__ void keep_best(const uint32_t (&k)[4], const int (&id)[4], int have) {
+    auto above = [&](auto&& f) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n += count(__ballot(f(k[i], id[i])));
+      return n;
+    };
+    uint32_t t = 1;      // the top-th largest key, bit by bit (all candidates when there are no more)
+    int last = INT32_MAX;
+    if (have > top) {
+      t = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        if (above([&](uint32_t a, int) { return a >= c; }) >= top) t = c;
+      }
+      const int more = above([&](uint32_t a, int) { return a > t; });
+      const int equal = above([&](uint32_t a, int) { return a == t; });
+      if (more + equal > top) {   // of equal ones the lowest ids
+        last = 0;
+        for (int bit = 30; bit >= 0; --bit) {
+          const int c = last | (1 << bit);
+          // ids below c are too few: the (top - more)-th lowest is c or more
+          if (above([&](uint32_t a, int i) { return a == t && i < c; }) < top - more) last = c;
+        }
+      }
+      bar = t;
+      bar_id = last;
+    }
+    wave_lds_sync();   // (the list has been read)
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool stays = k[i] > t || (k[i] == t && id[i] <= last);
+      const uint64_t mask = __ballot(stays);
+      if (stays) {
+        keys[n + below(mask)] = k[i];
+        ids[n + below(mask)] = id[i];
+      }
+      n += count(mask);
+    }
+    cnt = n;
+    wave_lds_sync();
+  }
+  __device__ void cut(int lane) {
+    wave_lds_sync();
+    uint32_t k[4];
+    int id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = i * kWave + lane < cnt;
+      k[i] = in ? keys[i * kWave + lane] : 0u;
+      id[i] = in ? ids[i * kWave + lane] : INT32_MAX;
+    }
+    keep_best(k, id, cnt);
+  }
+  // Every lane's candidate (if it has one that beats the bar); the whole wavefront calls it.
+  __device__ __forceinline__ void add(bool has, uint32_t key, int id, int lane) {
+    has = has && beats(key, id);
+    uint64_t mask = __ballot(has);
+    if (mask == 0) return;
+    if (cnt + count(mask) > kList) {
+      cut(lane);
+      has = has && beats(key, id);
+      mask = __ballot(has);
+    }
+    if (has) {
+      keys[cnt + below(mask)] = key;
+      ids[cnt + below(mask)] = id;
+    }
+    cnt += count(mask);
+  }
+};
+
+// The lanes' best `top` (key, id) in order and the row's numbers, by one wavefront.
+template <int K>
+__device__ __forceinline__ void finish(const Params& p, int row, const char* x, Stat t, const List& list, int lane) {
+  const float z = t.m == INFINITY ? NAN : log1pf(t.s);   // (inf - inf: no probabilities)
+  const bool none = t.m == -INFINITY;                    // every element is -inf: no distribution
+  if (lane == 0) {
+    const int64_t tok = p.tokens[row];
+    p.logprob[row] = tok >= 0 && tok < p.vocab ? (element<K>(x, tok) - t.m) - z : NAN;
+    p.entropy[row] = none ? NAN : z + t.w / (1.0f + t.s);
+  }
+  if (p.top == 0) return;
+  wave_lds_sync();
+  const uint32_t key = lane < p.top ? list.keys[lane] : 0u;
+  const int id = lane < p.top ? list.ids[lane] : INT32_MAX;
+  int rank = 0;
+  for (int i = 0; i < p.top; ++i) {
+    const uint32_t k = list.keys[i];
+    rank += k > key || (k == key && list.ids[i] < id) ? 1 : 0;
+  }
+  if (lane < p.top) {
+    const int64_t at = static_cast<int64_t>(row) * p.top + rank;
+    p.top_lp[at] = (key_score(key) - t.m) - z;
+    p.top_ids[at] = id;
+  }
+}
+
+// The wavefronts' lists and numbers as one: in wavefront 0.
+__device__ __forceinline__ void join_waves(uint32_t (&keys)[kWaves][kList], int (&ids)[kWaves][kList],
+                                           Stat (&stats)[kWaves], int (&counts)[kWaves], int wave, int lane, Stat& t,
+                                           List& list) {
+  if (list.cnt > list.top) list.cut(lane);
+  if (lane == 0) {
+    stats[wave] = t;
+    counts[wave] = list.cnt;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) t = join(t, stats[i]);
+  uint32_t k[4];
+  int id[4], have = 0;
+  static_assert(kWaves == 4, "one list a slot");
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const bool in = lane < counts[i];
+    k[i] = in ? keys[i][lane] : 0u;
+    id[i] = in ? ids[i][lane] : INT32_MAX;
+    have += counts[i];
+  }
+  list.keep_best(k, id, have);
+}
+
+template <int K>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
+  constexpr int E = 16 / kBytes<K>;    // elements a load
+  constexpr int U = kEach / E;         // loads an iteration
+  __shared__ uint32_t keys[kWaves][kList];
+  __shared__ int ids[kWaves][kList];
+  __shared__ Stat stats[kWaves];
+  __shared__ int counts[kWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x / static_cast<unsigned>(p.splits);
+  const int split = blockIdx.x % static_cast<unsigned>(p.splits);
+  const char* x = p.x + static_cast<int64_t>(row) * p.stride * kBytes<K>;
+  // 16-byte pieces from the boundary at or before the row: element i is in piece (i + head) / E
+  const int head = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / kBytes<K>);
+  const int64_t pieces = (static_cast<int64_t>(p.vocab) + head + E - 1) / E;
+  constexpr int kStep = U * kWave;     // pieces of an iteration: runs are whole ones but for the row's end
+  const int64_t per = (pieces + static_cast<int64_t>(p.splits) * kWaves * kStep - 1) / (p.splits * kWaves * kStep) * kStep;
+  const int64_t lo = min(per * (split * kWaves + wave), pieces), hi = min(lo + per, pieces);
+
+  List list{keys[wave], ids[wave], 0, p.top, 0u, INT32_MAX};
+  float bar = p.top > 0 ? -INFINITY : INFINITY;   // the list's, as a value
+  float m = -INFINITY, s = 0.0f, w = 0.0f;        // m is the wavefront's, s and w the lane's part
+  auto widen = [&](const uint4& raw, float (&f)[E]) {
+    const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      f[e] = K == kF32 ? __uint_as_float(r[e & 3])
+                       : K == kBf16 ? (e & 1 ? bf16_hi(r[(e >> 1) & 3]) : bf16_lo(r[(e >> 1) & 3]))
+                                    : f16_bits_to_f32(static_cast<uint16_t>(r[(e >> 1) & 3] >> (16 * (e & 1))));
+  };
+  // a piece whose elements do not all exist (the row's ends, the run's end)
+  auto load_some = [&](int64_t q, float (&f)[E]) {
+    const int64_t first = q * E - head;
+    if (q < hi && first >= 0 && first + E <= p.vocab) {
+      widen(*reinterpret_cast<const uint4*>(x + first * kBytes<K>), f);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int64_t i = first + e;
+      f[e] = q < hi && i >= 0 && i < p.vocab ? element<K>(x, i) : -INFINITY;
+    }
+  };
+  for (int64_t q0 = lo; q0 < hi; q0 += U * kWave) {
+    float v[U][E];
+    const int64_t first = q0 * E - head;
+    if (first >= 0 && q0 + U * kWave <= hi && first + U * kWave * E <= p.vocab) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + first * kBytes<K>) + lane;
+      uint4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = src[u * kWave];
+#pragma unroll
+      for (int u = 0; u < U; ++u) widen(raw[u], v[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_some(q0 + u * kWave + lane, v[u]);
+    }
+    float top = v[0][0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = fmaxf(top, v[u][e]);
+    const float old = m == -INFINITY ? 0.0f : m;
+    if (__any(top > m)) {
+      float t = top;
+#pragma unroll
+      for (int o = kWave / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+      // the sums move to the new maximum; the old one becomes an element like others (lane 0 has it)
+      if (m != -INFINITY) {
+        const float d = fminf(t - m, 200.0f), r = exp_neg(d);
+        w = r * (w + d * s);
+        s = r * s;
+        if (lane == 0) {
+          s += r;
+          w += d * r;
+        }
+      }
+      m = t;
+      // one element that is the maximum stays out
+      const uint64_t owners = __ballot(top == m);
+      bool skip = owners != 0 && lane == __ffsll(static_cast<long long>(owners)) - 1;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float y = m - v[u][e];
+          float ex = exp_neg(y);
+          if (skip && v[u][e] == m) {
+            ex = 0.0f;
+            skip = false;
+          }
+          s += ex;
+          w += fminf(y, 200.0f) * ex;   // (e^-200 is 0: an infinite y adds nothing)
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float y = old - v[u][e];
+          const float ex = exp_neg(y);
+          s += ex;
+          w += fminf(y, 200.0f) * ex;
+        }
+    }
+    if (q0 == lo && p.top > 0) {
+      // the first bar: the top-th largest of the lanes' maxima
+      const uint32_t k = score_key(top);
+      uint32_t t = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        if (count(__ballot(k >= c)) >= p.top) t = c;
+      }
+      list.bar = t;
+      bar = key_score(t);
+    }
+    if (p.top > 0 && __any(top >= bar)) {
+      // (all 64 lanes' element e at once; an element outside the row or run is none)
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float f = u == 0 ? v[0][e] : u == 1 ? v[1 % U][e] : u == 2 ? v[2 % U][e] : v[3 % U][e];
+          if (!__any(f >= bar)) continue;
+          const int64_t q = q0 + u * kWave + lane, i = q * E - head + e;
+          list.add(f >= bar && q < hi && i >= 0 && i < p.vocab, score_key(f), static_cast<int>(i), lane);
+          bar = key_score(list.bar);
+        }
+    }
+  }
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o);
+    w += __shfl_xor(w, o);
+  }
+  Stat t{m, s, w};
+  if (p.top > 0 && s != s) {
+    // a NaN or +inf: the row has no probabilities, but an order (NaN first): by keys
+    list.cnt = 0;
+    list.bar = 0;
+    list.bar_id = INT32_MAX;
+    for (int64_t q0 = lo; q0 < hi; q0 += kWave) {
+      float v[E];
+      load_some(q0 + lane, v);
+      for (int e = 0; e < E; ++e) {
+        float f = v[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) f = e == j ? v[j] : f;
+        const int64_t i = (q0 + lane) * E - head + e;
+        list.add(q0 + lane < hi && i >= 0 && i < p.vocab, score_key(f), static_cast<int>(i), lane);
+      }
+    }
+  }
+  join_waves(keys, ids, stats, counts, wave, lane, t, list);
+  if (wave != 0) return;
+  if (p.splits == 1) {
+    finish<K>(p, row, x, t, list, lane);
+    return;
+  }
+  float* rec = p.ws + static_cast<int64_t>(blockIdx.x) * (4 + 2 * p.top);
+  wave_lds_sync();
+  if (lane == 0) {
+    rec[0] = t.m;
+    rec[1] = t.s;
+    rec[2] = t.w;
+    rec[3] = __int_as_float(list.cnt);
+  }
+  if (lane < list.cnt) {
+    rec[4 + lane] = __uint_as_float(list.keys[lane]);
+    rec[4 + p.top + lane] = __int_as_float(list.ids[lane]);
+  }
+}
+
+// The pieces of a row joined: wavefront i takes records i, i + 4, ...
+template <int K>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const Params p) {
+  __shared__ uint32_t keys[kWaves][kList];
+  __shared__ int ids[kWaves][kList];
+  __shared__ Stat stats[kWaves];
+  __shared__ int counts[kWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x;
+  const float* recs = p.ws + static_cast<int64_t>(row) * p.splits * (4 + 2 * p.top);
+  List list{keys[wave], ids[wave], 0, p.top, 0u, INT32_MAX};
+  // a record a lane, then lanes joined
+  Stat t{-INFINITY, 0.0f, 0.0f};
+  const int mine = wave + kWaves * lane;
+  if (mine < p.splits) {
+    const float* r = recs + static_cast<int64_t>(mine) * (4 + 2 * p.top);
+    t = Stat{r[0], r[1], r[2]};
+  }
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1)
+    t = join(t, Stat{__shfl_xor(t.m, o), __shfl_xor(t.s, o), __shfl_xor(t.w, o)});
+  if (p.top > 0)
+    for (int i = wave; i < p.splits; i += kWaves) {
+      const float* r = recs + static_cast<int64_t>(i) * (4 + 2 * p.top);
+      const bool in = lane < __float_as_int(r[3]);
+      const uint32_t key = in ? __float_as_uint(r[4 + lane]) : 0u;
+      const int id = in ? __float_as_int(r[4 + p.top + lane]) : INT32_MAX;
+      list.add(in, key, id, lane);
+    }
+  join_waves(keys, ids, stats, counts, wave, lane, t, list);
+  if (wave == 0)
+    finish<K>(p, row, p.x + static_cast<int64_t>(row) * p.stride * kBytes<K>, t, list, lane);
+}
+
+// Pieces of a row: rows alone fill the device from about 1024 workgroups on, and a
+// piece is at least one iteration of its four wavefronts.
+int splits_of(int rows, int vocab) {
+  const int most = std::max(1, vocab / (kThreads * kEach));
+  return std::max(1, std::min({1024 / std::max(rows, 1), most, kMaxSplits}));
+}
+
+template <int K>
+void launch(const Params& p, hipStream_t s) {
+  logprobs_kernel<K><<<static_cast<unsigned>(p.rows) * p.splits, kThreads, 0, s>>>(p);
+  if (p.splits > 1) logprobs_join_kernel<K><<<p.rows, kThreads, 0, s>>>(p);
+}
+
+}  // namespace
+}  // namespace nkv
+
+using namespace nkv;
+
+extern "C" int64_t nkv_token_logprobs_workspace(int rows, int vocab, int top) {
+  const int s = splits_of(rows, vocab);
+  return s > 1 ? static_cast<int64_t>(rows) * s * (4 + 2 * top) : 0;
+}
+
+extern "C" int nkv_token_logprobs(const void* logits, int kind, int64_t row_stride, int rows, int vocab,
+                                  const int64_t* tokens, int top, float* logprob, float* entropy, float* top_logprobs,
+                                  int64_t* top_ids, float* workspace, void* stream) {
+  NKV_CHECK_ARG(kind >= kF32 && kind <= kF16, "nkv_token_logprobs: unknown type of logits %d", kind);
+  NKV_CHECK_ARG(rows >= 0 && vocab >= 1 && vocab <= INT32_MAX - 65536,
+                "nkv_token_logprobs: rows must not be negative, vocab from 1 to 2^31 - 65537");
+  NKV_CHECK_ARG(top >= 0 && top <= kMaxTop && top <= vocab,
+                "nkv_token_logprobs: top must be from 0 to %d and at most vocab (got %d)", kMaxTop, top);
+  if (rows == 0) return NKV_OK;
+  NKV_CHECK_ARG(rows <= INT32_MAX / 2, "nkv_token_logprobs: at most 2^30 rows");
+  NKV_CHECK_ARG(logits && tokens && logprob && entropy && (top == 0 || (top_logprobs && top_ids)),
+                "nkv_token_logprobs: NULL input or output");
+  NKV_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % (kind == kF32 ? 4 : 2) == 0 && row_stride >= 0,
+                "nkv_token_logprobs: logits must be aligned to their elements");
+  const int splits = splits_of(rows, vocab);
+  NKV_CHECK_ARG(splits == 1 || workspace, "nkv_token_logprobs: these sizes need a workspace");
+  const Params p{static_cast<const char*>(logits), row_stride, rows,    vocab,        top,     splits,
+                 tokens,                           logprob,    entropy, top_logprobs, top_ids, workspace};
+  const auto s = static_cast<hipStream_t>(stream);
+  if (kind == kF32) launch<kF32>(p, s);
+  else if (kind == kBf16) launch<kBf16>(p, s);
+  else launch<kF16>(p, s);
+  return launch_status("nkv_token_logprobs");
+}

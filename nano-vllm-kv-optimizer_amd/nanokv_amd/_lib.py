@@ -61,6 +61,9 @@ _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _SP = ctypes.POINTER(NkvStore)
 
+# a paged cache: k, v, their scales, three strides, pages, KV heads, page size, head dim
+_CACHE = [_P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _I]
+
 # name -> (restype, argtypes); the exported symbol set of include/nanokv.h
 SIGNATURES = {
     "nkv_abi_version": (_I, []),
@@ -111,6 +114,13 @@ SIGNATURES = {
     "nkv_attend_packed_workspace_floats": (_I64, [_I, _I, _I, _I]),
     "nkv_prefill_attend_tiled": (_I, [_SP, _I, _I, _P, _I64, _I, _P, _P, _I64, _P, _I64, _I64, _I, _I, _I, _I,
                                       _I, _I, _F, _I, _P, _P, _P]),
+    "nkv_paged_append": (_I, [*_CACHE, _P, _I64, _P, _I64, _P, _I64, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _F,
+                              _P, _P]),
+    "nkv_paged_read": (_I, [*_CACHE, _P, _I, _P, _P, _P]),
+    "nkv_paged_move": (_I, [*_CACHE, _P, _P, _I, _P, _P]),
+    "nkv_paged_move_workspace": (_I64, [_I, _I, _I, _I]),
+    "nkv_token_logprobs": (_I, [_P, _I, _I64, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "nkv_token_logprobs_workspace": (_I64, [_I, _I, _I]),
     "nkv_step_select_ns": (_I64, []),
     "nkv_decode_step_noalloc": (_I, [_SP, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F,
                                      _I, _P, _P, _P]),

@@ -120,7 +120,8 @@ def _call(name: str, device: int, *args) -> None:
         _lib.check(rc, name)
 
 
-def _no_gradients(who: str, *operands) -> None:
+def _asks_gradient(*operands) -> bool:
+    """Whether an operand (or None) asks for a gradient, backwards or forwards."""
     asks = False
     if _grad_enabled():
         for t in operands:
@@ -128,7 +129,11 @@ def _no_gradients(who: str, *operands) -> None:
                 asks = True
     if forward_ad._current_level >= 0:       # inside a dual_level
         asks = asks or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands)
-    if asks:
+    return asks
+
+
+def _no_gradients(who: str, *operands) -> None:
+    if _asks_gradient(*operands):
         raise ValueError(f"{who}: an operand asks for a gradient, and the 8-bit operators have none")
 
 
