@@ -756,6 +756,34 @@ int nkv_paged_move(void* k, void* v, float* k_scale, float* v_scale, int64_t pag
 int64_t nkv_paged_move_workspace(int num_kv_heads, int head_dim, int int8, int rows);
 
 /*
+ * Attention of every sequence's new tokens over its keys in the cache (the
+ * flash_attn_with_kvcache and block-table flash_attn_varlen_func calls of
+ * nanovllm/layers/attention.py:100-119, and drafted trees).
+ *
+ * Sequence b: lengths[b] keys, the slots of tables[b table_stride ..] (page ids; page j
+ * holds keys j page_size ..), its new tokens' among them as the last; its queries are rows
+ * starts[b] .. starts[b + 1] - 1 of q [rows][Hq][D] (row stride q_stride), or with
+ * starts NULL rows b max_new .. (rows == batch * max_new).  Query i of n sees keys
+ * j <= length - n + i; with tree (int64 [rows], n <= 64) the keys before length - n, and new
+ * token j where bit j of its mask is set.  out [rows][Hq][D] = softmax(scale q k^T) v,
+ * fp32 softmax; 0 for a query that sees nothing and for rows of no sequence.
+ * Lengths are taken up to the table's max_pages pages; page ids outside the cache
+ * hide their keys; values of hidden keys (NaN, infinite, never written) reach no output.
+ * max_new: at least every sequence's new tokens (rows behind it give 0).
+ * workspace: nkv_paged_attend_workspace(...) floats, 16-byte aligned (NULL where that is 0;
+ * ragged: starts != NULL), asked with the launch's device current.  Calls that may overlap take two.
+ * Constraints: batch <= 65535, Hq / Hkv <= 64, max_new <= 2^20, scale > 0,
+ * max_pages * page_size < 2^31 - 4095.
+ */
+int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride, int64_t head_stride,
+                     int64_t token_stride, int pages, int num_kv_heads, int page_size, int head_dim,
+                     const uint16_t* q, int64_t q_stride, int rows, int num_heads, const int32_t* tables,
+                     int64_t table_stride, int max_pages, const int32_t* lengths, int batch, const int32_t* starts,
+                     int max_new, const int64_t* tree, float scale, uint16_t* out, float* workspace, void* stream);
+int64_t nkv_paged_attend_workspace(int batch, int rows, int max_new, int num_heads, int num_kv_heads, int head_dim,
+                                   int max_pages, int page_size, int ragged);
+
+/*
  * Log probabilities of rows of logits [rows][vocab] (kind 0: fp32, 1: bf16, 2:
  * fp16; row_stride elements from row to row): logprob[t] of tokens[t] (NaN for
  * a token outside [0, vocab)), entropy[t] of the distribution, and the top most

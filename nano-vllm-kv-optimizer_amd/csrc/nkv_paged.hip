@@ -26,6 +26,8 @@ int fill_paged(const char* who, void* k, void* v, float* k_scale, float* v_scale
                       "%s: page_size must be a power of two from 16 to 4096 (got %d)", who, page_size);
   NKV_CHECK_ARG(k && v, "%s: the cache is NULL", who);
   NKV_CHECK_ARG((k_scale != nullptr) == (v_scale != nullptr), "%s: keys and values have both scales or none", who);
+  NKV_CHECK_ARG((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 16 == 0,
+                "%s: scales must lie on a 16-byte boundary", who);
   NKV_CHECK_ARG(pages >= 1 && num_kv_heads >= 1, "%s: pages and num_kv_heads must be positive", who);
   NKV_CHECK_ARG(static_cast<int64_t>(pages) * page_size <= INT32_MAX, "%s: a cache holds fewer than 2^31 tokens", who);
   const int elem = k_scale ? 1 : 2;

@@ -1,0 +1,1001 @@
+// Attention of every sequence's new tokens over its keys in a paged cache.
+//
+// Sequence b holds L keys (its page table's first L slots), the last n of them its new
+// tokens'; query i of it sees the keys up to L - n + i, or with a tree the keys before
+// L - n and those new ones whose bit its mask has.  o = softmax(scale q k^T) v with the
+// softmax in fp32, one pass over the keys with a running maximum; a query that sees nothing gives 0.
+//
+// The G query heads of a KV head share its keys, so (query, head) pairs are the columns of
+// one product S^T = K Q^T and O^T = V^T P^T on the matrix cores (16x16x32 bf16):
+//   * few_kernel, up to 16 columns (a token, a short draft): bound by reading the keys once.
+//     Every wavefront takes 32-key tiles of its own: K goes from HBM to the operand
+//     registers, V through the wavefront's LDS (read back transposed), both a tile
+//     ahead; P enters the second product as bf16 high and low parts, as good as fp32.
+//   * many_kernel, tiles of 64 or 128 columns (trees, prompts): 64-key tiles staged in LDS
+//     for all four wavefronts, the next one on its way; bound by the matrix cores for
+//     long prompts, by the keys for trees.  P is rounded to bf16 for the second product (2^-9
+//     of each weight, fewer than the output's own rounding), numerator and denominator alike.
+// 8-bit caches: the codes are bf16 exactly; a key's scale multiplies its logits, a
+// value's its weights, both in fp32.
+//
+// Few columns over long caches are split over workgroups by a plan that each of them makes
+// from the lengths (they are in device memory): runs of C 64-key tiles, C such that all
+// sequences together give about `target` runs, so one long sequence among short ones is cut
+// finer than they are.  merge_kernel joins the runs' partial sums.
+//
+// Hidden keys get weight 0, which times an infinite or NaN value is NaN: a column whose
+// result holds a NaN is computed again key by key (redo_column), hidden keys left out.  Keys
+// past the length are never read (rows are clamped or bounds-checked), page ids outside the
+// cache hide their keys.
+#include <algorithm>
+
+#include "nkv_paged.h"
+#include "nkv_stage.h"
+
+namespace nkv {
+namespace {
+using attend_detail::bf16x8;
+using attend_detail::f32x4;
+using attend_detail::i8x8_to_bf16x8;
+using attend_detail::max_over_rows;
+using attend_detail::sum_over_rows;
+using namespace stage;
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kKeys = 64;          // keys of a tile, the unit of runs
+constexpr int kFewCols = 16;
+constexpr int kMaxTree = 64;       // tokens of a tree: bits of a mask
+constexpr int kMaxSplits = 256;
+constexpr float kHeadroom = 8.0f;  // a running maximum moves once a logit passes it by 2^8 (log2 units)
+
+struct Plan {
+  int few, nct, cols, tpw, qtiles;      // columns and tokens of a workgroup's tile, tiles of max_new tokens
+  int max_splits, target, min_tiles;
+};
+
+struct Params {
+  PagedCache c;
+  const uint16_t* q;
+  int64_t q_ls;
+  uint16_t* out;
+  const int32_t* tables;
+  int64_t table_ls;
+  int max_pages;
+  const int32_t* lengths;
+  const int32_t* starts;     // nullptr: n tokens each
+  const uint64_t* tree;      // nullptr: in order
+  int B, T, n, hq, G;
+  float scale_log2;
+  float* part;
+  Plan plan;
+};
+
+template <int D> constexpr int kPart = D + 4;   // a column's partial record: m, l, two of padding, acc
+
+typedef __attribute__((address_space(4))) const int32_t cint32;
+
+struct Seq {
+  int begin, count, len, older;   // first row of q, new tokens, keys, keys before the new tokens
+};
+__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
+  Seq s;
+  int end;
+  if (p.starts) {
+    s.begin = min(max(((const cint32*)p.starts)[b], 0), p.T);
+    end = min(max(((const cint32*)p.starts)[b + 1], s.begin), p.T);
+  } else {
+    s.begin = b * p.n;
+    end = s.begin + p.n;
+  }
+  s.count = end - s.begin;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(((const cint32*)p.lengths)[b], 0)),
+                               static_cast<int64_t>(p.max_pages) << p.c.shift));
+  s.older = s.len - s.count;
+  return s;
+}
+
+// Tiles of a run (C): all lanes of the wavefront call it.
+__device__ __forceinline__ int run_tiles(const Params& p, int lane) {
+  if (p.plan.max_splits == 1) return INT32_MAX;
+  int64_t total = 0;
+  for (int b = lane; b < p.B; b += kWave) {
+    const int len = static_cast<int>(min(static_cast<int64_t>(max(p.lengths[b], 0)),
+                                         static_cast<int64_t>(p.max_pages) << p.c.shift));
+    int tiles = 1;
+    if (p.plan.qtiles > 1) {
+      const int count = p.starts ? min(max(p.starts[b + 1] - p.starts[b], 0), p.n) : p.n;
+      tiles = (count + p.plan.tpw - 1) / p.plan.tpw;
+    }
+    total += static_cast<int64_t>((len + kKeys - 1) / kKeys) * tiles;
+  }
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) total += __shfl_xor(total, o);
+  const int64_t cap = ((static_cast<int64_t>(p.max_pages) << p.c.shift) + kKeys - 1) / kKeys;
+  const int64_t c = max((total * p.c.hkv + p.plan.target - 1) / p.plan.target,
+                        max((cap + p.plan.max_splits - 1) / p.plan.max_splits, static_cast<int64_t>(p.plan.min_tiles)));
+  return __builtin_amdgcn_readfirstlane(static_cast<int>(c));
+}
+__device__ __forceinline__ int splits_of(int tiles, int run) { return max(1, tiles / run + (tiles % run != 0 ? 1 : 0)); }
+
+// Keys that the queries [t0, t1] of a sequence may see: [0, this).
+__device__ __forceinline__ int keys_of(const Params& p, const Seq& s, int t1) {
+  return p.tree ? s.len : min(max(s.older + t1 + 1, 0), s.len);
+}
+
+// The page of the 16-key group that starts at key0 (-1: none); key0 is the same in all lanes.
+__device__ __forceinline__ int page_of(const Params& p, const cint32* table, const Seq& s, int key0) {
+  if (key0 >= s.len) return -1;
+  const int id = table[key0 >> p.c.shift];
+  return id >= 0 && id < p.c.pages ? id : -1;
+}
+
+// The keys of [key0, key0 + 64) that a query of sequence s sees, as bits: those up
+// to `limit`, or with a tree the ones before its tokens and those that its mask names.
+__device__ __forceinline__ uint64_t seen_bits(uint64_t mask, bool tree, int limit, const Seq& s, int key0) {
+  if (tree) {
+    const int at = key0 - s.older;   // the first key's place among the new tokens
+    const uint64_t bits = at >= kMaxTree ? 0 : at >= 0 ? mask >> at : at <= -64 ? ~0ull : mask << -at | ((1ull << -at) - 1);
+    const int rows = s.len - key0;
+    return rows >= 64 ? bits : rows <= 0 ? 0 : bits & ((1ull << rows) - 1);
+  }
+  const int last = limit - key0;
+  return last >= 63 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
+}
+// x where the bit holds, else -inf.
+__device__ __forceinline__ float where_bit(float x, uint32_t bits, int bit) {
+  const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - bit)) >> 31);
+  return __uint_as_float((__float_as_uint(x) & keep) | (0xff800000u & ~keep));
+}
+
+// One column again, by one wavefront, key by key: m (log2 units), l and the sums of
+// the lane's D / 64 dims over the visible keys of [k0, k1).
+template <int D, bool INT8>
+__device__ void redo_column(const Params& p, const Seq& s, const cint32* table, int h, int t, int head, int k0, int k1,
+                            int lane, float& m, float& l, float (&o)[D / 64]) {
+  constexpr int N = D / 64;
+  const uint16_t* qrow = p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + head * D;
+  float q[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    q[e] = bf16_to_f32(qrow[lane * N + e]);
+    o[e] = 0.0f;
+  }
+  const uint64_t mask = p.tree ? p.tree[s.begin + t] : 0;
+  m = -INFINITY;
+  l = 0.0f;
+  for (int key = k0; key < min(k1, s.len); ++key) {
+    if (!(seen_bits(mask, p.tree != nullptr, s.older + t, s, key) & 1)) continue;
+    const int id = page_of(p, table, s, key);
+    if (id < 0) continue;
+    const int slot = (id << p.c.shift) + (key & (p.c.page - 1));
+    const int64_t row = paged_row(p.c, slot, h) + lane * N;
+    float k[N], v[N], vs = 1.0f, dot = 0.0f, ks = 1.0f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (INT8) {
+        k[e] = static_cast<float>(reinterpret_cast<const int8_t*>(p.c.k)[row + e]);
+        v[e] = static_cast<float>(reinterpret_cast<const int8_t*>(p.c.v)[row + e]);
+      } else {
+        k[e] = bf16_to_f32(reinterpret_cast<const uint16_t*>(p.c.k)[row + e]);
+        v[e] = bf16_to_f32(reinterpret_cast<const uint16_t*>(p.c.v)[row + e]);
+      }
+      dot += q[e] * k[e];
+    }
+    if (INT8) {
+      const int64_t at = paged_scale(p.c, slot, h);
+      ks = p.c.ks[at];
+      vs = p.c.vs[at];
+    }
+#pragma unroll
+    for (int x = kWave / 2; x > 0; x >>= 1) dot += __shfl_xor(dot, x);
+    const float y = dot * ks * p.scale_log2;
+    const float mn = fmaxf(m, y);
+    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float w = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y - mn);   // (NaN stays)
+    m = mn;
+    l = l * alpha + w;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = o[e] * alpha + w * (v[e] * vs);
+  }
+}
+
+// A column's result, by the lanes of a wavefront that hold D / 64 dims each.
+template <int D>
+__device__ __forceinline__ void store_column(const Params& p, bool whole, uint16_t* orow, float* rec, int lane, float m,
+                                             float l, const float (&o)[D / 64]) {
+  constexpr int N = D / 64;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    if (whole)
+      orow[lane * N + e] = f32_to_bf16(l == 0.0f ? 0.0f : o[e] / l);
+    else
+      rec[4 + lane * N + e] = o[e];
+  }
+  if (!whole && lane == 0) {
+    rec[0] = m;
+    rec[1] = l;
+  }
+}
+
+// Rows of q that belong to no sequence, or lie behind a sequence's max_new-th: zeros for head group h.
+__device__ __forceinline__ void clear_rows(const Params& p, int h, int from, int to, int d) {
+  const int per = p.G * d / 8;
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(to - from) * per; i += kThreads) {
+    const int64_t row = from + i / per;
+    reinterpret_cast<uint4*>(p.out + (row * p.hq + h * p.G) * d)[i % per] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+__device__ __forceinline__ void clear_others(const Params& p, const Seq& s, int b, int h, int d) {
+  if (!p.starts) return;
+  if (s.count > p.n) clear_rows(p, h, s.begin + p.n, s.begin + s.count, d);
+  if (b == 0) {
+    clear_rows(p, h, 0, s.begin, d);
+    clear_rows(p, h, min(max(((const cint32*)p.starts)[p.B], 0), p.T), p.T, d);
+  }
+}
+
+__device__ __forceinline__ bf16x8 as_bf16(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
+
+// ---------------------------------------------------------------- few columns --
+// Operand layout of the 16x16x32 product: lane (ln, lg) holds A[ln][8 lg ..] and
+// B[8 lg ..][ln], and of the result rows 4 lg .. + 3 of column ln.  The 32 keys of the
+// second product are ordered as the first one's results lie: 4 lg + e of the
+// first 16, then of the second, so P never leaves its lane.  In 8 bits a lane takes 16
+// neighbouring codes of a row for two steps of the first product, and q is laid out alike.
+template <int D, bool INT8>
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
+  constexpr int KS = D / 32;                    // steps of the first product
+  constexpr int DT = D / 16;                    // 16-dim tiles of the second
+  constexpr int RB = 2 * D;                     // bytes of a V row in LDS
+  constexpr int KL = INT8 ? D / 64 : D / 32;    // 16-byte loads of a K row's quarter
+  constexpr int VR = INT8 ? 1024 / D : 512 / D; // V rows a load of the wavefront covers
+  constexpr int VL = 16 / VR;                   // loads of a 16-key group
+  constexpr int kBuf = 32 * RB;
+  constexpr int kLds = kWaves * kBuf + kWaves * kFewCols * 8;
+  static_assert(kWaves * kFewCols * D * 4 <= kWaves * kBuf, "the join's sums fit where V was");
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int ln = lane & 15, lg = lane >> 4;
+  const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y;
+  const Seq s = seq_of(p, b);
+  if (split == 0) clear_others(p, s, b, h, D);
+  const int count = min(s.count, p.n);
+  if (count == 0) return;
+  const int keys = keys_of(p, s, count - 1);
+  const int tiles = (keys + kKeys - 1) / kKeys;
+  const int run = run_tiles(p, lane);
+  const int splits = splits_of(tiles, run);
+  if (split >= splits) return;
+  const int lo = static_cast<int>(static_cast<int64_t>(split) * tiles / splits) * kKeys;
+  const int hi = min(static_cast<int>(static_cast<int64_t>(split + 1) * tiles / splits) * kKeys, keys);
+  const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
+
+  // column ln: query token, head, what it sees
+  const int t = ln / p.G;
+  const bool mine = t < count;
+  const int head = h * p.G + ln % p.G;
+  const int limit = mine ? s.older + t : -1;
+  const uint64_t mask = p.tree && mine ? p.tree[s.begin + t] : 0;
+  bf16x8 bq[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    const int d0 = INT8 ? 64 * (ks >> 1) + 16 * lg + 8 * (ks & 1) : 32 * ks + 8 * lg;
+    if (mine) v = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + head * D + d0);
+    bq[ks] = as_bf16(v);
+  }
+
+  char* buf = lds + wave * kBuf;
+  constexpr int E = INT8 ? 1 : 2;
+  uint4 kr[2][KL], vr[2][VL];
+  float4 ksc[2], vsc[2];
+  // the tile's keys are in which 16-key groups' pages (bit 0, 1)
+  auto load = [&](int key, uint4 (&kd)[2][KL], uint4 (&vd)[2][VL], float4 (&kss)[2], float4 (&vss)[2]) {
+    int have = 0;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key0 = key + 16 * g;
+      const int id = page_of(p, table, s, key0);
+      if (id < 0) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kd[g][i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) vd[g][i] = make_uint4(0u, 0u, 0u, 0u);
+        kss[g] = vss[g] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        continue;
+      }
+      have |= 1 << g;
+      const int in = key0 & (p.c.page - 1);
+      const int64_t base = (p.c.sp * id + p.c.sh * h + p.c.st * in) * E;
+      const int last = s.len - 1 - key0;     // rows behind it are read as it is
+      const char* kp = p.c.k + base + static_cast<int64_t>(min(ln, last)) * (p.c.st * E);
+#pragma unroll
+      for (int i = 0; i < KL; ++i) kd[g][i] = *reinterpret_cast<const uint4*>(kp + i * 64 + lg * 16);
+      constexpr int PC = 64 / VR;            // 16-byte pieces of a row
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int row = min(VR * i + lane / PC, last);
+        vd[g][i] = *reinterpret_cast<const uint4*>(p.c.v + base + static_cast<int64_t>(row) * (p.c.st * E) + (lane % PC) * 16);
+      }
+      if (INT8) {
+        const int64_t at = ((static_cast<int64_t>(id) * p.c.hkv + h) << p.c.shift) + in + 4 * lg;
+        kss[g] = *reinterpret_cast<const float4*>(p.c.ks + at);
+        vss[g] = *reinterpret_cast<const float4*>(p.c.vs + at);
+      }
+    }
+    return have;
+  };
+  // V rows to LDS: row r at r RB, its 16-byte chunk c at position c ^ 2 (r & 3)
+  auto put = [&](const uint4 (&vd)[2][VL]) {
+    constexpr int PC = 64 / VR;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int row = 16 * g + VR * i + lane / PC;
+        const int c = lane % PC;
+        if (INT8) {
+          const uint4 w = vd[g][i];
+          *reinterpret_cast<uint4*>(buf + row * RB + (((2 * c) ^ (2 * (row & 3))) << 4)) = i8x8_to_bf16x8(w.x, w.y);
+          *reinterpret_cast<uint4*>(buf + row * RB + (((2 * c + 1) ^ (2 * (row & 3))) << 4)) = i8x8_to_bf16x8(w.z, w.w);
+        } else {
+          *reinterpret_cast<uint4*>(buf + row * RB + ((c ^ (2 * (row & 3))) << 4)) = vd[g][i];
+        }
+      }
+  };
+  // transposing read: keys 4 lg .. + 3 (+ 16 g) of dims 16 dt + ln
+  int vtr[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    vtr[x] = (4 * lg + (ln >> 2)) * RB + ((2 * (x ^ (ln >> 2)) + ((ln & 3) >> 1)) << 4) + 8 * (ln & 1);
+
+  f32x4 acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;   // the column's maximum (log2 units), the lane's part of its sum
+
+  int key = lo + 32 * wave, have = 0;
+  if (key < hi) {
+    have = load(key, kr, vr, ksc, vsc);
+    put(vr);
+  }
+  while (key < hi) {
+    const int next = key + 32 * kWaves;
+    uint4 kn[2][KL], vn[2][VL];
+    float4 ksn[2], vsn[2];
+    int have_n = 0;
+    if (next < hi) have_n = load(next, kn, vn, ksn, vsn);
+
+    f32x4 S[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        bf16x8 a;
+        if (INT8) {
+          const uint4 w = kr[g][ks >> 1];
+          a = as_bf16(ks & 1 ? i8x8_to_bf16x8(w.z, w.w) : i8x8_to_bf16x8(w.x, w.y));
+        } else {
+          a = as_bf16(kr[g][ks % KL]);
+        }
+        S[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ks], S[g], 0, 0, 0);
+      }
+    float y[2][4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float sc[4] = {ksc[g].x, ksc[g].y, ksc[g].z, ksc[g].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[g][e] = S[g][e] * (INT8 ? sc[e] * p.scale_log2 : p.scale_log2);
+    }
+    if (have != 3 || key + 31 > (p.tree ? s.older - 1 : s.older)) {
+      uint64_t bits = mine ? seen_bits(mask, p.tree != nullptr, limit, s, key) : 0;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (!((have >> g) & 1)) bits &= ~(0xffffull << (16 * g));
+        const uint32_t own = static_cast<uint32_t>(bits >> (16 * g + 4 * lg));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[g][e] = where_bit(y[g][e], own, e);
+      }
+    }
+    float top = y[0][0];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, y[g][e]);
+    if (__any(top > m + kHeadroom || (m == -INFINITY && top > m))) {
+      const float mn = fmaxf(m, max_over_rows(top));
+      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    bf16x8 hi8, lo8;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float sc[4] = {vsc[g].x, vsc[g].y, vsc[g].z, vsc[g].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float w = __builtin_amdgcn_exp2f(y[g][e] - base);
+        l += w;
+        if (INT8) w = w == 0.0f ? 0.0f : w * sc[e];   // (the scale of a hidden key may be anything)
+        const __bf16 a = static_cast<__bf16>(w);
+        hi8[4 * g + e] = a;
+        lo8[4 * g + e] = static_cast<__bf16>(w - static_cast<float>(a));
+      }
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      const char* vp = buf + vtr[i & 3] + (i >> 2) * 128;
+      const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
+      const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
+      const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi8, acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo8, acc[i], 0, 0, 0);
+    }
+    wave_lds_sync();
+    if (next < hi) {
+      put(vn);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kr[g][i] = kn[g][i];
+        ksc[g] = ksn[g];
+        vsc[g] = vsn[g];
+      }
+    }
+    have = have_n;
+    key = next;
+  }
+  l = sum_over_rows(l);
+
+  // ---- the wavefronts' sums joined: thread (column, D / 16 dims) -------------
+  float* sums = reinterpret_cast<float*>(lds);                        // [wave][column][D]
+  float* ml = reinterpret_cast<float*>(lds + kWaves * kBuf);          // [wave][column][2]
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(sums + (wave * kFewCols + ln) * D + 16 * i + 4 * lg) = acc[i];
+  if (lg == 0) {
+    ml[(wave * kFewCols + ln) * 2] = m;
+    ml[(wave * kFewCols + ln) * 2 + 1] = l;
+  }
+  __syncthreads();
+  const int col = threadIdx.x >> 4;
+  const int cols = count * p.G;
+  const int d0 = (threadIdx.x & 15) * (D / 16);
+  float mt = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) mt = fmaxf(mt, ml[(i * kFewCols + col) * 2]);
+  float lt = 0.0f, o[D / 16];
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) o[e] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float mi = ml[(i * kFewCols + col) * 2];
+    const float li = ml[(i * kFewCols + col) * 2 + 1];
+    const float w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mt);
+    if (mi == -INFINITY && li == 0.0f) continue;      // saw nothing (hidden values may have made its sums NaN)
+    lt += li * w;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) o[e] += sums[(i * kFewCols + col) * D + d0 + e] * w;
+  }
+  bool odd = lt != lt;
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) odd = odd || o[e] != o[e];
+  const uint64_t redo = __ballot(odd && col < cols);
+  const bool whole = splits == 1;
+  auto orow = [&](int c) {
+    return p.out + (static_cast<int64_t>(s.begin + c / p.G) * p.hq + h * p.G + c % p.G) * D;
+  };
+  auto rec = [&](int c) {
+    return p.part + (((static_cast<int64_t>(b) * p.c.hkv + h) * p.plan.max_splits + split) * p.plan.cols + c) * kPart<D>;
+  };
+  const bool again = (redo >> (lane & 48)) & 0xffff;   // the lane's column
+  if (col < cols && !again) {
+    if (whole) {
+      uint16_t* dst = orow(col) + d0;
+      const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+#pragma unroll
+      for (int e = 0; e < D / 16; e += 4)
+        *reinterpret_cast<u32x2*>(dst + e) = u32x2{pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv)};
+    } else {
+      float* r = rec(col);
+      if (d0 == 0) {
+        r[0] = mt;
+        r[1] = lt;
+      }
+#pragma unroll
+      for (int e = 0; e < D / 16; e += 4) *reinterpret_cast<f32x4*>(r + 4 + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+    }
+  }
+  if (redo == 0) return;
+  for (int i = 0; i < 4; ++i) {   // the wavefront's four columns
+    if (((redo >> (16 * i)) & 0xffff) == 0) continue;
+    const int c = 4 * wave + i;
+    float mc, lc, oc[D / 64];
+    redo_column<D, INT8>(p, s, table, h, c / p.G, h * p.G + c % p.G, lo, hi, lane, mc, lc, oc);
+    store_column<D>(p, whole, whole ? orow(c) : nullptr, whole ? nullptr : rec(c), lane, mc, lc, oc);
+  }
+}
+
+// --------------------------------------------------------------- many columns --
+// LDS of a stage: K tile, V tile (64 rows of 2 D bytes each), in 8 bits the 64
+// keys' and values' scales.  K row r's 16-byte chunk c lies at position c ^ (r mod chunks), V's
+// at c ^ 2 (r & 3): the 16-byte reads of 8 keys and the transposing reads of
+// 4 keys x 16 dims touch every bank once.
+template <int D> constexpr int kTile = kKeys * 2 * D;
+template <int D> constexpr int kStage = 2 * kTile<D> + 2 * kKeys * 4;
+
+template <int D, bool INT8, int NCT>
+__global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params p) {
+  constexpr int KS = D / 32, DT = D / 16, CH = D / 8, RB = 2 * D;
+  constexpr int kCols = 64 * NCT;
+  __shared__ __attribute__((aligned(16))) char lds0[kStage<D>];
+  __shared__ __attribute__((aligned(16))) char lds1[kStage<D>];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int ln = lane & 15, lg = lane >> 4;
+  const int h = blockIdx.x;
+  const int b = blockIdx.z / static_cast<unsigned>(p.plan.max_splits);
+  const int split = blockIdx.z % static_cast<unsigned>(p.plan.max_splits);
+  const int qt = p.plan.qtiles - 1 - static_cast<int>(blockIdx.y);   // the longest first
+  const Seq s = seq_of(p, b);
+  if (split == 0 && qt == 0) clear_others(p, s, b, h, D);
+  const int count = min(s.count, p.n);
+  const int tpw = p.plan.tpw;
+  const int t0 = qt * tpw;
+  if (t0 >= count) return;
+  const int t_last = min(t0 + tpw, count) - 1;
+  const int keys = keys_of(p, s, t_last);
+  const int tiles = (keys + kKeys - 1) / kKeys;
+  const int splits = splits_of(tiles, run_tiles(p, lane));
+  if (split >= splits) return;
+  const int lo = static_cast<int>(static_cast<int64_t>(split) * tiles / splits);
+  const int hi = static_cast<int>(static_cast<int64_t>(split + 1) * tiles / splits);
+  const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
+
+  // column c = 16 NCT wave + 16 ct + ln: token t0 + c / G, head c % G
+  int limit[NCT];
+  uint64_t mask[NCT];
+  bf16x8 bq[NCT][KS];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const int c = wave * 16 * NCT + ct * 16 + ln;
+    const int t = t0 + c / p.G;
+    const bool mine = t <= t_last;
+    limit[ct] = mine ? s.older + t : -1;
+    mask[ct] = p.tree && mine ? p.tree[s.begin + t] : 0;
+    const uint16_t* qrow = p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + (h * p.G + c % p.G) * D;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (mine) v = *reinterpret_cast<const uint4*>(qrow + 32 * ks + 8 * lg);
+      bq[ct][ks] = as_bf16(v);
+    }
+  }
+  f32x4 acc[DT][NCT], lsum[NCT];
+  float m[NCT];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    lsum[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    m[ct] = -INFINITY;
+  }
+
+  // Staging of a tile: wavefront w brings its keys 16 w .. + 15, which lie in one page.
+  // bf16 goes to LDS without registers, rows past the length (or of a page outside the
+  // cache) as zeros; 8-bit codes through registers, widened on the way.
+  constexpr int PC = INT8 ? D / 16 : D / 8;     // 16-byte pieces of a row in the cache
+  constexpr int RL = kWave / PC;                // rows a load of the wavefront covers
+  constexpr int NL = 16 / RL;                   // loads of its 16 rows
+  uint4 kreg[NL], vreg[NL];
+  float sreg = 0.0f;
+  int have = 0;                                 // bit g: the tile's 16-key group g has a page
+  auto begin_stage = [&](int tile, char* buf) {
+    const int key0 = tile * kKeys + 16 * wave;
+    have = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) have |= page_of(p, table, s, tile * kKeys + 16 * g) >= 0 ? 1 << g : 0;
+    const int id = page_of(p, table, s, key0);
+    const int rows = id < 0 ? 0 : min(16, s.len - key0);
+    const int in = key0 & (p.c.page - 1);
+    const int64_t at = p.c.sp * max(id, 0) + p.c.sh * h + p.c.st * in;
+    if constexpr (INT8) {
+      const int row_bytes = static_cast<int>(p.c.st);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int r = RL * i + lane / PC;
+        kreg[i] = vreg[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+          kreg[i] = *reinterpret_cast<const uint4*>(p.c.k + at + static_cast<int64_t>(r) * row_bytes + (lane % PC) * 16);
+          vreg[i] = *reinterpret_cast<const uint4*>(p.c.v + at + static_cast<int64_t>(r) * row_bytes + (lane % PC) * 16);
+        }
+      }
+      // lanes 0 .. 15 the keys' scales, 16 .. 31 the values'
+      sreg = 0.0f;
+      if (lane < 32 && ln < rows)
+        sreg = (lane < 16 ? p.c.ks : p.c.vs)[((static_cast<int64_t>(id) * p.c.hkv + h) << p.c.shift) + in + ln];
+    } else {
+      const int row_bytes = static_cast<int>(p.c.st) * 2;
+      const uint32_t bytes = static_cast<uint32_t>(rows) * row_bytes;
+      const rsrc_words rk = rsrc_of(p.c.k + 2 * at, bytes);
+      const rsrc_words rv = rsrc_of(p.c.v + 2 * at, bytes);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int r = RL * i + lane / PC, c = lane % PC;
+        const char* dst = buf + (16 * wave + RL * i) * RB;
+        lds_copy16(rk, dst, r * row_bytes + ((c ^ (r & (CH - 1))) << 4));
+        lds_copy16(rv, dst + kTile<D>, r * row_bytes + ((c ^ (2 * (r & 3))) << 4));
+      }
+    }
+  };
+  auto finish_stage = [&](char* buf) {
+    if constexpr (INT8) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int r = 16 * wave + RL * i + lane / PC, c = 2 * (lane % PC);
+        char* kd = buf + r * RB;
+        char* vd = kd + kTile<D>;
+        *reinterpret_cast<uint4*>(kd + ((c ^ (r & (CH - 1))) << 4)) = i8x8_to_bf16x8(kreg[i].x, kreg[i].y);
+        *reinterpret_cast<uint4*>(kd + (((c + 1) ^ (r & (CH - 1))) << 4)) = i8x8_to_bf16x8(kreg[i].z, kreg[i].w);
+        *reinterpret_cast<uint4*>(vd + ((c ^ (2 * (r & 3))) << 4)) = i8x8_to_bf16x8(vreg[i].x, vreg[i].y);
+        *reinterpret_cast<uint4*>(vd + (((c + 1) ^ (2 * (r & 3))) << 4)) = i8x8_to_bf16x8(vreg[i].z, vreg[i].w);
+      }
+      if (lane < 32)
+        reinterpret_cast<float*>(buf + 2 * kTile<D>)[(lane < 16 ? 0 : kKeys) + 16 * wave + ln] =
+            lane < 16 ? sreg * p.scale_log2 : sreg;
+    } else {
+      __builtin_amdgcn_s_waitcnt(0);   // the copies have landed
+    }
+    __syncthreads();
+  };
+
+  // operand addresses of the lane in a stage
+  int koff[KS], vtr[4];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = ln * RB + (((4 * ks + lg) ^ (ln & (CH - 1))) << 4);
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    vtr[x] = kTile<D> + (4 * lg + (ln >> 2)) * RB + ((2 * (x ^ (ln >> 2)) + ((ln & 3) >> 1)) << 4) + 8 * (ln & 1);
+
+  if (lo < hi) {
+    begin_stage(lo, lds0);
+    finish_stage(lds0);
+  }
+  for (int tile = lo; tile < hi; ++tile) {
+    char* buf = (tile - lo) & 1 ? lds1 : lds0;
+    char* other = (tile - lo) & 1 ? lds0 : lds1;
+    const int got = have;
+    const bool more = tile + 1 < hi;
+    if (more) begin_stage(tile + 1, other);
+
+    // ---- S^T = K Q^T: S[kt][ct][e] is key 16 kt + 4 lg + e of column ct -------
+    f32x4 S[4][NCT];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) S[kt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(buf + kt * 16 * RB + koff[ks]);
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) S[kt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ct][ks], S[kt][ct], 0, 0, 0);
+      }
+    }
+    const float* scales = reinterpret_cast<const float*>(buf + 2 * kTile<D>);
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      if (INT8) {
+        const f32x4 sc = *reinterpret_cast<const f32x4*>(scales + 16 * kt + 4 * lg);
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) S[kt][ct] *= sc;
+      } else {
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) S[kt][ct] *= p.scale_log2;
+      }
+    }
+    if (got != 15 || tile * kKeys + kKeys - 1 > (p.tree ? s.older - 1 : s.older + t0)) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        uint64_t bits = seen_bits(mask[ct], p.tree != nullptr, limit[ct], s, tile * kKeys);
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          if (!((got >> kt) & 1)) bits &= ~(0xffffull << (16 * kt));
+          const uint32_t own = static_cast<uint32_t>(bits >> (16 * kt + 4 * lg));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[kt][ct][e] = where_bit(S[kt][ct][e], own, e);
+        }
+      }
+    }
+    // ---- softmax: the maximum moves only where a logit passes it by 2^8 -------
+    float top[NCT];
+    bool move = false;
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      top[ct] = S[0][ct][0];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[ct] = fmaxf(top[ct], S[kt][ct][e]);
+      move = move || top[ct] > m[ct] + kHeadroom || (m[ct] == -INFINITY && top[ct] > m[ct]);
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        const float mn = fmaxf(m[ct], max_over_rows(top[ct]));
+        const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - mn);
+        m[ct] = mn;
+        lsum[ct] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i][ct] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      const float base = m[ct] == -INFINITY ? 0.0f : m[ct];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[kt][ct][e] = __builtin_amdgcn_exp2f(S[kt][ct][e] - base);
+    }
+    if (INT8) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        const f32x4 sc = *reinterpret_cast<const f32x4*>(scales + kKeys + 16 * kt + 4 * lg);
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          lsum[ct] += S[kt][ct];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[kt][ct][e] = S[kt][ct][e] == 0.0f ? 0.0f : S[kt][ct][e] * sc[e];
+        }
+      }
+    }
+    // ---- O^T += V^T P^T, the row sums a product with ones ----------------------
+    const bf16x8 ones = as_bf16(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2) {
+      bf16x8 bp[NCT];
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        const f32x4 a0 = S[2 * k2][ct], a1 = S[2 * k2 + 1][ct];
+        bp[ct] = as_bf16(make_uint4(pack_bf16(a0[0], a0[1]), pack_bf16(a0[2], a0[3]), pack_bf16(a1[0], a1[1]), pack_bf16(a1[2], a1[3])));
+        if (!INT8) lsum[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, bp[ct], lsum[ct], 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        const char* vp = buf + vtr[i & 3] + (i >> 2) * 128 + k2 * 32 * RB;
+        const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
+        const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
+        const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) acc[i][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, bp[ct], acc[i][ct], 0, 0, 0);
+      }
+    }
+    if (more)
+      finish_stage(other);
+  }
+
+  // ---- store: acc[i][ct][e] is dim 16 i + 4 lg + e ----------------------------
+  const bool whole = splits == 1;
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const int c0 = wave * 16 * NCT + ct * 16;
+    const int c = c0 + ln;
+    const bool mine = t0 + c / p.G <= t_last && c < tpw * p.G;
+    const float l = INT8 ? sum_over_rows(lsum[ct][0] + lsum[ct][1] + lsum[ct][2] + lsum[ct][3]) : lsum[ct][0];
+    bool odd = l != l;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd = odd || acc[i][ct][e] != acc[i][ct][e];
+    const uint64_t lanes = __ballot(odd && mine);
+    const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
+    auto orow = [&](int col) {
+      return p.out + (static_cast<int64_t>(s.begin + t0 + col / p.G) * p.hq + h * p.G + col % p.G) * D;
+    };
+    auto rec = [&](int col) {
+      return p.part + ((((static_cast<int64_t>(b) * p.plan.qtiles + qt) * p.c.hkv + h) * p.plan.max_splits + split) * kCols + col) * kPart<D>;
+    };
+    if (mine && !((redo >> ln) & 1)) {
+      if (whole) {
+        uint16_t* dst = orow(c) + 4 * lg;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const f32x4 o = acc[i][ct];
+          *reinterpret_cast<u32x2*>(dst + 16 * i) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+        }
+      } else {
+        float* r = rec(c);
+        if (lg == 0) {
+          r[0] = m[ct];
+          r[1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i][ct];
+      }
+    }
+    for (uint32_t left = redo; left != 0; left &= left - 1) {
+      const int col = c0 + __builtin_ctz(left);
+      float mc, lc, oc[D / 64];
+      redo_column<D, INT8>(p, s, table, h, t0 + col / p.G, h * p.G + col % p.G, lo * kKeys, hi * kKeys, lane, mc, lc, oc);
+      store_column<D>(p, whole, whole ? orow(col) : nullptr, whole ? nullptr : rec(col), lane, mc, lc, oc);
+    }
+  }
+}
+
+// ----------------------------------------------------------------- the join --
+// One workgroup a column: D / 4 lanes a run, 256 / (D / 4) runs at a time.  Bound by
+// reading the records once (and the launch).
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
+  constexpr int L = D / 4, N = kThreads / L;
+  __shared__ float sm[N], sl[N];
+  __shared__ f32x4 so[N][L];
+  const int lane = threadIdx.x & 63;
+  const int h = blockIdx.x, b = blockIdx.z;
+  const int qt = blockIdx.y / static_cast<unsigned>(p.plan.tpw * p.G);
+  const int col = blockIdx.y % static_cast<unsigned>(p.plan.tpw * p.G);
+  const Seq s = seq_of(p, b);
+  const int t = qt * p.plan.tpw + col / p.G;
+  const int count = min(s.count, p.n);
+  if (t >= count) return;
+  const int keys = keys_of(p, s, min((qt + 1) * p.plan.tpw, count) - 1);
+  const int splits = splits_of((keys + kKeys - 1) / kKeys, run_tiles(p, lane));
+  if (splits == 1) return;
+  const int slot = threadIdx.x / L, j = threadIdx.x % L;
+  const float* base = p.part + ((((static_cast<int64_t>(b) * p.plan.qtiles + qt) * p.c.hkv + h) * p.plan.max_splits) *
+                                p.plan.cols + col) * kPart<D>;
+  const int64_t step = static_cast<int64_t>(p.plan.cols) * kPart<D>;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = slot; i < splits; i += N) {
+    const float* r = base + i * step;
+    const float mi = r[0], li = r[1];
+    const f32x4 a = *reinterpret_cast<const f32x4*>(r + 4 + 4 * j);
+    if (mi == -INFINITY && li == 0.0f) continue;   // saw nothing
+    const float mn = fmaxf(m, mi);
+    const float wa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(mi - mn);
+    l = l * wa + li * wb;
+    o = o * wa + a * wb;
+    m = mn;
+  }
+  if (j == 0) {
+    sm[slot] = m;
+    sl[slot] = l;
+  }
+  so[slot][j] = o;
+  __syncthreads();
+  if (slot != 0) return;
+  float mt = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mt = fmaxf(mt, sm[i]);
+  float lt = 0.0f;
+  f32x4 ot = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (sm[i] == -INFINITY && sl[i] == 0.0f) continue;
+    const float w = __builtin_amdgcn_exp2f(sm[i] - mt);
+    lt += sl[i] * w;
+    ot += so[i][j] * w;
+  }
+  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  uint16_t* dst = p.out + (static_cast<int64_t>(s.begin + t) * p.hq + h * p.G + col % p.G) * D + 4 * j;
+  *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16(ot[0] * inv, ot[1] * inv), pack_bf16(ot[2] * inv, ot[3] * inv)};
+}
+
+// ----------------------------------------------------------------- the plan --
+Plan plan_of(int B, int T, int n, int hkv, int G, int64_t cap_tokens, bool ragged) {
+  Plan q{};
+  const int64_t rows = static_cast<int64_t>(n) * G;
+  q.few = rows <= kFewCols;
+  q.nct = q.few ? 0 : rows <= 64 ? 1 : 2;
+  q.cols = q.few ? static_cast<int>(rows) : 64 * q.nct;
+  q.tpw = q.few ? n : q.cols / G;
+  q.qtiles = (n + q.tpw - 1) / q.tpw;
+  const int cus = std::max(1, device_cus());
+  const int64_t cap = (cap_tokens + kKeys - 1) / kKeys;
+  // query tiles there are at least: a sequence has one, and all rows fill this many
+  const int64_t least = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw);
+  q.target = (q.few ? 8 : 2) * cus;
+  q.min_tiles = q.few ? 2 : 4;
+  int64_t most = (4 * static_cast<int64_t>(q.target) + least * hkv - 1) / (least * hkv);
+  if (!q.few && least * hkv >= q.target) most = 1;   // the tiles alone fill the device
+  most = std::min({most, (cap + q.min_tiles - 1) / q.min_tiles, static_cast<int64_t>(kMaxSplits), INT64_C(65535) / std::max(B, 1)});
+  q.max_splits = static_cast<int>(std::max<int64_t>(1, most));
+  return q;
+}
+
+template <int D, bool I8>
+void launch(const Params& p, hipStream_t s) {
+  const Plan& q = p.plan;
+  if (q.few)
+    few_kernel<D, I8><<<dim3(p.c.hkv, q.max_splits, p.B), kThreads, 0, s>>>(p);
+  else if (q.nct == 1)
+    many_kernel<D, I8, 1><<<dim3(p.c.hkv, q.qtiles, p.B * q.max_splits), kThreads, 0, s>>>(p);
+  else
+    many_kernel<D, I8, 2><<<dim3(p.c.hkv, q.qtiles, p.B * q.max_splits), kThreads, 0, s>>>(p);
+  if (q.max_splits > 1) merge_kernel<D><<<dim3(p.c.hkv, q.qtiles * q.tpw * p.G, p.B), kThreads, 0, s>>>(p);
+}
+
+int check_sizes(const char* who, int batch, int rows, int max_new, int num_heads, int num_kv_heads, int max_pages,
+                int page_size) {
+  NKV_CHECK_ARG(batch >= 0 && batch <= 65535, "%s: from 0 to 65535 sequences (got %d)", who, batch);
+  NKV_CHECK_ARG(rows >= 0 && max_new >= 1 && max_new <= (1 << 20), "%s: max_new must be from 1 to 2^20 (got %d)", who, max_new);
+  NKV_CHECK_ARG(num_kv_heads >= 1 && num_heads >= num_kv_heads && num_heads % num_kv_heads == 0 && num_kv_heads <= 65535,
+                "%s: num_heads (%d) must be a positive multiple of num_kv_heads (%d)", who, num_heads, num_kv_heads);
+  NKV_CHECK_SUPPORTED(num_heads / num_kv_heads <= 64, "%s: at most 64 query heads a KV head", who);
+  NKV_CHECK_ARG(max_pages >= 1 && static_cast<int64_t>(max_pages) * page_size <= INT32_MAX - 4096,
+                "%s: a page table covers from 1 page to 2^31 - 4096 tokens", who);
+  return NKV_OK;
+}
+
+}  // namespace
+}  // namespace nkv
+
+using namespace nkv;
+
+extern "C" int64_t nkv_paged_attend_workspace(int batch, int rows, int max_new, int num_heads, int num_kv_heads,
+                                              int head_dim, int max_pages, int page_size, int ragged) {
+  if (batch <= 0 || rows <= 0 || check_sizes("", batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return 0;
+  const Plan q = plan_of(batch, rows, max_new, num_kv_heads, num_heads / num_kv_heads,
+                         static_cast<int64_t>(max_pages) * page_size, ragged != 0);
+  return q.max_splits == 1 ? 0 : static_cast<int64_t>(batch) * q.qtiles * num_kv_heads * q.max_splits * q.cols * (head_dim + 4);
+}
+
+extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride,
+                                int64_t head_stride, int64_t token_stride, int pages, int num_kv_heads, int page_size,
+                                int head_dim, const uint16_t* q, int64_t q_stride, int rows, int num_heads,
+                                const int32_t* tables, int64_t table_stride, int max_pages, const int32_t* lengths,
+                                int batch, const int32_t* starts, int max_new, const int64_t* tree, float scale,
+                                uint16_t* out, float* workspace, void* stream) {
+  const char* who = "nkv_paged_attend";
+  Params p{};
+  if (int rc = fill_paged(who, k, v, k_scale, v_scale, page_stride, head_stride, token_stride, pages, num_kv_heads,
+                          page_size, head_dim, &p.c))
+    return rc;
+  if (int rc = check_sizes(who, batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return rc;
+  NKV_CHECK_ARG(starts != nullptr || static_cast<int64_t>(batch) * max_new == rows,
+                "%s: without starts every sequence has max_new rows", who);
+  NKV_CHECK_ARG(tree == nullptr || max_new <= kMaxTree, "%s: a tree has at most %d tokens (got %d)", who, kMaxTree, max_new);
+  NKV_CHECK_ARG(scale > 0.0f && scale < INFINITY, "%s: scale must be positive and finite", who);
+  if (rows == 0) return NKV_OK;
+  NKV_CHECK_ARG(batch >= 1, "%s: rows need a sequence", who);
+  NKV_CHECK_ARG(q && out && tables && lengths, "%s: q, out, tables and lengths must be non-NULL", who);
+  NKV_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 && q_stride % 8 == 0,
+                "%s: rows must lie on 16-byte boundaries", who);
+  const int G = num_heads / num_kv_heads;
+  p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
+  NKV_CHECK_ARG(p.plan.qtiles <= 65535 && static_cast<int64_t>(p.plan.qtiles) * p.plan.tpw * G <= 65535 * (p.plan.max_splits > 1 ? INT64_C(1) : INT64_C(1 << 20)),
+                "%s: too many query rows", who);
+  NKV_CHECK_ARG(p.plan.max_splits == 1 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                "%s: these sizes need a workspace on a 16-byte boundary", who);
+  p.q = q;
+  p.q_ls = q_stride;
+  p.out = out;
+  p.tables = tables;
+  p.table_ls = table_stride;
+  p.max_pages = max_pages;
+  p.lengths = lengths;
+  p.starts = starts;
+  p.tree = reinterpret_cast<const uint64_t*>(tree);
+  p.B = batch;
+  p.T = rows;
+  p.n = max_new;
+  p.hq = num_heads;
+  p.G = G;
+  p.scale_log2 = scale * 1.44269504088896340736f;
+  p.part = workspace;
+  const auto s = static_cast<hipStream_t>(stream);
+  if (head_dim == 128)
+    k_scale ? launch<128, true>(p, s) : launch<128, false>(p, s);
+  else
+    k_scale ? launch<64, true>(p, s) : launch<64, false>(p, s);
+  return launch_status(who);
+}

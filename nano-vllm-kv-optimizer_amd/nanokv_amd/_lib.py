@@ -119,6 +119,8 @@ SIGNATURES = {
     "nkv_paged_read": (_I, [*_CACHE, _P, _I, _P, _P, _P]),
     "nkv_paged_move": (_I, [*_CACHE, _P, _P, _I, _P, _P]),
     "nkv_paged_move_workspace": (_I64, [_I, _I, _I, _I]),
+    "nkv_paged_attend": (_I, [*_CACHE, _P, _I64, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _F, _P, _P, _P]),
+    "nkv_paged_attend_workspace": (_I64, [_I] * 9),
     "nkv_token_logprobs": (_I, [_P, _I, _I64, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P]),
     "nkv_token_logprobs_workspace": (_I64, [_I, _I, _I]),
     "nkv_step_select_ns": (_I64, []),

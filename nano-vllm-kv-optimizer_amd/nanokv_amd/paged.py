@@ -31,7 +31,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .q8 import _asks_gradient, _call, _fine, _quantize_formula
+from .q8 import _asks_gradient, _call, _current_device, _fine, _quantize_formula
 
 _BF16, _I8, _I32, _I64, _F32 = torch.bfloat16, torch.int8, torch.int32, torch.int64, torch.float32
 MAX_TREE = 64          # drafted tokens of a tree: bits of a mask
@@ -300,4 +300,143 @@ def move_paged(cache: PagedKV, src: torch.Tensor, dst: torch.Tensor) -> None:
         _call("paged_move", device, *args, src.data_ptr(), dst.data_ptr(), rows, ws.data_ptr())
 
 
-__all__ = ["PagedKV", "append_paged", "move_paged", "new_paged_kv", "qkv_append_paged", "read_paged"]
+# -- attention -----------------------------------------------------------------
+def tree_masks(parents: torch.Tensor) -> torch.Tensor:
+    """The masks of drafted trees: parents [..., n] (integers, n <= 64) gives for each
+    token the one of its tree that it follows, before it in the tree, or -1 for the cache;
+    int64 [..., n], bit j of token i's mask: it is j or follows j.
+
+    One operation a token: made once for a tree's shape and kept."""
+    if parents.dtype not in (_I32, _I64) or parents.dim() < 1 or not 1 <= parents.shape[-1] <= MAX_TREE:
+        raise ValueError(f"tree_masks: parents must be int32 or int64 [..., n], n from 1 to {MAX_TREE} "
+                         f"(got {parents.dtype} {tuple(parents.shape)})")
+    n = parents.shape[-1]
+    if not parents.is_cuda:
+        order = torch.arange(n)
+        if bool(((parents >= order) | (parents < -1)).any()):
+            raise ValueError("tree_masks: a token's parent comes before it in the tree, or is -1")
+    parents = parents.to(_I64)
+    masks = torch.zeros(parents.shape, dtype=_I64, device=parents.device)
+    for i in range(n):
+        p = parents[..., i:i + 1]
+        above = torch.where(p < 0, torch.zeros_like(p), masks.gather(-1, p.clamp(0, n - 1)))
+        masks[..., i:i + 1] = above | ((1 << i) - (1 << 64) if i == 63 else 1 << i)
+    return masks
+
+
+def _attend_formula(q, cache, tables, lengths, starts, max_new, tree, scale) -> torch.Tensor:
+    pages, hkv, page, d = cache.k.shape
+    T, hq, _ = q.shape
+    out = torch.zeros(T, hq, d)
+    B = lengths.shape[0]
+    starts = [b * max_new for b in range(B + 1)] if starts is None else starts.tolist()
+    for b in range(B):
+        n = min(starts[b + 1] - starts[b], max_new)
+        length = min(max(int(lengths[b]), 0), tables.shape[1] * page)
+        older = length - (starts[b + 1] - starts[b])
+        key = torch.arange(length)
+        ids = tables[b].long()[key // page]
+        ok = (ids >= 0) & (ids < pages)
+        at, off = ids.clamp(0, pages - 1), key % page
+        k, v = (t[at, :, off].float() * (1.0 if c is None else c[at, :, off].unsqueeze(-1))
+                for t, c in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        for i in range(n):
+            t = starts[b] + i
+            seen = key <= older + i
+            if tree is not None:
+                bit = (tree[t] >> (key - older).clamp(0, 63)) & 1
+                seen = (key < older) | (bit.bool() & (key - older < MAX_TREE))
+            seen = seen & ok
+            if not bool(seen.any()):
+                continue
+            x = q[t].float().view(hkv, hq // hkv, d)
+            w = torch.softmax(torch.matmul(x, k[seen].permute(1, 2, 0)) * scale, dim=-1)
+            out[t] = torch.matmul(w, v[seen].transpose(0, 1)).reshape(hq, d)
+    return out.to(q.dtype)
+
+
+def attend_paged(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor, lengths: torch.Tensor, *,
+                 starts: torch.Tensor | None = None, max_new: int | None = None, tree: torch.Tensor | None = None,
+                 scale: float | None = None) -> torch.Tensor:
+    """Attention of new tokens q [T, Hq, D] over their sequences' keys: [T, Hq, D].
+
+    Sequence b has lengths[b] keys in the pages tables[b] (int32 [B, most pages]), its new
+    tokens' (appended before) the last of them.  Its queries are rows starts[b] ..
+    starts[b + 1] - 1 (starts ascending [B + 1]), at most max_new of them (default T; a
+    closer bound launches less; rows behind it give 0); without starts every sequence has T / B.  A
+    query sees the keys up to its own token's, or with ``tree`` (int64 masks [T], at most
+    64 new tokens a sequence: ``tree_masks``) the keys before the new ones and those that its mask names.
+    Rows that see nothing, or that belong to no sequence, are 0.  scale: of the
+    logits (default D^-0.5)."""
+    who = "attend_paged"
+    args = _cache_args(cache, who)
+    pages, hkv, page, d = args[7:]
+    device = cache.k.get_device()
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] < 1 or q.shape[1] % hkv or q.get_device() != device:
+        raise ValueError(f"{who}: q must be [T, a multiple of {hkv}, {d}] on the cache's device "
+                         f"(got {tuple(q.shape)} on {q.device})")
+    T, hq, _ = q.shape
+    if hq // hkv > 64:
+        raise ValueError(f"{who}: at most 64 query heads share a KV head (got {hq // hkv})")
+    _no_gradients(who, q)
+    if (tables.dtype is not _I32 and tables.dtype is not _I64) or tables.dim() != 2 or tables.get_device() != device:
+        raise ValueError(f"{who}: tables must be int32 [B, pages] on the cache's device "
+                         f"(got {tables.dtype} {tuple(tables.shape)} on {tables.device})")
+    B, most = tables.shape
+    lengths = _ints(lengths, _I32, B, device, who, "lengths")
+    if starts is None:
+        if B == 0 and T or B and T % B:
+            raise ValueError(f"{who}: without starts all {B} sequences have as many rows (got {T})")
+        each = T // B if B else 0
+        if max_new is not None and max_new != each:
+            raise ValueError(f"{who}: without starts max_new is T / B = {each} (got {max_new})")
+        max_new = each
+    else:
+        starts = _ints(starts, _I32, B + 1, device, who, "starts")
+        max_new = T if max_new is None else min(int(max_new), T)
+        if T and max_new < 1:
+            raise ValueError(f"{who}: max_new must be positive (got {max_new})")
+    if tree is not None:
+        tree = _ints(tree, _I64, T, device, who, "tree")
+        if max_new > MAX_TREE:
+            raise ValueError(f"{who}: a tree has at most {MAX_TREE} tokens (max_new is {max_new})")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"{who}: scale must be positive and finite (got {scale})")
+    if T and B and (most < 1 or most * page > 2 ** 31 - 4097):
+        raise ValueError(f"{who}: a page table covers from one page to 2^31 - 4097 tokens (got {most} pages of {page})")
+    if device < 0:
+        return _attend_formula(q, cache, tables, lengths, starts, max_new, tree, scale) if T else torch.empty_like(q)
+    if q.dtype is not _BF16:
+        raise ValueError(f"{who}: q must be bfloat16 on the GPU (got {q.dtype})")
+    s = q.stride()
+    if s[2] != 1 or (hq > 1 and s[1] != d) or s[0] % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty_strided((T, hq, d), (hq * d, d, 1), dtype=_BF16, device=q.device)
+    if T == 0:
+        return out
+    if B == 0:
+        return out.zero_()
+    if tables.dtype is not _I32:
+        tables = tables.to(_I32)
+    if tables.stride(1) != 1:
+        tables = tables.contiguous()
+    need = _workspace(device, B, T, max_new, hq, hkv, d, most, page, starts is not None)
+    # (dropped behind the launch: the stream orders its reuse)
+    ws = torch.empty(need, dtype=_F32, device=q.device) if need else None
+    _call("paged_attend", device, *args, q.data_ptr(), q.stride(0), T, hq, tables.data_ptr(), tables.stride(0), most,
+          lengths.data_ptr(), B, None if starts is None else starts.data_ptr(), max_new,
+          None if tree is None else tree.data_ptr(), scale, out.data_ptr(), ws.data_ptr() if need else None)
+    return out
+
+
+def _workspace(device: int, *sizes) -> int:
+    fn = _lib.load().nkv_paged_attend_workspace
+    if device == _current_device():
+        return fn(*sizes)
+    with torch.cuda.device(device):
+        return fn(*sizes)
+
+
+__all__ = ["PagedKV", "append_paged", "attend_paged", "move_paged", "new_paged_kv", "qkv_append_paged", "read_paged",
+           "tree_masks"]

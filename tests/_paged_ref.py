@@ -73,6 +73,7 @@ def attend_ref(q, cache, tables, lengths, starts=None, tree=None, scale=None, n_
         at = torch.tensor([max(0, min(p, pages - 1)) for p in ids], dtype=torch.long)
         off = torch.arange(L) % page
         older = L - n
+        keys, values = k[at, :, off], v[at, :, off]                            # [L, hkv, d]
         for i in range(n):
             t = starts[b] + i
             seen = torch.arange(L) <= older + i
@@ -83,7 +84,7 @@ def attend_ref(q, cache, tables, lengths, starts=None, tree=None, scale=None, n_
             seen &= ok
             if not bool(seen.any()):
                 continue
-            kk, vv = k[at[seen], :, off[seen]], v[at[seen], :, off[seen]]      # [keys, hkv, d]
+            kk, vv = keys[seen], values[seen]
             qq = q[t].view(hkv, g, d)
             w = torch.softmax(torch.einsum("hgd,khd->hgk", qq, kk) * scale, dim=-1)
             out[t] = torch.einsum("hgk,khd->hgd", w, vv).reshape(hq, d)
