@@ -8,7 +8,7 @@
 // The G query heads of a KV head share its keys, so (query, head) pairs are the columns of
 // one product S^T = K Q^T and O^T = V^T P^T on the matrix cores (16x16x32 bf16):
 //   * few_kernel, up to 16 columns (a token, a short draft): bound by reading the keys once.
-//     Every wavefront takes 32-key tiles of its own: K goes from HBM to the operand
+//     Every wavefront works on 32-key tiles by itself: K goes from HBM to the operand
 //     registers, V through the wavefront's LDS (read back transposed), both a tile
 //     ahead; P enters the second product as bf16 high and low parts, as good as fp32.
 //   * many_kernel, tiles of 64 or 128 columns (trees, prompts): 64-key tiles staged in LDS
@@ -18,10 +18,11 @@
 // 8-bit caches: the codes are bf16 exactly; a key's scale multiplies its logits, a
 // value's its weights, both in fp32.
 //
-// Few columns over long caches are split over workgroups by a plan that each of them makes
-// from the lengths (they are in device memory): runs of C 64-key tiles, C such that all
-// sequences together give about `target` runs, so one long sequence among short ones is cut
-// finer than they are.  merge_kernel joins the runs' partial sums.
+// Work split, from the lengths, which are in device memory: few columns: the 32-key tiles of all
+// (sequence, KV head) pairs are one list, and every wavefront of one resident round takes an
+// equal run of it, whatever the sequences' lengths; many columns over long caches: runs of
+// C 64-key tiles, C such that all sequences together give about `target` runs. A pair that
+// several wavefronts (or runs) share is joined from their partial sums by a second kernel.
 //
 // Hidden keys get weight 0, which times an infinite or NaN value is NaN: a column whose
 // result holds a NaN is computed again key by key (redo_column), hidden keys left out.  Keys
@@ -51,7 +52,8 @@ constexpr float kHeadroom = 8.0f;  // a running maximum moves once a logit passe
 
 struct Plan {
   int few, nct, cols, tpw, qtiles;      // columns and tokens of a workgroup's tile, tiles of max_new tokens
-  int max_splits, target, min_tiles;
+  int max_splits, target, min_tiles;    // many columns: the runs
+  int waves;                            // few columns: the wavefronts (0: no pair has two tiles)
 };
 
 struct Params {
@@ -238,11 +240,108 @@ __device__ __forceinline__ void clear_others(const Params& p, const Seq& s, int 
 __device__ __forceinline__ bf16x8 as_bf16(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
 // ---------------------------------------------------------------- few columns --
+// A key or value is read by one workgroup: its line need not stay in the caches.
+__device__ __forceinline__ u32x4 load_once(const char* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
+
 // Operand layout of the 16x16x32 product: lane (ln, lg) holds A[ln][8 lg ..] and
 // B[8 lg ..][ln], and of the result rows 4 lg .. + 3 of column ln.  The 32 keys of the
 // second product are ordered as the first one's results lie: 4 lg + e of the
 // first 16, then of the second, so P never leaves its lane.  In 8 bits a lane takes 16
 // neighbouring codes of a row for two steps of the first product, and q is laid out alike.
+constexpr int kFewKeys = 32;       // keys of a wavefront's tile
+
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Tiles of sequence b for one KV head: at least one if it has queries.
+__device__ __forceinline__ int few_tiles(const Params& p, int b) {
+  int begin = b * p.n, count = p.n;
+  if (p.starts) {
+    begin = min(max(p.starts[b], 0), p.T);
+    count = min(max(p.starts[b + 1], begin), p.T) - begin;
+  }
+  if (count == 0) return 0;
+  const int len = static_cast<int>(min(static_cast<int64_t>(max(p.lengths[b], 0)), static_cast<int64_t>(p.max_pages) << p.c.shift));
+  const int keys = p.tree ? len : min(max(len - count + min(count, p.n), 0), len);
+  return max(1, (keys + kFewKeys - 1) / kFewKeys);
+}
+// The list of all pairs' tiles, sequence by sequence and in it head by head: its length.
+// The wavefronts [0, active) take [w total / active, (w + 1) total / active).
+struct List {
+  int64_t total;
+  int active;
+  __device__ __forceinline__ int64_t lo(int w) const { return static_cast<uint64_t>(w * total) / static_cast<uint32_t>(active); }
+  __device__ __forceinline__ int wave_of(int64_t x) const {
+    return static_cast<int>((static_cast<uint64_t>(x + 1) * active - 1) / static_cast<uint64_t>(total));
+  }
+};
+// The list, and of the tiles before sequence `until` the number of one head: all lanes of the wavefront call it.
+__device__ __forceinline__ List few_list(const Params& p, int lane, int until, int64_t& before) {
+  int64_t all = 0, some = 0;
+  for (int b = lane; b < p.B; b += kWave) {
+    const int t = few_tiles(p, b);
+    all += t;
+    some += b < until ? t : 0;
+  }
+#pragma unroll
+  for (int o = kWave / 2; o > 0; o >>= 1) {
+    all += __shfl_xor(all, o);
+    some += __shfl_xor(some, o);
+  }
+  before = some;
+  List l;
+  l.total = all * p.c.hkv;
+  l.active = static_cast<int>(min(l.total, static_cast<int64_t>(max(p.plan.waves, 1))));
+  return l;
+}
+// The sequence that holds entry x of the list, and the entries before it.
+__device__ __forceinline__ int few_find(const Params& p, int64_t x, int lane, int64_t& before) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kWave) {
+    const int64_t t = b0 + lane < p.B ? static_cast<int64_t>(few_tiles(p, b0 + lane)) * p.c.hkv : 0;
+    int64_t sum = t;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int64_t u = __shfl_up(sum, o);
+      if (lane >= o) sum += u;
+    }
+    const uint64_t past = __ballot(base + sum > x);
+    if (past != 0) {
+      const int at = __ffsll(static_cast<long long>(past)) - 1;
+      before = base + __shfl(sum - t, at);
+      return b0 + at;
+    }
+    base += __shfl(sum, kWave - 1);
+  }
+  before = base;
+  return p.B;
+}
+
+// Zeros for the rows of no sequence and those behind a sequence's max_new-th, by one workgroup.
+__device__ __forceinline__ void clear_rest(const Params& p, int wave, int lane, int d) {
+  auto clear = [&](int from, int to) {
+    const int64_t per = p.hq * d / 8;
+    for (int64_t i = lane; i < (to - from) * per; i += kWave)
+      reinterpret_cast<uint4*>(p.out + from * per * 8)[i] = make_uint4(0u, 0u, 0u, 0u);
+  };
+  if (wave == 0) clear(0, min(max(p.starts[0], 0), p.T));
+  if (wave == 1) clear(min(max(p.starts[p.B], 0), p.T), p.T);
+  for (int b0 = wave * kWave; b0 < p.B; b0 += kThreads) {
+    const int b = min(b0 + lane, p.B - 1);
+    const int begin = min(max(p.starts[b], 0), p.T);
+    const int end = min(max(p.starts[b + 1], begin), p.T);
+    for (uint64_t more = __ballot(b0 + lane < p.B && end - begin > p.n); more != 0; more &= more - 1) {
+      const int at = __ffsll(static_cast<long long>(more)) - 1;
+      clear(__shfl(begin, at) + p.n, __shfl(end, at));
+    }
+  }
+}
+
 template <int D, bool INT8>
 __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
   constexpr int KS = D / 32;                    // steps of the first product
@@ -251,275 +350,258 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
   constexpr int KL = INT8 ? D / 64 : D / 32;    // 16-byte loads of a K row's quarter
   constexpr int VR = INT8 ? 1024 / D : 512 / D; // V rows a load of the wavefront covers
   constexpr int VL = 16 / VR;                   // loads of a 16-key group
-  constexpr int kBuf = 32 * RB;
-  constexpr int kLds = kWaves * kBuf + kWaves * kFewCols * 8;
-  static_assert(kWaves * kFewCols * D * 4 <= kWaves * kBuf, "the join's sums fit where V was");
-  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  constexpr int kBuf = kFewKeys * RB;
+  constexpr int E = INT8 ? 1 : 2;
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kBuf];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int ln = lane & 15, lg = lane >> 4;
-  const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y;
-  const Seq s = seq_of(p, b);
-  if (split == 0) clear_others(p, s, b, h, D);
-  const int count = min(s.count, p.n);
-  if (count == 0) return;
-  const int keys = keys_of(p, s, count - 1);
-  const int tiles = (keys + kKeys - 1) / kKeys;
-  const int run = run_tiles(p, lane);
-  const int splits = splits_of(tiles, run);
-  if (split >= splits) return;
-  const int lo = static_cast<int>(static_cast<int64_t>(split) * tiles / splits) * kKeys;
-  const int hi = min(static_cast<int>(static_cast<int64_t>(split + 1) * tiles / splits) * kKeys, keys);
-  const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
-
-  // column ln: query token, head, what it sees
-  const int t = ln / p.G;
-  const bool mine = t < count;
-  const int head = h * p.G + ln % p.G;
-  const int limit = mine ? s.older + t : -1;
-  const uint64_t mask = p.tree && mine ? p.tree[s.begin + t] : 0;
-  bf16x8 bq[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    const int d0 = INT8 ? 64 * (ks >> 1) + 16 * lg + 8 * (ks & 1) : 32 * ks + 8 * lg;
-    if (mine) v = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + head * D + d0);
-    bq[ks] = as_bf16(v);
+  const int groups = p.plan.waves / kWaves;
+  if (static_cast<int>(blockIdx.x) == groups) {   // (there is one more with starts)
+    clear_rest(p, wave, lane, D);
+    return;
   }
-
+  // wavefront w: the first ones of all workgroups, then the second ones (few tiles lie on all CUs)
+  const int w = blockIdx.x + groups * wave;
+  int64_t before;
+  const List list = few_list(p, lane, 0, before);
+  if (w >= list.active) return;
+  const int64_t from = uniform(list.lo(w)), to = uniform(list.lo(w + 1));
+  int b = __builtin_amdgcn_readfirstlane(few_find(p, from, lane, before));
   char* buf = lds + wave * kBuf;
-  constexpr int E = INT8 ? 1 : 2;
-  uint4 kr[2][KL], vr[2][VL];
-  float4 ksc[2], vsc[2];
-  // the tile's keys are in which 16-key groups' pages (bit 0, 1)
-  auto load = [&](int key, uint4 (&kd)[2][KL], uint4 (&vd)[2][VL], float4 (&kss)[2], float4 (&vss)[2]) {
-    int have = 0;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int key0 = key + 16 * g;
-      const int id = page_of(p, table, s, key0);
-      if (id < 0) {
-#pragma unroll
-        for (int i = 0; i < KL; ++i) kd[g][i] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int i = 0; i < VL; ++i) vd[g][i] = make_uint4(0u, 0u, 0u, 0u);
-        kss[g] = vss[g] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        continue;
-      }
-      have |= 1 << g;
-      const int in = key0 & (p.c.page - 1);
-      const int64_t base = (p.c.sp * id + p.c.sh * h + p.c.st * in) * E;
-      const int last = s.len - 1 - key0;     // rows behind it are read as it is
-      const char* kp = p.c.k + base + static_cast<int64_t>(min(ln, last)) * (p.c.st * E);
-#pragma unroll
-      for (int i = 0; i < KL; ++i) kd[g][i] = *reinterpret_cast<const uint4*>(kp + i * 64 + lg * 16);
-      constexpr int PC = 64 / VR;            // 16-byte pieces of a row
-#pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        const int row = min(VR * i + lane / PC, last);
-        vd[g][i] = *reinterpret_cast<const uint4*>(p.c.v + base + static_cast<int64_t>(row) * (p.c.st * E) + (lane % PC) * 16);
-      }
-      if (INT8) {
-        const int64_t at = ((static_cast<int64_t>(id) * p.c.hkv + h) << p.c.shift) + in + 4 * lg;
-        kss[g] = *reinterpret_cast<const float4*>(p.c.ks + at);
-        vss[g] = *reinterpret_cast<const float4*>(p.c.vs + at);
-      }
-    }
-    return have;
-  };
-  // V rows to LDS: row r at r RB, its 16-byte chunk c at position c ^ 2 (r & 3)
-  auto put = [&](const uint4 (&vd)[2][VL]) {
-    constexpr int PC = 64 / VR;
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        const int row = 16 * g + VR * i + lane / PC;
-        const int c = lane % PC;
-        if (INT8) {
-          const uint4 w = vd[g][i];
-          *reinterpret_cast<uint4*>(buf + row * RB + (((2 * c) ^ (2 * (row & 3))) << 4)) = i8x8_to_bf16x8(w.x, w.y);
-          *reinterpret_cast<uint4*>(buf + row * RB + (((2 * c + 1) ^ (2 * (row & 3))) << 4)) = i8x8_to_bf16x8(w.z, w.w);
-        } else {
-          *reinterpret_cast<uint4*>(buf + row * RB + ((c ^ (2 * (row & 3))) << 4)) = vd[g][i];
-        }
-      }
-  };
   // transposing read: keys 4 lg .. + 3 (+ 16 g) of dims 16 dt + ln
   int vtr[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x)
     vtr[x] = (4 * lg + (ln >> 2)) * RB + ((2 * (x ^ (ln >> 2)) + ((ln & 3) >> 1)) << 4) + 8 * (ln & 1);
+  const int t = ln / p.G;   // column ln: query token, head of its group
+  const int e0 = ln % p.G;
 
-  f32x4 acc[DT];
+  int64_t left = to - from;                                    // tiles to do
+  int first = static_cast<int>(from - uniform(before));        // the first one's place in the sequence
+  for (; left > 0 && b < p.B; ++b) {
+    const Seq s = seq_of(p, b);
+    const int count = min(s.count, p.n);
+    if (count == 0) continue;
+    const int keys = keys_of(p, s, count - 1);
+    const int per_head = max(1, (keys + kFewKeys - 1) / kFewKeys);
+    const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
+    const bool mine = t < count;
+    const int limit = mine ? s.older + t : -1;
+    const uint64_t mask = p.tree && mine ? p.tree[s.begin + t] : 0;
+    for (int h = first / per_head; h < p.c.hkv && left > 0; ++h) {
+      const int tile0 = first - h * per_head;       // (0 from the second pair on)
+      const int ntile = static_cast<int>(min(static_cast<int64_t>(per_head - tile0), left));
+      first = (h + 1) * per_head;
+      left -= ntile;
+      const int lo = tile0 * kFewKeys, hi = min(lo + ntile * kFewKeys, keys);
+      const int head = h * p.G + e0;
+      bf16x8 bq[KS];
 #pragma unroll
-  for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -INFINITY, l = 0.0f;   // the column's maximum (log2 units), the lane's part of its sum
-
-  int key = lo + 32 * wave, have = 0;
-  if (key < hi) {
-    have = load(key, kr, vr, ksc, vsc);
-    put(vr);
-  }
-  while (key < hi) {
-    const int next = key + 32 * kWaves;
-    uint4 kn[2][KL], vn[2][VL];
-    float4 ksn[2], vsn[2];
-    int have_n = 0;
-    if (next < hi) have_n = load(next, kn, vn, ksn, vsn);
-
-    f32x4 S[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        bf16x8 a;
+      for (int ks = 0; ks < KS; ++ks) {
+        u32x4 v = u32x4{0u, 0u, 0u, 0u};
+        const int d0 = INT8 ? 64 * (ks >> 1) + 16 * lg + 8 * (ks & 1) : 32 * ks + 8 * lg;
+        if (mine) v = *reinterpret_cast<const u32x4*>(p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + head * D + d0);
+        bq[ks] = __builtin_bit_cast(bf16x8, v);
+      }
+      u32x4 kr[2][KL], vr[2][VL];
+      f32x4 ksc[2], vsc[2];
+      // 16 keys of one page from key0; whether they have one (page 0 is read where not: loads
+      // without branches leave the compiler nothing to merge behind them, 30 registers less)
+      auto load_group = [&](int key0, u32x4 (&kd)[KL], u32x4 (&vd)[VL], f32x4& kss, f32x4& vss) {
+        const int id = page_of(p, table, s, key0);
+        const int page = max(id, 0);
+        const int in = key0 & (p.c.page - 1);
+        const int64_t base = (p.c.sp * page + p.c.sh * h + p.c.st * in) * E;
+        const int last = max(s.len - 1 - key0, 0);     // rows behind it are read as it is
+        const int row_bytes = static_cast<int>(p.c.st) * E;
+        const char* kp = p.c.k + base + min(ln, last) * row_bytes + lg * 16;
+    #pragma unroll
+        for (int i = 0; i < KL; ++i) kd[i] = load_once(kp + i * 64);
+        constexpr int PC = 64 / VR;            // 16-byte pieces of a row
+    #pragma unroll
+        for (int i = 0; i < VL; ++i)
+          vd[i] = load_once(p.c.v + base + min(VR * i + lane / PC, last) * row_bytes + (lane % PC) * 16);
         if (INT8) {
-          const uint4 w = kr[g][ks >> 1];
-          a = as_bf16(ks & 1 ? i8x8_to_bf16x8(w.z, w.w) : i8x8_to_bf16x8(w.x, w.y));
-        } else {
-          a = as_bf16(kr[g][ks % KL]);
+          const int64_t at = ((static_cast<int64_t>(page) * p.c.hkv + h) << p.c.shift) + in + 4 * lg;
+          kss = *reinterpret_cast<const f32x4*>(p.c.ks + at);
+          vss = *reinterpret_cast<const f32x4*>(p.c.vs + at);
         }
-        S[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ks], S[g], 0, 0, 0);
+        return id >= 0;
+      };
+      // a tile of 32: bit g of the result: its group g has a page
+      auto load = [&](int key, u32x4 (&kd)[2][KL], u32x4 (&vd)[2][VL], f32x4 (&kss)[2], f32x4 (&vss)[2]) {
+        const bool a = load_group(key, kd[0], vd[0], kss[0], vss[0]);
+        const bool b = load_group(key + 16, kd[1], vd[1], kss[1], vss[1]);
+        return (a ? 1 : 0) | (b ? 2 : 0);
+      };
+      // V rows to LDS: row r at r RB, its 16-byte chunk c at position c ^ 2 (r & 3)
+      auto put = [&](const u32x4 (&vd)[2][VL]) {
+        constexpr int PC = 64 / VR;
+    #pragma unroll
+        for (int g = 0; g < 2; ++g)
+    #pragma unroll
+          for (int i = 0; i < VL; ++i) {
+            const int row = 16 * g + VR * i + lane / PC;
+            const int c = lane % PC;
+            if (INT8) {
+              const u32x4 w = vd[g][i];
+              *reinterpret_cast<uint4*>(buf + row * RB + (((2 * c) ^ (2 * (row & 3))) << 4)) = i8x8_to_bf16x8(w[0], w[1]);
+              *reinterpret_cast<uint4*>(buf + row * RB + (((2 * c + 1) ^ (2 * (row & 3))) << 4)) = i8x8_to_bf16x8(w[2], w[3]);
+            } else {
+              *reinterpret_cast<u32x4*>(buf + row * RB + ((c ^ (2 * (row & 3))) << 4)) = vd[g][i];
+            }
+          }
+      };
+      f32x4 acc[DT];
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      float m = -INFINITY, l = 0.0f;   // the column's maximum (log2 units), the lane's part of its sum
+      int key = lo, have = 0;
+      if (key < hi) {
+        have = load(key, kr, vr, ksc, vsc);
+        put(vr);
       }
-    float y[2][4];
+      while (key < hi) {
+        const int next = key + kFewKeys;
+        u32x4 kn[2][KL], vn[2][VL];
+        f32x4 ksn[2], vsn[2];
+        int have_n = 0;
+        if (next < hi) have_n = load(next, kn, vn, ksn, vsn);
+        if (INT8) {
+          // (an empty asm: the compiler would take the codes apart an iteration ahead, in 64 more
+          // registers than there are)
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float sc[4] = {ksc[g].x, ksc[g].y, ksc[g].z, ksc[g].w};
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[g][e] = S[g][e] * (INT8 ? sc[e] * p.scale_log2 : p.scale_log2);
-    }
-    if (have != 3 || key + 31 > (p.tree ? s.older - 1 : s.older)) {
-      uint64_t bits = mine ? seen_bits(mask, p.tree != nullptr, limit, s, key) : 0;
+            for (int i = 0; i < KL; ++i) asm volatile("" : "+v"(kr[g][i]));
+        }
+        f32x4 S[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (!((have >> g) & 1)) bits &= ~(0xffffull << (16 * g));
-        const uint32_t own = static_cast<uint32_t>(bits >> (16 * g + 4 * lg));
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[g][e] = where_bit(y[g][e], own, e);
+          for (int g = 0; g < 2; ++g) {
+            bf16x8 a;
+            if (INT8) {
+              const u32x4 w = kr[g][ks >> 1];
+              a = as_bf16(ks & 1 ? i8x8_to_bf16x8(w[2], w[3]) : i8x8_to_bf16x8(w[0], w[1]));
+            } else {
+              a = __builtin_bit_cast(bf16x8, kr[g][ks % KL]);
+            }
+            S[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ks], S[g], 0, 0, 0);
+          }
+        float y[2][4];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 sc = ksc[g];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[g][e] = S[g][e] * (INT8 ? sc[e] * p.scale_log2 : p.scale_log2);
+        }
+        if (have != 3 || key + 31 > (p.tree ? s.older - 1 : s.older)) {
+          uint64_t bits = mine ? seen_bits(mask, p.tree != nullptr, limit, s, key) : 0;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!((have >> g) & 1)) bits &= ~(0xffffull << (16 * g));
+            const uint32_t own = static_cast<uint32_t>(bits >> (16 * g + 4 * lg));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[g][e] = where_bit(y[g][e], own, e);
+          }
+        }
+        float top = y[0][0];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, y[g][e]);
+        if (__any(top > m + kHeadroom || (m == -INFINITY && top > m))) {
+          const float mn = fmaxf(m, max_over_rows(top));
+          const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= alpha;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        bf16x8 hi8, lo8;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 sc = vsc[g];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float w = __builtin_amdgcn_exp2f(y[g][e] - base);
+            l += w;
+            if (INT8) w = w == 0.0f ? 0.0f : w * sc[e];   // (the scale of a hidden key may be anything)
+            const __bf16 a = static_cast<__bf16>(w);
+            hi8[4 * g + e] = a;
+            lo8[4 * g + e] = static_cast<__bf16>(w - static_cast<float>(a));
+          }
+        }
+        wave_lds_sync();
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const char* vp = buf + vtr[i & 3] + (i >> 2) * 128;
+          const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
+          const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
+          const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi8, acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo8, acc[i], 0, 0, 0);
+        }
+        wave_lds_sync();
+        if (next < hi) {
+          put(vn);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+#pragma unroll
+            for (int i = 0; i < KL; ++i) kr[g][i] = kn[g][i];
+            ksc[g] = ksn[g];
+            vsc[g] = vsn[g];
+          }
+        }
+        have = have_n;
+        key = next;
       }
-    }
-    float top = y[0][0];
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, y[g][e]);
-    if (__any(top > m + kHeadroom || (m == -INFINITY && top > m))) {
-      const float mn = fmaxf(m, max_over_rows(top));
-      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i] *= alpha;
-    }
-    const float base = m == -INFINITY ? 0.0f : m;
-    bf16x8 hi8, lo8;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float sc[4] = {vsc[g].x, vsc[g].y, vsc[g].z, vsc[g].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float w = __builtin_amdgcn_exp2f(y[g][e] - base);
-        l += w;
-        if (INT8) w = w == 0.0f ? 0.0f : w * sc[e];   // (the scale of a hidden key may be anything)
-        const __bf16 a = static_cast<__bf16>(w);
-        hi8[4 * g + e] = a;
-        lo8[4 * g + e] = static_cast<__bf16>(w - static_cast<float>(a));
-      }
-    }
-    wave_lds_sync();
-#pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      const char* vp = buf + vtr[i & 3] + (i >> 2) * 128;
-      const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
-      const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
-      const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
-      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi8, acc[i], 0, 0, 0);
-      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo8, acc[i], 0, 0, 0);
-    }
-    wave_lds_sync();
-    if (next < hi) {
-      put(vn);
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-#pragma unroll
-        for (int i = 0; i < KL; ++i) kr[g][i] = kn[g][i];
-        ksc[g] = ksn[g];
-        vsc[g] = vsn[g];
-      }
-    }
-    have = have_n;
-    key = next;
-  }
-  l = sum_over_rows(l);
+      l = sum_over_rows(l);
 
-  // ---- the wavefronts' sums joined: thread (column, D / 16 dims) -------------
-  float* sums = reinterpret_cast<float*>(lds);                        // [wave][column][D]
-  float* ml = reinterpret_cast<float*>(lds + kWaves * kBuf);          // [wave][column][2]
-  __syncthreads();
+      // ---- the pair's result, or this wavefront's part of it: record 2 w of a pair that
+      // began before the wavefront's run, 2 w + 1 of one that goes on behind it
+      const bool whole = ntile == per_head;
+      bool odd = l != l;
 #pragma unroll
-  for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(sums + (wave * kFewCols + ln) * D + 16 * i + 4 * lg) = acc[i];
-  if (lg == 0) {
-    ml[(wave * kFewCols + ln) * 2] = m;
-    ml[(wave * kFewCols + ln) * 2 + 1] = l;
-  }
-  __syncthreads();
-  const int col = threadIdx.x >> 4;
-  const int cols = count * p.G;
-  const int d0 = (threadIdx.x & 15) * (D / 16);
-  float mt = -INFINITY;
+      for (int i = 0; i < DT; ++i)
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) mt = fmaxf(mt, ml[(i * kFewCols + col) * 2]);
-  float lt = 0.0f, o[D / 16];
+        for (int e = 0; e < 4; ++e) odd = odd || acc[i][e] != acc[i][e];
+      const int cols = count * p.G;
+      const uint64_t lanes = __ballot(odd && ln < cols);
+      const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
+      auto orow = [&](int c) { return p.out + (static_cast<int64_t>(s.begin + c / p.G) * p.hq + h * p.G + c % p.G) * D; };
+      auto rec = [&](int c) { return p.part + (static_cast<int64_t>(2 * w + (tile0 > 0 ? 0 : 1)) * p.plan.cols + c) * kPart<D>; };
+      if (ln < cols && !((redo >> ln) & 1)) {
+        if (whole) {
+          uint16_t* dst = orow(ln) + 4 * lg;
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e) o[e] = 0.0f;
+          for (int i = 0; i < DT; ++i)
+            *reinterpret_cast<u32x2*>(dst + 16 * i) =
+                u32x2{pack_bf16(acc[i][0] * inv, acc[i][1] * inv), pack_bf16(acc[i][2] * inv, acc[i][3] * inv)};
+        } else {
+          float* r = rec(ln);
+          if (lg == 0) {
+            r[0] = m;
+            r[1] = l;
+          }
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    const float mi = ml[(i * kFewCols + col) * 2];
-    const float li = ml[(i * kFewCols + col) * 2 + 1];
-    const float w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mt);
-    if (mi == -INFINITY && li == 0.0f) continue;      // saw nothing (hidden values may have made its sums NaN)
-    lt += li * w;
-#pragma unroll
-    for (int e = 0; e < D / 16; ++e) o[e] += sums[(i * kFewCols + col) * D + d0 + e] * w;
-  }
-  bool odd = lt != lt;
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e) odd = odd || o[e] != o[e];
-  const uint64_t redo = __ballot(odd && col < cols);
-  const bool whole = splits == 1;
-  auto orow = [&](int c) {
-    return p.out + (static_cast<int64_t>(s.begin + c / p.G) * p.hq + h * p.G + c % p.G) * D;
-  };
-  auto rec = [&](int c) {
-    return p.part + (((static_cast<int64_t>(b) * p.c.hkv + h) * p.plan.max_splits + split) * p.plan.cols + c) * kPart<D>;
-  };
-  const bool again = (redo >> (lane & 48)) & 0xffff;   // the lane's column
-  if (col < cols && !again) {
-    if (whole) {
-      uint16_t* dst = orow(col) + d0;
-      const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-#pragma unroll
-      for (int e = 0; e < D / 16; e += 4)
-        *reinterpret_cast<u32x2*>(dst + e) = u32x2{pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv)};
-    } else {
-      float* r = rec(col);
-      if (d0 == 0) {
-        r[0] = mt;
-        r[1] = lt;
+          for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i];
+        }
       }
-#pragma unroll
-      for (int e = 0; e < D / 16; e += 4) *reinterpret_cast<f32x4*>(r + 4 + d0 + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+      for (uint32_t todo = redo; todo != 0; todo &= todo - 1) {
+        const int c = __builtin_ctz(todo);
+        float mc, lc, oc[D / 64];
+        redo_column<D, INT8>(p, s, table, h, c / p.G, h * p.G + c % p.G, lo, hi, lane, mc, lc, oc);
+        store_column<D>(p, whole, whole ? orow(c) : nullptr, whole ? nullptr : rec(c), lane, mc, lc, oc);
+      }
+      wave_lds_sync();
     }
-  }
-  if (redo == 0) return;
-  for (int i = 0; i < 4; ++i) {   // the wavefront's four columns
-    if (((redo >> (16 * i)) & 0xffff) == 0) continue;
-    const int c = 4 * wave + i;
-    float mc, lc, oc[D / 64];
-    redo_column<D, INT8>(p, s, table, h, c / p.G, h * p.G + c % p.G, lo, hi, lane, mc, lc, oc);
-    store_column<D>(p, whole, whole ? orow(c) : nullptr, whole ? nullptr : rec(c), lane, mc, lc, oc);
+    first = 0;
   }
 }
 
@@ -846,17 +928,34 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
   const int t = qt * p.plan.tpw + col / p.G;
   const int count = min(s.count, p.n);
   if (t >= count) return;
-  const int keys = keys_of(p, s, min((qt + 1) * p.plan.tpw, count) - 1);
-  const int splits = splits_of((keys + kKeys - 1) / kKeys, run_tiles(p, lane));
-  if (splits == 1) return;
   const int slot = threadIdx.x / L, j = threadIdx.x % L;
-  const float* base = p.part + ((((static_cast<int64_t>(b) * p.plan.qtiles + qt) * p.c.hkv + h) * p.plan.max_splits) *
-                                p.plan.cols + col) * kPart<D>;
-  const int64_t step = static_cast<int64_t>(p.plan.cols) * kPart<D>;
+  int splits;
+  int64_t first, next;    // the first record, and the second (those that follow lie `step` on)
+  int64_t step;
+  if (p.plan.few) {
+    int64_t before;
+    const List list = few_list(p, lane, b, before);
+    const int tiles = few_tiles(p, b);
+    const int64_t x = before * p.c.hkv + static_cast<int64_t>(h) * tiles;
+    const int w0 = list.wave_of(x), w1 = list.wave_of(x + tiles - 1);
+    splits = w1 - w0 + 1;
+    first = 2 * static_cast<int64_t>(w0) + 1;
+    next = 2 * static_cast<int64_t>(w0) + 2;
+    step = 2;
+  } else {
+    const int keys = keys_of(p, s, min((qt + 1) * p.plan.tpw, count) - 1);
+    splits = splits_of((keys + kKeys - 1) / kKeys, run_tiles(p, lane));
+    first = ((static_cast<int64_t>(b) * p.plan.qtiles + qt) * p.c.hkv + h) * p.plan.max_splits;
+    next = first + 1;
+    step = 1;
+  }
+  if (splits == 1) return;
+  const int64_t size = static_cast<int64_t>(p.plan.cols) * kPart<D>;
+  const float* base = p.part + col * kPart<D>;
   float m = -INFINITY, l = 0.0f;
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int i = slot; i < splits; i += N) {
-    const float* r = base + i * step;
+    const float* r = base + (i == 0 ? first : next + (i - 1) * step) * size;
     const float mi = r[0], li = r[1];
     const f32x4 a = *reinterpret_cast<const f32x4*>(r + 4 + 4 * j);
     if (mi == -INFINITY && li == 0.0f) continue;   // saw nothing
@@ -903,10 +1002,15 @@ Plan plan_of(int B, int T, int n, int hkv, int G, int64_t cap_tokens, bool ragge
   const int64_t cap = (cap_tokens + kKeys - 1) / kKeys;
   // query tiles there are at least: a sequence has one, and all rows fill this many
   const int64_t least = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw);
-  q.target = (q.few ? 8 : 2) * cus;
-  q.min_tiles = q.few ? 2 : 4;
+  if (q.few) {   // one resident round: two workgroups a CU
+    q.max_splits = 1;
+    q.waves = cap_tokens > kFewKeys ? 2 * kWaves * cus : 0;
+    return q;
+  }
+  q.target = 2 * cus;
+  q.min_tiles = 4;
   int64_t most = (4 * static_cast<int64_t>(q.target) + least * hkv - 1) / (least * hkv);
-  if (!q.few && least * hkv >= q.target) most = 1;   // the tiles alone fill the device
+  if (least * hkv >= q.target) most = 1;   // the tiles alone fill the device
   most = std::min({most, (cap + q.min_tiles - 1) / q.min_tiles, static_cast<int64_t>(kMaxSplits), INT64_C(65535) / std::max(B, 1)});
   q.max_splits = static_cast<int>(std::max<int64_t>(1, most));
   return q;
@@ -915,13 +1019,25 @@ Plan plan_of(int B, int T, int n, int hkv, int G, int64_t cap_tokens, bool ragge
 template <int D, bool I8>
 void launch(const Params& p, hipStream_t s) {
   const Plan& q = p.plan;
-  if (q.few)
-    few_kernel<D, I8><<<dim3(p.c.hkv, q.max_splits, p.B), kThreads, 0, s>>>(p);
-  else if (q.nct == 1)
+  if (q.few) {
+    // (no pair has two tiles: a wavefront takes as many as it needs)
+    const int waves = q.waves > 0 ? q.waves : kWaves * static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.B) * p.c.hkv + kWaves - 1) / kWaves, 4096));
+    Params f = p;
+    f.plan.waves = waves;
+    few_kernel<D, I8><<<waves / kWaves + (p.starts ? 1 : 0), kThreads, 0, s>>>(f);
+  } else if (q.nct == 1) {
     many_kernel<D, I8, 1><<<dim3(p.c.hkv, q.qtiles, p.B * q.max_splits), kThreads, 0, s>>>(p);
-  else
+  } else {
     many_kernel<D, I8, 2><<<dim3(p.c.hkv, q.qtiles, p.B * q.max_splits), kThreads, 0, s>>>(p);
-  if (q.max_splits > 1) merge_kernel<D><<<dim3(p.c.hkv, q.qtiles * q.tpw * p.G, p.B), kThreads, 0, s>>>(p);
+  }
+  if (q.max_splits > 1 || q.waves > 0) merge_kernel<D><<<dim3(p.c.hkv, q.qtiles * q.tpw * p.G, p.B), kThreads, 0, s>>>(p);
+}
+
+// Floats of the partial sums.
+int64_t part_floats(const Plan& q, int B, int hkv, int head_dim) {
+  const int64_t records = q.few ? 2 * static_cast<int64_t>(q.waves)
+                                : q.max_splits == 1 ? 0 : static_cast<int64_t>(B) * q.qtiles * hkv * q.max_splits;
+  return records * q.cols * (head_dim + 4);
 }
 
 int check_sizes(const char* who, int batch, int rows, int max_new, int num_heads, int num_kv_heads, int max_pages,
@@ -946,7 +1062,7 @@ extern "C" int64_t nkv_paged_attend_workspace(int batch, int rows, int max_new, 
   if (batch <= 0 || rows <= 0 || check_sizes("", batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return 0;
   const Plan q = plan_of(batch, rows, max_new, num_kv_heads, num_heads / num_kv_heads,
                          static_cast<int64_t>(max_pages) * page_size, ragged != 0);
-  return q.max_splits == 1 ? 0 : static_cast<int64_t>(batch) * q.qtiles * num_kv_heads * q.max_splits * q.cols * (head_dim + 4);
+  return part_floats(q, batch, num_kv_heads, head_dim);
 }
 
 extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride,
@@ -963,6 +1079,8 @@ extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale
   if (int rc = check_sizes(who, batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return rc;
   NKV_CHECK_ARG(starts != nullptr || static_cast<int64_t>(batch) * max_new == rows,
                 "%s: without starts every sequence has max_new rows", who);
+  NKV_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size / kFewKeys * num_kv_heads <= INT32_MAX - num_kv_heads,
+                "%s: a page table and KV heads past 2^31 pieces of 32 keys", who);
   NKV_CHECK_ARG(tree == nullptr || max_new <= kMaxTree, "%s: a tree has at most %d tokens (got %d)", who, kMaxTree, max_new);
   NKV_CHECK_ARG(scale > 0.0f && scale < INFINITY, "%s: scale must be positive and finite", who);
   if (rows == 0) return NKV_OK;
@@ -974,7 +1092,7 @@ extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale
   p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
   NKV_CHECK_ARG(p.plan.qtiles <= 65535 && static_cast<int64_t>(p.plan.qtiles) * p.plan.tpw * G <= 65535 * (p.plan.max_splits > 1 ? INT64_C(1) : INT64_C(1 << 20)),
                 "%s: too many query rows", who);
-  NKV_CHECK_ARG(p.plan.max_splits == 1 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+  NKV_CHECK_ARG(part_floats(p.plan, batch, num_kv_heads, head_dim) == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "%s: these sizes need a workspace on a 16-byte boundary", who);
   p.q = q;
   p.q_ls = q_stride;
