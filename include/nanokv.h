@@ -773,7 +773,8 @@ int64_t nkv_paged_move_workspace(int num_kv_heads, int head_dim, int int8, int r
  * workspace: nkv_paged_attend_workspace(...) floats, 16-byte aligned (NULL where that is 0;
  * ragged: starts != NULL), asked with the launch's device current.  Calls that may overlap take two.
  * Constraints: batch <= 65535, Hq / Hkv <= 64, max_new <= 2^20, scale > 0,
- * max_pages * page_size < 2^31 - 4095.
+ * max_pages * page_size < 2^31 - 4096, and fewer than 2^31 pieces of 32 keys in batch such
+ * tables times Hkv.
  */
 int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride, int64_t head_stride,
                      int64_t token_stride, int pages, int num_kv_heads, int page_size, int head_dim,

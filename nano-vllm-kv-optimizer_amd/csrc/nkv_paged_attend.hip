@@ -97,6 +97,23 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   return s;
 }
 
+// The same for a sequence of the lane's own.
+__device__ __forceinline__ Seq lane_seq(const Params& p, int b) {
+  Seq s;
+  int end;
+  if (p.starts) {
+    s.begin = min(max(p.starts[b], 0), p.T);
+    end = min(max(p.starts[b + 1], s.begin), p.T);
+  } else {
+    s.begin = b * p.n;
+    end = s.begin + p.n;
+  }
+  s.count = end - s.begin;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(p.lengths[b], 0)), static_cast<int64_t>(p.max_pages) << p.c.shift));
+  s.older = s.len - s.count;
+  return s;
+}
+
 // Tiles of a run (C): all lanes of the wavefront call it.
 __device__ __forceinline__ int run_tiles(const Params& p, int lane) {
   if (p.plan.max_splits == 1) return INT32_MAX;
@@ -252,74 +269,55 @@ __device__ __forceinline__ u32x4 load_once(const char* p) {
 // neighbouring codes of a row for two steps of the first product, and q is laid out alike.
 constexpr int kFewKeys = 32;       // keys of a wavefront's tile
 
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
-  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+// Inclusive sum over the lanes of the wavefront (row shifts, then the rows' ends carried on).
+__device__ __forceinline__ int lane_sums(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
 }
 
-// Tiles of sequence b for one KV head: at least one if it has queries.
-__device__ __forceinline__ int few_tiles(const Params& p, int b) {
-  int begin = b * p.n, count = p.n;
-  if (p.starts) {
-    begin = min(max(p.starts[b], 0), p.T);
-    count = min(max(p.starts[b + 1], begin), p.T) - begin;
-  }
-  if (count == 0) return 0;
-  const int len = static_cast<int>(min(static_cast<int64_t>(max(p.lengths[b], 0)), static_cast<int64_t>(p.max_pages) << p.c.shift));
-  const int keys = p.tree ? len : min(max(len - count + min(count, p.n), 0), len);
-  return max(1, (keys + kFewKeys - 1) / kFewKeys);
+// Tiles of a sequence for one KV head: at least one if it has queries.
+__device__ __forceinline__ int few_tiles(const Params& p, const Seq& s) {
+  const int count = min(s.count, p.n);
+  return count == 0 ? 0 : max(1, (keys_of(p, s, count - 1) + kFewKeys - 1) / kFewKeys);
 }
-// The list of all pairs' tiles, sequence by sequence and in it head by head: its length.
-// The wavefronts [0, active) take [w total / active, (w + 1) total / active).
+// The tiles of all pairs are one list, sequence by sequence and in it head by head
+// (fewer than 2^31: the caller checked).  The wavefronts [0, active) take equal runs of it.
 struct List {
-  int64_t total;
-  int active;
-  __device__ __forceinline__ int64_t lo(int w) const { return static_cast<uint64_t>(w * total) / static_cast<uint32_t>(active); }
-  __device__ __forceinline__ int wave_of(int64_t x) const {
-    return static_cast<int>((static_cast<uint64_t>(x + 1) * active - 1) / static_cast<uint64_t>(total));
+  int total, active, share, more;   // the first `more` wavefronts take share + 1
+  __device__ __forceinline__ void split(int tiles, int waves) {
+    total = tiles;
+    active = min(total, waves);
+    share = active == total ? 1 : static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(active));
+    more = total - share * active;
+  }
+  __device__ __forceinline__ int lo(int w) const { return w * share + min(w, more); }
+  __device__ __forceinline__ int wave_of(int x) const {
+    if (share == 1 && more == 0) return x;
+    const uint32_t edge = static_cast<uint32_t>(more) * (share + 1), at = x;
+    return at < edge ? at / static_cast<uint32_t>(share + 1) : more + (at - edge) / static_cast<uint32_t>(share);
   }
 };
-// The list, and of the tiles before sequence `until` the number of one head: all lanes of the wavefront call it.
-__device__ __forceinline__ List few_list(const Params& p, int lane, int until, int64_t& before) {
-  int64_t all = 0, some = 0;
-  for (int b = lane; b < p.B; b += kWave) {
-    const int t = few_tiles(p, b);
-    all += t;
-    some += b < until ? t : 0;
-  }
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) {
-    all += __shfl_xor(all, o);
-    some += __shfl_xor(some, o);
-  }
-  before = some;
-  List l;
-  l.total = all * p.c.hkv;
-  l.active = static_cast<int>(min(l.total, static_cast<int64_t>(max(p.plan.waves, 1))));
-  return l;
-}
-// The sequence that holds entry x of the list, and the entries before it.
-__device__ __forceinline__ int few_find(const Params& p, int64_t x, int lane, int64_t& before) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kWave) {
-    const int64_t t = b0 + lane < p.B ? static_cast<int64_t>(few_tiles(p, b0 + lane)) * p.c.hkv : 0;
-    int64_t sum = t;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int64_t u = __shfl_up(sum, o);
-      if (lane >= o) sum += u;
+// Sums over the sequences before b0 and of all, 64 at a time; `inc` and `mine` are those of the
+// 64 from b0 = 64 * chunk: the inclusive sum and the lane's sequence.
+__device__ __forceinline__ int few_sums(const Params& p, int lane, int chunk, int& before, int& inc, Seq& mine) {
+  int all = 0;
+  for (int c = 0; c * kWave < p.B; ++c) {
+    const int b = c * kWave + lane;
+    Seq s = lane_seq(p, min(b, p.B - 1));
+    const int sum = lane_sums(b < p.B ? few_tiles(p, s) : 0);
+    if (c == chunk) {
+      before = all;
+      inc = sum;
+      mine = s;
     }
-    const uint64_t past = __ballot(base + sum > x);
-    if (past != 0) {
-      const int at = __ffsll(static_cast<long long>(past)) - 1;
-      before = base + __shfl(sum - t, at);
-      return b0 + at;
-    }
-    base += __shfl(sum, kWave - 1);
+    all += __builtin_amdgcn_readlane(sum, kWave - 1);
   }
-  before = base;
-  return p.B;
+  return all;
 }
 
 // Zeros for the rows of no sequence and those behind a sequence's max_new-th, by one workgroup.
@@ -364,11 +362,27 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
   }
   // wavefront w: the first ones of all workgroups, then the second ones (few tiles lie on all CUs)
   const int w = blockIdx.x + groups * wave;
-  int64_t before;
-  const List list = few_list(p, lane, 0, before);
+  int before, inc;
+  Seq seqs;
+  List list;
+  list.split(few_sums(p, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.waves);
   if (w >= list.active) return;
-  const int64_t from = uniform(list.lo(w)), to = uniform(list.lo(w + 1));
-  int b = __builtin_amdgcn_readfirstlane(few_find(p, from, lane, before));
+  const int from = list.lo(w);
+  // the sequence that holds the run's first tile
+  int chunk = 0;
+  uint64_t past = __ballot(inc * p.c.hkv > from);
+  while (past == 0) {   // (the list is longer than `from`)
+    few_sums(p, lane, ++chunk, before, inc, seqs);
+    past = __ballot((before + inc) * p.c.hkv > from);
+  }
+  const int at = __ffsll(static_cast<long long>(past)) - 1;
+  int b = chunk * kWave + at;
+  before += at > 0 ? __builtin_amdgcn_readlane(inc, at - 1) : 0;
+  Seq s;
+  s.begin = __builtin_amdgcn_readlane(seqs.begin, at);
+  s.count = __builtin_amdgcn_readlane(seqs.count, at);
+  s.len = __builtin_amdgcn_readlane(seqs.len, at);
+  s.older = s.len - s.count;
   char* buf = lds + wave * kBuf;
   // transposing read: keys 4 lg .. + 3 (+ 16 g) of dims 16 dt + ln
   int vtr[4];
@@ -378,12 +392,10 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
   const int t = ln / p.G;   // column ln: query token, head of its group
   const int e0 = ln % p.G;
 
-  int64_t left = to - from;                                    // tiles to do
-  int first = static_cast<int>(from - uniform(before));        // the first one's place in the sequence
-  for (; left > 0 && b < p.B; ++b) {
-    const Seq s = seq_of(p, b);
+  int left = list.lo(w + 1) - from;            // tiles to do
+  int first = from - before * p.c.hkv;         // the first one's place in the sequence
+  while (left > 0) {
     const int count = min(s.count, p.n);
-    if (count == 0) continue;
     const int keys = keys_of(p, s, count - 1);
     const int per_head = max(1, (keys + kFewKeys - 1) / kFewKeys);
     const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
@@ -392,7 +404,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
     const uint64_t mask = p.tree && mine ? p.tree[s.begin + t] : 0;
     for (int h = first / per_head; h < p.c.hkv && left > 0; ++h) {
       const int tile0 = first - h * per_head;       // (0 from the second pair on)
-      const int ntile = static_cast<int>(min(static_cast<int64_t>(per_head - tile0), left));
+      const int ntile = min(per_head - tile0, left);
       first = (h + 1) * per_head;
       left -= ntile;
       const int lo = tile0 * kFewKeys, hi = min(lo + ntile * kFewKeys, keys);
@@ -602,6 +614,8 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
       wave_lds_sync();
     }
     first = 0;
+    if (left <= 0) break;
+    do s = seq_of(p, ++b); while (s.count == 0 && b + 1 < p.B);
   }
 }
 
@@ -933,10 +947,12 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
   int64_t first, next;    // the first record, and the second (those that follow lie `step` on)
   int64_t step;
   if (p.plan.few) {
-    int64_t before;
-    const List list = few_list(p, lane, b, before);
-    const int tiles = few_tiles(p, b);
-    const int64_t x = before * p.c.hkv + static_cast<int64_t>(h) * tiles;
+    int before, inc;
+    Seq seqs;
+    List list;
+    list.split(few_sums(p, lane, b / kWave, before, inc, seqs) * p.c.hkv, p.plan.waves);
+    const int tiles = few_tiles(p, s);
+    const int x = (before + __builtin_amdgcn_readlane(inc, b % kWave) - tiles) * p.c.hkv + h * tiles;
     const int w0 = list.wave_of(x), w1 = list.wave_of(x + tiles - 1);
     splits = w1 - w0 + 1;
     first = 2 * static_cast<int64_t>(w0) + 1;
@@ -954,16 +970,34 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
   const float* base = p.part + col * kPart<D>;
   float m = -INFINITY, l = 0.0f;
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = slot; i < splits; i += N) {
-    const float* r = base + (i == 0 ? first : next + (i - 1) * step) * size;
-    const float mi = r[0], li = r[1];
-    const f32x4 a = *reinterpret_cast<const f32x4*>(r + 4 + 4 * j);
-    if (mi == -INFINITY && li == 0.0f) continue;   // saw nothing
-    const float mn = fmaxf(m, mi);
-    const float wa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(mi - mn);
-    l = l * wa + li * wb;
-    o = o * wa + a * wb;
+  constexpr int U = 4;    // records in flight
+  for (int i0 = slot; i0 < splits; i0 += U * N) {
+    float mi[U], li[U];
+    f32x4 a[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * N, splits - 1);
+      const float* r = base + (i == 0 ? first : next + (i - 1) * step) * size;
+      mi[u] = r[0];
+      li[u] = r[1];
+      a[u] = *reinterpret_cast<const f32x4*>(r + 4 + 4 * j);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, mi[u]);
+    const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= old;
+    o *= old;
     m = mn;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // (a run that saw nothing, or one past the last, read again: nothing)
+      const bool none = i0 + u * N >= splits || (mi[u] == -INFINITY && li[u] == 0.0f);
+      const float w = __builtin_amdgcn_exp2f(mi[u] - mn);
+      l += none ? 0.0f : li[u] * w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += none ? 0.0f : a[u][e] * w;
+    }
   }
   if (j == 0) {
     sm[slot] = m;
@@ -1048,7 +1082,10 @@ int check_sizes(const char* who, int batch, int rows, int max_new, int num_heads
                 "%s: num_heads (%d) must be a positive multiple of num_kv_heads (%d)", who, num_heads, num_kv_heads);
   NKV_CHECK_SUPPORTED(num_heads / num_kv_heads <= 64, "%s: at most 64 query heads a KV head", who);
   NKV_CHECK_ARG(max_pages >= 1 && static_cast<int64_t>(max_pages) * page_size <= INT32_MAX - 4096,
-                "%s: a page table covers from 1 page to 2^31 - 4096 tokens", who);
+                "%s: a page table covers from 1 page to 2^31 - 4097 tokens", who);
+  const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size / kFewKeys + 1) * num_kv_heads;
+  NKV_CHECK_ARG(tiles * std::max(batch, 1) <= INT32_MAX,
+                "%s: the page tables cover 2^31 pieces of 32 keys of a KV head or more", who);
   return NKV_OK;
 }
 
@@ -1079,8 +1116,6 @@ extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale
   if (int rc = check_sizes(who, batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return rc;
   NKV_CHECK_ARG(starts != nullptr || static_cast<int64_t>(batch) * max_new == rows,
                 "%s: without starts every sequence has max_new rows", who);
-  NKV_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size / kFewKeys * num_kv_heads <= INT32_MAX - num_kv_heads,
-                "%s: a page table and KV heads past 2^31 pieces of 32 keys", who);
   NKV_CHECK_ARG(tree == nullptr || max_new <= kMaxTree, "%s: a tree has at most %d tokens (got %d)", who, kMaxTree, max_new);
   NKV_CHECK_ARG(scale > 0.0f && scale < INFINITY, "%s: scale must be positive and finite", who);
   if (rows == 0) return NKV_OK;
