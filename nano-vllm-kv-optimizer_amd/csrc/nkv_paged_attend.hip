@@ -18,11 +18,11 @@
 // 8-bit caches: the codes are bf16 exactly; a key's scale multiplies its logits, a
 // value's its weights, both in fp32.
 //
-// Work split, from the lengths, which are in device memory: few columns: the 32-key tiles of all
-// (sequence, KV head) pairs are one list, and every wavefront of one resident round takes an
-// equal run of it, whatever the sequences' lengths; many columns over long caches: runs of
-// C 64-key tiles, C such that all sequences together give about `target` runs. A pair that
-// several wavefronts (or runs) share is joined from their partial sums by a second kernel.
+// Work split, from the lengths, which are in device memory: the key tiles of all (sequence, KV
+// head, query tile) units are one list, and every worker of one resident round (a wavefront of
+// few_kernel, a workgroup of many_kernel) takes an equal run of it, whatever the sequences' lengths.
+// A unit that several workers share is joined from their partial sums by a second
+// kernel.  Query tiles that fill the device for several rounds are not cut: a workgroup each.
 //
 // Hidden keys get weight 0, which times an infinite or NaN value is NaN: a column whose
 // result holds a NaN is computed again key by key (redo_column), hidden keys left out.  Keys
@@ -47,13 +47,15 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kKeys = 64;          // keys of a tile, the unit of runs
 constexpr int kFewCols = 16;
 constexpr int kMaxTree = 64;       // tokens of a tree: bits of a mask
-constexpr int kMaxSplits = 256;
+#ifndef ROUNDS
+#define ROUNDS 1
+#endif
+constexpr int kRounds = ROUNDS;
 constexpr float kHeadroom = 8.0f;  // a running maximum moves once a logit passes it by 2^8 (log2 units)
 
 struct Plan {
-  int few, nct, cols, tpw, qtiles;      // columns and tokens of a workgroup's tile, tiles of max_new tokens
-  int max_splits, target, min_tiles;    // many columns: the runs
-  int waves;                            // few columns: the wavefronts (0: no pair has two tiles)
+  int few, nct, cols, tpw, qtiles;   // columns and tokens of a workgroup's tile, tiles of max_new tokens
+  int workers;                       // wavefronts (few columns) or workgroups that share the list; 0: nothing is cut
 };
 
 struct Params {
@@ -73,7 +75,29 @@ struct Params {
   Plan plan;
 };
 
-template <int D> constexpr int kPart = D + 4;   // a column's partial record: m, l, two of padding, acc
+// The arguments loaded again: what only a kernel's end or its rare paths use would
+// otherwise be held in registers all along.
+__device__ __forceinline__ const Params& again() {
+  typedef __attribute__((address_space(4))) const Params kernarg;
+  kernarg* k = (kernarg*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(k));
+  return *(const Params*)k;
+}
+
+// Workspace: a note of each unit that has queries, then two records of each worker: a column's
+// m, l, two floats of padding and its sums.  A unit that several workers share has
+// record 2 w + 1 of the first one and 2 w of each that follows.
+struct Note {
+  int records, worker;   // records 1: the unit is whole
+  int row, cols;         // first row of out, columns
+};
+__device__ __forceinline__ Note* note_of(const Params& p, int unit) { return reinterpret_cast<Note*>(p.part) + unit; }
+template <int D> constexpr int kPart = D + 4;
+template <int D>
+__device__ __forceinline__ float* record_of(const Params& p, int record, int c) {
+  return p.part + 4 * static_cast<int64_t>(p.B) * p.plan.qtiles * p.c.hkv +
+         (static_cast<int64_t>(record) * p.plan.cols + c) * kPart<D>;
+}
 
 typedef __attribute__((address_space(4))) const int32_t cint32;
 
@@ -113,29 +137,6 @@ __device__ __forceinline__ Seq lane_seq(const Params& p, int b) {
   s.older = s.len - s.count;
   return s;
 }
-
-// Tiles of a run (C): all lanes of the wavefront call it.
-__device__ __forceinline__ int run_tiles(const Params& p, int lane) {
-  if (p.plan.max_splits == 1) return INT32_MAX;
-  int64_t total = 0;
-  for (int b = lane; b < p.B; b += kWave) {
-    const int len = static_cast<int>(min(static_cast<int64_t>(max(p.lengths[b], 0)),
-                                         static_cast<int64_t>(p.max_pages) << p.c.shift));
-    int tiles = 1;
-    if (p.plan.qtiles > 1) {
-      const int count = p.starts ? min(max(p.starts[b + 1] - p.starts[b], 0), p.n) : p.n;
-      tiles = (count + p.plan.tpw - 1) / p.plan.tpw;
-    }
-    total += static_cast<int64_t>((len + kKeys - 1) / kKeys) * tiles;
-  }
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  const int64_t cap = ((static_cast<int64_t>(p.max_pages) << p.c.shift) + kKeys - 1) / kKeys;
-  const int64_t c = max((total * p.c.hkv + p.plan.target - 1) / p.plan.target,
-                        max((cap + p.plan.max_splits - 1) / p.plan.max_splits, static_cast<int64_t>(p.plan.min_tiles)));
-  return __builtin_amdgcn_readfirstlane(static_cast<int>(c));
-}
-__device__ __forceinline__ int splits_of(int tiles, int run) { return max(1, tiles / run + (tiles % run != 0 ? 1 : 0)); }
 
 // Keys that the queries [t0, t1] of a sequence may see: [0, this).
 __device__ __forceinline__ int keys_of(const Params& p, const Seq& s, int t1) {
@@ -280,36 +281,39 @@ __device__ __forceinline__ int lane_sums(int x) {
   return x;
 }
 
-// Tiles of a sequence for one KV head: at least one if it has queries.
-__device__ __forceinline__ int few_tiles(const Params& p, const Seq& s) {
-  const int count = min(s.count, p.n);
-  return count == 0 ? 0 : max(1, (keys_of(p, s, count - 1) + kFewKeys - 1) / kFewKeys);
+// Key tiles of query tile qt of a sequence: none without queries, at least one with.
+__device__ __forceinline__ int key_tiles(const Params& p, const Seq& s, int qt, int keys) {
+  const int count = min(s.count, p.n), t0 = qt * p.plan.tpw;
+  return t0 >= count ? 0 : max(1, (keys_of(p, s, min(t0 + p.plan.tpw, count) - 1) + keys - 1) / keys);
 }
-// The tiles of all pairs are one list, sequence by sequence and in it head by head
-// (fewer than 2^31: the caller checked).  The wavefronts [0, active) take equal runs of it.
+// The list of all units' tiles (fewer than 2^31: the caller checked), of which the
+// workers [0, active) take equal runs.
 struct List {
-  int total, active, share, more;   // the first `more` wavefronts take share + 1
-  __device__ __forceinline__ void split(int tiles, int waves) {
+  int total, active, share, more;   // the first `more` workers take share + 1
+  __device__ __forceinline__ void split(int tiles, int workers) {
     total = tiles;
-    active = min(total, waves);
+    active = min(total, workers);
     share = active == total ? 1 : static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(active));
     more = total - share * active;
   }
   __device__ __forceinline__ int lo(int w) const { return w * share + min(w, more); }
-  __device__ __forceinline__ int wave_of(int x) const {
+  __device__ __forceinline__ int worker_of(int x) const {
     if (share == 1 && more == 0) return x;
     const uint32_t edge = static_cast<uint32_t>(more) * (share + 1), at = x;
     return at < edge ? at / static_cast<uint32_t>(share + 1) : more + (at - edge) / static_cast<uint32_t>(share);
   }
 };
-// Sums over the sequences before b0 and of all, 64 at a time; `inc` and `mine` are those of the
-// 64 from b0 = 64 * chunk: the inclusive sum and the lane's sequence.
-__device__ __forceinline__ int few_sums(const Params& p, int lane, int chunk, int& before, int& inc, Seq& mine) {
+// The tiles of all units of one KV head, `keys` keys each.  Unit u is query tile u % qtiles of
+// sequence u / qtiles; of the 64 units from u0 = 64 * chunk, `before` is the sum over
+// those in front of u0, `inc` the inclusive sum and `mine` the sequence of the lane's.
+__device__ __forceinline__ int unit_sums(const Params& p, int keys, int lane, int chunk, int& before, int& inc, Seq& mine) {
   int all = 0;
-  for (int c = 0; c * kWave < p.B; ++c) {
-    const int b = c * kWave + lane;
-    Seq s = lane_seq(p, min(b, p.B - 1));
-    const int sum = lane_sums(b < p.B ? few_tiles(p, s) : 0);
+  const int units = p.B * p.plan.qtiles;
+  for (int c = 0; c * kWave < units; ++c) {
+    const int u = min(c * kWave + lane, units - 1);
+    const int b = p.plan.qtiles == 1 ? u : static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(p.plan.qtiles));
+    const Seq s = lane_seq(p, b);
+    const int sum = lane_sums(c * kWave + lane < units ? key_tiles(p, s, u - b * p.plan.qtiles, keys) : 0);
     if (c == chunk) {
       before = all;
       inc = sum;
@@ -341,7 +345,8 @@ __device__ __forceinline__ void clear_rest(const Params& p, int wave, int lane, 
 }
 
 template <int D, bool INT8>
-__global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
+  const Params& p = args;
   constexpr int KS = D / 32;                    // steps of the first product
   constexpr int DT = D / 16;                    // 16-dim tiles of the second
   constexpr int RB = 2 * D;                     // bytes of a V row in LDS
@@ -355,24 +360,25 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int ln = lane & 15, lg = lane >> 4;
-  const int groups = p.plan.waves / kWaves;
+  const int groups = p.plan.workers / kWaves;
   if (static_cast<int>(blockIdx.x) == groups) {   // (there is one more with starts)
     clear_rest(p, wave, lane, D);
     return;
   }
+  const bool cut = p.part != nullptr;
   // wavefront w: the first ones of all workgroups, then the second ones (few tiles lie on all CUs)
   const int w = blockIdx.x + groups * wave;
   int before, inc;
   Seq seqs;
   List list;
-  list.split(few_sums(p, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.waves);
+  list.split(unit_sums(p, kFewKeys, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.workers);
   if (w >= list.active) return;
   const int from = list.lo(w);
   // the sequence that holds the run's first tile
   int chunk = 0;
   uint64_t past = __ballot(inc * p.c.hkv > from);
   while (past == 0) {   // (the list is longer than `from`)
-    few_sums(p, lane, ++chunk, before, inc, seqs);
+    unit_sums(p, kFewKeys, lane, ++chunk, before, inc, seqs);
     past = __ballot((before + inc) * p.c.hkv > from);
   }
   const int at = __ffsll(static_cast<long long>(past)) - 1;
@@ -392,9 +398,10 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
   const int t = ln / p.G;   // column ln: query token, head of its group
   const int e0 = ln % p.G;
 
-  int left = list.lo(w + 1) - from;            // tiles to do
+  int left = list.lo(w + 1) - from, done = 0;  // tiles to do, done
   int first = from - before * p.c.hkv;         // the first one's place in the sequence
   while (left > 0) {
+    const Params& p = again();
     const int count = min(s.count, p.n);
     const int keys = keys_of(p, s, count - 1);
     const int per_head = max(1, (keys + kFewKeys - 1) / kFewKeys);
@@ -574,9 +581,12 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
       }
       l = sum_over_rows(l);
 
-      // ---- the pair's result, or this wavefront's part of it: record 2 w of a pair that
-      // began before the wavefront's run, 2 w + 1 of one that goes on behind it
+      // ---- the pair's result, or this wavefront's part of it
+      const Params& p = again();
       const bool whole = ntile == per_head;
+      if (cut && tile0 == 0 && lane == 0)
+        *note_of(p, b * p.c.hkv + h) = Note{whole ? 1 : list.worker_of(from + done + per_head - 1) - w + 1, w, s.begin, count * p.G};
+      done += ntile;
       bool odd = l != l;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -586,7 +596,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
       const uint64_t lanes = __ballot(odd && ln < cols);
       const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
       auto orow = [&](int c) { return p.out + (static_cast<int64_t>(s.begin + c / p.G) * p.hq + h * p.G + c % p.G) * D; };
-      auto rec = [&](int c) { return p.part + (static_cast<int64_t>(2 * w + (tile0 > 0 ? 0 : 1)) * p.plan.cols + c) * kPart<D>; };
+      auto rec = [&](int c) { return record_of<D>(p, 2 * w + (tile0 > 0 ? 0 : 1), c); };
       if (ln < cols && !((redo >> ln) & 1)) {
         if (whole) {
           uint16_t* dst = orow(ln) + 4 * lg;
@@ -627,131 +637,65 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params p) {
 template <int D> constexpr int kTile = kKeys * 2 * D;
 template <int D> constexpr int kStage = 2 * kTile<D> + 2 * kKeys * 4;
 
-template <int D, bool INT8, int NCT>
-__global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params p) {
+// The maximum that keeps a NaN (v_maximum3_f32 on pairs: no quieting of the operands first).
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Softmax state of a column: nm is minus the reference maximum (log2 units), a logit above
+// thr moves it (both as before any key: 0 and -inf).
+struct Col {
+  float nm, thr;
+};
+
+// SHARED: the workgroups share the list; else one a unit: grid (KV head, query tile, sequence).
+template <int D, bool INT8, int NCT, bool SHARED>
+__global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
+  const Params& p = args;
   constexpr int KS = D / 32, DT = D / 16, CH = D / 8, RB = 2 * D;
-  constexpr int kCols = 64 * NCT;
-  __shared__ __attribute__((aligned(16))) char lds0[kStage<D>];
-  __shared__ __attribute__((aligned(16))) char lds1[kStage<D>];
+  constexpr int KT = INT8 && NCT > 1 ? 2 : 4;   // 16-key groups a pass: half the logits live
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage<D>];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int ln = lane & 15, lg = lane >> 4;
-  const int h = blockIdx.x;
-  const int b = blockIdx.z / static_cast<unsigned>(p.plan.max_splits);
-  const int split = blockIdx.z % static_cast<unsigned>(p.plan.max_splits);
-  const int qt = p.plan.qtiles - 1 - static_cast<int>(blockIdx.y);   // the longest first
-  const Seq s = seq_of(p, b);
-  if (split == 0 && qt == 0) clear_others(p, s, b, h, D);
-  const int count = min(s.count, p.n);
-  const int tpw = p.plan.tpw;
-  const int t0 = qt * tpw;
-  if (t0 >= count) return;
-  const int t_last = min(t0 + tpw, count) - 1;
-  const int keys = keys_of(p, s, t_last);
-  const int tiles = (keys + kKeys - 1) / kKeys;
-  const int splits = splits_of(tiles, run_tiles(p, lane));
-  if (split >= splits) return;
-  const int lo = static_cast<int>(static_cast<int64_t>(split) * tiles / splits);
-  const int hi = static_cast<int>(static_cast<int64_t>(split + 1) * tiles / splits);
-  const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
+  const int tpw = p.plan.tpw, qtiles = p.plan.qtiles;
 
-  // column c = 16 NCT wave + 16 ct + ln: token t0 + c / G, head c % G
-  int limit[NCT];
-  uint64_t mask[NCT];
-  bf16x8 bq[NCT][KS];
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    const int c = wave * 16 * NCT + ct * 16 + ln;
-    const int t = t0 + c / p.G;
-    const bool mine = t <= t_last;
-    limit[ct] = mine ? s.older + t : -1;
-    mask[ct] = p.tree && mine ? p.tree[s.begin + t] : 0;
-    const uint16_t* qrow = p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + (h * p.G + c % p.G) * D;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (mine) v = *reinterpret_cast<const uint4*>(qrow + 32 * ks + 8 * lg);
-      bq[ct][ks] = as_bf16(v);
+  // ---- the workgroup's first unit (KV head, sequence, query tile), its tile there, its run
+  int h, b, qt, tile0 = 0, left = INT32_MAX, worker = 0;
+  List list;
+  if (!SHARED) {
+    h = blockIdx.x;
+    b = blockIdx.z;
+    qt = qtiles - 1 - static_cast<int>(blockIdx.y);   // the longest first
+  } else {
+    if (static_cast<int>(blockIdx.x) == p.plan.workers) {   // (there is one more with starts)
+      clear_rest(p, wave, lane, D);
+      return;
     }
-  }
-  f32x4 acc[DT][NCT], lsum[NCT];
-  float m[NCT];
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i) acc[i][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    lsum[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    m[ct] = -INFINITY;
+    // runs that follow one another on one XCD (workgroups go round them): units of a head share its keys in that L2
+    const int per = p.plan.workers / 8;
+    worker = p.plan.workers % 8 == 0 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    int before, inc;
+    Seq seqs;
+    const int sum = unit_sums(p, kKeys, lane, 0, before, inc, seqs);
+    list.split(sum * p.c.hkv, p.plan.workers);
+    if (worker >= list.active) return;
+    const int from = list.lo(worker);
+    left = list.lo(worker + 1) - from;
+    h = static_cast<int>(static_cast<uint32_t>(from) / static_cast<uint32_t>(sum));
+    const int rest = from - h * sum;
+    int chunk = 0;
+    uint64_t past = __ballot(inc > rest);
+    while (past == 0) {   // (rest < sum)
+      unit_sums(p, kKeys, lane, ++chunk, before, inc, seqs);
+      past = __ballot(before + inc > rest);
+    }
+    const int at = __ffsll(static_cast<long long>(past)) - 1;
+    const int unit = chunk * kWave + at;
+    tile0 = rest - before - (at > 0 ? __builtin_amdgcn_readlane(inc, at - 1) : 0);
+    b = unit / qtiles;
+    qt = unit - b * qtiles;
   }
 
-  // Staging of a tile: wavefront w brings its keys 16 w .. + 15, which lie in one page.
-  // bf16 goes to LDS without registers, rows past the length (or of a page outside the
-  // cache) as zeros; 8-bit codes through registers, widened on the way.
-  constexpr int PC = INT8 ? D / 16 : D / 8;     // 16-byte pieces of a row in the cache
-  constexpr int RL = kWave / PC;                // rows a load of the wavefront covers
-  constexpr int NL = 16 / RL;                   // loads of its 16 rows
-  uint4 kreg[NL], vreg[NL];
-  float sreg = 0.0f;
-  int have = 0;                                 // bit g: the tile's 16-key group g has a page
-  auto begin_stage = [&](int tile, char* buf) {
-    const int key0 = tile * kKeys + 16 * wave;
-    have = 0;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) have |= page_of(p, table, s, tile * kKeys + 16 * g) >= 0 ? 1 << g : 0;
-    const int id = page_of(p, table, s, key0);
-    const int rows = id < 0 ? 0 : min(16, s.len - key0);
-    const int in = key0 & (p.c.page - 1);
-    const int64_t at = p.c.sp * max(id, 0) + p.c.sh * h + p.c.st * in;
-    if constexpr (INT8) {
-      const int row_bytes = static_cast<int>(p.c.st);
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int r = RL * i + lane / PC;
-        kreg[i] = vreg[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) {
-          kreg[i] = *reinterpret_cast<const uint4*>(p.c.k + at + static_cast<int64_t>(r) * row_bytes + (lane % PC) * 16);
-          vreg[i] = *reinterpret_cast<const uint4*>(p.c.v + at + static_cast<int64_t>(r) * row_bytes + (lane % PC) * 16);
-        }
-      }
-      // lanes 0 .. 15 the keys' scales, 16 .. 31 the values'
-      sreg = 0.0f;
-      if (lane < 32 && ln < rows)
-        sreg = (lane < 16 ? p.c.ks : p.c.vs)[((static_cast<int64_t>(id) * p.c.hkv + h) << p.c.shift) + in + ln];
-    } else {
-      const int row_bytes = static_cast<int>(p.c.st) * 2;
-      const uint32_t bytes = static_cast<uint32_t>(rows) * row_bytes;
-      const rsrc_words rk = rsrc_of(p.c.k + 2 * at, bytes);
-      const rsrc_words rv = rsrc_of(p.c.v + 2 * at, bytes);
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int r = RL * i + lane / PC, c = lane % PC;
-        const char* dst = buf + (16 * wave + RL * i) * RB;
-        lds_copy16(rk, dst, r * row_bytes + ((c ^ (r & (CH - 1))) << 4));
-        lds_copy16(rv, dst + kTile<D>, r * row_bytes + ((c ^ (2 * (r & 3))) << 4));
-      }
-    }
-  };
-  auto finish_stage = [&](char* buf) {
-    if constexpr (INT8) {
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int r = 16 * wave + RL * i + lane / PC, c = 2 * (lane % PC);
-        char* kd = buf + r * RB;
-        char* vd = kd + kTile<D>;
-        *reinterpret_cast<uint4*>(kd + ((c ^ (r & (CH - 1))) << 4)) = i8x8_to_bf16x8(kreg[i].x, kreg[i].y);
-        *reinterpret_cast<uint4*>(kd + (((c + 1) ^ (r & (CH - 1))) << 4)) = i8x8_to_bf16x8(kreg[i].z, kreg[i].w);
-        *reinterpret_cast<uint4*>(vd + ((c ^ (2 * (r & 3))) << 4)) = i8x8_to_bf16x8(vreg[i].x, vreg[i].y);
-        *reinterpret_cast<uint4*>(vd + (((c + 1) ^ (2 * (r & 3))) << 4)) = i8x8_to_bf16x8(vreg[i].z, vreg[i].w);
-      }
-      if (lane < 32)
-        reinterpret_cast<float*>(buf + 2 * kTile<D>)[(lane < 16 ? 0 : kKeys) + 16 * wave + ln] =
-            lane < 16 ? sreg * p.scale_log2 : sreg;
-    } else {
-      __builtin_amdgcn_s_waitcnt(0);   // the copies have landed
-    }
-    __syncthreads();
-  };
-
+  const uint32_t lds_base = lds_address(lds);
   // operand addresses of the lane in a stage
   int koff[KS], vtr[4];
 #pragma unroll
@@ -760,318 +704,476 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params p) {
   for (int x = 0; x < 4; ++x)
     vtr[x] = kTile<D> + (4 * lg + (ln >> 2)) * RB + ((2 * (x ^ (ln >> 2)) + ((ln & 3) >> 1)) << 4) + 8 * (ln & 1);
 
-  if (lo < hi) {
-    begin_stage(lo, lds0);
-    finish_stage(lds0);
-  }
-  for (int tile = lo; tile < hi; ++tile) {
-    char* buf = (tile - lo) & 1 ? lds1 : lds0;
-    char* other = (tile - lo) & 1 ? lds0 : lds1;
-    const int got = have;
-    const bool more = tile + 1 < hi;
-    if (more) begin_stage(tile + 1, other);
+  for (;;) {
+    const Params& p = SHARED ? again() : args;
+    const Seq s = seq_of(p, b);
+    if (!SHARED && qt == 0) clear_others(p, s, b, h, D);
+    const int t0 = qt * tpw;
+    const int tiles = key_tiles(p, s, qt, kKeys);
+    if (tiles > 0) {
+    const int t_last = min(t0 + tpw, min(s.count, p.n)) - 1;
+    const int lo = tile0, hi = min(tiles, left < tiles ? lo + left : tiles);
+    const int32_t* table = p.tables + b * p.table_ls;
+    const float sl = INT8 ? 1.0f : p.scale_log2;   // (8 bits: in the keys' scales)
+    // the head's rows in a page
+    constexpr int E = INT8 ? 1 : 2;
+    const char* kbase = p.c.k + p.c.sh * h * E;
+    const char* vbase = p.c.v + p.c.sh * h * E;
+    const int row_bytes = static_cast<int>(p.c.st) * E;
 
-    // ---- S^T = K Q^T: S[kt][ct][e] is key 16 kt + 4 lg + e of column ct -------
-    f32x4 S[4][NCT];
+    // column c = 16 NCT wave + 16 ct + ln: token t0 + c / G, head c % G
+    int tcol[NCT];
+    bf16x8 bq[NCT][KS];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) S[kt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int ct = 0; ct < NCT; ++ct) {
+      const int c = wave * 16 * NCT + ct * 16 + ln;
+      const int t = t0 + static_cast<int>(static_cast<uint32_t>(c) / static_cast<uint32_t>(p.G));
+      tcol[ct] = t;
+      const uint16_t* qrow = p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + (h * p.G + c - (t - t0) * p.G) * D;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(buf + kt * 16 * RB + koff[ks]);
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) S[kt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ct][ks], S[kt][ct], 0, 0, 0);
+        u32x4 v = u32x4{0u, 0u, 0u, 0u};
+        if (t <= t_last) v = *reinterpret_cast<const u32x4*>(qrow + 32 * ks + 8 * lg);
+        bq[ct][ks] = __builtin_bit_cast(bf16x8, v);
       }
     }
-    const float* scales = reinterpret_cast<const float*>(buf + 2 * kTile<D>);
+    f32x4 acc[DT][NCT], lsum[NCT];
+    Col col[NCT];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      if (INT8) {
-        const f32x4 sc = *reinterpret_cast<const f32x4*>(scales + 16 * kt + 4 * lg);
+    for (int ct = 0; ct < NCT; ++ct) {
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) S[kt][ct] *= sc;
+      for (int i = 0; i < DT; ++i) acc[i][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      lsum[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      col[ct] = Col{0.0f, -INFINITY};
+    }
+
+    // Staging of a tile: wavefront w brings its keys 16 w .. + 15, which lie in one page.
+    // bf16 goes to LDS without registers, rows past the length (or of a page outside the
+    // cache) as zeros; 8-bit codes through registers, widened on the way.
+    constexpr int PC = INT8 ? D / 16 : D / 8;     // 16-byte pieces of a row in the cache
+    constexpr int RL = kWave / PC;                // rows a load of the wavefront covers
+    constexpr int NL = 16 / RL;                   // loads of its 16 rows
+    u32x4 kreg[NL], vreg[NL];
+    float sreg = 0.0f;
+    // the pages of the 64 16-key groups from tile id0, one a lane (-1: none), and who has one
+    int ids = -1, id0 = lo;
+    uint64_t paged = 0;
+    auto fetch_ids = [&](int tile) {
+      const int key0 = tile * kKeys + 16 * lane;
+      ids = key0 < s.len ? table[key0 >> p.c.shift] : -1;
+      paged = __ballot(ids >= 0 && ids < p.c.pages);
+      id0 = tile;
+    };
+    int have = 0;                                 // bit g: the tile's 16-key group g has a page
+    auto begin_stage = [&](int tile, char* buf) {
+      if (tile - id0 >= 16) fetch_ids(tile);
+      const int at = (tile - id0) * 4;
+      have = static_cast<int>(paged >> at) & 15;
+      const int id = (have >> wave) & 1 ? __builtin_amdgcn_readlane(ids, at + wave) : 0;
+      const int key0 = tile * kKeys + 16 * wave;
+      const int rows = (have >> wave) & 1 ? min(16, s.len - key0) : 0;
+      const int in = key0 & (p.c.page - 1);
+      const int64_t row0 = p.c.sp * E * id + static_cast<int64_t>(in) * row_bytes;
+      if constexpr (INT8) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int r = RL * i + lane / PC;
+          kreg[i] = vreg[i] = u32x4{0u, 0u, 0u, 0u};
+          if (r < rows) {
+            kreg[i] = *reinterpret_cast<const u32x4*>(kbase + row0 + static_cast<int64_t>(r) * row_bytes + (lane % PC) * 16);
+            vreg[i] = *reinterpret_cast<const u32x4*>(vbase + row0 + static_cast<int64_t>(r) * row_bytes + (lane % PC) * 16);
+          }
+        }
+        // lanes 0 .. 15 the keys' scales, 16 .. 31 the values'
+        sreg = 0.0f;
+        if (lane < 32 && ln < rows)
+          sreg = (lane < 16 ? p.c.ks : p.c.vs)[((static_cast<int64_t>(id) * p.c.hkv + h) << p.c.shift) + in + ln];
       } else {
+        const uint32_t bytes = static_cast<uint32_t>(rows) * row_bytes;
+        const rsrc_words rk = rsrc_of(kbase + row0, bytes);
+        const rsrc_words rv = rsrc_of(vbase + row0, bytes);
+        // (made opaque: the offsets of all loads, kept from tile to tile, would not fit the registers)
+        int row = lane / PC;
+        asm volatile("" : "+v"(row));
+        const int c = lane % PC, ko = (c ^ (row & (CH - 1))) << 4, vo = (c ^ (2 * (row & 3))) << 4;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(static_cast<int>(lds_base + (buf - lds) + 16 * wave * RB));
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) S[kt][ct] *= p.scale_log2;
-      }
-    }
-    if (got != 15 || tile * kKeys + kKeys - 1 > (p.tree ? s.older - 1 : s.older + t0)) {
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) {
-        uint64_t bits = seen_bits(mask[ct], p.tree != nullptr, limit[ct], s, tile * kKeys);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          if (!((got >> kt) & 1)) bits &= ~(0xffffull << (16 * kt));
-          const uint32_t own = static_cast<uint32_t>(bits >> (16 * kt + 4 * lg));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[kt][ct][e] = where_bit(S[kt][ct][e], own, e);
+        for (int i = 0; i < NL; ++i) {
+          const int at_row = (row + RL * i) * row_bytes;
+          lds_copy16(rk, dst + i * RL * RB, at_row + (ko ^ ((RL * i & (CH - 1)) << 4)));
+          lds_copy16(rv, dst + i * RL * RB + kTile<D>, at_row + vo);
         }
       }
-    }
-    // ---- softmax: the maximum moves only where a logit passes it by 2^8 -------
-    float top[NCT];
-    bool move = false;
+    };
+    auto finish_stage = [&](char* buf) {
+      if constexpr (INT8) {
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      top[ct] = S[0][ct][0];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top[ct] = fmaxf(top[ct], S[kt][ct][e]);
-      move = move || top[ct] > m[ct] + kHeadroom || (m[ct] == -INFINITY && top[ct] > m[ct]);
-    }
-    if (__any(move)) {
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) {
-        const float mn = fmaxf(m[ct], max_over_rows(top[ct]));
-        const float alpha = m[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[ct] - mn);
-        m[ct] = mn;
-        lsum[ct] *= alpha;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i][ct] *= alpha;
+        for (int i = 0; i < NL; ++i) {
+          const int r = 16 * wave + RL * i + lane / PC, c = 2 * (lane % PC);
+          char* kd = buf + r * RB;
+          char* vd = kd + kTile<D>;
+          *reinterpret_cast<uint4*>(kd + ((c ^ (r & (CH - 1))) << 4)) = i8x8_to_bf16x8(kreg[i][0], kreg[i][1]);
+          *reinterpret_cast<uint4*>(kd + (((c + 1) ^ (r & (CH - 1))) << 4)) = i8x8_to_bf16x8(kreg[i][2], kreg[i][3]);
+          *reinterpret_cast<uint4*>(vd + ((c ^ (2 * (r & 3))) << 4)) = i8x8_to_bf16x8(vreg[i][0], vreg[i][1]);
+          *reinterpret_cast<uint4*>(vd + (((c + 1) ^ (2 * (r & 3))) << 4)) = i8x8_to_bf16x8(vreg[i][2], vreg[i][3]);
+        }
+        if (lane < 32)
+          reinterpret_cast<float*>(buf + 2 * kTile<D>)[(lane < 16 ? 0 : kKeys) + 16 * wave + ln] =
+              lane < 16 ? sreg * p.scale_log2 : sreg;
+      } else {
+        __builtin_amdgcn_s_waitcnt(0);   // the copies have landed
       }
-    }
+      __syncthreads();
+    };
+
+    // One tile in `buf`.  Operand reads run two products ahead through a ring of three
+    // registers; the scheduling barriers keep that order.
+    auto attend = [&](int tile, int got, const char* buf) {
+      const float* scales = reinterpret_cast<const float*>(buf + 2 * kTile<D>);
+      const bool mask = got != 15 || tile * kKeys + kKeys - 1 > (p.tree ? s.older - 1 : s.older + t0);
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      const float base = m[ct] == -INFINITY ? 0.0f : m[ct];
+      for (int pass = 0; pass < 4 / KT; ++pass) {
+        constexpr int kQ = KS * KT;
+        auto read_k = [&](int i) {   // ks outer, kt inner
+          return *reinterpret_cast<const bf16x8*>(buf + (pass * KT + i % KT) * 16 * RB + koff[i / KT]);
+        };
+        auto read_v = [&](int i) {   // 32-key group outer, 16 dims inner
+          const char* vp = buf + vtr[(i % DT) & 3] + ((i % DT) >> 2) * 128 + (pass * (KT / 2) + i / DT) * 32 * RB;
+          const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
+          const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
+          return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        // ---- S^T = K Q^T: S[kt][ct][e] is key 16 kt + 4 lg + e of the pass, column ct
+        f32x4 S[KT][NCT];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[kt][ct][e] = __builtin_amdgcn_exp2f(S[kt][ct][e] - base);
-    }
-    if (INT8) {
+          for (int ct = 0; ct < NCT; ++ct) S[kt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        bf16x8 ka[3];
+        ka[0] = read_k(0);
+        ka[1] = read_k(1);
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        const f32x4 sc = *reinterpret_cast<const f32x4*>(scales + kKeys + 16 * kt + 4 * lg);
+        for (int i = 0; i < kQ; ++i) {
+          if (i + 2 < kQ) ka[(i + 2) % 3] = read_k(i + 2);
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct)
+            S[i % KT][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[i % 3], bq[ct][i / KT], S[i % KT][ct], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // the first values load while the softmax runs
+        constexpr int kV = DT * (KT / 2);
+        bf16x8 va[3];
+        va[0] = read_v(0);
+        va[1] = read_v(1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (INT8) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const f32x4 sc = *reinterpret_cast<const f32x4*>(scales + 16 * (pass * KT + kt) + 4 * lg);
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) S[kt][ct] *= sc;
+          }
+        }
+        if (mask) {
+          const Params& p = again();
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            const bool mine = tcol[ct] <= t_last;
+            const uint64_t names = p.tree && mine ? p.tree[s.begin + tcol[ct]] : 0;
+            uint64_t bits = seen_bits(names, p.tree != nullptr, mine ? s.older + tcol[ct] : -1, s, tile * kKeys);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              const int g = pass * KT + kt;
+              if (!((got >> g) & 1)) bits &= ~(0xffffull << (16 * g));
+              const uint32_t own = static_cast<uint32_t>(bits >> (16 * g + 4 * lg));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) S[kt][ct][e] = where_bit(S[kt][ct][e], own, e);
+            }
+          }
+        }
+        // ---- softmax: a maximum moves only where a logit passes it by 2^8
+        float top[NCT];
+        bool move = false;
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) {
-          lsum[ct] += S[kt][ct];
+          top[ct] = S[0][ct][0];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) S[kt][ct][e] = S[kt][ct][e] == 0.0f ? 0.0f : S[kt][ct][e] * sc[e];
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[ct] = max_nan(top[ct], S[kt][ct][e]);
+          move = move || top[ct] > col[ct].thr;
+        }
+        if (__any(move)) {
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            const float old = col[ct].thr == -INFINITY ? -INFINITY : -col[ct].nm;
+            const float cand = max_over_rows(top[ct]) * sl;
+            const float m = cand > old + kHeadroom ? cand : old;
+            const float ref = m == -INFINITY ? 0.0f : m;
+            const float alpha = old == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(old - ref);
+            col[ct].nm = -ref;
+            col[ct].thr = m == -INFINITY ? -INFINITY : (m + kHeadroom) / sl;
+            lsum[ct] *= alpha;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i][ct] *= alpha;
+          }
+        }
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              S[kt][ct][e] = __builtin_amdgcn_exp2f(INT8 ? S[kt][ct][e] + col[ct].nm : __builtin_fmaf(S[kt][ct][e], sl, col[ct].nm));
+        if (INT8) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const f32x4 sc = *reinterpret_cast<const f32x4*>(scales + kKeys + 16 * (pass * KT + kt) + 4 * lg);
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) {
+              lsum[ct] += S[kt][ct];
+              // (the scale of a hidden key may be anything)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) S[kt][ct][e] = S[kt][ct][e] == 0.0f ? 0.0f : S[kt][ct][e] * sc[e];
+            }
+          }
+        }
+        // ---- O^T += V^T P^T, the row sums a product with ones
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const int j = i / DT, dt = i % DT;
+          if (dt == 0) __builtin_amdgcn_sched_barrier(0);
+          bf16x8 bp[NCT];
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            const f32x4 a0 = S[2 * j][ct], a1 = S[2 * j + 1][ct];
+            const u32x4 w = u32x4{pack_bf16(a0[0], a0[1]), pack_bf16(a0[2], a0[3]), pack_bf16(a1[0], a1[1]), pack_bf16(a1[2], a1[3])};
+            bp[ct] = __builtin_bit_cast(bf16x8, w);
+            if (!INT8 && dt == 0) {
+              const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+              lsum[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, bp[ct], lsum[ct], 0, 0, 0);
+            }
+          }
+          if (i + 2 < kV) va[(i + 2) % 3] = read_v(i + 2);
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct)
+            acc[dt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[i % 3], bp[ct], acc[dt][ct], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-    }
-    // ---- O^T += V^T P^T, the row sums a product with ones ----------------------
-    const bf16x8 ones = as_bf16(make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
-#pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2) {
-      bf16x8 bp[NCT];
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) {
-        const f32x4 a0 = S[2 * k2][ct], a1 = S[2 * k2 + 1][ct];
-        bp[ct] = as_bf16(make_uint4(pack_bf16(a0[0], a0[1]), pack_bf16(a0[2], a0[3]), pack_bf16(a1[0], a1[1]), pack_bf16(a1[2], a1[3])));
-        if (!INT8) lsum[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, bp[ct], lsum[ct], 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        const char* vp = buf + vtr[i & 3] + (i >> 2) * 128 + k2 * 32 * RB;
-        const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
-        const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
-        const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) acc[i][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, bp[ct], acc[i][ct], 0, 0, 0);
-      }
-    }
-    if (more)
-      finish_stage(other);
-  }
+    };
 
-  // ---- store: acc[i][ct][e] is dim 16 i + 4 lg + e ----------------------------
-  const bool whole = splits == 1;
+    fetch_ids(lo);
+    begin_stage(lo, lds);
+    finish_stage(lds);
+    for (int tile = lo; tile < hi; ++tile) {
+      char* buf = lds + ((tile - lo) & 1) * kStage<D>;
+      char* other = lds + ((tile - lo + 1) & 1) * kStage<D>;
+      const int got = have;
+      if (tile + 1 < hi) begin_stage(tile + 1, other);
+      attend(tile, got, buf);
+      if (tile + 1 < hi) finish_stage(other);
+    }
+
+    // ---- store: acc[i][ct][e] is dim 16 i + 4 lg + e
+    const bool whole = hi - lo == tiles;
+    {
+    const Params& p = again();
+    if (SHARED && lo == 0 && threadIdx.x == 0)   // (one that is cut is the run's last)
+      *note_of(p, (h * p.B + b) * qtiles + qt) =
+          Note{whole ? 1 : list.worker_of(list.lo(worker + 1) - hi + tiles - 1) - worker + 1, worker, s.begin + t0, (t_last + 1 - t0) * p.G};
 #pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    const int c0 = wave * 16 * NCT + ct * 16;
-    const int c = c0 + ln;
-    const bool mine = t0 + c / p.G <= t_last && c < tpw * p.G;
-    const float l = INT8 ? sum_over_rows(lsum[ct][0] + lsum[ct][1] + lsum[ct][2] + lsum[ct][3]) : lsum[ct][0];
-    bool odd = l != l;
+    for (int ct = 0; ct < NCT; ++ct) {
+      const int c0 = wave * 16 * NCT + ct * 16;
+      const int c = c0 + ln;
+      const bool mine = tcol[ct] <= t_last;
+      const float l = INT8 ? sum_over_rows(lsum[ct][0] + lsum[ct][1] + lsum[ct][2] + lsum[ct][3]) : lsum[ct][0];
+      bool odd = l != l;
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+      for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) odd = odd || acc[i][ct][e] != acc[i][ct][e];
-    const uint64_t lanes = __ballot(odd && mine);
-    const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
-    auto orow = [&](int col) {
-      return p.out + (static_cast<int64_t>(s.begin + t0 + col / p.G) * p.hq + h * p.G + col % p.G) * D;
-    };
-    auto rec = [&](int col) {
-      return p.part + ((((static_cast<int64_t>(b) * p.plan.qtiles + qt) * p.c.hkv + h) * p.plan.max_splits + split) * kCols + col) * kPart<D>;
-    };
-    if (mine && !((redo >> ln) & 1)) {
-      if (whole) {
-        uint16_t* dst = orow(c) + 4 * lg;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int e = 0; e < 4; ++e) odd = odd || acc[i][ct][e] != acc[i][ct][e];
+      const uint64_t lanes = __ballot(odd && mine);
+      const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
+      auto orow = [&](int cc) {
+        return p.out + (static_cast<int64_t>(s.begin + t0 + cc / p.G) * p.hq + h * p.G + cc % p.G) * D;
+      };
+      auto rec = [&](int cc) { return record_of<D>(p, 2 * worker + (lo > 0 ? 0 : 1), cc); };
+      if (mine && !((redo >> ln) & 1)) {
+        if (!SHARED || whole) {
+          uint16_t* dst = orow(c) + 4 * lg;
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          const f32x4 o = acc[i][ct];
-          *reinterpret_cast<u32x2*>(dst + 16 * i) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+          for (int i = 0; i < DT; ++i) {
+            const f32x4 o = acc[i][ct];
+            *reinterpret_cast<u32x2*>(dst + 16 * i) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+          }
+        } else {
+          float* r = rec(c);
+          if (lg == 0) {
+            r[0] = col[ct].thr == -INFINITY ? -INFINITY : -col[ct].nm;
+            r[1] = l;
+          }
+#pragma unroll
+          for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i][ct];
         }
-      } else {
-        float* r = rec(c);
-        if (lg == 0) {
-          r[0] = m[ct];
-          r[1] = l;
-        }
-#pragma unroll
-        for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i][ct];
+      }
+      for (uint32_t todo = redo; todo != 0; todo &= todo - 1) {
+        const int cc = c0 + __builtin_ctz(todo);
+        float mc, lc, oc[D / 64];
+        redo_column<D, INT8>(p, s, (const cint32*)table, h, t0 + cc / p.G, h * p.G + cc % p.G, lo * kKeys, hi * kKeys, lane, mc, lc, oc);
+        store_column<D>(p, whole, whole ? orow(cc) : nullptr, whole ? nullptr : rec(cc), lane, mc, lc, oc);
       }
     }
-    for (uint32_t left = redo; left != 0; left &= left - 1) {
-      const int col = c0 + __builtin_ctz(left);
-      float mc, lc, oc[D / 64];
-      redo_column<D, INT8>(p, s, table, h, t0 + col / p.G, h * p.G + col % p.G, lo * kKeys, hi * kKeys, lane, mc, lc, oc);
-      store_column<D>(p, whole, whole ? orow(col) : nullptr, whole ? nullptr : rec(col), lane, mc, lc, oc);
     }
+    left -= hi - lo;
+    }
+    if (!SHARED || left <= 0) return;
+    // ---- the next unit of the list
+    const Params& next = again();
+    tile0 = 0;
+    if (++qt * tpw >= min(s.count, next.n)) {
+      qt = 0;
+      do {
+        if (++b == next.B) {
+          b = 0;
+          ++h;
+        }
+      } while (seq_of(next, b).count == 0);   // (there is a unit: the run goes on)
+    }
+    __syncthreads();   // (the stages have been read)
   }
 }
 
 // ----------------------------------------------------------------- the join --
-// One workgroup a column: D / 4 lanes a run, 256 / (D / 4) runs at a time.  Bound by
-// reading the records once (and the launch).
+// A wavefront a column of a unit that is cut: D / 4 lanes a record, 8 records of each such group
+// of lanes in flight.  Bound by the launch and three round trips, or by reading the records once.
 template <int D>
 __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
-  constexpr int L = D / 4, N = kThreads / L;
-  __shared__ float sm[N], sl[N];
-  __shared__ f32x4 so[N][L];
+  constexpr int L = D / 4, N = kWave / L;
   const int lane = threadIdx.x & 63;
-  const int h = blockIdx.x, b = blockIdx.z;
-  const int qt = blockIdx.y / static_cast<unsigned>(p.plan.tpw * p.G);
-  const int col = blockIdx.y % static_cast<unsigned>(p.plan.tpw * p.G);
-  const Seq s = seq_of(p, b);
-  const int t = qt * p.plan.tpw + col / p.G;
-  const int count = min(s.count, p.n);
-  if (t >= count) return;
-  const int slot = threadIdx.x / L, j = threadIdx.x % L;
-  int splits;
-  int64_t first, next;    // the first record, and the second (those that follow lie `step` on)
-  int64_t step;
+  const int unit = blockIdx.x, col = blockIdx.y * kWaves + static_cast<int>(threadIdx.x >> 6);
+  int h, u;
   if (p.plan.few) {
-    int before, inc;
-    Seq seqs;
-    List list;
-    list.split(few_sums(p, lane, b / kWave, before, inc, seqs) * p.c.hkv, p.plan.waves);
-    const int tiles = few_tiles(p, s);
-    const int x = (before + __builtin_amdgcn_readlane(inc, b % kWave) - tiles) * p.c.hkv + h * tiles;
-    const int w0 = list.wave_of(x), w1 = list.wave_of(x + tiles - 1);
-    splits = w1 - w0 + 1;
-    first = 2 * static_cast<int64_t>(w0) + 1;
-    next = 2 * static_cast<int64_t>(w0) + 2;
-    step = 2;
+    u = unit / p.c.hkv;
+    h = unit - u * p.c.hkv;
   } else {
-    const int keys = keys_of(p, s, min((qt + 1) * p.plan.tpw, count) - 1);
-    splits = splits_of((keys + kKeys - 1) / kKeys, run_tiles(p, lane));
-    first = ((static_cast<int64_t>(b) * p.plan.qtiles + qt) * p.c.hkv + h) * p.plan.max_splits;
-    next = first + 1;
-    step = 1;
+    h = unit / (p.B * p.plan.qtiles);
+    u = unit - h * p.B * p.plan.qtiles;
   }
-  if (splits == 1) return;
-  const int64_t size = static_cast<int64_t>(p.plan.cols) * kPart<D>;
-  const float* base = p.part + col * kPart<D>;
+  const Note note = *note_of(p, unit);
+  const Seq s = seq_of(p, u / p.plan.qtiles);
+  // (a unit without queries has no note)
+  if (u % p.plan.qtiles * p.plan.tpw >= min(s.count, p.n) || note.records == 1 || col >= note.cols) return;
+  const int slot = lane / L, j = lane % L;
   float m = -INFINITY, l = 0.0f;
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int U = 4;    // records in flight
-  for (int i0 = slot; i0 < splits; i0 += U * N) {
+  constexpr int U = 8;
+  for (int i0 = slot; i0 - slot < note.records; i0 += U * N) {
     float mi[U], li[U];
     f32x4 a[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = min(i0 + u * N, splits - 1);
-      const float* r = base + (i == 0 ? first : next + (i - 1) * step) * size;
-      mi[u] = r[0];
-      li[u] = r[1];
-      a[u] = *reinterpret_cast<const f32x4*>(r + 4 + 4 * j);
+    for (int k = 0; k < U; ++k) {
+      const int i = min(i0 + k * N, note.records - 1);
+      const float* r = record_of<D>(p, 2 * (note.worker + i) + (i == 0 ? 1 : 0), col);
+      mi[k] = r[0];
+      li[k] = r[1];
+      a[k] = *reinterpret_cast<const f32x4*>(r + 4 + 4 * j);
     }
     float mn = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, mi[u]);
+    for (int k = 0; k < U; ++k) mn = fmaxf(mn, mi[k]);
     const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
     l *= old;
     o *= old;
     m = mn;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (a run that saw nothing, or one past the last, read again: nothing)
-      const bool none = i0 + u * N >= splits || (mi[u] == -INFINITY && li[u] == 0.0f);
-      const float w = __builtin_amdgcn_exp2f(mi[u] - mn);
-      l += none ? 0.0f : li[u] * w;
+    for (int k = 0; k < U; ++k) {
+      // (one that saw nothing, or one past the last, read again: nothing)
+      const bool none = i0 + k * N >= note.records || (mi[k] == -INFINITY && li[k] == 0.0f);
+      const float wt = __builtin_amdgcn_exp2f(mi[k] - mn);
+      l += none ? 0.0f : li[k] * wt;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += none ? 0.0f : a[u][e] * w;
+      for (int e = 0; e < 4; ++e) o[e] += none ? 0.0f : a[k][e] * wt;
     }
   }
-  if (j == 0) {
-    sm[slot] = m;
-    sl[slot] = l;
+#pragma unroll
+  for (int x = L; x < kWave; x <<= 1) {
+    const float mo = __shfl_xor(m, x), lo = __shfl_xor(l, x);
+    const float mn = fmaxf(m, mo);
+    const float wa = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float wb = mo == -INFINITY && lo == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
+    l = l * wa + lo * wb;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * wa + __shfl_xor(o[e], x) * wb;
+    m = mn;
   }
-  so[slot][j] = o;
-  __syncthreads();
   if (slot != 0) return;
-  float mt = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < N; ++i) mt = fmaxf(mt, sm[i]);
-  float lt = 0.0f;
-  f32x4 ot = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (sm[i] == -INFINITY && sl[i] == 0.0f) continue;
-    const float w = __builtin_amdgcn_exp2f(sm[i] - mt);
-    lt += sl[i] * w;
-    ot += so[i][j] * w;
-  }
-  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-  uint16_t* dst = p.out + (static_cast<int64_t>(s.begin + t) * p.hq + h * p.G + col % p.G) * D + 4 * j;
-  *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16(ot[0] * inv, ot[1] * inv), pack_bf16(ot[2] * inv, ot[3] * inv)};
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const uint32_t t = static_cast<uint32_t>(col) / static_cast<uint32_t>(p.G);
+  uint16_t* dst = p.out + (static_cast<int64_t>(note.row + t) * p.hq + h * p.G + col - t * p.G) * D + 4 * j;
+  *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
 }
 
 // ----------------------------------------------------------------- the plan --
-Plan plan_of(int B, int T, int n, int hkv, int G, int64_t cap_tokens, bool ragged) {
+Plan plan_of(int B, int T, int n, int hkv, int G, int head_dim, int64_t cap_tokens, bool ragged) {
   Plan q{};
   const int64_t rows = static_cast<int64_t>(n) * G;
-  q.few = rows <= kFewCols;
-  q.nct = q.few ? 0 : rows <= 64 ? 1 : 2;
-  q.cols = q.few ? static_cast<int>(rows) : 64 * q.nct;
-  q.tpw = q.few ? n : q.cols / G;
-  q.qtiles = (n + q.tpw - 1) / q.tpw;
   const int cus = std::max(1, device_cus());
-  const int64_t cap = (cap_tokens + kKeys - 1) / kKeys;
-  // query tiles there are at least: a sequence has one, and all rows fill this many
-  const int64_t least = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw);
-  if (q.few) {   // one resident round: two workgroups a CU
-    q.max_splits = 1;
-    q.waves = cap_tokens > kFewKeys ? 2 * kWaves * cus : 0;
+  q.few = rows <= kFewCols;
+  if (q.few) {
+    q.cols = static_cast<int>(rows);
+    q.tpw = n;
+    q.qtiles = 1;
+    q.workers = cap_tokens > kFewKeys ? 2 * kWaves * cus : 0;   // two workgroups a CU
     return q;
   }
-  q.target = 2 * cus;
-  q.min_tiles = 4;
-  int64_t most = (4 * static_cast<int64_t>(q.target) + least * hkv - 1) / (least * hkv);
-  if (least * hkv >= q.target) most = 1;   // the tiles alone fill the device
-  most = std::min({most, (cap + q.min_tiles - 1) / q.min_tiles, static_cast<int64_t>(kMaxSplits), INT64_C(65535) / std::max(B, 1)});
-  q.max_splits = static_cast<int>(std::max<int64_t>(1, most));
+  q.nct = rows <= 64 ? 1 : 2;
+#ifdef MAXNCT
+  if (rows > 64) q.nct = std::min(q.nct, MAXNCT);
+#endif
+  q.cols = 64 * q.nct;
+  q.tpw = q.cols / G;
+  q.qtiles = (n + q.tpw - 1) / q.tpw;
+  // units of one head there are at least: a sequence has one, and all rows fill this many
+  const int64_t least = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw);
+  const int64_t cap = (cap_tokens + kKeys - 1) / kKeys;
+  const bool fits = static_cast<int64_t>(B) * q.qtiles <= 1024 && cap * B * q.qtiles * hkv <= INT32_MAX;
+  // workgroups that a CU holds: 128-dim heads 2, 64-dim ones 3
+  const int slots = (head_dim == 128 ? 2 : 3) * cus;
+  q.workers = fits && cap > 1 && least * hkv < kRounds * slots ? slots : 0;
   return q;
+}
+
+template <int D, bool I8, int NCT>
+void launch_many(const Params& p, hipStream_t s) {
+  const Plan& q = p.plan;
+  if (q.workers > 0)
+    many_kernel<D, I8, NCT, true><<<q.workers + (p.starts ? 1 : 0), kThreads, 0, s>>>(p);
+  else
+    many_kernel<D, I8, NCT, false><<<dim3(p.c.hkv, q.qtiles, p.B), kThreads, 0, s>>>(p);
 }
 
 template <int D, bool I8>
 void launch(const Params& p, hipStream_t s) {
   const Plan& q = p.plan;
   if (q.few) {
-    // (no pair has two tiles: a wavefront takes as many as it needs)
-    const int waves = q.waves > 0 ? q.waves : kWaves * static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.B) * p.c.hkv + kWaves - 1) / kWaves, 4096));
+    // (where no pair has two tiles a wavefront takes some of them)
     Params f = p;
-    f.plan.waves = waves;
-    few_kernel<D, I8><<<waves / kWaves + (p.starts ? 1 : 0), kThreads, 0, s>>>(f);
-  } else if (q.nct == 1) {
-    many_kernel<D, I8, 1><<<dim3(p.c.hkv, q.qtiles, p.B * q.max_splits), kThreads, 0, s>>>(p);
+    if (q.workers == 0) f.part = nullptr;
+    if (q.workers == 0)
+      f.plan.workers = kWaves * static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.B) * p.c.hkv + kWaves - 1) / kWaves, 4096));
+    few_kernel<D, I8><<<f.plan.workers / kWaves + (p.starts ? 1 : 0), kThreads, 0, s>>>(f);
   } else {
-    many_kernel<D, I8, 2><<<dim3(p.c.hkv, q.qtiles, p.B * q.max_splits), kThreads, 0, s>>>(p);
+    q.nct == 1 ? launch_many<D, I8, 1>(p, s) : launch_many<D, I8, 2>(p, s);
   }
-  if (q.max_splits > 1 || q.waves > 0) merge_kernel<D><<<dim3(p.c.hkv, q.qtiles * q.tpw * p.G, p.B), kThreads, 0, s>>>(p);
+  if (q.workers > 0) merge_kernel<D><<<dim3(p.B * q.qtiles * p.c.hkv, (q.cols + kWaves - 1) / kWaves), kThreads, 0, s>>>(p);
 }
 
-// Floats of the partial sums.
+// Floats of the workspace: the notes and two records a worker.
 int64_t part_floats(const Plan& q, int B, int hkv, int head_dim) {
-  const int64_t records = q.few ? 2 * static_cast<int64_t>(q.waves)
-                                : q.max_splits == 1 ? 0 : static_cast<int64_t>(B) * q.qtiles * hkv * q.max_splits;
-  return records * q.cols * (head_dim + 4);
+  if (q.workers == 0) return 0;
+  return 4 * static_cast<int64_t>(B) * q.qtiles * hkv + 2 * static_cast<int64_t>(q.workers) * q.cols * (head_dim + 4);
 }
 
 int check_sizes(const char* who, int batch, int rows, int max_new, int num_heads, int num_kv_heads, int max_pages,
@@ -1097,7 +1199,7 @@ using namespace nkv;
 extern "C" int64_t nkv_paged_attend_workspace(int batch, int rows, int max_new, int num_heads, int num_kv_heads,
                                               int head_dim, int max_pages, int page_size, int ragged) {
   if (batch <= 0 || rows <= 0 || check_sizes("", batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return 0;
-  const Plan q = plan_of(batch, rows, max_new, num_kv_heads, num_heads / num_kv_heads,
+  const Plan q = plan_of(batch, rows, max_new, num_kv_heads, num_heads / num_kv_heads, head_dim,
                          static_cast<int64_t>(max_pages) * page_size, ragged != 0);
   return part_floats(q, batch, num_kv_heads, head_dim);
 }
@@ -1124,8 +1226,8 @@ extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale
   NKV_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 && q_stride % 8 == 0,
                 "%s: rows must lie on 16-byte boundaries", who);
   const int G = num_heads / num_kv_heads;
-  p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
-  NKV_CHECK_ARG(p.plan.qtiles <= 65535 && static_cast<int64_t>(p.plan.qtiles) * p.plan.tpw * G <= 65535 * (p.plan.max_splits > 1 ? INT64_C(1) : INT64_C(1 << 20)),
+  p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, head_dim, static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
+  NKV_CHECK_ARG(p.plan.qtiles <= 65535,
                 "%s: too many query rows", who);
   NKV_CHECK_ARG(part_floats(p.plan, batch, num_kv_heads, head_dim) == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "%s: these sizes need a workspace on a 16-byte boundary", who);

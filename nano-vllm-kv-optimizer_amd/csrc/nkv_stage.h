@@ -78,9 +78,12 @@ __device__ __forceinline__ rsrc_words rsrc_of(const void* base, uint32_t bytes) 
 // vmcnt waits.  The memory clobber keeps every LDS access on its side of the
 // copy.  M0 (the LDS base, read when the copy issues) is restored after it;
 // the s_nops cover the descriptor-write and M0-write hazards.
-__device__ __forceinline__ void lds_copy16(rsrc_words rsrc, const char* lds, int voffset) {
-  const uint32_t m0 = static_cast<uint32_t>(
+// (`lds` as an address in LDS: of a generic pointer the compiler would test for null first.)
+__device__ __forceinline__ uint32_t lds_address(const char* lds) {
+  return static_cast<uint32_t>(
       __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>((lds_void*)lds))));
+}
+__device__ __forceinline__ void lds_copy16(rsrc_words rsrc, uint32_t m0, int voffset) {
   uint32_t saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
@@ -92,6 +95,9 @@ __device__ __forceinline__ void lds_copy16(rsrc_words rsrc, const char* lds, int
       : "=&s"(saved)
       : "s"(m0), "v"(voffset), "s"(rsrc)
       : "memory");
+}
+__device__ __forceinline__ void lds_copy16(rsrc_words rsrc, const char* lds, int voffset) {
+  lds_copy16(rsrc, lds_address(lds), voffset);
 }
 // The same, 4 bytes a lane (buffer_load_dword ... lds): lane u lands at lds + 4 u.
 __device__ __forceinline__ void lds_copy4(rsrc_words rsrc, const char* lds, int voffset) {
