@@ -47,10 +47,7 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kKeys = 64;          // keys of a tile, the unit of runs
 constexpr int kFewCols = 16;
 constexpr int kMaxTree = 64;       // tokens of a tree: bits of a mask
-#ifndef ROUNDS
-#define ROUNDS 1
-#endif
-constexpr int kRounds = ROUNDS;
+constexpr int kLeastRun = 4;       // tiles of a workgroup's run at least
 constexpr float kHeadroom = 8.0f;  // a running maximum moves once a logit passes it by 2^8 (log2 units)
 
 struct Plan {
@@ -290,9 +287,9 @@ __device__ __forceinline__ int key_tiles(const Params& p, const Seq& s, int qt, 
 // workers [0, active) take equal runs.
 struct List {
   int total, active, share, more;   // the first `more` workers take share + 1
-  __device__ __forceinline__ void split(int tiles, int workers) {
+  __device__ __forceinline__ void split(int tiles, int workers, int least) {
     total = tiles;
-    active = min(total, workers);
+    active = min((total + least - 1) / least, workers);   // (a run of fewer is not worth its records)
     share = active == total ? 1 : static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(active));
     more = total - share * active;
   }
@@ -371,7 +368,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
   int before, inc;
   Seq seqs;
   List list;
-  list.split(unit_sums(p, kFewKeys, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.workers);
+  list.split(unit_sums(p, kFewKeys, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.workers, 1);
   if (w >= list.active) return;
   const int from = list.lo(w);
   // the sequence that holds the run's first tile
@@ -676,7 +673,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     int before, inc;
     Seq seqs;
     const int sum = unit_sums(p, kKeys, lane, 0, before, inc, seqs);
-    list.split(sum * p.c.hkv, p.plan.workers);
+    list.split(sum * p.c.hkv, p.plan.workers, kLeastRun);
     if (worker >= list.active) return;
     const int from = list.lo(worker);
     left = list.lo(worker + 1) - from;
@@ -1046,15 +1043,16 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
 }
 
 // ----------------------------------------------------------------- the join --
-// A wavefront a column of a unit that is cut: D / 4 lanes a record, 8 records of each such group
+// A wavefront a column of a unit that is cut, or with WIDE (few columns, which may be cut
+// into many runs) a workgroup: D / 4 lanes a record, 8 records of each such group
 // of lanes in flight.  Bound by the launch and three round trips, or by reading the records once.
-template <int D>
+template <int D, bool WIDE>
 __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
-  constexpr int L = D / 4, N = kWave / L;
-  const int lane = threadIdx.x & 63;
-  const int unit = blockIdx.x, col = blockIdx.y * kWaves + static_cast<int>(threadIdx.x >> 6);
+  constexpr int L = D / 4, N = (WIDE ? kThreads : kWave) / L;
+  const int lane = WIDE ? threadIdx.x : threadIdx.x & 63;
+  const int unit = blockIdx.x, col = WIDE ? blockIdx.y : blockIdx.y * kWaves + static_cast<int>(threadIdx.x >> 6);
   int h, u;
-  if (p.plan.few) {
+  if (WIDE) {   // (the list of few columns goes sequence by sequence)
     u = unit / p.c.hkv;
     h = unit - u * p.c.hkv;
   } else {
@@ -1097,6 +1095,8 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
       for (int e = 0; e < 4; ++e) o[e] += none ? 0.0f : a[k][e] * wt;
     }
   }
+  __shared__ float sm[kWaves], sl[kWaves];
+  __shared__ f32x4 so[kWaves][L];
 #pragma unroll
   for (int x = L; x < kWave; x <<= 1) {
     const float mo = __shfl_xor(m, x), lo = __shfl_xor(l, x);
@@ -1107,6 +1107,26 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = o[e] * wa + __shfl_xor(o[e], x) * wb;
     m = mn;
+  }
+  if (WIDE) {
+    if (lane % kWave < L) {
+      sm[lane / kWave] = m;
+      sl[lane / kWave] = l;
+      so[lane / kWave][j] = o;
+    }
+    __syncthreads();
+    if (slot != 0) return;
+    m = -INFINITY;
+    l = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sm[i]);
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const float wt = sm[i] == -INFINITY && sl[i] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm[i] - m);
+      l += sl[i] * wt;
+      o += so[i][j] * wt;
+    }
   }
   if (slot != 0) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1129,19 +1149,18 @@ Plan plan_of(int B, int T, int n, int hkv, int G, int head_dim, int64_t cap_toke
     return q;
   }
   q.nct = rows <= 64 ? 1 : 2;
-#ifdef MAXNCT
-  if (rows > 64) q.nct = std::min(q.nct, MAXNCT);
-#endif
   q.cols = 64 * q.nct;
   q.tpw = q.cols / G;
   q.qtiles = (n + q.tpw - 1) / q.tpw;
-  // units of one head there are at least: a sequence has one, and all rows fill this many
-  const int64_t least = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw);
+  // A workgroup a unit takes as long as the longest unit; shared, the units take their mean
+  // share of the slots, and about 32 tiles' time more for records of 64 KiB, written and
+  // read (us, a workgroup a unit / shared: 500 tokens 21 / 37, 2000 56 / 97, 1000 behind 8192
+  // 187 / 176, 2 x 947 behind 9882 217 / 137, 200 behind 32768 638 / 151)
+  const int slots = (head_dim == 128 ? 2 : 3) * cus;   // workgroups that the CUs hold
   const int64_t cap = (cap_tokens + kKeys - 1) / kKeys;
+  const int64_t units = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw) * hkv;   // at least
   const bool fits = static_cast<int64_t>(B) * q.qtiles <= 1024 && cap * B * q.qtiles * hkv <= INT32_MAX;
-  // workgroups that a CU holds: 128-dim heads 2, 64-dim ones 3
-  const int slots = (head_dim == 128 ? 2 : 3) * cus;
-  q.workers = fits && cap > 1 && least * hkv < kRounds * slots ? slots : 0;
+  q.workers = fits && units < slots && cap * (slots - units) > 32 * static_cast<int64_t>(slots) ? slots : 0;
   return q;
 }
 
@@ -1167,7 +1186,12 @@ void launch(const Params& p, hipStream_t s) {
   } else {
     q.nct == 1 ? launch_many<D, I8, 1>(p, s) : launch_many<D, I8, 2>(p, s);
   }
-  if (q.workers > 0) merge_kernel<D><<<dim3(p.B * q.qtiles * p.c.hkv, (q.cols + kWaves - 1) / kWaves), kThreads, 0, s>>>(p);
+  if (q.workers == 0) return;
+  const unsigned units = static_cast<unsigned>(p.B) * q.qtiles * p.c.hkv;
+  if (q.few)
+    merge_kernel<D, true><<<dim3(units, q.cols), kThreads, 0, s>>>(p);
+  else
+    merge_kernel<D, false><<<dim3(units, q.cols / kWaves), kThreads, 0, s>>>(p);
 }
 
 // Floats of the workspace: the notes and two records a worker.
