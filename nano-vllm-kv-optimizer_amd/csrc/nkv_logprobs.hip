@@ -11,13 +11,17 @@
 //   s = s1 + r (s2 + 1),  w = w1 + r (w2 + d (s2 + 1)).
 //
 // Work split: a wavefront takes a run of its row; its maximum is the same in
-// all lanes and moves rarely, so an element costs a subtraction, a product, an exp2, two
-// additions and the comparisons.  Alternatives: an element that beats the
-// wavefront's n-th best so far goes to its list of up to 256 in LDS; a full list is
-// cut to its best n, which raises the bar.  The bar starts at the n-th largest of
-// the lanes' maxima over the first piece, so few elements ever pass it.  Order:
+// all lanes and moves rarely, so an element costs a product, an exp2, two
+// additions and the comparisons.  Alternatives: elements that reach the
+// wavefront's bar go to its list of up to 256 in LDS; a list grown long is
+// cut to its best, which raises the bar.  The bar starts below the n-th largest of
+// the lanes' maxima over the first piece, so few elements ever reach it.  Order:
 // value descending (NaN above all), index ascending.  Bound by reading the
 // logits once, or by the launches (one row).
+//
+// Exponents are in log2 units: 2^-z with z = M - x log2 e in one fused operation, M = m
+// log2 e rounded.  What M's rounding is off by, e, scales every term by 2^e alike, and adds
+// to every z: both are mended in the sums (settle), not in the terms.
 #include <algorithm>
 
 #include "nkv_common.h"
@@ -30,7 +34,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kList = 256;       // candidates a wavefront keeps at most
 constexpr int kMaxTop = 64;      // alternatives: one a lane in the final order
 constexpr int kEach = 16;        // elements a lane takes per iteration
-constexpr int kMaxSplits = 64;   // pieces of a row
+constexpr int kMaxSplits = 128;  // pieces of a row
 constexpr float kLog2e = 1.44269504088896340736f;
 
 enum Kind { kF32 = 0, kBf16 = 1, kF16 = 2 };
@@ -59,6 +63,8 @@ __device__ __forceinline__ float element(const char* row, int64_t i) {
 struct Stat { float m, s, w; };
 
 __device__ __forceinline__ float exp_neg(float y) { return __builtin_amdgcn_exp2f(y * -kLog2e); }
+// The maximum that keeps a NaN (v_maximum3_f32: two elements an instruction, none quieted first).
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
   if (b.m > a.m) { const Stat t = a; a = b; b = t; }
@@ -74,6 +80,29 @@ __device__ __forceinline__ int below(uint64_t mask) {   // set bits under this l
                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
+// Inclusive sum over the lanes of the wavefront.
+__device__ __forceinline__ int lane_sums(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+__device__ __forceinline__ float lane_total(float x) {
+#define NKV_ADD(ctrl, rows) x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), ctrl, rows, 0xf, false))
+  NKV_ADD(0x111, 0xf);
+  NKV_ADD(0x112, 0xf);
+  NKV_ADD(0x114, 0xf);
+  NKV_ADD(0x118, 0xf);
+  NKV_ADD(0x142, 0xa);
+  NKV_ADD(0x143, 0xc);
+#undef NKV_ADD
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), kWave - 1));
+}
+
 // A wavefront's candidates: (key, id) in LDS, and the bar that a new one has to
 // beat: a larger key, or the same with a lower id.
 struct List {
@@ -85,26 +114,31 @@ struct List {
 
   __device__ __forceinline__ bool beats(uint32_t key, int id) const { return key > bar || (key == bar && id < bar_id); }
 
-  // The best `top` of up to four candidates a lane (an empty one has key 0,
-  // below every element's): they become the list, the last of them the bar.
-  __device__ void keep_best(const uint32_t (&k)[4], const int (&id)[4], int have) {
+  // Of up to four candidates a lane (an empty one has key 0, below every element's) the
+  // best: at least `top` of them and at most `most` (top <= most <= 64).  They become the
+  // list, and the bar keeps out what would not be among them.
+  __device__ void keep_best(const uint32_t (&k)[4], const int (&id)[4], int have, int most) {
     auto above = [&](auto&& f) {
       int n = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) n += count(__ballot(f(k[i], id[i])));
       return n;
     };
-    uint32_t t = 1;      // the top-th largest key, bit by bit (all candidates when there are no more)
+    uint32_t t = 1;      // the smallest key kept (all candidates when there are few)
     int last = INT32_MAX;
-    if (have > top) {
-      t = 0;
-      for (int bit = 31; bit >= 0; --bit) {
+    if (have > most) {
+      t = 0;             // at least `top` keys are t or more, bit by bit, until they are few enough
+      int kept = have;
+      for (int bit = 31; bit >= 0 && kept > most; --bit) {
         const uint32_t c = t | (1u << bit);
-        if (above([&](uint32_t a, int) { return a >= c; }) >= top) t = c;
+        const int n = above([&](uint32_t a, int) { return a >= c; });
+        if (n >= top) {
+          t = c;
+          kept = n;
+        }
       }
-      const int more = above([&](uint32_t a, int) { return a > t; });
-      const int equal = above([&](uint32_t a, int) { return a == t; });
-      if (more + equal > top) {   // of equal ones the lowest ids
+      if (kept > most) {   // too many are equal: of those the lowest ids
+        const int more = above([&](uint32_t a, int) { return a > t; });
         last = 0;
         for (int bit = 30; bit >= 0; --bit) {
           const int c = last | (1 << bit);
@@ -130,7 +164,7 @@ struct List {
     cnt = n;
     wave_lds_sync();
   }
-  __device__ void cut(int lane) {
+  __device__ void cut(int lane, int most) {
     wave_lds_sync();
     uint32_t k[4];
     int id[4];
@@ -140,7 +174,7 @@ struct List {
       k[i] = in ? keys[i * kWave + lane] : 0u;
       id[i] = in ? ids[i * kWave + lane] : INT32_MAX;
     }
-    keep_best(k, id, cnt);
+    keep_best(k, id, cnt, most);
   }
   // Every lane's candidate (if it has one that beats the bar); the whole wavefront calls it.
   __device__ __forceinline__ void add(bool has, uint32_t key, int id, int lane) {
@@ -148,7 +182,7 @@ struct List {
     uint64_t mask = __ballot(has);
     if (mask == 0) return;
     if (cnt + count(mask) > kList) {
-      cut(lane);
+      cut(lane, kWave);
       has = has && beats(key, id);
       mask = __ballot(has);
     }
@@ -160,14 +194,18 @@ struct List {
   }
 };
 
-// The lanes' best `top` (key, id) in order and the row's numbers, by one wavefront.
+// The logit of the row's token (NaN: no such token).
 template <int K>
-__device__ __forceinline__ void finish(const Params& p, int row, const char* x, Stat t, const List& list, int lane) {
+__device__ __forceinline__ float token_logit(const Params& p, int row, const char* x) {
+  const int64_t tok = p.tokens[row];
+  return tok >= 0 && tok < p.vocab ? element<K>(x, tok) : NAN;
+}
+// The lanes' best `top` (key, id) in order and the row's numbers, by one wavefront; xt: the token's logit.
+__device__ __forceinline__ void finish(const Params& p, int row, float xt, Stat t, const List& list, int lane) {
   const float z = t.m == INFINITY ? NAN : log1pf(t.s);   // (inf - inf: no probabilities)
   const bool none = t.m == -INFINITY;                    // every element is -inf: no distribution
   if (lane == 0) {
-    const int64_t tok = p.tokens[row];
-    p.logprob[row] = tok >= 0 && tok < p.vocab ? (element<K>(x, tok) - t.m) - z : NAN;
+    p.logprob[row] = (xt - t.m) - z;
     p.entropy[row] = none ? NAN : z + t.w / (1.0f + t.s);
   }
   if (p.top == 0) return;
@@ -190,13 +228,14 @@ __device__ __forceinline__ void finish(const Params& p, int row, const char* x, 
 __device__ __forceinline__ void join_waves(uint32_t (&keys)[kWaves][kList], int (&ids)[kWaves][kList],
                                            Stat (&stats)[kWaves], int (&counts)[kWaves], int wave, int lane, Stat& t,
                                            List& list) {
-  if (list.cnt > list.top) list.cut(lane);
+  if (list.cnt > kWave) list.cut(lane, kWave);   // (one of the four lists a lane below)
   if (lane == 0) {
     stats[wave] = t;
     counts[wave] = list.cnt;
   }
   __syncthreads();
   if (wave != 0) return;
+  t = stats[0];   // (in all lanes)
 #pragma unroll
   for (int i = 1; i < kWaves; ++i) t = join(t, stats[i]);
   uint32_t k[4];
@@ -209,7 +248,7 @@ __device__ __forceinline__ void join_waves(uint32_t (&keys)[kWaves][kList], int 
     id[i] = in ? ids[i][lane] : INT32_MAX;
     have += counts[i];
   }
-  list.keep_best(k, id, have);
+  list.keep_best(k, id, have, list.top);
 }
 
 template <int K>
@@ -232,9 +271,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
   const int64_t per = (pieces + static_cast<int64_t>(p.splits) * kWaves * kStep - 1) / (p.splits * kWaves * kStep) * kStep;
   const int64_t lo = min(per * (split * kWaves + wave), pieces), hi = min(lo + per, pieces);
 
+  // (early: two round trips that nothing waits for)
+  const float xt = p.splits == 1 && wave == 0 ? token_logit<K>(p, row, x) : 0.0f;
   List list{keys[wave], ids[wave], 0, p.top, 0u, INT32_MAX};
   float bar = p.top > 0 ? -INFINITY : INFINITY;   // the list's, as a value
   float m = -INFINITY, s = 0.0f, w = 0.0f;        // m is the wavefront's, s and w the lane's part
+  // since m moved: the sums of 2^-z and z 2^-z, big_m = m log2 e rounded (0 of -inf), off what it lacks
+  float sz = 0.0f, wz = 0.0f, big_m = 0.0f, off = 0.0f;
+  auto settle = [&]() {
+    const float f = __builtin_amdgcn_exp2f(-off);
+    s += sz * f;
+    w += (wz + off * sz) * f * (1.0f / kLog2e);
+    sz = wz = 0.0f;
+  };
   auto widen = [&](const uint4& raw, float (&f)[E]) {
     const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
@@ -274,14 +323,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = fmaxf(top, v[u][e]);
-    const float old = m == -INFINITY ? 0.0f : m;
-    if (__any(top > m)) {
-      float t = top;
+      for (int e = 0; e < E; ++e) top = max_nan(top, v[u][e]);
+    if (__any(top > m) || !(fabsf(m) < 0x1p126f)) {   // (m log2 e may be infinite: never in M's form)
+      float t = top;      // (a lane's NaN gives way to the others' values)
 #pragma unroll
       for (int o = kWave / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+      t = fmaxf(t, m);
+      settle();
       // the sums move to the new maximum; the old one becomes an element like others (lane 0 has it)
-      if (m != -INFINITY) {
+      const bool moves = t > m;
+      if (m != -INFINITY && moves) {
         const float d = fminf(t - m, 200.0f), r = exp_neg(d);
         w = r * (w + d * s);
         s = r * s;
@@ -291,14 +342,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
         }
       }
       m = t;
+      big_m = m * kLog2e;
+      off = __builtin_fmaf(m, kLog2e, -big_m);
+      if (!(fabsf(m) < 0x1p126f)) big_m = off = 0.0f;
       // one element that is the maximum stays out
-      const uint64_t owners = __ballot(top == m);
+      const uint64_t owners = moves ? __ballot(top == m) : 0;
+      const float ref = m == -INFINITY ? 0.0f : m;
       bool skip = owners != 0 && lane == __ffsll(static_cast<long long>(owners)) - 1;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float y = m - v[u][e];
+          const float y = ref - v[u][e];
           float ex = exp_neg(y);
           if (skip && v[u][e] == m) {
             ex = 0.0f;
@@ -312,24 +367,58 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float y = old - v[u][e];
-          const float ex = exp_neg(y);
-          s += ex;
-          w += fminf(y, 200.0f) * ex;
+          const float z = __builtin_fmaf(v[u][e], -kLog2e, big_m);
+          const float ex = __builtin_amdgcn_exp2f(-z);
+          sz += ex;
+          wz += fminf(z, 300.0f) * ex;   // (likewise 2^-300)
         }
     }
-    if (q0 == lo && p.top > 0) {
-      // the first bar: the top-th largest of the lanes' maxima
+    if (p.top == 0) continue;
+    if (q0 == lo) {
+      // the first bar: at least `top` lanes have a maximum that reaches it, not many more
       const uint32_t k = score_key(top);
       uint32_t t = 0;
-      for (int bit = 31; bit >= 0; --bit) {
+      int n = kWave;
+      for (int bit = 31; bit >= 0 && n > p.top + 8; --bit) {
         const uint32_t c = t | (1u << bit);
-        if (count(__ballot(k >= c)) >= p.top) t = c;
+        const int a = count(__ballot(k >= c));
+        if (a >= p.top) {
+          t = c;
+          n = a;
+        }
       }
       list.bar = t;
-      bar = key_score(t);
+      bar = t <= score_key(-INFINITY) ? -INFINITY : key_score(t);
     }
-    if (p.top > 0 && __any(top >= bar)) {
+    if (!__any(top >= bar)) continue;
+    // how many of the lane's elements reach the bar: then each has its places in the list
+    const bool whole = first >= 0 && q0 + U * kWave <= hi && first + U * kWave * E <= p.vocab;
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) mine += v[u][e] >= bar ? 1 : 0;
+    const int upto = lane_sums(mine);
+    const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (whole && list.cnt + all <= kList) {
+      int at = list.cnt + upto - mine;
+      if (mine > 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (v[u][e] >= bar) {
+              list.keys[at] = score_key(v[u][e]);
+              list.ids[at] = static_cast<int>((q0 + u * kWave + lane) * E - head + e);
+              ++at;
+            }
+      }
+      list.cnt += all;
+      if (list.cnt > 2 * p.top + 32) {
+        list.cut(lane, min(p.top + 8, kWave));
+        bar = key_score(list.bar);
+      }
+    } else {
       // (all 64 lanes' element e at once; an element outside the row or run is none)
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -338,15 +427,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
           if (!__any(f >= bar)) continue;
           const int64_t q = q0 + u * kWave + lane, i = q * E - head + e;
           list.add(f >= bar && q < hi && i >= 0 && i < p.vocab, score_key(f), static_cast<int>(i), lane);
-          bar = key_score(list.bar);
+          bar = list.bar <= score_key(-INFINITY) ? -INFINITY : key_score(list.bar);
         }
     }
   }
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) {
-    s += __shfl_xor(s, o);
-    w += __shfl_xor(w, o);
-  }
+  settle();
+  s = lane_total(s);
+  w = lane_total(w);
   Stat t{m, s, w};
   if (p.top > 0 && s != s) {
     // a NaN or +inf: the row has no probabilities, but an order (NaN first): by keys
@@ -368,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
   join_waves(keys, ids, stats, counts, wave, lane, t, list);
   if (wave != 0) return;
   if (p.splits == 1) {
-    finish<K>(p, row, x, t, list, lane);
+    finish(p, row, xt, t, list, lane);
     return;
   }
   float* rec = p.ws + static_cast<int64_t>(blockIdx.x) * (4 + 2 * p.top);
@@ -397,33 +484,43 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const Params p)
   const int row = blockIdx.x;
   const float* recs = p.ws + static_cast<int64_t>(row) * p.splits * (4 + 2 * p.top);
   List list{keys[wave], ids[wave], 0, p.top, 0u, INT32_MAX};
-  // a record a lane, then lanes joined
-  Stat t{-INFINITY, 0.0f, 0.0f};
+  const float xt = wave == 0 ? token_logit<K>(p, row, p.x + static_cast<int64_t>(row) * p.stride * kBytes<K>) : 0.0f;
+  Stat t{-INFINITY, 0.0f, 0.0f};   // a record a lane
   const int mine = wave + kWaves * lane;
   if (mine < p.splits) {
     const float* r = recs + static_cast<int64_t>(mine) * (4 + 2 * p.top);
     t = Stat{r[0], r[1], r[2]};
   }
+  // the records' candidates as one run, four loads of each in flight
+  const int size = 4 + 2 * p.top, all = p.splits * p.top;
+  for (int e0 = wave * kWave; e0 < all; e0 += 4 * kThreads) {
+    uint32_t key[4];
+    int id[4];
 #pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1)
-    t = join(t, Stat{__shfl_xor(t.m, o), __shfl_xor(t.s, o), __shfl_xor(t.w, o)});
-  if (p.top > 0)
-    for (int i = wave; i < p.splits; i += kWaves) {
-      const float* r = recs + static_cast<int64_t>(i) * (4 + 2 * p.top);
-      const bool in = lane < __float_as_int(r[3]);
-      const uint32_t key = in ? __float_as_uint(r[4 + lane]) : 0u;
-      const int id = in ? __float_as_int(r[4 + p.top + lane]) : INT32_MAX;
-      list.add(in, key, id, lane);
+    for (int i = 0; i < 4; ++i) {
+      const int e = min(e0 + i * kThreads + lane, all - 1);
+      const int rec = static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(p.top)), at = e - rec * p.top;
+      const float* r = recs + rec * size;
+      const bool in = e0 + i * kThreads + lane < all && at < __float_as_int(r[3]);
+      key[i] = in ? __float_as_uint(r[4 + at]) : 0u;
+      id[i] = in ? __float_as_int(r[4 + p.top + at]) : INT32_MAX;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) list.add(key[i] != 0, key[i], id[i], lane);
+  }
+  // the lanes that have a record joined
+  int lanes = 1;
+  while (lanes * kWaves < p.splits) lanes <<= 1;
+  for (int o = lanes >> 1; o > 0; o >>= 1)
+    t = join(t, Stat{__shfl_xor(t.m, o), __shfl_xor(t.s, o), __shfl_xor(t.w, o)});
   join_waves(keys, ids, stats, counts, wave, lane, t, list);
-  if (wave == 0)
-    finish<K>(p, row, p.x + static_cast<int64_t>(row) * p.stride * kBytes<K>, t, list, lane);
+  if (wave == 0) finish(p, row, xt, t, list, lane);
 }
 
 // Pieces of a row: rows alone fill the device from about 1024 workgroups on, and a
 // piece is at least one iteration of its four wavefronts.
 int splits_of(int rows, int vocab) {
-  const int most = std::max(1, vocab / (kThreads * kEach));
+  const int most = (vocab + 8 + kThreads * kEach - 1) / (kThreads * kEach);   // (8: up to the boundary before the row)
   return std::max(1, std::min({1024 / std::max(rows, 1), most, kMaxSplits}));
 }
 
