@@ -14,8 +14,8 @@
 // all lanes and moves rarely, so an element costs a product, an exp2, two
 // additions and the comparisons.  Alternatives: elements that reach the
 // wavefront's bar go to its list of up to 256 in LDS; a list grown long is
-// cut to its best, which raises the bar.  The bar starts below the n-th largest of
-// the lanes' maxima over the first piece, so few elements ever reach it.  Order:
+// cut to its best.  The bar lies below the n-th largest of the lanes' maxima so
+// far, so few elements ever reach it.  Order:
 // value descending (NaN above all), index ascending.  Bound by reading the
 // logits once, or by the launches (one row).
 //
@@ -80,17 +80,7 @@ __device__ __forceinline__ int below(uint64_t mask) {   // set bits under this l
                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
-// Inclusive sum over the lanes of the wavefront.
-__device__ __forceinline__ int lane_sums(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
-
+// The sum over the lanes of the wavefront (row shifts, then the rows' ends carried on).
 __device__ __forceinline__ float lane_total(float x) {
 #define NKV_ADD(ctrl, rows) x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), ctrl, rows, 0xf, false))
   NKV_ADD(0x111, 0xf);
@@ -274,6 +264,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
   // (early: two round trips that nothing waits for)
   const float xt = p.splits == 1 && wave == 0 ? token_logit<K>(p, row, x) : 0.0f;
   List list{keys[wave], ids[wave], 0, p.top, 0u, INT32_MAX};
+  int until = 1, iterations = 1;                  // iterations until the bar is set anew
+  float best = -INFINITY;                         // the lane's maximum so far
   float bar = p.top > 0 ? -INFINITY : INFINITY;   // the list's, as a value
   float m = -INFINITY, s = 0.0f, w = 0.0f;        // m is the wavefront's, s and w the lane's part
   // since m moved: the sums of 2^-z and z 2^-z, big_m = m log2 e rounded (0 of -inf), off what it lacks
@@ -374,12 +366,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
         }
     }
     if (p.top == 0) continue;
-    if (q0 == lo) {
-      // the first bar: at least `top` lanes have a maximum that reaches it, not many more
-      const uint32_t k = score_key(top);
+    best = max_nan(best, top);
+    if (--until == 0) {
+      // the bar from the lanes' maxima so far: `top` lanes have one that reaches it, and not many
+      // more; again after 1, 2, 4, ... iterations, so that an octave brings few candidates
+      until = iterations += iterations;
+      const uint32_t k = score_key(best);
       uint32_t t = 0;
       int n = kWave;
-      for (int bit = 31; bit >= 0 && n > p.top + 8; --bit) {
+      for (int bit = 31; bit >= 0 && n > p.top + 2; --bit) {
         const uint32_t c = t | (1u << bit);
         const int a = count(__ballot(k >= c));
         if (a >= p.top) {
@@ -387,33 +382,36 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
           n = a;
         }
       }
-      list.bar = t;
-      bar = t <= score_key(-INFINITY) ? -INFINITY : key_score(t);
-    }
-    if (!__any(top >= bar)) continue;
-    // how many of the lane's elements reach the bar: then each has its places in the list
-    const bool whole = first >= 0 && q0 + U * kWave <= hi && first + U * kWave * E <= p.vocab;
-    int mine = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) mine += v[u][e] >= bar ? 1 : 0;
-    const int upto = lane_sums(mine);
-    const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
-    if (whole && list.cnt + all <= kList) {
-      int at = list.cnt + upto - mine;
-      if (mine > 0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (v[u][e] >= bar) {
-              list.keys[at] = score_key(v[u][e]);
-              list.ids[at] = static_cast<int>((q0 + u * kWave + lane) * E - head + e);
-              ++at;
-            }
+      if (t > list.bar) {
+        list.bar = t;
+        list.bar_id = INT32_MAX;
       }
-      list.cnt += all;
+      bar = list.bar <= score_key(-INFINITY) ? -INFINITY : key_score(list.bar);
+    }
+    const uint64_t lanes = __ballot(top >= bar);
+    if (lanes == 0) continue;
+    int most = kEach * count(lanes);   // candidates at most, or where that is too many, as they are
+    if (list.cnt + most > kList) {
+      most = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) most += count(__ballot(v[u][e] >= bar));
+    }
+    if (first >= 0 && q0 + U * kWave <= hi && first + U * kWave * E <= p.vocab && list.cnt + most <= kList) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool has = v[u][e] >= bar;
+          const uint64_t mask = __ballot(has);
+          if (mask == 0) continue;
+          if (has) {
+            list.keys[list.cnt + below(mask)] = score_key(v[u][e]);
+            list.ids[list.cnt + below(mask)] = static_cast<int>((q0 + u * kWave + lane) * E - head + e);
+          }
+          list.cnt += count(mask);
+        }
       if (list.cnt > 2 * p.top + 32) {
         list.cut(lane, min(p.top + 8, kWave));
         bar = key_score(list.bar);
