@@ -30,7 +30,10 @@ projections as nanovllm/utils/loader.py:12-28 does) or are random-initialised
 for measurement (``init_random_``).  ``prefill`` / ``decode`` drive the model
 the way the reference's ModelRunner does for one sequence: prefill in chunks
 (the first chunk dense within itself, later chunks sparse), then one token
-per decode step.
+per decode step.  With paged caches instead of the sparse runtimes
+(``attach_paged``) ``paged_step`` runs one step of several sequences at once:
+prompts, tokens or drafted trees, attending densely; the norms, the rotation
+and the writes to the cache are one launch (``nanokv_amd.paged``).
 """
 
 from __future__ import annotations
@@ -46,7 +49,9 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _lib
-from .attention import Attention, attach_m12_runtimes, set_context
+from .attention import Attention, attach_m12_runtimes, attach_paged_cache, get_context, reset_context, set_context
+from .logprobs import TokenLogprobs, token_logprobs
+from .paged import qkv_append_paged
 from .q8 import Q8, linear_q8, linear_silu_mul_q8, norm_linear_q8, norm_linear_silu_mul_q8, quantize_q8
 from .sparse.m12_runtime import M12Config
 from .store import _ptr, _stream
@@ -431,8 +436,31 @@ class Qwen3Attention(nn.Module):
     def forward(self, positions: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
         return self.attend(positions, self.qkv_proj(h))
 
+    def _paged(self, qkv: torch.Tensor):
+        """(cache, norm weights, eps, cos, sin) if norms, rotation and the writes to a
+        paged cache may run as one launch: this file's modules without hooks, bf16 on the GPU."""
+        attn, rope = self.attn, self.rotary_emb
+        if not (_own(attn, Attention) and attn.dense() is not None and _fused(qkv) and _own(rope, RotaryEmbedding)
+                and self.head_dim in (64, 128)) or nn.modules.module._has_any_global_hook():
+            return None
+        weights, eps = (None, None), 0.0
+        if self.qk_norm:
+            qn, kn = self.q_norm, self.k_norm
+            if not (_own(qn, RMSNorm) and _own(kn, RMSNorm) and qn.eps == kn.eps
+                    and qn.weight.dtype == kn.weight.dtype == torch.bfloat16):
+                return None
+            weights, eps = (qn.weight, kn.weight), qn.eps
+        return (attn.dense(), weights, eps, *rope.table(qkv.device))
+
     def attend(self, positions: torch.Tensor, qkv: torch.Tensor) -> torch.Tensor:
         """Everything after the fused q|k|v projection."""
+        held = self._paged(qkv)
+        if held is not None:
+            cache, weights, eps, cos, sin = held
+            context = get_context()
+            q = qkv_append_paged(cache, qkv, self.attn.slots(context), positions, cos, sin, self.num_heads,
+                                 q_norm=weights[0], k_norm=weights[1], eps=eps)
+            return self.o_proj(self.attn.attend(q, context).flatten(1))
         if self.qk_norm and self.head_dim == 128 and _fused(qkv):
             qn, kn, rope = self.q_norm, self.k_norm, self.rotary_emb
             if _own(qn, RMSNorm) and _own(kn, RMSNorm) and _own(rope, RotaryEmbedding):
@@ -508,7 +536,8 @@ class Qwen3DecoderLayer(nn.Module):
         return mlp(h), residual
 
 
-_FORWARDS.update((c, c.forward) for c in (Linear, Q8Linear, RMSNorm, RotaryEmbedding, Qwen3Attention, Qwen3MLP))
+_FORWARDS.update((c, c.forward) for c in (Attention, Linear, Q8Linear, RMSNorm, RotaryEmbedding, Qwen3Attention,
+                                          Qwen3MLP))
 
 
 class Qwen3Model(nn.Module):
@@ -562,6 +591,48 @@ class Qwen3ForCausalLM(nn.Module):
             return gemv_dev(h, self.lm_head_weight)
         return F.linear(h, self.lm_head_weight)
 
+    def token_logprobs(self, h: torch.Tensor, tokens: torch.Tensor, top: int = 0, rows: int = 512) -> TokenLogprobs:
+        """logprobs.token_logprobs of what compute_logits makes of hidden rows h [T, hidden],
+        `rows` rows of logits at a time (a vocabulary's logits of a prompt are gigabytes)."""
+        if rows < 1:
+            raise ValueError(f"token_logprobs takes at least one row at a time (got {rows})")
+        if tokens.shape != h.shape[:1]:
+            raise ValueError(f"tokens must be [{h.shape[0]}] (got {tuple(tokens.shape)})")
+        parts = [token_logprobs(self.compute_logits(h[i:i + rows]), tokens[i:i + rows], top)
+                 for i in range(0, max(h.shape[0], 1), rows)]
+        return parts[0] if len(parts) == 1 else TokenLogprobs(*(torch.cat(t) for t in zip(*parts)))
+
+    # -- dense attention over paged caches ----------------------------------------
+    def attach_paged(self, pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16) -> list:
+        """One paged cache per layer (attention.attach_paged_cache), in the place of sparse runtimes."""
+        self.release_graph()
+        self.runtimes = []
+        return attach_paged_cache(self, pages, page_size, dtype)
+
+    @torch.inference_mode()
+    def paged_step(self, input_ids: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, tables: torch.Tensor,
+                   lengths: torch.Tensor, *, starts: torch.Tensor | None = None, max_new: int | None = None,
+                   tree: torch.Tensor | None = None) -> torch.Tensor:
+        """One step of several sequences: the hidden rows [T, hidden] of their new tokens
+        input_ids [T] at `positions` [T] (compute_logits, token_logprobs take them).
+
+        The tokens' keys and values go to `slots` [T] of every layer's cache and attend
+        to their sequences' keys: tables, lengths, starts, max_new and tree as
+        paged.attend_paged takes them.  Nothing is read back, so a step of fixed sizes can be
+        captured in a graph, its inputs changed in place."""
+        if self.model.layers and self.model.layers[0].self_attn.attn.dense() is None:
+            raise RuntimeError("attach_paged() the caches first")
+        n = input_ids.numel()
+        if positions.shape != (n,) or slots.shape != (n,) or input_ids.dim() != 1:
+            raise ValueError(f"input_ids, positions and slots must be alike, [T] (got {tuple(input_ids.shape)}, "
+                             f"{tuple(positions.shape)}, {tuple(slots.shape)})")
+        set_context(starts is not None, cu_seqlens_q=starts, max_seqlen_q=max_new or 0, slot_mapping=slots,
+                    context_lens=lengths, block_tables=tables, tree_masks=tree)
+        try:
+            return self(input_ids, positions)
+        finally:
+            reset_context()
+
     # -- sparse runtime wiring and one-sequence driving -------------------------
     def attach(self, m12: M12Config, device=None) -> list:
         """One M12 runtime per layer over one shared HBM store (model_runner.py:125-183)."""
@@ -590,6 +661,18 @@ class Qwen3ForCausalLM(nn.Module):
     def prefill(self, input_ids: torch.Tensor, chunk: int = 4096) -> torch.Tensor:
         """Prefill a new sequence in chunks of `chunk` tokens; returns the
         logits of its last token ([vocab] fp32)."""
+        return self._prefill(input_ids, chunk, None)
+
+    @torch.inference_mode()
+    def prefill_logprobs(self, input_ids: torch.Tensor, top: int = 0, chunk: int = 4096) -> tuple:
+        """prefill, and the log probabilities of the prompt's tokens after its first
+        (token_logprobs with `top` alternatives): (logits of the last token, TokenLogprobs of [n - 1])."""
+        parts = []
+        logits = self._prefill(input_ids, chunk, lambda h, s, e: parts.append(
+            self.token_logprobs(h[:min(e, input_ids.numel() - 1) - s], input_ids[s + 1:e + 1], top)))
+        return logits, TokenLogprobs(*(torch.cat(t) for t in zip(*parts)))
+
+    def _prefill(self, input_ids: torch.Tensor, chunk: int, each) -> torch.Tensor:
         if not self.runtimes:
             raise RuntimeError("attach() the sparse runtimes first")
         if self.runtimes[0].valid_len:
@@ -605,6 +688,8 @@ class Qwen3ForCausalLM(nn.Module):
             pos = torch.arange(s, e, device=ids.device)
             set_context(True, max_seqlen_q=ids.numel(), max_seqlen_k=s + ids.numel())
             h = self(ids, pos)
+            if each is not None:
+                each(h, s, e)
         return self.compute_logits(h[-1:]).float()[0]
 
     @torch.inference_mode()
