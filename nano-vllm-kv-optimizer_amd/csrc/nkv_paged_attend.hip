@@ -13,8 +13,8 @@
 //     ahead; P enters the second product as bf16 high and low parts, as good as fp32.
 //   * many_kernel, tiles of 64 or 128 columns (trees, prompts): 64-key tiles staged in LDS
 //     for all four wavefronts, the next one on its way; bound by the matrix cores for
-//     long prompts, by the keys for trees.  P is rounded to bf16 for the second product (2^-9
-//     of each weight, fewer than the output's own rounding), numerator and denominator alike.
+//     long prompts, by the keys for trees.  P is rounded to bf16 for the second product (2^-8
+//     of each weight, as the output's own rounding), in 16 bits numerator and denominator alike.
 // 8-bit caches: the codes are bf16 exactly; a key's scale multiplies its logits, a
 // value's its weights, both in fp32.
 //
@@ -214,6 +214,7 @@ __device__ void redo_column(const Params& p, const Seq& s, const cint32* table, 
     l = l * alpha + w;
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] = o[e] * alpha + w * (v[e] * vs);
+    if (l != l) break;   // (NaN, whatever follows)
   }
 }
 
@@ -707,7 +708,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     if (!SHARED && qt == 0) clear_others(p, s, b, h, D);
     const int t0 = qt * tpw;
     const int tiles = key_tiles(p, s, qt, kKeys);
-    if (tiles > 0) {
+    if (!SHARED && tiles == 0) return;   // (the list has units with queries only)
     const int t_last = min(t0 + tpw, min(s.count, p.n)) - 1;
     const int lo = tile0, hi = min(tiles, left < tiles ? lo + left : tiles);
     const int32_t* table = p.tables + b * p.table_ls;
@@ -974,11 +975,10 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
 
     // ---- store: acc[i][ct][e] is dim 16 i + 4 lg + e
     const bool whole = hi - lo == tiles;
-    {
-    const Params& p = again();
+    const Params& late = again();
     if (SHARED && lo == 0 && threadIdx.x == 0)   // (one that is cut is the run's last)
-      *note_of(p, (h * p.B + b) * qtiles + qt) =
-          Note{whole ? 1 : list.worker_of(list.lo(worker + 1) - hi + tiles - 1) - worker + 1, worker, s.begin + t0, (t_last + 1 - t0) * p.G};
+      *note_of(late, (h * late.B + b) * qtiles + qt) =
+          Note{whole ? 1 : list.worker_of(list.lo(worker + 1) - hi + tiles - 1) - worker + 1, worker, s.begin + t0, (t_last + 1 - t0) * late.G};
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct) {
       const int c0 = wave * 16 * NCT + ct * 16;
@@ -993,9 +993,9 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
       const uint64_t lanes = __ballot(odd && mine);
       const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
       auto orow = [&](int cc) {
-        return p.out + (static_cast<int64_t>(s.begin + t0 + cc / p.G) * p.hq + h * p.G + cc % p.G) * D;
+        return late.out + (static_cast<int64_t>(s.begin + t0 + cc / late.G) * late.hq + h * late.G + cc % late.G) * D;
       };
-      auto rec = [&](int cc) { return record_of<D>(p, 2 * worker + (lo > 0 ? 0 : 1), cc); };
+      auto rec = [&](int cc) { return record_of<D>(late, 2 * worker + (lo > 0 ? 0 : 1), cc); };
       if (mine && !((redo >> ln) & 1)) {
         if (!SHARED || whole) {
           uint16_t* dst = orow(c) + 4 * lg;
@@ -1018,25 +1018,22 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
       for (uint32_t todo = redo; todo != 0; todo &= todo - 1) {
         const int cc = c0 + __builtin_ctz(todo);
         float mc, lc, oc[D / 64];
-        redo_column<D, INT8>(p, s, (const cint32*)table, h, t0 + cc / p.G, h * p.G + cc % p.G, lo * kKeys, hi * kKeys, lane, mc, lc, oc);
-        store_column<D>(p, whole, whole ? orow(cc) : nullptr, whole ? nullptr : rec(cc), lane, mc, lc, oc);
+        redo_column<D, INT8>(late, s, (const cint32*)table, h, t0 + cc / late.G, h * late.G + cc % late.G, lo * kKeys, hi * kKeys, lane, mc, lc, oc);
+        store_column<D>(late, whole, whole ? orow(cc) : nullptr, whole ? nullptr : rec(cc), lane, mc, lc, oc);
       }
     }
-    }
     left -= hi - lo;
-    }
     if (!SHARED || left <= 0) return;
     // ---- the next unit of the list
-    const Params& next = again();
     tile0 = 0;
-    if (++qt * tpw >= min(s.count, next.n)) {
+    if (++qt * tpw >= min(s.count, late.n)) {
       qt = 0;
       do {
-        if (++b == next.B) {
+        if (++b == late.B) {
           b = 0;
           ++h;
         }
-      } while (seq_of(next, b).count == 0);   // (there is a unit: the run goes on)
+      } while (seq_of(late, b).count == 0);   // (there is a unit: the run goes on)
     }
     __syncthreads();   // (the stages have been read)
   }

@@ -341,3 +341,45 @@ def test_far_offsets_in_a_cache_past_32_bits():
         a = attend_paged(q, cache, torch.tensor([far], dtype=torch.int32, device="cuda"), lens)
         b = attend_paged(q, small, torch.arange(4, dtype=torch.int32, device="cuda")[None], lens)
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_more_sequences_than_lanes(kv):
+    """A token of each of 150 sequences, some empty, some of no new token."""
+    from nanokv_amd.paged import attend_paged
+    lengths = [(37 * b) % 230 for b in range(150)]
+    cache, tables, lens = _setup(lengths, 2, 16, 64, kv, seed=5)
+    q = _q(150, 4, 64, 9)
+    _check(attend_paged(q, cache, tables, lens), q, cache, tables, lens)
+    counts = [0] * 70 + [b % 3 for b in range(80)]                     # (the first 64 hold no query)
+    starts = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    n = int(starts[-1])
+    got = attend_paged(q[:n], cache, tables, lens, starts=starts, max_new=2)
+    _check(got, q[:n], cache, tables, lens, starts)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("cap", [300, 4608])
+def test_more_query_tiles_than_lanes(kv, cap):
+    """100 sequences of up to 20 new tokens under tables of `cap` tokens: a workgroup a unit, or a shared list."""
+    from nanokv_amd.paged import attend_paged
+    lengths = [20 + (53 * b) % 200 for b in range(100)]
+    cache, tables, lens = _setup(lengths, 1, 16, 64, kv, seed=6)
+    tables = torch.nn.functional.pad(tables, (0, max(0, cap // 16 - tables.shape[1])), value=-1)
+    q = _q(2000, 4, 64, 10)
+    _check(attend_paged(q, cache, tables, lens), q, cache, tables, lens, n_each=20)
+    counts = [0] * 66 + [(7 * b) % 21 for b in range(34)]
+    starts = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    n = int(starts[-1])
+    got = attend_paged(q[:n], cache, tables, lens, starts=starts, max_new=20)
+    _check(got, q[:n], cache, tables, lens, starts, many=True)
+
+
+def test_nan_keys_make_nan_outputs():
+    """A NaN key that a query sees: its output is NaN, other queries' are not."""
+    from nanokv_amd.paged import attend_paged
+    cache, tables, lens = _setup([200, 200], 1, 16, 64, "bf16", seed=7)
+    cache.k[int(tables[0, 3]), 0, 5] = float("nan")                     # key 53 of the first sequence
+    for each in (1, 40):
+        got = attend_paged(_q(2 * each, 4, 64, 11), cache, tables, lens)
+        assert bool(got[:each].isnan().all()) and not bool(got[each:].isnan().any())
