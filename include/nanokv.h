@@ -710,7 +710,8 @@ int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale
  * head to head and token to token (rows on 16-byte boundaries, at most 64 MiB
  * from token to token), so other orders of the first three dimensions are read in place.
  * Slot s is token s % page_size of page s / page_size.
- * Constraints: D 64 or 128; page_size a power of two from 16 to 4096.
+ * Constraints: D 64 or 128; page_size a power of two from 16 to 4096; at most 2^27
+ * rows of heads written, read or moved in a call.
  * ---------------------------------------------------------------------- */
 
 /*
@@ -772,9 +773,9 @@ int64_t nkv_paged_move_workspace(int num_kv_heads, int head_dim, int int8, int r
  * max_new: at least every sequence's new tokens (rows behind it give 0).
  * workspace: nkv_paged_attend_workspace(...) floats, 16-byte aligned (NULL where that is 0;
  * ragged: starts != NULL), asked with the launch's device current.  Calls that may overlap take two.
- * Constraints: batch <= 65535, Hq / Hkv <= 64, max_new <= 2^20, scale > 0,
- * max_pages * page_size < 2^31 - 4096, and fewer than 2^31 pieces of 32 keys in batch such
- * tables times Hkv.
+ * Constraints: batch <= 65535, batch * Hkv < 2^24, Hq / Hkv <= 64, max_new <= 2^20 and at most 65535
+ * times 128 / (Hq / Hkv) rounded down, scale > 0, max_pages * page_size < 2^31 - 4096, and fewer than
+ * 2^31 pieces of 32 keys in batch such tables times Hkv.
  */
 int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale, int64_t page_stride, int64_t head_stride,
                      int64_t token_stride, int pages, int num_kv_heads, int page_size, int head_dim,
@@ -792,7 +793,7 @@ int64_t nkv_paged_attend_workspace(int batch, int rows, int max_new, int num_hea
  * ties to the lower id).  -inf logits have no probability; a row of -inf alone,
  * or with a NaN or +inf, has NaN for all of its numbers.  fp32 throughout.
  * workspace: nkv_token_logprobs_workspace(rows, vocab, top) floats (NULL where that is 0).
- * Constraints: top <= min(64, vocab).
+ * Constraints: top <= min(64, vocab), rows < 2^24.
  */
 int nkv_token_logprobs(const void* logits, int kind, int64_t row_stride, int rows, int vocab, const int64_t* tokens,
                        int top, float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids,

@@ -35,6 +35,7 @@ constexpr int kList = 256;       // candidates a wavefront keeps at most
 constexpr int kMaxTop = 64;      // alternatives: one a lane in the final order
 constexpr int kEach = 16;        // elements a lane takes per iteration
 constexpr int kMaxSplits = 128;  // pieces of a row
+constexpr int kMaxRows = (1 << 24) - 1;   // (a launch has fewer than 2^32 threads)
 constexpr float kLog2e = 1.44269504088896340736f;
 
 enum Kind { kF32 = 0, kBf16 = 1, kF16 = 2 };
@@ -547,7 +548,7 @@ extern "C" int nkv_token_logprobs(const void* logits, int kind, int64_t row_stri
   NKV_CHECK_ARG(top >= 0 && top <= kMaxTop && top <= vocab,
                 "nkv_token_logprobs: top must be from 0 to %d and at most vocab (got %d)", kMaxTop, top);
   if (rows == 0) return NKV_OK;
-  NKV_CHECK_ARG(rows <= INT32_MAX / 2, "nkv_token_logprobs: at most 2^30 rows");
+  NKV_CHECK_ARG(rows <= kMaxRows, "nkv_token_logprobs: at most 2^24 - 1 rows");
   NKV_CHECK_ARG(logits && tokens && logprob && entropy && (top == 0 || (top_logprobs && top_ids)),
                 "nkv_token_logprobs: NULL input or output");
   NKV_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % (kind == kF32 ? 4 : 2) == 0 && row_stride >= 0,

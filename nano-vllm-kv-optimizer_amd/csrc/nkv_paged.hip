@@ -56,6 +56,7 @@ int fill_paged(const char* who, void* k, void* v, float* k_scale, float* v_scale
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxUnits = 1 << 27;   // (16 lanes each: a launch has fewer than 2^32 threads)
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -303,7 +304,7 @@ extern "C" int nkv_paged_append(void* k, void* v, float* k_scale, float* v_scale
     return rc;
   NKV_CHECK_ARG(rows >= 0 && num_heads >= 0, "nkv_paged_append: rows and num_heads must not be negative");
   const int64_t units = static_cast<int64_t>(rows) * (num_heads + 2LL * num_kv_heads);
-  NKV_CHECK_ARG(units <= INT32_MAX / 2, "nkv_paged_append: at most 2^30 rows of heads");
+  NKV_CHECK_ARG(units <= kMaxUnits, "nkv_paged_append: at most 2^27 rows of heads");
   NKV_CHECK_ARG(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0,
                 "nkv_paged_append: rotary_dim must be a multiple of 16 up to head_dim (got %d)", rotary_dim);
   if (rows == 0) return NKV_OK;
@@ -337,7 +338,7 @@ extern "C" int nkv_paged_read(void* k, void* v, float* k_scale, float* v_scale, 
                           num_kv_heads, page_size, head_dim, &c))
     return rc;
   const int64_t units = static_cast<int64_t>(rows) * 2 * num_kv_heads;
-  NKV_CHECK_ARG(rows >= 0 && units <= INT32_MAX / 2, "nkv_paged_read: from 0 to 2^30 rows of heads");
+  NKV_CHECK_ARG(rows >= 0 && units <= kMaxUnits, "nkv_paged_read: from 0 to 2^27 rows of heads");
   if (rows == 0) return NKV_OK;
   NKV_CHECK_ARG(slots && k_out && v_out, "nkv_paged_read: slots and outputs must be non-NULL");
   NKV_CHECK_ARG((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 == 0,
@@ -364,7 +365,7 @@ extern "C" int nkv_paged_move(void* k, void* v, float* k_scale, float* v_scale, 
                           num_kv_heads, page_size, head_dim, &c))
     return rc;
   const int64_t units = static_cast<int64_t>(rows) * 2 * num_kv_heads;
-  NKV_CHECK_ARG(rows >= 0 && units <= INT32_MAX / 2, "nkv_paged_move: from 0 to 2^30 rows of heads");
+  NKV_CHECK_ARG(rows >= 0 && units <= kMaxUnits, "nkv_paged_move: from 0 to 2^27 rows of heads");
   if (rows == 0) return NKV_OK;
   NKV_CHECK_ARG(src && dst && workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                 "nkv_paged_move: src, dst and a workspace on a 16-byte boundary are needed");

@@ -1156,7 +1156,7 @@ Plan plan_of(int B, int T, int n, int hkv, int G, int head_dim, int64_t cap_toke
   const int slots = (head_dim == 128 ? 2 : 3) * cus;   // workgroups that the CUs hold
   const int64_t cap = (cap_tokens + kKeys - 1) / kKeys;
   const int64_t units = std::max<int64_t>(ragged ? 1 : B, (static_cast<int64_t>(T) + q.tpw - 1) / q.tpw) * hkv;   // at least
-  const bool fits = static_cast<int64_t>(B) * q.qtiles <= 1024 && cap * B * q.qtiles * hkv <= INT32_MAX;
+  const bool fits = static_cast<int64_t>(B) * q.qtiles <= 1024 && hkv <= 1024 && cap * B * q.qtiles * hkv <= INT32_MAX;
   q.workers = fits && units < slots && cap * (slots - units) > 32 * static_cast<int64_t>(slots) ? slots : 0;
   return q;
 }
@@ -1204,6 +1204,8 @@ int check_sizes(const char* who, int batch, int rows, int max_new, int num_heads
   NKV_CHECK_ARG(num_kv_heads >= 1 && num_heads >= num_kv_heads && num_heads % num_kv_heads == 0 && num_kv_heads <= 65535,
                 "%s: num_heads (%d) must be a positive multiple of num_kv_heads (%d)", who, num_heads, num_kv_heads);
   NKV_CHECK_SUPPORTED(num_heads / num_kv_heads <= 64, "%s: at most 64 query heads a KV head", who);
+  // (a launch has fewer than 2^32 threads)
+  NKV_CHECK_ARG(static_cast<int64_t>(batch) * num_kv_heads < 1 << 24, "%s: fewer than 2^24 pairs of a sequence and a KV head", who);
   NKV_CHECK_ARG(max_pages >= 1 && static_cast<int64_t>(max_pages) * page_size <= INT32_MAX - 4096,
                 "%s: a page table covers from 1 page to 2^31 - 4097 tokens", who);
   const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size / kFewKeys + 1) * num_kv_heads;
@@ -1248,8 +1250,7 @@ extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale
                 "%s: rows must lie on 16-byte boundaries", who);
   const int G = num_heads / num_kv_heads;
   p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, head_dim, static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
-  NKV_CHECK_ARG(p.plan.qtiles <= 65535,
-                "%s: too many query rows", who);
+  NKV_CHECK_ARG(p.plan.qtiles <= 65535, "%s: at most 65535 query tiles of a sequence (max_new is %d)", who, max_new);
   NKV_CHECK_ARG(part_floats(p.plan, batch, num_kv_heads, head_dim) == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "%s: these sizes need a workspace on a 16-byte boundary", who);
   p.q = q;

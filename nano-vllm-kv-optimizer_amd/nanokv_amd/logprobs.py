@@ -24,6 +24,7 @@ from .q8 import INT_MAX, _asks_gradient, _call
 
 MAX_TOP = 64
 MAX_VOCAB = INT_MAX - 65536
+MAX_ROWS = 2 ** 24 - 1
 _KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -69,8 +70,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if _asks_gradient(logits):
         raise ValueError(f"{who}: the logits ask for a gradient, and this operator has none")
     rows = logits.numel() // vocab
-    if rows > INT_MAX // 2:
-        raise ValueError(f"{who}: at most {INT_MAX // 2} rows (got {rows})")
+    if rows > MAX_ROWS:
+        raise ValueError(f"{who}: at most {MAX_ROWS} rows (got {rows})")
     if not logits.is_cuda:
         return _formula(logits, tokens.long(), top)
     device = logits.device

@@ -44,6 +44,7 @@ def test_rows_without_a_distribution():
     (dict(tokens=torch.zeros(2)), "tokens must be"),
     (dict(top=9), "top must be"), (dict(top=-1), "top must be"), (dict(top=2.0), "top must be"),
     (dict(top=True), "top must be"),
+    (dict(logits=torch.zeros(1, 8).expand(2 ** 24, 8), tokens=torch.zeros(1, dtype=torch.long).expand(2 ** 24)), "16777215 rows"),
     (dict(logits=torch.zeros(2, 8, requires_grad=True)), "gradient")])
 def test_refusals(change, words):
     args = dict(logits=torch.zeros(2, 8), tokens=torch.zeros(2, dtype=torch.long), top=2) | change
@@ -64,7 +65,7 @@ def test_the_library_refuses_before_any_device_work():
     for change, words in ((dict(kind=3), b"type of logits"), (dict(vocab=0), b"vocab"), (dict(rows=-1), b"rows"),
                           (dict(top=65), b"top must be"), (dict(top=101), b"top must be"), (dict(logits=None), b"NULL"),
                           (dict(tl=None), b"NULL"), (dict(logits=ctypes.c_void_p(66)), b"aligned"),
-                          (dict(vocab=151936, ws=None, rows=1), b"workspace")):
+                          (dict(vocab=151936, ws=None, rows=1), b"workspace"), (dict(rows=2 ** 24), b"2^24 - 1")):
         assert call(**change) == _lib.NKV_ERR_ARG and words in lib.nkv_last_error(), change
     assert call(rows=0) == _lib.NKV_OK
     assert lib.nkv_token_logprobs_workspace(1, 151936, 20) > 0

@@ -84,6 +84,9 @@ def test_the_library_refuses_before_any_device_work():
     for change, words in BAD_CACHES:
         assert refused(call(change), words), change
     assert refused(call(dict(ks=ctypes.c_void_p(72), vs=P)), b"scales must lie")
+    assert refused(call(dict(hkv=300), batch=65535, rows=65535, new=1, heads=300, most=1), b"2^24 pairs")
+    assert refused(call(dict(hkv=1), batch=1, rows=2 ** 20, new=2 ** 20, heads=64, most=4096), b"65535 query tiles")
+    assert refused(call(dict(hkv=300), batch=4096, rows=4096, new=1, heads=300, most=65536), b"2^31 pieces of 32 keys")
     for change, words in ((dict(batch=-1), b"65535 sequences"), (dict(batch=65536, rows=131072), b"65535 sequences"),
                           (dict(new=0), b"max_new"), (dict(new=2 ** 20 + 1), b"max_new"), (dict(heads=3), b"multiple"),
                           (dict(heads=130), b"64 query heads"), (dict(most=0), b"page table"),

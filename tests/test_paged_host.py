@@ -147,7 +147,7 @@ def test_the_library_refuses_rows():
     lib, c = _lib.load(), list(CACHE.values())
     good = dict(q=P, qs=512, k=P, ks=512, v=P, vs=512, rows=1, heads=4, slots=P, pos=P, cos=P, sin=P, most=8, rot=64,
                 inter=0, qw=P, kw=P, eps=1e-6, out=P)
-    for change, words in ((dict(rows=-1), b"negative"), (dict(rows=2 ** 30), b"2^30"), (dict(rot=72), b"rotary_dim"),
+    for change, words in ((dict(rows=-1), b"negative"), (dict(rows=2 ** 27), b"2^27"), (dict(rot=72), b"rotary_dim"),
                           (dict(rot=80), b"rotary_dim"), (dict(rot=-16), b"rotary_dim"), (dict(k=None), b"non-NULL"),
                           (dict(slots=None), b"non-NULL"), (dict(out=None), b"q_rows and q_out"),
                           (dict(pos=None), b"rotation"), (dict(most=0), b"rotation"), (dict(qs=511), b"16-byte"),
