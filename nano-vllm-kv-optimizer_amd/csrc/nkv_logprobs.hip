@@ -44,6 +44,7 @@ struct Params {
   const char* x;
   int64_t stride;          // elements from row to row
   int rows, vocab, top, splits;
+  int per;                 // 16-byte pieces of a wavefront's run
   const int64_t* tokens;
   float* logprob;
   float* entropy;
@@ -81,17 +82,38 @@ __device__ __forceinline__ int below(uint64_t mask) {   // set bits under this l
                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
-// The sum over the lanes of the wavefront (row shifts, then the rows' ends carried on).
+// A reduction over the lanes of the wavefront (row shifts, then the rows' ends carried on), `none` its
+// neutral element.
+template <typename F>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t x, uint32_t none, F&& f) {
+#define NKV_STEP(ctrl, rows) \
+  x = f(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(x), ctrl, rows, 0xf, false)))
+  NKV_STEP(0x111, 0xf);
+  NKV_STEP(0x112, 0xf);
+  NKV_STEP(0x114, 0xf);
+  NKV_STEP(0x118, 0xf);
+  NKV_STEP(0x142, 0xa);
+  NKV_STEP(0x143, 0xc);
+#undef NKV_STEP
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), kWave - 1));
+}
 __device__ __forceinline__ float lane_total(float x) {
-#define NKV_ADD(ctrl, rows) x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), ctrl, rows, 0xf, false))
-  NKV_ADD(0x111, 0xf);
-  NKV_ADD(0x112, 0xf);
-  NKV_ADD(0x114, 0xf);
-  NKV_ADD(0x118, 0xf);
-  NKV_ADD(0x142, 0xa);
-  NKV_ADD(0x143, 0xc);
-#undef NKV_ADD
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), kWave - 1));
+  return __uint_as_float(over_lanes(__float_as_uint(x), 0u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ float lane_top(float x) {   // (a NaN gives way)
+  return __uint_as_float(over_lanes(__float_as_uint(x), 0xff800000u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ uint32_t lane_max(uint32_t x) {
+  return over_lanes(x, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+// What keys from lo to hi have in common, as the least number that has it; bit: the first in which they differ (-1: none).
+__device__ __forceinline__ uint32_t prefix_of(uint32_t lo, uint32_t hi, int& bit) {
+  bit = lo == hi ? -1 : 31 - __builtin_clz(lo ^ hi);
+  return bit < 0 ? hi : hi & ~((2u << bit) - 1);
 }
 
 // A wavefront's candidates: (key, id) in LDS, and the bar that a new one has to
@@ -118,9 +140,11 @@ struct List {
     uint32_t t = 1;      // the smallest key kept (all candidates when there are few)
     int last = INT32_MAX;
     if (have > most) {
-      t = 0;             // at least `top` keys are t or more, bit by bit, until they are few enough
-      int kept = have;
-      for (int bit = 31; bit >= 0 && kept > most; --bit) {
+      // at least `top` keys are t or more, bit by bit, until they are few enough
+      const uint32_t hi = lane_max(max(max(k[0], k[1]), max(k[2], k[3])));
+      const uint32_t lo = ~lane_max(max(max(~(k[0] - 1), ~(k[1] - 1)), max(~(k[2] - 1), ~(k[3] - 1)))) + 1;   // (of those not 0)
+      int kept = have, bit;
+      for (t = prefix_of(lo, hi, bit); bit >= 0 && kept > most; --bit) {
         const uint32_t c = t | (1u << bit);
         const int n = above([&](uint32_t a, int) { return a >= c; });
         if (n >= top) {
@@ -131,7 +155,7 @@ struct List {
       if (kept > most) {   // too many are equal: of those the lowest ids
         const int more = above([&](uint32_t a, int) { return a > t; });
         last = 0;
-        for (int bit = 30; bit >= 0; --bit) {
+        for (bit = 30; bit >= 0; --bit) {
           const int c = last | (1 << bit);
           // ids below c are too few: the (top - more)-th lowest is c or more
           if (above([&](uint32_t a, int i) { return a == t && i < c; }) < top - more) last = c;
@@ -215,11 +239,10 @@ __device__ __forceinline__ void finish(const Params& p, int row, float xt, Stat 
   }
 }
 
-// The wavefronts' lists and numbers as one: in wavefront 0.
+// The wavefronts' lists (up to 64 each) and numbers as one: in wavefront 0.
 __device__ __forceinline__ void join_waves(uint32_t (&keys)[kWaves][kList], int (&ids)[kWaves][kList],
                                            Stat (&stats)[kWaves], int (&counts)[kWaves], int wave, int lane, Stat& t,
                                            List& list) {
-  if (list.cnt > kWave) list.cut(lane, kWave);   // (one of the four lists a lane below)
   if (lane == 0) {
     stats[wave] = t;
     counts[wave] = list.cnt;
@@ -258,9 +281,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
   // 16-byte pieces from the boundary at or before the row: element i is in piece (i + head) / E
   const int head = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / kBytes<K>);
   const int64_t pieces = (static_cast<int64_t>(p.vocab) + head + E - 1) / E;
-  constexpr int kStep = U * kWave;     // pieces of an iteration: runs are whole ones but for the row's end
-  const int64_t per = (pieces + static_cast<int64_t>(p.splits) * kWaves * kStep - 1) / (p.splits * kWaves * kStep) * kStep;
-  const int64_t lo = min(per * (split * kWaves + wave), pieces), hi = min(lo + per, pieces);
+  const int64_t lo = min(static_cast<int64_t>(p.per) * (split * kWaves + wave), pieces), hi = min(lo + p.per, pieces);
 
   // (early: two round trips that nothing waits for)
   const float xt = p.splits == 1 && wave == 0 ? token_logit<K>(p, row, x) : 0.0f;
@@ -318,10 +339,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
 #pragma unroll
       for (int e = 0; e < E; ++e) top = max_nan(top, v[u][e]);
     if (__any(top > m) || !(fabsf(m) < 0x1p126f)) {   // (m log2 e may be infinite: never in M's form)
-      float t = top;      // (a lane's NaN gives way to the others' values)
-#pragma unroll
-      for (int o = kWave / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
-      t = fmaxf(t, m);
+      const float t = fmaxf(lane_top(top), m);
       settle();
       // the sums move to the new maximum; the old one becomes an element like others (lane 0 has it)
       const bool moves = t > m;
@@ -373,9 +391,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
       // more; again after 1, 2, 4, ... iterations, so that an octave brings few candidates
       until = iterations += iterations;
       const uint32_t k = score_key(best);
-      uint32_t t = 0;
-      int n = kWave;
-      for (int bit = 31; bit >= 0 && n > p.top + 2; --bit) {
+      int n = kWave, bit;
+      uint32_t t = prefix_of(~lane_max(~k), lane_max(k), bit);
+      for (; bit >= 0 && n > p.top + 2; --bit) {
         const uint32_t c = t | (1u << bit);
         const int a = count(__ballot(k >= c));
         if (a >= p.top) {
@@ -419,15 +437,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
       }
     } else {
       // (all 64 lanes' element e at once; an element outside the row or run is none)
-      for (int u = 0; u < U; ++u)
+#pragma unroll 1
+      for (int j = 0; j < U * E; ++j) {
+        float f = v[0][0];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float f = u == 0 ? v[0][e] : u == 1 ? v[1 % U][e] : u == 2 ? v[2 % U][e] : v[3 % U][e];
-          if (!__any(f >= bar)) continue;
-          const int64_t q = q0 + u * kWave + lane, i = q * E - head + e;
-          list.add(f >= bar && q < hi && i >= 0 && i < p.vocab, score_key(f), static_cast<int>(i), lane);
-          bar = list.bar <= score_key(-INFINITY) ? -INFINITY : key_score(list.bar);
-        }
+        for (int i = 1; i < U * E; ++i) f = i == j ? v[i / E][i % E] : f;
+        if (!__any(f >= bar)) continue;
+        const int64_t q = q0 + j / E * kWave + lane, i = q * E - head + j % E;
+        list.add(f >= bar && q < hi && i >= 0 && i < p.vocab, score_key(f), static_cast<int>(i), lane);
+        bar = list.bar <= score_key(-INFINITY) ? -INFINITY : key_score(list.bar);
+      }
     }
   }
   settle();
@@ -451,6 +470,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
       }
     }
   }
+  if (list.cnt > kWave) list.cut(lane, kWave);
   join_waves(keys, ids, stats, counts, wave, lane, t, list);
   if (wave != 0) return;
   if (p.splits == 1) {
@@ -490,22 +510,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const Params p)
     const float* r = recs + static_cast<int64_t>(mine) * (4 + 2 * p.top);
     t = Stat{r[0], r[1], r[2]};
   }
-  // the records' candidates as one run, four loads of each in flight
+  // the records' candidates as one run, three of each lane beside the best 64 so far
   const int size = 4 + 2 * p.top, all = p.splits * p.top;
-  for (int e0 = wave * kWave; e0 < all; e0 += 4 * kThreads) {
+  for (int e0 = 0; e0 < all; e0 += 3 * kThreads) {
     uint32_t key[4];
-    int id[4];
+    int id[4], have = list.cnt;
+    key[0] = lane < list.cnt ? keys[wave][lane] : 0u;
+    id[0] = lane < list.cnt ? ids[wave][lane] : INT32_MAX;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = min(e0 + i * kThreads + lane, all - 1);
+    for (int i = 1; i < 4; ++i) {
+      const int x = e0 + (i - 1) * kThreads + static_cast<int>(threadIdx.x), e = min(x, all - 1);
       const int rec = static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(p.top)), at = e - rec * p.top;
       const float* r = recs + rec * size;
-      const bool in = e0 + i * kThreads + lane < all && at < __float_as_int(r[3]);
-      key[i] = in ? __float_as_uint(r[4 + at]) : 0u;
-      id[i] = in ? __float_as_int(r[4 + p.top + at]) : INT32_MAX;
+      const int entries = __float_as_int(r[3]);
+      key[i] = __float_as_uint(r[4 + at]);   // (what lies behind the entries may be anything)
+      id[i] = __float_as_int(r[4 + p.top + at]);
+      const bool in = x < all && at < entries;
+      key[i] = in ? key[i] : 0u;
+      id[i] = in ? id[i] : INT32_MAX;
+      have += count(__ballot(in));
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) list.add(key[i] != 0, key[i], id[i], lane);
+    list.keep_best(key, id, have, kWave);
   }
   // the lanes that have a record joined
   int lanes = 1;
@@ -524,7 +549,11 @@ int splits_of(int rows, int vocab) {
 }
 
 template <int K>
-void launch(const Params& p, hipStream_t s) {
+void launch(Params p, hipStream_t s) {
+  // runs are whole iterations but for the row's end (which may lie a piece further than it need)
+  constexpr int E = 16 / kBytes<K>, step = kEach / E * kWave;
+  const int64_t pieces = (p.vocab + 2LL * (E - 1)) / E, runs = static_cast<int64_t>(p.splits) * kWaves * step;
+  p.per = static_cast<int>((pieces + runs - 1) / runs * step);
   logprobs_kernel<K><<<static_cast<unsigned>(p.rows) * p.splits, kThreads, 0, s>>>(p);
   if (p.splits > 1) logprobs_join_kernel<K><<<p.rows, kThreads, 0, s>>>(p);
 }
@@ -555,7 +584,7 @@ extern "C" int nkv_token_logprobs(const void* logits, int kind, int64_t row_stri
                 "nkv_token_logprobs: logits must be aligned to their elements");
   const int splits = splits_of(rows, vocab);
   NKV_CHECK_ARG(splits == 1 || workspace, "nkv_token_logprobs: these sizes need a workspace");
-  const Params p{static_cast<const char*>(logits), row_stride, rows,    vocab,        top,     splits,
+  const Params p{static_cast<const char*>(logits), row_stride, rows,    vocab,   top,          splits,  0,
                  tokens,                           logprob,    entropy, top_logprobs, top_ids, workspace};
   const auto s = static_cast<hipStream_t>(stream);
   if (kind == kF32) launch<kF32>(p, s);
