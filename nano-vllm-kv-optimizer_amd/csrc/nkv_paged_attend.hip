@@ -825,7 +825,9 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     };
 
     // One tile in `buf`.  Operand reads run two products ahead through a ring of three
-    // registers; the scheduling barriers keep that order.
+    // registers; the scheduling barriers keep that order.  The priority takes one of a SIMD's
+    // wavefronts through its products, so that the others' softmax falls beside them (4096 tokens behind
+    // 12288: 871 us without, 823 with it).
     auto attend = [&](int tile, int got, const char* buf) {
       const float* scales = reinterpret_cast<const float*>(buf + 2 * kTile<D>);
       const bool mask = got != 15 || tile * kKeys + kKeys - 1 > (p.tree ? s.older - 1 : s.older + t0);
@@ -842,6 +844,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
           return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         };
         // ---- S^T = K Q^T: S[kt][ct][e] is key 16 kt + 4 lg + e of the pass, column ct
+        __builtin_amdgcn_s_setprio(1);
         f32x4 S[KT][NCT];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
@@ -889,6 +892,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
             }
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         // ---- softmax: a maximum moves only where a logit passes it by 2^8
         float top[NCT];
         bool move = false;
@@ -937,6 +941,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
           }
         }
         // ---- O^T += V^T P^T, the row sums a product with ones
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
           const int j = i / DT, dt = i % DT;
@@ -958,6 +963,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
             acc[dt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[i % 3], bp[ct], acc[dt][ct], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
     };
 
