@@ -47,7 +47,6 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kKeys = 64;          // keys of a tile, the unit of runs
 constexpr int kFewCols = 16;
 constexpr int kMaxTree = 64;       // tokens of a tree: bits of a mask
-constexpr int kLeastRun = 4;       // tiles of a workgroup's run at least
 constexpr float kHeadroom = 8.0f;  // a running maximum moves once a logit passes it by 2^8 (log2 units)
 
 struct Plan {
@@ -288,9 +287,9 @@ __device__ __forceinline__ int key_tiles(const Params& p, const Seq& s, int qt, 
 // workers [0, active) take equal runs.
 struct List {
   int total, active, share, more;   // the first `more` workers take share + 1
-  __device__ __forceinline__ void split(int tiles, int workers, int least) {
+  __device__ __forceinline__ void split(int tiles, int workers) {
     total = tiles;
-    active = min((total + least - 1) / least, workers);   // (a run of fewer is not worth its records)
+    active = min(total, workers);
     share = active == total ? 1 : static_cast<int>(static_cast<uint32_t>(total) / static_cast<uint32_t>(active));
     more = total - share * active;
   }
@@ -369,7 +368,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
   int before, inc;
   Seq seqs;
   List list;
-  list.split(unit_sums(p, kFewKeys, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.workers, 1);
+  list.split(unit_sums(p, kFewKeys, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.workers);
   if (w >= list.active) return;
   const int from = list.lo(w);
   // the sequence that holds the run's first tile
@@ -674,7 +673,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     int before, inc;
     Seq seqs;
     const int sum = unit_sums(p, kKeys, lane, 0, before, inc, seqs);
-    list.split(sum * p.c.hkv, p.plan.workers, kLeastRun);
+    list.split(sum * p.c.hkv, p.plan.workers);
     if (worker >= list.active) return;
     const int from = list.lo(worker);
     left = list.lo(worker + 1) - from;
@@ -1139,7 +1138,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
 }
 
 // ----------------------------------------------------------------- the plan --
-Plan plan_of(int B, int T, int n, int hkv, int G, int head_dim, int64_t cap_tokens, bool ragged) {
+Plan plan_of(int B, int T, int n, int hkv, int G, int head_dim, bool int8, int64_t cap_tokens, bool ragged) {
   Plan q{};
   const int64_t rows = static_cast<int64_t>(n) * G;
   const int cus = std::max(1, device_cus());
@@ -1148,7 +1147,12 @@ Plan plan_of(int B, int T, int n, int hkv, int G, int head_dim, int64_t cap_toke
     q.cols = static_cast<int>(rows);
     q.tpw = n;
     q.qtiles = 1;
-    q.workers = cap_tokens > kFewKeys ? 2 * kWaves * cus : 0;   // two workgroups a CU
+    // Workgroups a CU by the bytes of a row, which a tile's loads in flight go by (us with 1 / 2 / 3: 256 bytes,
+    // 64 x 8192 keys 195 / 201 / 208, 32768 38.7 / 40.8 / 47.5; 128 bytes, int8 3 x 131072 146 / 111 / 127,
+    // bf16 64 x 8192 122 / 107 / 112; 64 bytes, 64 x 8192 131 / 87 / 79)
+    const int row_bytes = int8 ? head_dim : 2 * head_dim;
+    const int groups = row_bytes == 256 ? 1 : row_bytes == 128 ? 2 : 3;
+    q.workers = cap_tokens > kFewKeys ? groups * kWaves * cus : 0;
     return q;
   }
   q.nct = rows <= 64 ? 1 : 2;
@@ -1228,7 +1232,8 @@ using namespace nkv;
 extern "C" int64_t nkv_paged_attend_workspace(int batch, int rows, int max_new, int num_heads, int num_kv_heads,
                                               int head_dim, int max_pages, int page_size, int ragged) {
   if (batch <= 0 || rows <= 0 || check_sizes("", batch, rows, max_new, num_heads, num_kv_heads, max_pages, page_size)) return 0;
-  const Plan q = plan_of(batch, rows, max_new, num_kv_heads, num_heads / num_kv_heads, head_dim,
+  // (an 8-bit cache has as many workers as one of bf16, or more)
+  const Plan q = plan_of(batch, rows, max_new, num_kv_heads, num_heads / num_kv_heads, head_dim, true,
                          static_cast<int64_t>(max_pages) * page_size, ragged != 0);
   return part_floats(q, batch, num_kv_heads, head_dim);
 }
@@ -1255,7 +1260,8 @@ extern "C" int nkv_paged_attend(void* k, void* v, float* k_scale, float* v_scale
   NKV_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 && q_stride % 8 == 0,
                 "%s: rows must lie on 16-byte boundaries", who);
   const int G = num_heads / num_kv_heads;
-  p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, head_dim, static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
+  p.plan = plan_of(batch, rows, max_new, num_kv_heads, G, head_dim, k_scale != nullptr,
+                   static_cast<int64_t>(max_pages) * page_size, starts != nullptr);
   NKV_CHECK_ARG(p.plan.qtiles <= 65535, "%s: at most 65535 query tiles of a sequence (max_new is %d)", who, max_new);
   NKV_CHECK_ARG(part_floats(p.plan, batch, num_kv_heads, head_dim) == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "%s: these sizes need a workspace on a 16-byte boundary", who);
