@@ -17,7 +17,9 @@
 // cut to its best.  The bar lies below the n-th largest of the lanes' maxima so
 // far, so few elements ever reach it.  Order:
 // value descending (NaN above all), index ascending.  Bound by reading the
-// logits once, or by the launches (one row).
+// logits once, or by the launches (one row).  Measured, rows of 151936: 2048 in bf16 with 5
+// alternatives 143 us (4.3 TB/s; 127 with none, 196 with 50: the vector instructions, 6 and an exp2 an
+// element, run beside the loads and are not all hidden); one row of fp32 with 20: 9.3 and 7.1 us.
 //
 // Exponents are in log2 units: 2^-z with z = M - x log2 e in one fused operation, M = m
 // log2 e rounded.  What M's rounding is off by, e, scales every term by 2^e alike, and adds
@@ -542,7 +544,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const Params p)
 }
 
 // Pieces of a row: rows alone fill the device from about 1024 workgroups on, and a
-// piece is at least one iteration of its four wavefronts.
+// piece is at least one iteration of its four wavefronts (us with 512 / 1024 / 2048 workgroups: 200 rows of
+// 151936 50 / 42 / -, 400 69 / 60.5 / -, 64 33 / 32.7 / 36.2, 300 rows of 32000 29.1 / 31.7 / 32.5).
 int splits_of(int rows, int vocab) {
   const int most = (vocab + 8 + kThreads * kEach - 1) / (kThreads * kEach);   // (8: up to the boundary before the row)
   return std::max(1, std::min({1024 / std::max(rows, 1), most, kMaxSplits}));
