@@ -137,7 +137,8 @@ class Attention(nn.Module):
             raise ValueError("dense attention needs the step's block_tables and context_lens (set_context)")
         ragged = c.cu_seqlens_q is not None
         return attend_paged(q, self.paged_cache, c.block_tables, lengths, starts=c.cu_seqlens_q,
-                            max_new=(c.max_seqlen_q or None) if ragged else None, tree=getattr(c, "tree_masks", None), scale=self.scale)
+                            max_new=(c.max_seqlen_q or None) if ragged else None,
+                            tree=getattr(c, "tree_masks", None), scale=self.scale)
 
 
 def attach_paged_cache(model: nn.Module, pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16,
@@ -187,4 +188,5 @@ def attach_m12_runtimes(model: nn.Module, cfg: M12Config, device=None) -> list[M
     return runtimes
 
 
-__all__ = ["Attention", "Context", "TreeContext", "attach_m12_runtimes", "attach_paged_cache", "get_context", "reset_context", "set_context"]
+__all__ = ["Attention", "Context", "TreeContext", "attach_m12_runtimes", "attach_paged_cache", "get_context",
+           "reset_context", "set_context"]
