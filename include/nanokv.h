@@ -757,9 +757,8 @@ int nkv_paged_move(void* k, void* v, float* k_scale, float* v_scale, int64_t pag
 int64_t nkv_paged_move_workspace(int num_kv_heads, int head_dim, int int8, int rows);
 
 /*
- * Attention of every sequence's new tokens over its keys in the cache (the
- * flash_attn_with_kvcache and block-table flash_attn_varlen_func calls of
- * nanovllm/layers/attention.py:100-119, and drafted trees).
+ * Attention of every sequence's new tokens over its keys in the cache (the dense
+ * calls over the block tables of nanovllm/layers/attention.py:100-119, and drafted trees).
  *
  * Sequence b: lengths[b] keys, the slots of tables[b table_stride ..] (page ids; page j
  * holds keys j page_size ..), its new tokens' among them as the last; its queries are rows
