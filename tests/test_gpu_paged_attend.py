@@ -383,3 +383,20 @@ def test_nan_keys_make_nan_outputs():
     for each in (1, 40):
         got = attend_paged(_q(2 * each, 4, 64, 11), cache, tables, lens)
         assert bool(got[:each].isnan().all()) and not bool(got[each:].isnan().any())
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("n", [3, 40])
+def test_trees_longer_than_their_sequences_or_than_max_new(kv, n):
+    """Sequences that hold fewer keys than their trees have tokens (the first ones lie before key 0), and
+    trees cut off at max_new: their rows behind it are 0."""
+    from nanokv_amd.paged import attend_paged, tree_masks
+    cache, tables, lens = _setup([n, n - 2, 0, 1, 70], 2, 16, 128, kv, seed=n)
+    masks = tree_masks(torch.stack([_random_tree(n, i) for i in range(5)]).cuda()).flatten()
+    q = _q(5 * n, 8, 128, n)
+    _check(attend_paged(q, cache, tables, lens, tree=masks), q, cache, tables, lens, tree=masks, n_each=n)
+    starts = torch.arange(0, 5 * n + 1, n, dtype=torch.int32, device="cuda")
+    got = attend_paged(q, cache, tables, lens, starts=starts, max_new=n - 1, tree=masks)
+    kept = torch.arange(5 * n, device="cuda") % n != n - 1
+    want = attend_paged(q, cache, tables, lens, starts=starts, max_new=n, tree=masks)
+    assert torch.equal(got[kept], want[kept]) and bool((got[~kept] == 0).all())

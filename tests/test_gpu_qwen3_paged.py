@@ -127,3 +127,15 @@ def test_log_probabilities_of_a_prompt():
         assert float((t.logprob.double() - ref).abs().max()) <= tol
         assert t.top_ids.shape == (199, 4) and bool((t.top_logprobs[:, :-1] >= t.top_logprobs[:, 1:]).all())
     assert torch.equal(model.token_logprobs(h, ids[1:], 4, rows=199).top_ids[:, 0], x.argmax(-1))
+
+
+def test_log_probabilities_of_a_prompt_of_one_token_are_refused_and_of_no_rows_are_none():
+    from nanokv_amd.sparse import M12Config
+    model = _model()
+    model.attach(M12Config(max_model_len=512, num_heads=8, num_kv_heads=2))
+    with pytest.raises(ValueError, match="at least 2 tokens"):          # (as prefill)
+        model.prefill_logprobs(torch.tensor([7], device="cuda"), top=3)
+    last, lp = model.prefill_logprobs(torch.tensor([7, 8], device="cuda"), top=3)
+    assert last.shape == (512,) and lp.logprob.shape == (1,) and lp.top_ids.shape == (1, 3)
+    lp = model.token_logprobs(torch.empty(0, 512, dtype=torch.bfloat16, device="cuda"), torch.empty(0, dtype=torch.long, device="cuda"))
+    assert lp.entropy.shape == (0,) and lp.top_logprobs.shape == (0, 0)
