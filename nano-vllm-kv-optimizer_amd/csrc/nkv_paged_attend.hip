@@ -30,9 +30,10 @@
 // kernel.  Query tiles that fill the device for several rounds are not cut: a workgroup each.
 //
 // Hidden keys get weight 0, which times an infinite or NaN value is NaN: a column whose
-// result holds a NaN is computed again key by key (redo_column), hidden keys left out.  Keys
-// past the length are never read (rows are clamped or bounds-checked), page ids outside the
-// cache hide their keys.
+// result holds a NaN is computed again key by key (redo_column), hidden keys left out; in
+// many_kernel only if a hidden key holds such a value (hidden_odd: in 8 bits none can), as the columns that see
+// one may be all of a prompt's.  Keys past the length are never read (rows are clamped or
+// bounds-checked), page ids outside the cache hide their keys.
 #include <algorithm>
 
 #include "nkv_paged.h"
@@ -167,6 +168,30 @@ __device__ __forceinline__ uint64_t seen_bits(uint64_t mask, bool tree, int limi
 __device__ __forceinline__ float where_bit(float x, uint32_t bits, int bit) {
   const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - bit)) >> 31);
   return __uint_as_float((__float_as_uint(x) & keep) | (0xff800000u & ~keep));
+}
+
+// Whether a key of [k0, k1) that row t's query does not see holds a value that is not finite.
+template <int D>
+__device__ bool hidden_odd(const Params& p, const Seq& s, const cint32* table, int h, int t, int k0, int k1, int lane) {
+  constexpr int N = D / 64;
+  const uint64_t mask = p.tree ? p.tree[s.begin + t] : 0;
+  const int end = min(k1, s.len);
+  for (int key0 = k0; key0 < end; key0 += 64) {
+    uint64_t hidden = ~seen_bits(mask, p.tree != nullptr, s.older + t, s, key0);
+    if (end - key0 < 64) hidden &= (1ull << (end - key0)) - 1;
+    for (; hidden != 0; hidden &= hidden - 1) {
+      const int key = key0 + __ffsll(static_cast<long long>(hidden)) - 1;
+      const int id = page_of(p, table, s, key);
+      if (id < 0) continue;   // (zeros were read)
+      const int slot = (id << p.c.shift) + (key & (p.c.page - 1));
+      const uint16_t* v = reinterpret_cast<const uint16_t*>(p.c.v) + paged_row(p.c, slot, h) + lane * N;
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < N; ++e) odd = odd || (v[e] & 0x7f80) == 0x7f80;
+      if (__any(odd)) return true;
+    }
+  }
+  return false;
 }
 
 // One column again, by one wavefront, key by key: m (log2 units), l and the sums of
@@ -1000,8 +1025,11 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
       for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd = odd || acc[i][ct][e] != acc[i][ct][e];
-      const uint64_t lanes = __ballot(odd && mine);
-      const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
+      const uint64_t lanes = __ballot(!INT8 && odd && mine);
+      uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
+      for (uint32_t todo = redo; todo != 0; todo &= todo - 1)
+        if (!hidden_odd<D>(late, s, (const cint32*)table, h, t0 + (c0 + __builtin_ctz(todo)) / late.G, lo * kKeys, hi * kKeys, lane))
+          redo &= ~(todo & -todo);
       auto orow = [&](int cc) {
         return late.out + (static_cast<int64_t>(s.begin + t0 + cc / late.G) * late.hq + h * late.G + cc % late.G) * D;
       };

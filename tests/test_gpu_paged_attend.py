@@ -400,3 +400,22 @@ def test_trees_longer_than_their_sequences_or_than_max_new(kv, n):
     kept = torch.arange(5 * n, device="cuda") % n != n - 1
     want = attend_paged(q, cache, tables, lens, starts=starts, max_new=n, tree=masks)
     assert torch.equal(got[kept], want[kept]) and bool((got[~kept] == 0).all())
+
+
+@pytest.mark.parametrize("n,older", [(1, 70), (5, 9000), (40, 70), (33, 9000)])
+def test_infinite_values_that_a_query_sees(n, older):
+    """A value of +inf in one dim: +inf there for the queries that see it, the others as without it."""
+    from nanokv_amd.paged import attend_paged
+    cache, tables, lens = _setup([older + n], 1, 16, 128, "bf16", seed=n)
+    q = _q(n, 4, 128, 5, scale=0.5)
+    at = older + n // 2
+    want = attend_paged(q, cache, tables, lens)
+    cache.v[int(tables[0, at // 16]), 0, at % 16, 7] = float("inf")
+    got = attend_paged(q, cache, tables, lens)
+    sees = torch.arange(n, device="cuda") >= n // 2
+    assert bool((got[sees, :, 7] == float("inf")).all())
+    got[sees, :, 7] = want[sees, :, 7]
+    # a column computed again has other roundings: each result is off by at most (1 + 2.02) 2^-8 of the largest
+    # value (the output's rounding and P's, the tolerance above), so two by twice that
+    top = float(cache.v.float().nan_to_num(0, 0, 0).abs().max())
+    assert float((got.float() - want.float()).abs().max()) <= 2 * 3.03 * 2.0 ** -8 * top
