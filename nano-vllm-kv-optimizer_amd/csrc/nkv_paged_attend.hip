@@ -17,8 +17,8 @@
 //     for all four wavefronts, the next one on its way; bound by the matrix cores for
 //     long prompts, by the keys for trees.  P is rounded to bf16 for the second product (2^-8
 //     of each weight, as the output's own rounding), in 16 bits numerator and denominator alike.
-//     Measured: 4096 tokens behind 12288 820 us (1.17 PFLOP/s; of 64 dims 528 and 0.91), at the chip's power
-//     limit; 7 prompts of up to 2000, 16 heads of 64 dims, 50 us (0.59: a CU may hold several of the longest tiles);
+//     Measured: 4096 tokens behind 12288 791-845 us by box (1.14-1.22 PFLOP/s; of 64 dims 528 and 0.91), at
+//     the chip's power limit; 7 prompts of up to 2000, 16 heads of 64 dims, 50 us (0.59: a CU may hold several of the longest tiles);
 //     5 trees of 26 over up to 16384 keys (243 MB) 60 + 9 us.
 // 8-bit caches: the codes are bf16 exactly; a key's scale multiplies its logits, a
 // value's its weights, both in fp32.
