@@ -91,13 +91,13 @@ __device__ __forceinline__ const Params& again() {
 // record 2 w + 1 of the first one and 2 w of each that follows.
 struct Note {
   int records, worker;   // records 1: the unit is whole
-  int row, cols;         // first row of out, columns
 };
+__host__ __device__ __forceinline__ int64_t note_floats(int64_t units) { return (2 * units + 3) & ~int64_t{3}; }
 __device__ __forceinline__ Note* note_of(const Params& p, int unit) { return reinterpret_cast<Note*>(p.part) + unit; }
 template <int D> constexpr int kPart = D + 4;
 template <int D>
 __device__ __forceinline__ float* record_of(const Params& p, int record, int c) {
-  return p.part + 4 * static_cast<int64_t>(p.B) * p.plan.qtiles * p.c.hkv +
+  return p.part + note_floats(static_cast<int64_t>(p.B) * p.plan.qtiles * p.c.hkv) +
          (static_cast<int64_t>(record) * p.plan.cols + c) * kPart<D>;
 }
 
@@ -404,8 +404,9 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
   // the sequence that holds the run's first tile
   int chunk = 0;
   uint64_t past = __ballot(inc * p.c.hkv > from);
-  while (past == 0) {   // (the list is longer than `from`)
-    unit_sums(p, kFewKeys, lane, ++chunk, before, inc, seqs);
+  while (past == 0) {   // (the list is longer than `from`, unless the lengths change under the call: it ends then, too)
+    if (++chunk * kWave >= p.B) return;
+    unit_sums(p, kFewKeys, lane, chunk, before, inc, seqs);
     past = __ballot((before + inc) * p.c.hkv > from);
   }
   const int at = __ffsll(static_cast<long long>(past)) - 1;
@@ -612,7 +613,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
       const Params& p = again();
       const bool whole = ntile == per_head;
       if (cut && tile0 == 0 && lane == 0)
-        *note_of(p, b * p.c.hkv + h) = Note{whole ? 1 : list.worker_of(from + done + per_head - 1) - w + 1, w, s.begin, count * p.G};
+        *note_of(p, b * p.c.hkv + h) = Note{whole ? 1 : list.worker_of(from + done + per_head - 1) - w + 1, w};
       done += ntile;
       bool odd = l != l;
 #pragma unroll
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
       wave_lds_sync();
     }
     first = 0;
-    if (left <= 0) break;
+    if (left <= 0 || b + 1 >= p.B) break;
     do s = seq_of(p, ++b); while (s.count == 0 && b + 1 < p.B);
   }
 }
@@ -711,8 +712,9 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     const int rest = from - h * sum;
     int chunk = 0;
     uint64_t past = __ballot(inc > rest);
-    while (past == 0) {   // (rest < sum)
-      unit_sums(p, kKeys, lane, ++chunk, before, inc, seqs);
+    while (past == 0) {   // (rest < sum; or as in few_kernel)
+      if (++chunk * kWave >= p.B * qtiles) return;
+      unit_sums(p, kKeys, lane, chunk, before, inc, seqs);
       past = __ballot(before + inc > rest);
     }
     const int at = __ffsll(static_cast<long long>(past)) - 1;
@@ -1013,7 +1015,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     const Params& late = again();
     if (SHARED && lo == 0 && threadIdx.x == 0)   // (one that is cut is the run's last)
       *note_of(late, (h * late.B + b) * qtiles + qt) =
-          Note{whole ? 1 : list.worker_of(list.lo(worker + 1) - hi + tiles - 1) - worker + 1, worker, s.begin + t0, (t_last + 1 - t0) * late.G};
+          Note{whole ? 1 : list.worker_of(list.lo(worker + 1) - hi + tiles - 1) - worker + 1, worker};
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct) {
       const int c0 = wave * 16 * NCT + ct * 16;
@@ -1069,7 +1071,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
       do {
         if (++b == late.B) {
           b = 0;
-          ++h;
+          if (++h == late.c.hkv) return;   // (as in few_kernel)
         }
       } while (seq_of(late, b).count == 0);   // (there is a unit: the run goes on)
     }
@@ -1097,8 +1099,12 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
   }
   const Note note = *note_of(p, unit);
   const Seq s = seq_of(p, u / p.plan.qtiles);
-  // (a unit without queries has no note)
-  if (u % p.plan.qtiles * p.plan.tpw >= min(s.count, p.n) || note.records == 1 || col >= note.cols) return;
+  const int t0 = u % p.plan.qtiles * p.plan.tpw;
+  // (a unit without queries has no note; one that points past the records was never written: the lengths
+  // have changed under the call)
+  if (col >= (min(s.count, min(t0 + p.plan.tpw, p.n)) - t0) * p.G || note.records <= 1 || note.worker < 0 ||
+      note.records > p.plan.workers - note.worker)
+    return;
   const int slot = lane / L, j = lane % L;
   float m = -INFINITY, l = 0.0f;
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1167,7 +1173,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Params p) {
   if (slot != 0) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const uint32_t t = static_cast<uint32_t>(col) / static_cast<uint32_t>(p.G);
-  uint16_t* dst = p.out + (static_cast<int64_t>(note.row + t) * p.hq + h * p.G + col - t * p.G) * D + 4 * j;
+  uint16_t* dst = p.out + (static_cast<int64_t>(s.begin + t0 + t) * p.hq + h * p.G + col - t * p.G) * D + 4 * j;
   *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
 }
 
@@ -1238,7 +1244,7 @@ void launch(const Params& p, hipStream_t s) {
 // Floats of the workspace: the notes and two records a worker.
 int64_t part_floats(const Plan& q, int B, int hkv, int head_dim) {
   if (q.workers == 0) return 0;
-  return 4 * static_cast<int64_t>(B) * q.qtiles * hkv + 2 * static_cast<int64_t>(q.workers) * q.cols * (head_dim + 4);
+  return note_floats(static_cast<int64_t>(B) * q.qtiles * hkv) + 2 * static_cast<int64_t>(q.workers) * q.cols * (head_dim + 4);
 }
 
 int check_sizes(const char* who, int batch, int rows, int max_new, int num_heads, int num_kv_heads, int max_pages,
