@@ -23,7 +23,9 @@
 //
 // Exponents are in log2 units: 2^-z with z = M - x log2 e in one fused operation, M = m
 // log2 e rounded.  What M's rounding is off by, e, scales every term by 2^e alike, and adds
-// to every z: both are mended in the sums (settle), not in the terms.
+// to every z: both are mended in the sums (settle), not in the terms.  e is up to half an ulp of M: 2^-8
+// for |m| < 2^16.  Larger maxima (runs that hold nothing but a mask's value) take m - x itself, since 2^e
+// leaves the range from |m| = 2^32 on.
 #include <algorithm>
 
 #include "nkv_common.h"
@@ -39,6 +41,7 @@ constexpr int kEach = 16;        // elements a lane takes per iteration
 constexpr int kMaxSplits = 128;  // pieces of a row
 constexpr int kMaxRows = (1 << 24) - 1;   // (a launch has fewer than 2^32 threads)
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kFar = 0x1p16f;  // maxima from here on are subtracted directly
 
 enum Kind { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) top = max_nan(top, v[u][e]);
-    if (__any(top > m) || !(fabsf(m) < 0x1p126f)) {   // (m log2 e may be infinite: never in M's form)
+    if (__any(top > m) || !(fabsf(m) < kFar)) {
       const float t = fmaxf(lane_top(top), m);
       settle();
       // the sums move to the new maximum; the old one becomes an element like others (lane 0 has it)
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const Params p) {
       m = t;
       big_m = m * kLog2e;
       off = __builtin_fmaf(m, kLog2e, -big_m);
-      if (!(fabsf(m) < 0x1p126f)) big_m = off = 0.0f;
+      if (!(fabsf(m) < kFar)) big_m = off = 0.0f;
       // one element that is the maximum stays out
       const uint64_t owners = moves ? __ballot(top == m) : 0;
       const float ref = m == -INFINITY ? 0.0f : m;
