@@ -84,13 +84,18 @@ def _cache_args(cache: PagedKV, who: str) -> tuple:
     return (k.data_ptr(), v.data_ptr(), None, None, *strides[:3], pages, hkv, page, d)
 
 
+def _to_i32(t: torch.Tensor) -> torch.Tensor:
+    """An int64 tensor as int32, what does not fit as the type's ends: they too lie outside every cache and table."""
+    return t.clamp(-2 ** 31, 2 ** 31 - 1).to(_I32)
+
+
 def _ints(t: torch.Tensor, dtype: torch.dtype, n: int | None, device: int, who: str, what: str) -> torch.Tensor:
     """t as a dense vector of dtype (converted from the other integer type)."""
     if t.dtype not in (_I32, _I64) or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.get_device() != device:
         raise ValueError(f"{who}: {what} must be int32 or int64 [{'n' if n is None else n}] on the cache's device "
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
     if t.dtype is not dtype:
-        t = t.to(dtype)
+        t = _to_i32(t) if dtype is _I32 else t.to(dtype)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -329,7 +334,7 @@ def _attend_formula(q, cache, tables, lengths, starts, max_new, tree, scale) -> 
     T, hq, _ = q.shape
     out = torch.zeros(T, hq, d)
     B = lengths.shape[0]
-    starts = [b * max_new for b in range(B + 1)] if starts is None else starts.tolist()
+    starts = [b * max_new for b in range(B + 1)] if starts is None else starts.clamp(0, T).tolist()
     for b in range(B):
         n = min(starts[b + 1] - starts[b], max_new)
         length = min(max(int(lengths[b]), 0), tables.shape[1] * page)
@@ -418,7 +423,7 @@ def attend_paged(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor, lengths:
     if B == 0:
         return out.zero_()
     if tables.dtype is not _I32:
-        tables = tables.to(_I32)
+        tables = _to_i32(tables)
     if tables.stride(1) != 1:
         tables = tables.contiguous()
     need = _workspace(device, B, T, max_new, hq, hkv, d, most, page, starts is not None)

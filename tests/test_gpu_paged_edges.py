@@ -1,0 +1,44 @@
+"""The paged operators on the GPU at the ends of their arguments: integers past 32 bits."""
+
+import pytest
+import torch
+
+from _paged_ref import make_cache
+from test_gpu_paged_attend import _check, _q, _setup
+
+pytestmark = pytest.mark.gpu
+FAR = [2 ** 32 + 5, -2 ** 63, 2 ** 63 - 1, 2 ** 32, 2 ** 31, -2 ** 32 + 7]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_slots_past_32_bits_lie_outside_the_cache(kv):
+    from nanokv_amd.paged import PagedKV, append_paged, move_paged, qkv_append_paged, read_paged
+    cache = make_cache(3, 2, 16, 64, kv, "cuda")
+    was = PagedKV(*(None if t is None else t.clone() for t in cache))
+    far, near = torch.tensor(FAR, device="cuda"), torch.arange(len(FAR), device="cuda")
+    rows = torch.ones(len(FAR), 2, 64, dtype=torch.bfloat16, device="cuda")
+    append_paged(cache, rows, rows, far)
+    qkv_append_paged(cache, torch.ones(len(FAR), 8 * 64, dtype=torch.bfloat16, device="cuda"), far, None, None, None, 4)
+    move_paged(cache, far, near)
+    move_paged(cache, near, far)
+    assert all(torch.equal(a, b) for a, b in zip(cache, was) if a is not None)
+    assert all(bool((t == 0).all()) for t in read_paged(cache, far))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("n", [1, 30])
+def test_lengths_tables_and_starts_past_32_bits(kv, n):
+    from nanokv_amd.paged import attend_paged
+    cache, tables, lens = _setup([160, 160], 2, 16, 64, kv, seed=1, poison=False)
+    tables = tables[:, :10].contiguous()
+    q = _q(2 * n, 8, 64, 2)
+    full = attend_paged(q, cache, tables, lens)
+    got = attend_paged(q, cache, tables, torch.tensor([2 ** 32 + 3, -2 ** 63 + 4], device="cuda"))
+    assert torch.equal(got[:n], full[:n]) and bool((got[n:] == 0).all())
+    far = tables.long()
+    far[0, 3], far[0, 5], far[1, 0], far[1, 9] = 2 ** 32, 2 ** 32 + 1, -2 ** 63, 2 ** 63 - 1
+    got = attend_paged(q, cache, far, lens)
+    _check(got, q, cache, far, lens, n_each=n)
+    starts = torch.tensor([0, n, 2 ** 32 + n], device="cuda")
+    assert torch.equal(attend_paged(q, cache, tables, lens, starts=starts, max_new=n),
+                       attend_paged(q, cache, tables, lens, starts=starts.clamp(max=2 * n), max_new=n))

@@ -1,0 +1,40 @@
+"""The paged operators' CPU forms at the ends of their integer arguments."""
+
+import torch
+
+from _paged_ref import attend_ref, make_cache
+from nanokv_amd.paged import PagedKV, append_paged, attend_paged, move_paged, read_paged
+
+FAR = [2 ** 32 + 5, -2 ** 63, 2 ** 63 - 1, 2 ** 32, 2 ** 31, -2 ** 32 + 7]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b) if x is not None)
+
+
+def test_slots_past_32_bits_lie_outside_the_cache():
+    for kv in ("bf16", "int8"):
+        cache = make_cache(3, 2, 16, 64, kv, "cpu")
+        was = PagedKV(*(None if t is None else t.clone() for t in cache))
+        rows = torch.ones(len(FAR), 2, 64)
+        append_paged(cache, rows, rows, torch.tensor(FAR))
+        move_paged(cache, torch.tensor(FAR), torch.arange(len(FAR)))
+        move_paged(cache, torch.arange(len(FAR)), torch.tensor(FAR))
+        assert _same(cache, was)
+        assert all(bool((t == 0).all()) for t in read_paged(cache, torch.tensor(FAR)))
+
+
+def test_lengths_tables_and_starts_past_32_bits():
+    cache = make_cache(5, 1, 16, 64, "bf16", "cpu")
+    q = torch.randn(4, 2, 64, generator=torch.Generator().manual_seed(0)).bfloat16()
+    tables = torch.tensor([[3, 1], [0, 2]])
+    full = attend_paged(q[:2], cache, tables, torch.tensor([32, 0]))
+    assert torch.equal(attend_paged(q[:2], cache, tables, torch.tensor([2 ** 32 + 3, -2 ** 63 + 4])), full)
+    far = torch.tensor([[3, 2 ** 32 + 1], [-2 ** 63, 2]])
+    ref, mag = attend_ref(q[:2], cache, far, torch.tensor([32, 32]))
+    got = attend_paged(q[:2], cache, far, torch.tensor([32, 32]))
+    assert bool(((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -10 * mag).all())
+    # starts past the rows are their end
+    want = attend_paged(q, cache, tables, torch.tensor([20, 9]), starts=torch.tensor([1, 3, 4]))
+    got = attend_paged(q, cache, tables, torch.tensor([20, 9]), starts=torch.tensor([1, 3, 2 ** 32 + 3]))
+    assert torch.equal(got, want)
