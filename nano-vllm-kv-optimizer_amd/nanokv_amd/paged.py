@@ -367,8 +367,8 @@ def attend_paged(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor, lengths:
 
     Sequence b has lengths[b] keys in the pages tables[b] (int32 [B, most pages]), its new
     tokens' (appended before) the last of them.  Its queries are rows starts[b] ..
-    starts[b + 1] - 1 (starts ascending [B + 1]), at most max_new of them (default T; a
-    closer bound launches less; rows behind it give 0); without starts every sequence has T / B.  A
+    starts[b + 1] - 1 (starts ascending [B + 1]), at most max_new of them (default T, of trees
+    at most 64; a closer bound launches less; rows behind it give 0); without starts every sequence has T / B.  A
     query sees the keys up to its own token's, or with ``tree`` (int64 masks [T], at most
     64 new tokens a sequence: ``tree_masks``) the keys before the new ones and those that its mask names.
     Rows that see nothing, or that belong to no sequence, are 0.  scale: of the
@@ -398,7 +398,9 @@ def attend_paged(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor, lengths:
         max_new = each
     else:
         starts = _ints(starts, _I32, B + 1, device, who, "starts")
-        max_new = T if max_new is None else min(int(max_new), T)
+        if max_new is None:
+            max_new = T if tree is None else MAX_TREE
+        max_new = min(int(max_new), T)
         if T and max_new < 1:
             raise ValueError(f"{who}: max_new must be positive (got {max_new})")
     if tree is not None:

@@ -1,5 +1,6 @@
 """The paged operators' CPU forms at the ends of their integer arguments."""
 
+import pytest
 import torch
 
 from _paged_ref import attend_ref, make_cache
@@ -38,3 +39,18 @@ def test_lengths_tables_and_starts_past_32_bits():
     want = attend_paged(q, cache, tables, torch.tensor([20, 9]), starts=torch.tensor([1, 3, 4]))
     got = attend_paged(q, cache, tables, torch.tensor([20, 9]), starts=torch.tensor([1, 3, 2 ** 32 + 3]))
     assert torch.equal(got, want)
+
+
+def test_trees_of_many_sequences_need_no_bound():
+    """More than 64 rows in all, at most 64 new tokens each: max_new may be left out."""
+    g = torch.Generator().manual_seed(3)
+    cache = make_cache(9, 1, 16, 64, "bf16", "cpu")
+    tables = torch.tensor([[3, 0, 5, 1, 8], [7, 6, 2, 4, 8]])
+    lengths, starts = torch.tensor([75, 70]), torch.tensor([0, 64, 104])
+    q = torch.randn(104, 2, 64, generator=g).bfloat16()
+    masks = torch.randint(-2 ** 62, 2 ** 62, (104,), generator=g)
+    got = attend_paged(q, cache, tables, lengths, starts=starts, tree=masks)
+    assert torch.equal(got, attend_paged(q, cache, tables, lengths, starts=starts, max_new=64, tree=masks))
+    assert not bool((got == 0).all(-1).any())
+    with pytest.raises(ValueError, match="at most 64 tokens"):
+        attend_paged(q, cache, tables, lengths, starts=starts, max_new=65, tree=masks)
