@@ -369,8 +369,8 @@ def attend_paged(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor, lengths:
     tokens' (appended before) the last of them.  Its queries are rows starts[b] ..
     starts[b + 1] - 1 (starts ascending [B + 1]), at most max_new of them (default T, of trees
     at most 64; a closer bound launches less; rows behind it give 0); without starts every sequence has T / B.  A
-    query sees the keys up to its own token's, or with ``tree`` (int64 masks [T], at most
-    64 new tokens a sequence: ``tree_masks``) the keys before the new ones and those that its mask names.
+    query sees the keys up to its own token's, or with ``tree`` (int64 masks [T], or
+    int32 ones of 32 tokens; at most 64 new tokens a sequence: ``tree_masks``) the keys before the new ones and those that its mask names.
     Rows that see nothing, or that belong to no sequence, are 0.  scale: of the
     logits (default D^-0.5)."""
     who = "attend_paged"
@@ -404,6 +404,8 @@ def attend_paged(q: torch.Tensor, cache: PagedKV, tables: torch.Tensor, lengths:
         if T and max_new < 1:
             raise ValueError(f"{who}: max_new must be positive (got {max_new})")
     if tree is not None:
+        if tree.dtype is _I32:
+            tree = tree.to(_I64) & 0xffffffff   # (bit 31 is a token's, not a sign)
         tree = _ints(tree, _I64, T, device, who, "tree")
         if max_new > MAX_TREE:
             raise ValueError(f"{who}: a tree has at most {MAX_TREE} tokens (max_new is {max_new})")

@@ -54,3 +54,14 @@ def test_trees_of_many_sequences_need_no_bound():
     assert not bool((got == 0).all(-1).any())
     with pytest.raises(ValueError, match="at most 64 tokens"):
         attend_paged(q, cache, tables, lengths, starts=starts, max_new=65, tree=masks)
+
+
+def test_masks_of_32_bits_name_no_further_tokens():
+    """int32 masks: bit 31 is token 31's, not that of all tokens behind it."""
+    g = torch.Generator().manual_seed(4)
+    cache = make_cache(4, 1, 16, 64, "bf16", "cpu")
+    q = torch.randn(40, 2, 64, generator=g).bfloat16()
+    masks = torch.randint(-2 ** 31, 2 ** 31, (40,), generator=g).int()
+    tables, lengths = torch.tensor([[3, 1, 2, 0]]), torch.tensor([50])
+    assert torch.equal(attend_paged(q, cache, tables, lengths, tree=masks),
+                       attend_paged(q, cache, tables, lengths, tree=masks.long() & 0xffffffff))
