@@ -331,25 +331,56 @@ struct List {
   }
 };
 // The tiles of all units of one KV head, `keys` keys each.  Unit u is query tile u % qtiles of
-// sequence u / qtiles; of the 64 units from u0 = 64 * chunk, `before` is the sum over
-// those in front of u0, `inc` the inclusive sum and `mine` the sequence of the lane's.
-__device__ __forceinline__ int unit_sums(const Params& p, int keys, int lane, int chunk, int& before, int& inc, Seq& mine) {
-  int all = 0;
-  const int units = p.B * p.plan.qtiles;
-  for (int c = 0; c * kWave < units; ++c) {
-    const int u = min(c * kWave + lane, units - 1);
+// sequence u / qtiles; a wavefront sums chunks of 64 units, a lane each, and goes over them once: lane
+// i keeps the sum up to the end of block i (a 64th of the chunks, or one), which leaves few chunks to look
+// through again for a tile's unit, however many sequences there are (a token each of 1024 / 4096 / 16384
+// sequences of up to 300, 300 and 64 keys: 172 / 615 / 969 us; all chunks again for each chunk
+// passed: 234 / 1629 / 18111).
+struct Units {
+  int chunks, per;      // chunks in all, of a block
+  int ends;             // lane i: tiles up to the end of block i
+  int before, inc;      // tiles before the chunk looked at, the inclusive sums of its units
+  Seq mine;             // the lane's sequence there
+
+  __device__ __forceinline__ void look(const Params& p, int keys, int lane, int c) {
+    const int units = p.B * p.plan.qtiles, at = c * kWave + lane, u = min(at, units - 1);
     const int b = p.plan.qtiles == 1 ? u : static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(p.plan.qtiles));
-    const Seq s = lane_seq(p, b);
-    const int sum = lane_sums(c * kWave + lane < units ? key_tiles(p, s, u - b * p.plan.qtiles, keys) : 0);
-    if (c == chunk) {
-      before = all;
-      inc = sum;
-      mine = s;
-    }
-    all += __builtin_amdgcn_readlane(sum, kWave - 1);
+    mine = lane_seq(p, b);
+    inc = lane_sums(at < units ? key_tiles(p, mine, u - b * p.plan.qtiles, keys) : 0);
   }
-  return all;
-}
+  // All tiles.
+  __device__ __forceinline__ int sum(const Params& p, int keys, int lane) {
+    chunks = (p.B * p.plan.qtiles + kWave - 1) / kWave;
+    per = (chunks + kWave - 1) / kWave;
+    before = ends = 0;
+    int all = 0;
+    for (int c = 0, block = 0, left = per; c < chunks; ++c) {
+      look(p, keys, lane, c);
+      all += __builtin_amdgcn_readlane(inc, kWave - 1);
+      ends = lane >= block ? all : ends;   // (those past the last block have all)
+      if (--left == 0) {
+        left = per;
+        ++block;
+      }
+    }
+    return all;
+  }
+  // The unit that holds tile x of the list in which every tile counts `each` times; -1: none (the lengths
+  // have changed under the call).  `before` and `inc` are those of its chunk.
+  __device__ __forceinline__ int find(const Params& p, int keys, int lane, int each, int x) {
+    const uint64_t blocks = __ballot(ends * each > x);
+    if (blocks == 0) return -1;
+    const int block = __ffsll(static_cast<long long>(blocks)) - 1;
+    before = block > 0 ? __builtin_amdgcn_readlane(ends, block - 1) : 0;
+    for (int c = block * per; c < min((block + 1) * per, chunks); ++c) {
+      if (chunks > 1) look(p, keys, lane, c);   // (one: as it was summed)
+      const uint64_t past = __ballot((before + inc) * each > x);
+      if (past != 0) return c * kWave + __ffsll(static_cast<long long>(past)) - 1;
+      before += __builtin_amdgcn_readlane(inc, kWave - 1);
+    }
+    return -1;
+  }
+};
 
 // Zeros for the rows of no sequence and those behind a sequence's max_new-th, by one workgroup.
 __device__ __forceinline__ void clear_rest(const Params& p, int wave, int lane, int d) {
@@ -395,27 +426,20 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
   const bool cut = p.part != nullptr;
   // wavefront w: the first ones of all workgroups, then the second ones (few tiles lie on all CUs)
   const int w = blockIdx.x + groups * wave;
-  int before, inc;
-  Seq seqs;
+  Units units;
   List list;
-  list.split(unit_sums(p, kFewKeys, lane, 0, before, inc, seqs) * p.c.hkv, p.plan.workers);
+  list.split(units.sum(p, kFewKeys, lane) * p.c.hkv, p.plan.workers);
   if (w >= list.active) return;
   const int from = list.lo(w);
   // the sequence that holds the run's first tile
-  int chunk = 0;
-  uint64_t past = __ballot(inc * p.c.hkv > from);
-  while (past == 0) {   // (the list is longer than `from`, unless the lengths change under the call: it ends then, too)
-    if (++chunk * kWave >= p.B) return;
-    unit_sums(p, kFewKeys, lane, chunk, before, inc, seqs);
-    past = __ballot((before + inc) * p.c.hkv > from);
-  }
-  const int at = __ffsll(static_cast<long long>(past)) - 1;
-  int b = chunk * kWave + at;
-  before += at > 0 ? __builtin_amdgcn_readlane(inc, at - 1) : 0;
+  int b = units.find(p, kFewKeys, lane, p.c.hkv, from);
+  if (b < 0) return;
+  const int at = b % kWave;
+  const int before = units.before + (at > 0 ? __builtin_amdgcn_readlane(units.inc, at - 1) : 0);
   Seq s;
-  s.begin = __builtin_amdgcn_readlane(seqs.begin, at);
-  s.count = __builtin_amdgcn_readlane(seqs.count, at);
-  s.len = __builtin_amdgcn_readlane(seqs.len, at);
+  s.begin = __builtin_amdgcn_readlane(units.mine.begin, at);
+  s.count = __builtin_amdgcn_readlane(units.mine.count, at);
+  s.len = __builtin_amdgcn_readlane(units.mine.len, at);
   s.older = s.len - s.count;
   char* buf = lds + wave * kBuf;
   // transposing read: keys 4 lg .. + 3 (+ 16 g) of dims 16 dt + ln
@@ -701,25 +725,18 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     // runs that follow one another on one XCD (workgroups go round them): units of a head share its keys in that L2
     const int per = p.plan.workers / 8;
     worker = p.plan.workers % 8 == 0 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
-    int before, inc;
-    Seq seqs;
-    const int sum = unit_sums(p, kKeys, lane, 0, before, inc, seqs);
+    Units units;
+    const int sum = units.sum(p, kKeys, lane);
     list.split(sum * p.c.hkv, p.plan.workers);
     if (worker >= list.active) return;
     const int from = list.lo(worker);
     left = list.lo(worker + 1) - from;
     h = static_cast<int>(static_cast<uint32_t>(from) / static_cast<uint32_t>(sum));
     const int rest = from - h * sum;
-    int chunk = 0;
-    uint64_t past = __ballot(inc > rest);
-    while (past == 0) {   // (rest < sum; or as in few_kernel)
-      if (++chunk * kWave >= p.B * qtiles) return;
-      unit_sums(p, kKeys, lane, chunk, before, inc, seqs);
-      past = __ballot(before + inc > rest);
-    }
-    const int at = __ffsll(static_cast<long long>(past)) - 1;
-    const int unit = chunk * kWave + at;
-    tile0 = rest - before - (at > 0 ? __builtin_amdgcn_readlane(inc, at - 1) : 0);
+    const int unit = units.find(p, kKeys, lane, 1, rest);
+    if (unit < 0) return;
+    const int at = unit % kWave;
+    tile0 = rest - units.before - (at > 0 ? __builtin_amdgcn_readlane(units.inc, at - 1) : 0);
     b = unit / qtiles;
     qt = unit - b * qtiles;
   }

@@ -1,4 +1,4 @@
-"""The paged operators on the GPU at the ends of their arguments: integers past 32 bits."""
+"""The paged operators on the GPU at the ends of their arguments: integers past 32 bits, thousands of sequences."""
 
 import pytest
 import torch
@@ -42,3 +42,33 @@ def test_lengths_tables_and_starts_past_32_bits(kv, n):
     starts = torch.tensor([0, n, 2 ** 32 + n], device="cuda")
     assert torch.equal(attend_paged(q, cache, tables, lens, starts=starts, max_new=n),
                        attend_paged(q, cache, tables, lens, starts=starts.clamp(max=2 * n), max_new=n))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_thousands_of_sequences(kv):
+    """A token of each of 4500 sequences (their chunks of 64 fall into blocks of two), a few of them long, many
+    empty; then without a new token for most."""
+    from nanokv_amd.paged import attend_paged
+    B = 4500
+    lengths = [(37 * b) % 40 if b % 3 else 0 for b in range(B)]
+    lengths[70], lengths[2500], lengths[-1] = 3000, 1500, 700
+    cache, tables, lens = _setup(lengths, 1, 16, 64, kv, seed=8, poison=False)
+    q = _q(B, 2, 64, 1)
+    _check(attend_paged(q, cache, tables, lens), q, cache, tables, lens)
+    counts = [1 if b % 50 == 7 or b > B - 9 else 0 for b in range(B)]
+    starts = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    n = int(starts[-1])
+    got = attend_paged(q[:n], cache, tables, lens, starts=starts, max_new=1)
+    _check(got, q[:n], cache, tables, lens, starts)
+
+
+@pytest.mark.parametrize("kv,hkv,d", [("bf16", 1, 128), ("int8", 1, 64)])
+def test_a_shared_list_of_many_query_tiles(kv, hkv, d):
+    """450 sequences of up to 20 new tokens whose tables are wide: one list of key tiles, several chunks of units."""
+    from nanokv_amd.paged import attend_paged
+    lengths = [20 + (53 * b) % 60 for b in range(450)]
+    lengths[200], lengths[449] = 2600, 900
+    cache, tables, lens = _setup(lengths, hkv, 16, d, kv, seed=9, poison=False)
+    tables = torch.nn.functional.pad(tables, (0, 2048 - tables.shape[1]), value=-1)
+    q = _q(9000, 2 * hkv, d, 2)
+    _check(attend_paged(q, cache, tables, lens), q, cache, tables, lens, n_each=20)
