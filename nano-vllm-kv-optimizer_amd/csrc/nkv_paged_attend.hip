@@ -265,23 +265,6 @@ __device__ __forceinline__ void store_column(const Params& p, bool whole, uint16
   }
 }
 
-// Rows of q that belong to no sequence, or lie behind a sequence's max_new-th: zeros for head group h.
-__device__ __forceinline__ void clear_rows(const Params& p, int h, int from, int to, int d) {
-  const int per = p.G * d / 8;
-  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(to - from) * per; i += kThreads) {
-    const int64_t row = from + i / per;
-    reinterpret_cast<uint4*>(p.out + (row * p.hq + h * p.G) * d)[i % per] = make_uint4(0u, 0u, 0u, 0u);
-  }
-}
-__device__ __forceinline__ void clear_others(const Params& p, const Seq& s, int b, int h, int d) {
-  if (!p.starts) return;
-  if (s.count > p.n) clear_rows(p, h, s.begin + p.n, s.begin + s.count, d);
-  if (b == 0) {
-    clear_rows(p, h, 0, s.begin, d);
-    clear_rows(p, h, min(max(((const cint32*)p.starts)[p.B], 0), p.T), p.T, d);
-  }
-}
-
 __device__ __forceinline__ bf16x8 as_bf16(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
 // ---------------------------------------------------------------- few columns --
@@ -382,24 +365,30 @@ struct Units {
   }
 };
 
-// Zeros for the rows of no sequence and those behind a sequence's max_new-th, by one workgroup.
-__device__ __forceinline__ void clear_rest(const Params& p, int wave, int lane, int d) {
-  auto clear = [&](int from, int to) {
-    const int64_t per = p.hq * d / 8;
-    for (int64_t i = lane; i < (to - from) * per; i += kWave)
-      reinterpret_cast<uint4*>(p.out + from * per * 8)[i] = make_uint4(0u, 0u, 0u, 0u);
-  };
-  if (wave == 0) clear(0, min(max(p.starts[0], 0), p.T));
-  if (wave == 1) clear(min(max(p.starts[p.B], 0), p.T), p.T);
-  for (int b0 = wave * kWave; b0 < p.B; b0 += kThreads) {
-    const int b = min(b0 + lane, p.B - 1);
-    const int begin = min(max(p.starts[b], 0), p.T);
-    const int end = min(max(p.starts[b + 1], begin), p.T);
-    for (uint64_t more = __ballot(b0 + lane < p.B && end - begin > p.n); more != 0; more &= more - 1) {
-      const int at = __ffsll(static_cast<long long>(more)) - 1;
-      clear(__shfl(begin, at) + p.n, __shfl(end, at));
+// Zeros for the rows of no sequence and those behind a sequence's max_new-th: by `waves` wavefronts,
+// 16 rows at a time (4096 rows of 32 heads of 128 dims, all but one of padding, one over 2048 keys: 17 us; with
+// all rows by one workgroup 830).
+constexpr int kClearRows = 16;
+__device__ __forceinline__ void clear_rest(const Params& p, int64_t wave, int64_t waves, int lane, int d) {
+  const int64_t per = p.hq * d / 8;   // 16-byte pieces of a row
+  for (int64_t r0 = wave * kClearRows; r0 < p.T; r0 += waves * kClearRows) {
+    const int row = static_cast<int>(min(r0 + lane % kClearRows, static_cast<int64_t>(p.T) - 1));
+    int b = -1, end = p.B + 1;        // the last sequence that starts at the row or before it (p.B: none)
+    while (end - b > 1) {
+      const int mid = (b + end) / 2;
+      if (p.starts[mid] <= row) b = mid; else end = mid;
+    }
+    const bool none = b < 0 || b == p.B || row - max(p.starts[b], 0) >= p.n;
+    uint32_t rows = static_cast<uint32_t>(__ballot(none && lane < kClearRows && r0 + lane < p.T));
+    for (; rows != 0; rows &= rows - 1) {
+      uint4* dst = reinterpret_cast<uint4*>(p.out) + (r0 + __builtin_ctz(rows)) * per;
+      for (int64_t i = lane; i < per; i += kWave) dst[i] = make_uint4(0u, 0u, 0u, 0u);
     }
   }
+}
+// Workgroups beside those that attend.
+int clear_groups(const Params& p) {
+  return p.starts ? std::min((p.T + kWaves * kClearRows - 1) / (kWaves * kClearRows), 256) : 0;
 }
 
 template <int D, bool INT8>
@@ -419,8 +408,8 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
   const int lane = threadIdx.x & 63;
   const int ln = lane & 15, lg = lane >> 4;
   const int groups = p.plan.workers / kWaves;
-  if (static_cast<int>(blockIdx.x) == groups) {   // (there is one more with starts)
-    clear_rest(p, wave, lane, D);
+  if (static_cast<int>(blockIdx.x) >= groups) {   // (there are more with starts)
+    clear_rest(p, (blockIdx.x - groups) * kWaves + wave, (gridDim.x - groups) * kWaves, lane, D);
     return;
   }
   const bool cut = p.part != nullptr;
@@ -717,9 +706,13 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     h = blockIdx.x;
     b = blockIdx.z;
     qt = qtiles - 1 - static_cast<int>(blockIdx.y);   // the longest first
+    if (p.starts) {   // (the shortest units' workgroups come first here)
+      const int64_t at = (static_cast<int64_t>(qt) * p.B + b) * p.c.hkv + h, all = static_cast<int64_t>(qtiles) * p.B * p.c.hkv;
+      clear_rest(p, at * kWaves + wave, all * kWaves, lane, D);
+    }
   } else {
-    if (static_cast<int>(blockIdx.x) == p.plan.workers) {   // (there is one more with starts)
-      clear_rest(p, wave, lane, D);
+    if (static_cast<int>(blockIdx.x) >= p.plan.workers) {   // (there are more with starts)
+      clear_rest(p, (blockIdx.x - p.plan.workers) * kWaves + wave, (gridDim.x - p.plan.workers) * kWaves, lane, D);
       return;
     }
     // runs that follow one another on one XCD (workgroups go round them): units of a head share its keys in that L2
@@ -753,7 +746,6 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
   for (;;) {
     const Params& p = SHARED ? again() : args;
     const Seq s = seq_of(p, b);
-    if (!SHARED && qt == 0) clear_others(p, s, b, h, D);
     const int t0 = qt * tpw;
     const int tiles = key_tiles(p, s, qt, kKeys);
     if (!SHARED && tiles == 0) return;   // (the list has units with queries only)
@@ -1232,7 +1224,7 @@ template <int D, bool I8, int NCT>
 void launch_many(const Params& p, hipStream_t s) {
   const Plan& q = p.plan;
   if (q.workers > 0)
-    many_kernel<D, I8, NCT, true><<<q.workers + (p.starts ? 1 : 0), kThreads, 0, s>>>(p);
+    many_kernel<D, I8, NCT, true><<<q.workers + clear_groups(p), kThreads, 0, s>>>(p);
   else
     many_kernel<D, I8, NCT, false><<<dim3(p.c.hkv, q.qtiles, p.B), kThreads, 0, s>>>(p);
 }
@@ -1246,7 +1238,7 @@ void launch(const Params& p, hipStream_t s) {
     if (q.workers == 0) f.part = nullptr;
     if (q.workers == 0)
       f.plan.workers = kWaves * static_cast<int>(std::min<int64_t>((static_cast<int64_t>(p.B) * p.c.hkv + kWaves - 1) / kWaves, 4096));
-    few_kernel<D, I8><<<f.plan.workers / kWaves + (p.starts ? 1 : 0), kThreads, 0, s>>>(f);
+    few_kernel<D, I8><<<f.plan.workers / kWaves + clear_groups(p), kThreads, 0, s>>>(f);
   } else {
     q.nct == 1 ? launch_many<D, I8, 1>(p, s) : launch_many<D, I8, 2>(p, s);
   }

@@ -1,4 +1,5 @@
-"""The paged operators on the GPU at the ends of their arguments: integers past 32 bits, thousands of sequences."""
+"""The paged operators on the GPU at the ends of their arguments: integers past 32 bits, thousands of sequences
+and of rows of padding."""
 
 import pytest
 import torch
@@ -72,3 +73,32 @@ def test_a_shared_list_of_many_query_tiles(kv, hkv, d):
     tables = torch.nn.functional.pad(tables, (0, 2048 - tables.shape[1]), value=-1)
     q = _q(9000, 2 * hkv, d, 2)
     _check(attend_paged(q, cache, tables, lens), q, cache, tables, lens, n_each=20)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("n,wide", [(1, 1), (3, 1), (30, 1), (30, 4096), (300, 1)])
+def test_rows_of_padding(kv, n, wide):
+    """Thousands of rows of no sequence before, behind and (past max_new) between the others: all 0, whatever
+    the memory held, and the others as without them."""
+    from nanokv_amd.paged import attend_paged
+    cache, tables, lens = _setup([n + 70, n, n + 5, 2 * n], 2, 16, 64, kv, seed=n, poison=False)
+    tables = torch.nn.functional.pad(tables, (0, wide), value=-1)
+    rows = [(3001, n), (3001 + n, 0), (3001 + n, 1500), (4501 + n, 1)]       # first row, rows of each sequence
+    starts = torch.tensor([r for r, _ in rows] + [4502 + n], dtype=torch.int32, device="cuda")
+    T = 4502 + n + 2017
+    q = _q(T, 8, 64, 3)
+    junk = torch.full((4, T, 8, 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+    del junk                                                                # (the output may take its memory)
+    got = attend_paged(q, cache, tables, lens, starts=starts, max_new=n)
+    live = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for first, count in rows:
+        live[first:first + min(count, n)] = True
+    assert bool((got[~live] == 0).all())
+    some = [0, 3]                                                           # sequences whose rows are all there
+    for b in some:
+        first, count = rows[b]
+        one = torch.tensor([0, count], dtype=torch.int32, device="cuda")
+        alone = attend_paged(q[first:first + count].contiguous(), cache, tables[b:b + 1], lens[b:b + 1], starts=one,
+                             max_new=n)
+        tol = 2 * 3.03 * 2.0 ** -8 * float(cache.v.float().abs().max()) * (1.0 if kv == "bf16" else 0.025)
+        assert float((got[first:first + count].float() - alone.float()).abs().max()) <= tol
