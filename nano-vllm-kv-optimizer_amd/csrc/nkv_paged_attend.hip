@@ -29,12 +29,13 @@
 // A unit that several workers share is joined from their partial sums by a second
 // kernel.  Query tiles that fill the device for several rounds are not cut: a workgroup each.
 //
-// Hidden keys get weight 0, which times an infinite or NaN value is NaN: a column whose
-// result holds a NaN is computed again key by key (redo_column), hidden keys left out; in
-// many_kernel only if a hidden key holds such a value (hidden_odd: in 8 bits none can), as the columns that see
-// one may be all of a prompt's.  Keys past the length are never read (rows are clamped or
-// bounds-checked), page ids outside the cache hide their keys.
+// Hidden keys get weight 0, which times an infinite or NaN value is NaN: such rows of V are zeros in LDS and
+// are added to the columns that see them one by one from the cache, when a run is done a second time because it
+// gave NaN (4096 tokens behind 12288, one of them NaN: 1040 us; 4 x 16384 keys 100, without 63).  In 8 bits the
+// codes are finite, and the weight 0 of a scale stays 0.  Keys past the length are never read (rows are
+// clamped or bounds-checked), page ids outside the cache hide their keys.
 #include <algorithm>
+#include <type_traits>
 
 #include "nkv_paged.h"
 #include "nkv_stage.h"
@@ -170,98 +171,32 @@ __device__ __forceinline__ float where_bit(float x, uint32_t bits, int bit) {
   return __uint_as_float((__float_as_uint(x) & keep) | (0xff800000u & ~keep));
 }
 
-// Whether a key of [k0, k1) that row t's query does not see holds a value that is not finite.
-template <int D>
-__device__ bool hidden_odd(const Params& p, const Seq& s, const cint32* table, int h, int t, int k0, int k1, int lane) {
-  constexpr int N = D / 64;
-  const uint64_t mask = p.tree ? p.tree[s.begin + t] : 0;
-  const int end = min(k1, s.len);
-  for (int key0 = k0; key0 < end; key0 += 64) {
-    uint64_t hidden = ~seen_bits(mask, p.tree != nullptr, s.older + t, s, key0);
-    if (end - key0 < 64) hidden &= (1ull << (end - key0)) - 1;
-    for (; hidden != 0; hidden &= hidden - 1) {
-      const int key = key0 + __ffsll(static_cast<long long>(hidden)) - 1;
-      const int id = page_of(p, table, s, key);
-      if (id < 0) continue;   // (zeros were read)
-      const int slot = (id << p.c.shift) + (key & (p.c.page - 1));
-      const uint16_t* v = reinterpret_cast<const uint16_t*>(p.c.v) + paged_row(p.c, slot, h) + lane * N;
-      bool odd = false;
+// Whether one of 8 bf16 values is infinite or NaN.
+__device__ __forceinline__ bool not_finite(u32x4 v) {
+  bool odd = false;
 #pragma unroll
-      for (int e = 0; e < N; ++e) odd = odd || (v[e] & 0x7f80) == 0x7f80;
-      if (__any(odd)) return true;
-    }
-  }
-  return false;
+  for (int i = 0; i < 4; ++i) odd = odd || (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+  return odd;
 }
-
-// One column again, by one wavefront, key by key: m (log2 units), l and the sums of
-// the lane's D / 64 dims over the visible keys of [k0, k1).
-template <int D, bool INT8>
-__device__ void redo_column(const Params& p, const Seq& s, const cint32* table, int h, int t, int head, int k0, int k1,
-                            int lane, float& m, float& l, float (&o)[D / 64]) {
-  constexpr int N = D / 64;
-  const uint16_t* qrow = p.q + static_cast<int64_t>(s.begin + t) * p.q_ls + head * D;
-  float q[N];
+// The bits of rows (L lanes each) that have a lane in `lanes`.
+template <int L>
+__device__ __forceinline__ uint32_t rows_of(uint64_t lanes) {
+  uint32_t rows = 0;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    q[e] = bf16_to_f32(qrow[lane * N + e]);
-    o[e] = 0.0f;
-  }
-  const uint64_t mask = p.tree ? p.tree[s.begin + t] : 0;
-  m = -INFINITY;
-  l = 0.0f;
-  for (int key = k0; key < min(k1, s.len); ++key) {
-    if (!(seen_bits(mask, p.tree != nullptr, s.older + t, s, key) & 1)) continue;
-    const int id = page_of(p, table, s, key);
-    if (id < 0) continue;
-    const int slot = (id << p.c.shift) + (key & (p.c.page - 1));
-    const int64_t row = paged_row(p.c, slot, h) + lane * N;
-    float k[N], v[N], vs = 1.0f, dot = 0.0f, ks = 1.0f;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if (INT8) {
-        k[e] = static_cast<float>(reinterpret_cast<const int8_t*>(p.c.k)[row + e]);
-        v[e] = static_cast<float>(reinterpret_cast<const int8_t*>(p.c.v)[row + e]);
-      } else {
-        k[e] = bf16_to_f32(reinterpret_cast<const uint16_t*>(p.c.k)[row + e]);
-        v[e] = bf16_to_f32(reinterpret_cast<const uint16_t*>(p.c.v)[row + e]);
-      }
-      dot += q[e] * k[e];
-    }
-    if (INT8) {
-      const int64_t at = paged_scale(p.c, slot, h);
-      ks = p.c.ks[at];
-      vs = p.c.vs[at];
-    }
-#pragma unroll
-    for (int x = kWave / 2; x > 0; x >>= 1) dot += __shfl_xor(dot, x);
-    const float y = dot * ks * p.scale_log2;
-    const float mn = fmaxf(m, y);
-    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float w = y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y - mn);   // (NaN stays)
-    m = mn;
-    l = l * alpha + w;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = o[e] * alpha + w * (v[e] * vs);
-    if (l != l) break;   // (NaN, whatever follows)
-  }
+  for (int r = 0; r < kWave / L; ++r) rows |= ((lanes >> (r * L)) & ((1ull << L) - 1)) != 0 ? 1u << r : 0u;
+  return rows;
 }
-
-// A column's result, by the lanes of a wavefront that hold D / 64 dims each.
-template <int D>
-__device__ __forceinline__ void store_column(const Params& p, bool whole, uint16_t* orow, float* rec, int lane, float m,
-                                             float l, const float (&o)[D / 64]) {
-  constexpr int N = D / 64;
+// acc += w V for a row of V as it lies in the cache; acc[i][e] is dim 16 i + 4 lg + e.
+template <int DT, typename F>
+__device__ __forceinline__ void add_row(const char* row, int lg, float w, F&& acc) {
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    if (whole)
-      orow[lane * N + e] = f32_to_bf16(l == 0.0f ? 0.0f : o[e] / l);
-    else
-      rec[4 + lane * N + e] = o[e];
-  }
-  if (!whole && lane == 0) {
-    rec[0] = m;
-    rec[1] = l;
+  for (int i = 0; i < DT; ++i) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(row + 32 * i + 8 * lg);
+    f32x4& a = acc(i);
+    a[0] += w * bf16_lo(v[0]);
+    a[1] += w * bf16_hi(v[0]);
+    a[2] += w * bf16_lo(v[1]);
+    a[3] += w * bf16_hi(v[1]);
   }
 }
 
@@ -366,8 +301,8 @@ struct Units {
 };
 
 // Zeros for the rows of no sequence and those behind a sequence's max_new-th: by `waves` wavefronts,
-// 16 rows at a time (4096 rows of 32 heads of 128 dims, all but one of padding, one over 2048 keys: 17 us; with
-// all rows by one workgroup 830).
+// 16 rows at a time (4096 rows of 32 heads of 128 dims, all but one of padding, one over 2048 keys: 17 us; by
+// one wavefront 830).
 constexpr int kClearRows = 16;
 __device__ __forceinline__ void clear_rest(const Params& p, int64_t wave, int64_t waves, int lane, int d) {
   const int64_t per = p.hq * d / 8;   // 16-byte pieces of a row
@@ -449,7 +384,10 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
     const cint32* table = (const cint32*)(p.tables + b * p.table_ls);
     const bool mine = t < count;
     const int limit = mine ? s.older + t : -1;
-    const uint64_t mask = p.tree && mine ? p.tree[s.begin + t] : 0;
+    const bool tree = p.tree != nullptr;
+    const uint64_t mask = tree && mine ? p.tree[s.begin + t] : 0;
+    const int older = tree ? s.older - 1 : s.older;   // all columns see the keys up to here
+    const float scale_log2 = p.scale_log2;
     for (int h = first / per_head; h < p.c.hkv && left > 0; ++h) {
       const int tile0 = first - h * per_head;       // (0 from the second pair on)
       const int ntile = min(per_head - tile0, left);
@@ -496,6 +434,22 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
         const bool b = load_group(key + 16, kd[1], vd[1], kss[1], vss[1]);
         return (a ? 1 : 0) | (b ? 2 : 0);
       };
+      // Zeros for the tile's rows of V that are not finite: their bits.
+      auto clean = [&](u32x4 (&vd)[2][VL]) {
+        constexpr int PC = 64 / VR;
+        uint32_t rows = 0;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < VL; ++i) {
+            const uint64_t lanes = __ballot(not_finite(vd[g][i]));
+            if (lanes == 0) continue;
+            const uint32_t odd = rows_of<PC>(lanes);
+            if ((odd >> (lane / PC)) & 1) vd[g][i] = u32x4{0u, 0u, 0u, 0u};
+            rows |= odd << (16 * g + VR * i);
+          }
+        return rows;
+      };
       // V rows to LDS: row r at r RB, its 16-byte chunk c at position c ^ 2 (r & 3)
       auto put = [&](const u32x4 (&vd)[2][VL]) {
         constexpr int PC = 64 / VR;
@@ -515,112 +469,148 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
           }
       };
       f32x4 acc[DT];
+      float m, l;   // the column's maximum (log2 units), the lane's part of its sum
+      auto run = [&](auto care) {
+        constexpr bool careful = decltype(care)::value;
 #pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      float m = -INFINITY, l = 0.0f;   // the column's maximum (log2 units), the lane's part of its sum
-      int key = lo, have = 0;
-      if (key < hi) {
-        have = load(key, kr, vr, ksc, vsc);
-        put(vr);
-      }
-      while (key < hi) {
-        const int next = key + kFewKeys;
-        u32x4 kn[2][KL], vn[2][VL];
-        f32x4 ksn[2], vsn[2];
-        int have_n = 0;
-        if (next < hi) have_n = load(next, kn, vn, ksn, vsn);
-        if (INT8) {
-          // (an empty asm: the compiler would take the codes apart an iteration ahead, in 64 more
-          // registers than there are)
+        for (int i = 0; i < DT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m = -INFINITY;
+        l = 0.0f;
+        int key = lo, have = 0;
+        uint32_t apart = 0;             // rows of V that lie in LDS as zeros
+        if (key < hi) {
+          have = load(key, kr, vr, ksc, vsc);
+          if (careful) apart = clean(vr);
+          put(vr);
+        }
+        while (key < hi) {
+          const int next = key + kFewKeys;
+          u32x4 kn[2][KL], vn[2][VL];
+          f32x4 ksn[2], vsn[2];
+          int have_n = 0;
+          if (next < hi) have_n = load(next, kn, vn, ksn, vsn);
+          if (INT8) {
+            // (an empty asm: the compiler would take the codes apart an iteration ahead, in 64 more
+            // registers than there are)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int i = 0; i < KL; ++i) asm volatile("" : "+v"(kr[g][i]));
+          }
+          f32x4 S[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              bf16x8 a;
+              if (INT8) {
+                const u32x4 w = kr[g][ks >> 1];
+                a = as_bf16(ks & 1 ? i8x8_to_bf16x8(w[2], w[3]) : i8x8_to_bf16x8(w[0], w[1]));
+              } else {
+                a = __builtin_bit_cast(bf16x8, kr[g][ks % KL]);
+              }
+              S[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ks], S[g], 0, 0, 0);
+            }
+          float y[2][4];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const f32x4 sc = ksc[g];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[g][e] = S[g][e] * (INT8 ? sc[e] * scale_log2 : scale_log2);
+          }
+          if (have != 3 || key + 31 > older) {
+            uint64_t bits = mine ? seen_bits(mask, tree, limit, s, key) : 0;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (!((have >> g) & 1)) bits &= ~(0xffffull << (16 * g));
+              const uint32_t own = static_cast<uint32_t>(bits >> (16 * g + 4 * lg));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[g][e] = where_bit(y[g][e], own, e);
+            }
+          }
+          float top = y[0][0];
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int i = 0; i < KL; ++i) asm volatile("" : "+v"(kr[g][i]));
-        }
-        f32x4 S[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, y[g][e]);
+          if (__any((top > m + kHeadroom) | ((m == -INFINITY) & (top > m)))) {
+            const float mn = fmaxf(m, max_over_rows(top));
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+            for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+          bf16x8 hi8, lo8;
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            bf16x8 a;
-            if (INT8) {
-              const u32x4 w = kr[g][ks >> 1];
-              a = as_bf16(ks & 1 ? i8x8_to_bf16x8(w[2], w[3]) : i8x8_to_bf16x8(w[0], w[1]));
-            } else {
-              a = __builtin_bit_cast(bf16x8, kr[g][ks % KL]);
+            const f32x4 sc = vsc[g];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float w = __builtin_amdgcn_exp2f(y[g][e] - base);
+              l += w;
+              if (INT8) w = w == 0.0f ? 0.0f : w * sc[e];   // (the scale of a hidden key may be anything)
+              const __bf16 a = static_cast<__bf16>(w);
+              hi8[4 * g + e] = a;
+              // (8 bits: behind a scale that is infinite the low part is finite)
+              const float rest = w - static_cast<float>(a);
+              lo8[4 * g + e] = static_cast<__bf16>(INT8 ? fmaxf(rest, -1e38f) : rest);
             }
-            S[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, bq[ks], S[g], 0, 0, 0);
           }
-        float y[2][4];
+          if (careful) {
+            for (uint32_t todo = apart; todo != 0; todo &= todo - 1) {
+              const int r = __builtin_ctz(todo);
+              const int id = page_of(p, table, s, key + r);
+              if (id < 0) continue;
+              float w = 0.0f;   // the row's weight: in the lanes that hold keys 4 (r / 4) .. + 3 of its group
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const f32x4 sc = ksc[g];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[g][e] = S[g][e] * (INT8 ? sc[e] * p.scale_log2 : p.scale_log2);
-        }
-        if (have != 3 || key + 31 > (p.tree ? s.older - 1 : s.older)) {
-          uint64_t bits = mine ? seen_bits(mask, p.tree != nullptr, limit, s, key) : 0;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (!((have >> g) & 1)) bits &= ~(0xffffull << (16 * g));
-            const uint32_t own = static_cast<uint32_t>(bits >> (16 * g + 4 * lg));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[g][e] = where_bit(y[g][e], own, e);
+              for (int x = 0; x < 8; ++x)
+                if (x == 4 * (r >> 4) + (r & 3)) w = static_cast<float>(hi8[x]) + static_cast<float>(lo8[x]);
+              w = __shfl(w, 16 * ((r >> 2) & 3) + ln);
+              const char* row = p.c.v + (p.c.sp * id + p.c.sh * h + p.c.st * ((key + r) & (p.c.page - 1))) * E;
+              if (mine && (seen_bits(mask, tree, limit, s, key + r) & 1))
+                add_row<DT>(row, lg, w, [&](int i) -> f32x4& { return acc[i]; });
+            }
           }
-        }
-        float top = y[0][0];
+          wave_lds_sync();
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, y[g][e]);
-        if (__any(top > m + kHeadroom || (m == -INFINITY && top > m))) {
-          const float mn = fmaxf(m, max_over_rows(top));
-          const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-          m = mn;
-          l *= alpha;
-#pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] *= alpha;
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-        bf16x8 hi8, lo8;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const f32x4 sc = vsc[g];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float w = __builtin_amdgcn_exp2f(y[g][e] - base);
-            l += w;
-            if (INT8) w = w == 0.0f ? 0.0f : w * sc[e];   // (the scale of a hidden key may be anything)
-            const __bf16 a = static_cast<__bf16>(w);
-            hi8[4 * g + e] = a;
-            lo8[4 * g + e] = static_cast<__bf16>(w - static_cast<float>(a));
+          for (int i = 0; i < DT; ++i) {
+            const char* vp = buf + vtr[i & 3] + (i >> 2) * 128;
+            const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
+            const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
+            const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi8, acc[i], 0, 0, 0);
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo8, acc[i], 0, 0, 0);
           }
-        }
-        wave_lds_sync();
+          wave_lds_sync();
+          if (next < hi) {
+            if (careful) apart = clean(vn);
+            put(vn);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          const char* vp = buf + vtr[i & 3] + (i >> 2) * 128;
-          const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp));
-          const i16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vp + 16 * RB));
-          const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7));
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi8, acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo8, acc[i], 0, 0, 0);
-        }
-        wave_lds_sync();
-        if (next < hi) {
-          put(vn);
+            for (int g = 0; g < 2; ++g) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-#pragma unroll
-            for (int i = 0; i < KL; ++i) kr[g][i] = kn[g][i];
-            ksc[g] = ksn[g];
-            vsc[g] = vsn[g];
+              for (int i = 0; i < KL; ++i) kr[g][i] = kn[g][i];
+              ksc[g] = ksn[g];
+              vsc[g] = vsn[g];
+            }
           }
+          have = have_n;
+          key = next;
         }
-        have = have_n;
-        key = next;
+        l = sum_over_rows(l);
+      };
+      run(std::false_type{});
+      if constexpr (!INT8) {
+        // A sum that is NaN (l is, too, if a logit is) may be one of a value that its column does not see, or of
+        // an infinite one, whose product with P's low part has any sign: again, such rows by themselves.
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = odd || acc[i][e] != acc[i][e];
+        if (__builtin_expect(__any(odd && mine && l == l), 0)) run(std::true_type{});
       }
-      l = sum_over_rows(l);
 
       // ---- the pair's result, or this wavefront's part of it
       const Params& p = again();
@@ -628,26 +618,16 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
       if (cut && tile0 == 0 && lane == 0)
         *note_of(p, b * p.c.hkv + h) = Note{whole ? 1 : list.worker_of(from + done + per_head - 1) - w + 1, w};
       done += ntile;
-      bool odd = l != l;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd = odd || acc[i][e] != acc[i][e];
-      const int cols = count * p.G;
-      const uint64_t lanes = __ballot(odd && ln < cols);
-      const uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
-      auto orow = [&](int c) { return p.out + (static_cast<int64_t>(s.begin + c / p.G) * p.hq + h * p.G + c % p.G) * D; };
-      auto rec = [&](int c) { return record_of<D>(p, 2 * w + (tile0 > 0 ? 0 : 1), c); };
-      if (ln < cols && !((redo >> ln) & 1)) {
+      if (ln < count * p.G) {
         if (whole) {
-          uint16_t* dst = orow(ln) + 4 * lg;
+          uint16_t* dst = p.out + (static_cast<int64_t>(s.begin + t) * p.hq + head) * D + 4 * lg;
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
           for (int i = 0; i < DT; ++i)
             *reinterpret_cast<u32x2*>(dst + 16 * i) =
                 u32x2{pack_bf16(acc[i][0] * inv, acc[i][1] * inv), pack_bf16(acc[i][2] * inv, acc[i][3] * inv)};
         } else {
-          float* r = rec(ln);
+          float* r = record_of<D>(p, 2 * w + (tile0 > 0 ? 0 : 1), ln);
           if (lg == 0) {
             r[0] = m;
             r[1] = l;
@@ -655,12 +635,6 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
 #pragma unroll
           for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i];
         }
-      }
-      for (uint32_t todo = redo; todo != 0; todo &= todo - 1) {
-        const int c = __builtin_ctz(todo);
-        float mc, lc, oc[D / 64];
-        redo_column<D, INT8>(p, s, table, h, c / p.G, h * p.G + c % p.G, lo, hi, lane, mc, lc, oc);
-        store_column<D>(p, whole, whole ? orow(c) : nullptr, whole ? nullptr : rec(c), lane, mc, lc, oc);
       }
       wave_lds_sync();
     }
@@ -688,8 +662,9 @@ struct Col {
 };
 
 // SHARED: the workgroups share the list; else one a unit: grid (KV head, query tile, sequence).
+// (64 dims in bf16 fit three workgroups a CU, which plan_of counts on, with at most 168 registers.)
 template <int D, bool INT8, int NCT, bool SHARED>
-__global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
+__global__ __launch_bounds__(kThreads, D == 64 && !INT8 ? 3 : 2) void many_kernel(const Params args) {
   const Params& p = args;
   constexpr int KS = D / 32, DT = D / 16, CH = D / 8, RB = 2 * D;
   constexpr int KT = INT8 && NCT > 1 ? 2 : 4;   // 16-key groups a pass: half the logits live
@@ -777,13 +752,6 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     }
     f32x4 acc[DT][NCT], lsum[NCT];
     Col col[NCT];
-#pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-#pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      lsum[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      col[ct] = Col{0.0f, -INFINITY};
-    }
 
     // Staging of a tile: wavefront w brings its keys 16 w .. + 15, which lie in one page.
     // bf16 goes to LDS without registers, rows past the length (or of a page outside the
@@ -843,7 +811,9 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
         }
       }
     };
-    auto finish_stage = [&](char* buf) {
+    // From here on keys are hidden from some column (others that have no page are zeros).
+    const int tail = max(p.tree ? s.older : s.older + t0 + 1, 0);
+    auto finish_stage = [&](auto careful, int tile, char* buf) {
       if constexpr (INT8) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -860,6 +830,22 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
               lane < 16 ? sreg * p.scale_log2 : sreg;
       } else {
         __builtin_amdgcn_s_waitcnt(0);   // the copies have landed
+        if (decltype(careful)::value && tile * kKeys + kKeys > tail) {
+          // zeros for the wavefront's rows of V that are not finite; their bits lie behind the tiles
+          asm volatile("" ::: "memory");   // (no read above the wait)
+          char* vd = buf + kTile<D> + 16 * wave * RB + lane * 16;
+          uint32_t rows = 0;
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            u32x4* piece = reinterpret_cast<u32x4*>(vd + i * RL * RB);
+            const uint64_t lanes = __ballot(not_finite(*piece));
+            if (lanes == 0) continue;
+            const uint32_t odd = rows_of<PC>(lanes);
+            if ((odd >> (lane / PC)) & 1) *piece = u32x4{0u, 0u, 0u, 0u};
+            rows |= odd << (RL * i);
+          }
+          if (lane == 0) reinterpret_cast<uint32_t*>(buf + 2 * kTile<D>)[wave] = rows;
+        }
       }
       __syncthreads();
     };
@@ -868,9 +854,9 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
     // registers; the scheduling barriers keep that order.  The priority takes one of a SIMD's
     // wavefronts through its products, so that the others' softmax falls beside them (4096 tokens behind
     // 12288: 871 us without, 823 with it).
-    auto attend = [&](int tile, int got, const char* buf) {
+    auto attend = [&](auto careful, int tile, int got, const char* buf) {
       const float* scales = reinterpret_cast<const float*>(buf + 2 * kTile<D>);
-      const bool mask = got != 15 || tile * kKeys + kKeys - 1 > (p.tree ? s.older - 1 : s.older + t0);
+      const bool hidden = tile * kKeys + kKeys > tail, mask = got != 15 || hidden;
 #pragma unroll
       for (int pass = 0; pass < 4 / KT; ++pass) {
         constexpr int kQ = KS * KT;
@@ -980,6 +966,32 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
             }
           }
         }
+        if (decltype(careful)::value && hidden) {
+          const uint32_t* bits = reinterpret_cast<const uint32_t*>(buf + 2 * kTile<D>);
+#pragma unroll 1
+          for (int kt = 0; kt < 4; ++kt) {
+            uint32_t todo = __builtin_amdgcn_readfirstlane(static_cast<int>(bits[kt]));
+#pragma unroll 1
+            for (; todo != 0; todo &= todo - 1) {
+              const int r = __builtin_ctz(todo), key = tile * kKeys + 16 * kt + r;
+              const Params& p = again();
+              const int id = page_of(p, (const cint32*)(p.tables + b * p.table_ls), s, key);   // (it has one)
+              const char* row = p.c.v + (p.c.sp * max(id, 0) + p.c.sh * h + p.c.st * (key & (p.c.page - 1))) * E;
+#pragma unroll
+              for (int ct = 0; ct < NCT; ++ct) {
+                float w = 0.0f;   // the row's weight: in the lanes that hold keys 4 (r / 4) .. + 3 of the group
+#pragma unroll
+                for (int x = 0; x < 4 * KT; ++x)
+                  if (x == 4 * kt + (r & 3)) w = S[x >> 2][ct][x & 3];
+                w = __shfl(w, 16 * (r >> 2) + ln);
+                const bool mine = tcol[ct] <= t_last;
+                const uint64_t names = p.tree && mine ? p.tree[s.begin + tcol[ct]] : 0;
+                if (mine && (seen_bits(names, p.tree != nullptr, s.older + tcol[ct], s, key) & 1))
+                  add_row<DT>(row, lg, w, [&](int i) -> f32x4& { return acc[i][ct]; });
+              }
+            }
+          }
+        }
         // ---- O^T += V^T P^T, the row sums a product with ones
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -1007,16 +1019,59 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
       }
     };
 
-    fetch_ids(lo);
-    begin_stage(lo, lds);
-    finish_stage(lds);
-    for (int tile = lo; tile < hi; ++tile) {
-      char* buf = lds + ((tile - lo) & 1) * kStage<D>;
-      char* other = lds + ((tile - lo + 1) & 1) * kStage<D>;
-      const int got = have;
-      if (tile + 1 < hi) begin_stage(tile + 1, other);
-      attend(tile, got, buf);
-      if (tile + 1 < hi) finish_stage(other);
+    auto run = [&](auto careful) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        lsum[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        col[ct] = Col{0.0f, -INFINITY};
+      }
+      fetch_ids(lo);
+      begin_stage(lo, lds);
+      finish_stage(careful, lo, lds);
+      for (int tile = lo; tile < hi; ++tile) {
+        char* buf = lds + ((tile - lo) & 1) * kStage<D>;
+        char* other = lds + ((tile - lo + 1) & 1) * kStage<D>;
+        const int got = have;
+        if (tile + 1 < hi) begin_stage(tile + 1, other);
+        attend(careful, tile, got, buf);
+        if (tile + 1 < hi) finish_stage(careful, tile + 1, other);
+      }
+    };
+    run(std::false_type{});
+    if constexpr (!INT8) {
+      // A sum that is NaN (with a logit's, the weights are) may be one of a value that its column does not see.
+      bool odd = false;
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = odd || (acc[i][ct][e] != acc[i][ct][e] && tcol[ct] <= t_last);
+      int* flags = reinterpret_cast<int*>(lds + 2 * kTile<D>) + kWaves;
+      const bool any = __any(odd);
+      if (lane == 0) flags[wave] = any;
+      __syncthreads();
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]), 0)) {
+        // the values in question (all wavefronts look through all of them)
+        bool found = false;
+        for (int key0 = max(tail, lo * kKeys) & -16; key0 < min(hi * kKeys, s.len) && !found; key0 += 16) {
+          const int id = page_of(p, (const cint32*)table, s, key0);
+          if (id < 0) continue;
+          const int in = key0 & (p.c.page - 1);
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const int r = RL * i + lane / PC;
+            if (key0 + r < s.len)
+              found = found || not_finite(*reinterpret_cast<const u32x4*>(
+                                   vbase + p.c.sp * E * id + static_cast<int64_t>(in + r) * row_bytes + (lane % PC) * 16));
+          }
+          found = __any(found);
+        }
+        __syncthreads();   // (the flags have been read)
+        if (found) run(std::true_type{});
+      }
     }
 
     // ---- store: acc[i][ct][e] is dim 16 i + 4 lg + e
@@ -1031,44 +1086,23 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Params args) {
       const int c = c0 + ln;
       const bool mine = tcol[ct] <= t_last;
       const float l = INT8 ? sum_over_rows(lsum[ct][0] + lsum[ct][1] + lsum[ct][2] + lsum[ct][3]) : lsum[ct][0];
-      bool odd = l != l;
+      if (!mine) continue;
+      if (!SHARED || whole) {
+        uint16_t* dst = late.out + (static_cast<int64_t>(s.begin + tcol[ct]) * late.hq + h * late.G + c - (tcol[ct] - t0) * late.G) * D + 4 * lg;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd = odd || acc[i][ct][e] != acc[i][ct][e];
-      const uint64_t lanes = __ballot(!INT8 && odd && mine);
-      uint32_t redo = static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffff);
-      for (uint32_t todo = redo; todo != 0; todo &= todo - 1)
-        if (!hidden_odd<D>(late, s, (const cint32*)table, h, t0 + (c0 + __builtin_ctz(todo)) / late.G, lo * kKeys, hi * kKeys, lane))
-          redo &= ~(todo & -todo);
-      auto orow = [&](int cc) {
-        return late.out + (static_cast<int64_t>(s.begin + t0 + cc / late.G) * late.hq + h * late.G + cc % late.G) * D;
-      };
-      auto rec = [&](int cc) { return record_of<D>(late, 2 * worker + (lo > 0 ? 0 : 1), cc); };
-      if (mine && !((redo >> ln) & 1)) {
-        if (!SHARED || whole) {
-          uint16_t* dst = orow(c) + 4 * lg;
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            const f32x4 o = acc[i][ct];
-            *reinterpret_cast<u32x2*>(dst + 16 * i) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
-          }
-        } else {
-          float* r = rec(c);
-          if (lg == 0) {
-            r[0] = col[ct].thr == -INFINITY ? -INFINITY : -col[ct].nm;
-            r[1] = l;
-          }
-#pragma unroll
-          for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i][ct];
+        for (int i = 0; i < DT; ++i) {
+          const f32x4 o = acc[i][ct];
+          *reinterpret_cast<u32x2*>(dst + 16 * i) = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
         }
-      }
-      for (uint32_t todo = redo; todo != 0; todo &= todo - 1) {
-        const int cc = c0 + __builtin_ctz(todo);
-        float mc, lc, oc[D / 64];
-        redo_column<D, INT8>(late, s, (const cint32*)table, h, t0 + cc / late.G, h * late.G + cc % late.G, lo * kKeys, hi * kKeys, lane, mc, lc, oc);
-        store_column<D>(late, whole, whole ? orow(cc) : nullptr, whole ? nullptr : rec(cc), lane, mc, lc, oc);
+      } else {
+        float* r = record_of<D>(late, 2 * worker + (lo > 0 ? 0 : 1), c);
+        if (lg == 0) {
+          r[0] = col[ct].thr == -INFINITY ? -INFINITY : -col[ct].nm;
+          r[1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) *reinterpret_cast<f32x4*>(r + 4 + 16 * i + 4 * lg) = acc[i][ct];
       }
     }
     left -= hi - lo;

@@ -102,3 +102,69 @@ def test_rows_of_padding(kv, n, wide):
                              max_new=n)
         tol = 2 * 3.03 * 2.0 ** -8 * float(cache.v.float().abs().max()) * (1.0 if kv == "bf16" else 0.025)
         assert float((got[first:first + count].float() - alone.float()).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("n,hq,hkv,d,older,wide", [
+    (4, 4, 1, 128, 60, 0), (16, 1, 1, 64, 1000, 0), (7, 4, 2, 64, 3, 0), (16, 4, 1, 128, 40, 0), (13, 5, 1, 64, 200, 0),
+    (60, 8, 2, 128, 37, 0), (64, 4, 1, 64, 100, 0), (50, 4, 2, 128, 500, 4096), (40, 8, 1, 64, 90, 4096), (12, 4, 1, 64, 5, 4096)])
+def test_values_that_some_queries_see(tree, n, hq, hkv, d, older, wide):
+    """NaN and infinities in some dims of several new tokens: the outputs are the formula's, infinities, NaN and
+    what is finite alike, whatever those that do not see them have beside them in a tile."""
+    from _paged_ref import attend_ref
+    from nanokv_amd.paged import attend_paged, tree_masks
+    g = torch.Generator().manual_seed(n)
+    cache, tables, lens = _setup([older + n, n, older // 2 + n], hkv, 16, d, "bf16", seed=n)
+    tables = torch.nn.functional.pad(tables, (0, wide // 16), value=-1)
+    for b in range(3):
+        first = int(lens[b]) - n
+        for i in {1, 2, n // 2, n - 1} if b < 2 else {n - 2}:
+            at = first + i
+            dims = torch.randint(0, d, (3,), generator=g)
+            for dim, bad in zip(dims.tolist(), (float("nan"), float("inf"), float("-inf"))):
+                cache.v[int(tables[b, at // 16]), :, at % 16, dim] = bad
+    masks = None
+    if tree:
+        parents = torch.tensor([-1] + [int(torch.randint(-1, i, (1,), generator=g)) for i in range(1, n)])
+        masks = tree_masks(parents.cuda()).repeat(3)
+    q = _q(3 * n, hq, d, 3, scale=0.7)
+    got = attend_paged(q, cache, tables, lens, tree=masks)
+    ref, mag = attend_ref(q, cache, tables, lens, tree=masks, n_each=n)
+    fine = ref.isfinite()
+    assert bool(fine.any()) and not bool(fine.all())
+    got = got.double().cpu()
+    same = (got == ref) | (got.isnan() & ref.isnan())
+    assert bool(same[~fine].all()), (got[~fine][~same[~fine]][:4], ref[~fine][~same[~fine]][:4])
+    many = n * hq // hkv > 16
+    c = 2.0 ** -13 + (2.02 * 2.0 ** -8 if many else 0.0)      # (logits below 20 and 2000 keys: 2 e + 2 n u < 2^-13)
+    tol = 2.0 ** -8 * (ref.abs() + c * mag) + c * mag
+    assert bool(((got - ref).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("kv,B,n,older", [("bf16", 1, 512, 1536), ("bf16", 4, 1, 16384), ("bf16", 2, 4, 8192),
+                                          ("int8", 2, 4, 8192), ("int8", 4, 1, 16384)])
+def test_values_that_are_not_finite_take_no_longer(kv, B, n, older):
+    """A NaN value that some queries see: the call takes the time of one without, or little more."""
+    from nanokv_amd.paged import attend_paged
+    cache, tables, lens = _setup([older + n] * B, 8, 64, 128, kv, seed=1, poison=False)
+    q = _q(B * n, 32, 128, 3)
+
+    def us():
+        times = []
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(4):
+                attend_paged(q, cache, tables, lens)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) * 250)
+        return min(times)
+
+    clean = us()
+    for at in (older + n // 2, older // 2):
+        if kv == "bf16":
+            cache.v[int(tables[0, at // 64]), :, at % 64, 3] = float("nan")
+        else:
+            cache.v_scale[int(tables[0, at // 64]), :, at % 64] = float("nan")
+        assert us() < 3 * clean + 50
