@@ -168,3 +168,34 @@ def test_values_that_are_not_finite_take_no_longer(kv, B, n, older):
         else:
             cache.v_scale[int(tables[0, at // 64]), :, at % 64] = float("nan")
         assert us() < 3 * clean + 50
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,hq,hkv,page,tree", [(26, 4, 2, 64, True), (9, 5, 1, 16, True), (33, 2, 2, 256, False),
+                                                (26, 8, 2, 16, True), (64, 5, 1, 64, True), (150, 8, 2, 64, False)])
+def test_shared_lists_of_every_kind(kv, d, n, hq, hkv, page, tree):
+    """Tiles of 64 and of 128 columns, shared and cut over workgroups, in both formats: trees and short chunks
+    behind a few thousand keys."""
+    from nanokv_amd import _lib
+    from nanokv_amd.paged import attend_paged, tree_masks
+    older = [3000, 0, 2111]
+    lengths = [o + n for o in older]
+    cache, tables, lens = _setup(lengths, hkv, page, d, kv, seed=n)
+    rows = n * (hq // hkv)
+    assert rows > 16
+    most = tables.shape[1]
+    assert _lib.load().nkv_paged_attend_workspace(3, 3 * n, n, hq, hkv, d, most, page, 0) > 0      # (the list is shared)
+    masks = None
+    if tree:
+        g = torch.Generator().manual_seed(n)
+        parents = [torch.tensor([-1] + [int(torch.randint(-1, i, (1,), generator=g)) for i in range(1, n)]) for _ in range(3)]
+        masks = tree_masks(torch.stack(parents).cuda()).flatten()
+    q = _q(3 * n, hq, d, n)
+    want = attend_paged(q, cache, tables, lens, tree=masks)
+    _check(want, q, cache, tables, lens, tree=masks, n_each=n)
+    starts = torch.tensor([3, n + 3, n + 3, 2 * n + 1], dtype=torch.int32, device="cuda")
+    q = _q(2 * n + 5, hq, d, n + 1)
+    masks = None if masks is None else masks[:2 * n + 5].contiguous()
+    got = attend_paged(q, cache, tables, lens, starts=starts, max_new=n, tree=masks)
+    _check(got, q, cache, tables, lens, starts, tree=masks)
