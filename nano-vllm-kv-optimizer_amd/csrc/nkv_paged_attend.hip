@@ -186,6 +186,18 @@ __device__ __forceinline__ uint32_t rows_of(uint64_t lanes) {
   for (int r = 0; r < kWave / L; ++r) rows |= ((lanes >> (r * L)) & ((1ull << L) - 1)) != 0 ? 1u << r : 0u;
   return rows;
 }
+// 0, or NaN if one of the values is infinite or NaN, in four chains (comparisons would each pass a scalar register).
+template <typename F>
+__device__ __forceinline__ float zero_if_finite(int n, F&& at) {
+  f32x4 z = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const f32x4 a = at(i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = __builtin_fmaf(a[e], 0.0f, z[e]);
+  }
+  return (z[0] + z[1]) + (z[2] + z[3]);
+}
 // acc += w V for a row of V as it lies in the cache; acc[i][e] is dim 16 i + 4 lg + e.
 template <int DT, typename F>
 __device__ __forceinline__ void add_row(const char* row, int lg, float w, F&& acc) {
@@ -586,6 +598,13 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
           wave_lds_sync();
           if (next < hi) {
             if (careful) apart = clean(vn);
+            if (INT8) {
+              // (likewise the values' codes, right behind their loads)
+#pragma unroll
+              for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < VL; ++i) asm volatile("" : "+v"(vn[g][i]));
+            }
             put(vn);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
@@ -602,14 +621,10 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
       };
       run(std::false_type{});
       if constexpr (!INT8) {
-        // A sum that is NaN (l is, too, if a logit is) may be one of a value that its column does not see, or of
-        // an infinite one, whose product with P's low part has any sign: again, such rows by themselves.
-        bool odd = false;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd = odd || acc[i][e] != acc[i][e];
-        if (__builtin_expect(__any(odd && mine && l == l), 0)) run(std::true_type{});
+        // A sum that is not finite (l is NaN if a logit is) may be one of a value that its column does not see, or
+        // of an infinite one, whose product with P's low part has any sign: again, such rows by themselves.
+        const float z = zero_if_finite(DT, [&](int i) { return acc[i]; });
+        if (__builtin_expect(__any((z != z) & mine & (l == l)), 0)) run(std::true_type{});
       }
 
       // ---- the pair's result, or this wavefront's part of it
@@ -1040,15 +1055,14 @@ __global__ __launch_bounds__(kThreads, D == 64 && !INT8 ? 3 : 2) void many_kerne
       }
     };
     run(std::false_type{});
-    if constexpr (!INT8) {
-      // A sum that is NaN (with a logit's, the weights are) may be one of a value that its column does not see.
+    if (!INT8 && hi * kKeys > tail) {
+      // A sum that is not finite may be one of a value that its column does not see.
       bool odd = false;
 #pragma unroll
-      for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd = odd || (acc[i][ct][e] != acc[i][ct][e] && tcol[ct] <= t_last);
+      for (int ct = 0; ct < NCT; ++ct) {
+        const float z = zero_if_finite(DT, [&](int i) { return acc[i][ct]; });
+        odd |= (z != z) & (tcol[ct] <= t_last);
+      }
       int* flags = reinterpret_cast<int*>(lds + 2 * kTile<D>) + kWaves;
       const bool any = __any(odd);
       if (lane == 0) flags[wave] = any;
