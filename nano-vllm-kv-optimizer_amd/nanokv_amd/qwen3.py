@@ -614,7 +614,9 @@ class Qwen3ForCausalLM(nn.Module):
                    lengths: torch.Tensor, *, starts: torch.Tensor | None = None, max_new: int | None = None,
                    tree: torch.Tensor | None = None) -> torch.Tensor:
         """One step of several sequences: the hidden rows [T, hidden] of their new tokens
-        input_ids [T] at `positions` [T] (compute_logits, token_logprobs take them).
+        input_ids [T] at `positions` [T] (compute_logits, token_logprobs take them).  Positions lie in
+        [0, max_position), padding's too: being in device memory they are not checked as prefill's and
+        decode's are, and the fused launch takes the rotary table's first or last row for others.
 
         The tokens' keys and values go to `slots` [T] of every layer's cache and attend
         to their sequences' keys: tables, lengths, starts, max_new and tree as
