@@ -1102,7 +1102,8 @@ __global__ __launch_bounds__(kThreads, D == 64 && !INT8 ? 3 : 2) void many_kerne
       const float l = INT8 ? sum_over_rows(lsum[ct][0] + lsum[ct][1] + lsum[ct][2] + lsum[ct][3]) : lsum[ct][0];
       if (!mine) continue;
       if (!SHARED || whole) {
-        uint16_t* dst = late.out + (static_cast<int64_t>(s.begin + tcol[ct]) * late.hq + h * late.G + c - (tcol[ct] - t0) * late.G) * D + 4 * lg;
+        const int head = h * late.G + c - (tcol[ct] - t0) * late.G;
+        uint16_t* dst = late.out + (static_cast<int64_t>(s.begin + tcol[ct]) * late.hq + head) * D + 4 * lg;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int i = 0; i < DT; ++i) {

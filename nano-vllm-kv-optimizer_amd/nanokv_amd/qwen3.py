@@ -51,7 +51,7 @@ from torch import nn
 from . import _lib
 from .attention import Attention, attach_m12_runtimes, attach_paged_cache, get_context, reset_context, set_context
 from .logprobs import TokenLogprobs, token_logprobs
-from .paged import qkv_append_paged
+from .paged import _to_i32, qkv_append_paged
 from .q8 import Q8, linear_q8, linear_silu_mul_q8, norm_linear_q8, norm_linear_silu_mul_q8, quantize_q8
 from .sparse.m12_runtime import M12Config
 from .store import _ptr, _stream
@@ -628,6 +628,9 @@ class Qwen3ForCausalLM(nn.Module):
         if positions.shape != (n,) or slots.shape != (n,) or input_ids.dim() != 1:
             raise ValueError(f"input_ids, positions and slots must be alike, [T] (got {tuple(input_ids.shape)}, "
                              f"{tuple(positions.shape)}, {tuple(slots.shape)})")
+        # (64-bit ones are narrowed once a step, not in every layer)
+        slots, tables, lengths, starts = (_to_i32(t) if t is not None and t.dtype is torch.int64 else t
+                                          for t in (slots, tables, lengths, starts))
         set_context(starts is not None, cu_seqlens_q=starts, max_seqlen_q=max_new or 0, slot_mapping=slots,
                     context_lens=lengths, block_tables=tables, tree_masks=tree)
         try:

@@ -65,3 +65,26 @@ def test_masks_of_32_bits_name_no_further_tokens():
     tables, lengths = torch.tensor([[3, 1, 2, 0]]), torch.tensor([50])
     assert torch.equal(attend_paged(q, cache, tables, lengths, tree=masks),
                        attend_paged(q, cache, tables, lengths, tree=masks.long() & 0xffffffff))
+
+
+def test_a_decoder_step_takes_64_bit_numbers():
+    """Slots, tables, lengths and starts of 64 bits, padding's far outside: the step's rows are those of 32 bits."""
+    from nanokv_amd.qwen3 import Qwen3Config, Qwen3ForCausalLM, init_random_
+    model = Qwen3ForCausalLM(Qwen3Config(vocab_size=64, hidden_size=128, intermediate_size=192, num_hidden_layers=2,
+                                         num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                                         max_position_embeddings=512))
+    init_random_(model, 3, std=0.2)
+    ids, pos = torch.arange(6), torch.tensor([0, 1, 2, 0, 1, 0])
+    slots, tables = torch.tensor([32, 33, 34, 0, 1, -1]), torch.tensor([[2, -1], [0, 1]])
+    lengths, starts = torch.tensor([3, 2]), torch.tensor([0, 3, 5])
+    out = []
+    for far in (False, True):
+        model.attach_paged(3, 16)
+        s, t = slots.clone(), tables.clone()
+        if far:
+            s[5], t[0, 1] = 2 ** 32 + 40, 2 ** 32
+        args = (s, t, lengths, starts) if far else (x.int() for x in (s, t, lengths, starts))
+        s, t, n, at = args
+        out.append(model.paged_step(ids, pos, s, t, n, starts=at, max_new=3))
+        out.append(model.model.layers[1].self_attn.attn.paged_cache.k.clone())
+    assert torch.equal(out[0][:5], out[2][:5]) and torch.equal(out[1], out[3])
