@@ -705,7 +705,8 @@ int nkv_norm_gemv_silu_mul_q8(const int8_t* gate_up_weight, const float* w_scale
  * libraries), and log probabilities.
  *
  * The cache of one layer: k, v [pages][Hkv][page_size][D], bf16, or int8 codes
- * with k_scale, v_scale fp32 [pages][Hkv][page_size] (dense); NULL scales: bf16.
+ * with k_scale, v_scale fp32 [pages][Hkv][page_size] (dense; finite, or NaN: as
+ * nkv_paged_append writes them); NULL scales: bf16.
  * page_stride, head_stride and token_stride are the elements from page to page,
  * head to head and token to token (rows on 16-byte boundaries, at most 64 MiB
  * from token to token), so other orders of the first three dimensions are read in place.

@@ -565,9 +565,9 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(const Params args) {
               if (INT8) w = w == 0.0f ? 0.0f : w * sc[e];   // (the scale of a hidden key may be anything)
               const __bf16 a = static_cast<__bf16>(w);
               hi8[4 * g + e] = a;
-              // (8 bits: behind a scale that is infinite the low part is finite)
+              // (8 bits: behind a scale that is infinite the low part is finite, and so are its products with codes)
               const float rest = w - static_cast<float>(a);
-              lo8[4 * g + e] = static_cast<__bf16>(INT8 ? fmaxf(rest, -1e38f) : rest);
+              lo8[4 * g + e] = static_cast<__bf16>(INT8 ? fmaxf(rest, -1e34f) : rest);
             }
           }
           if (careful) {

@@ -39,7 +39,7 @@ MAX_TREE = 64          # drafted tokens of a tree: bits of a mask
 
 class PagedKV(NamedTuple):
     """Keys and values [pages, Hkv, page, D] (bf16, or int8 codes) and the codes' fp32
-    scales [pages, Hkv, page].  Other orders in memory (views) are read in place as
+    scales [pages, Hkv, page] (finite, or NaN: as they are written here).  Other orders in memory (views) are read in place as
     long as a row's D values lie together and k and v lie alike."""
     k: torch.Tensor
     v: torch.Tensor

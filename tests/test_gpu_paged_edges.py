@@ -199,3 +199,25 @@ def test_shared_lists_of_every_kind(kv, d, n, hq, hkv, page, tree):
     masks = None if masks is None else masks[:2 * n + 5].contiguous()
     got = attend_paged(q, cache, tables, lens, starts=starts, max_new=n, tree=masks)
     _check(got, q, cache, tables, lens, starts, tree=masks)
+
+
+@pytest.mark.parametrize("n,older", [(1, 70), (3, 500), (20, 70), (24, 3000)])
+@pytest.mark.parametrize("which,bad", [(2, float("nan")), (3, float("nan")), (3, float("inf"))])
+def test_scales_that_are_not_finite(n, older, which, bad):
+    """A scale of a seen and of a drafted row of an 8-bit cache, of its key or of its value: the outputs are the
+    formula's (infinity times a code: infinite, or NaN for 0), those that do not see the row have none of it.
+    (Infinite scales of keys lie outside what a cache holds: their logits are infinite where those of infinite
+    keys would be NaN.)"""
+    from _paged_ref import attend_ref
+    from nanokv_amd.paged import attend_paged
+    cache, tables, lens = _setup([older + n, older + n], 2, 16, 128, "int8", seed=n)
+    cache[which][int(tables[0, 2]), :, 5] = bad                                    # key 37 of the first sequence
+    at = older + n // 2
+    cache[which][int(tables[1, at // 16]), :, at % 16] = bad                       # a new token of the second
+    q = _q(2 * n, 8, 128, 5, scale=0.1)
+    got = attend_paged(q, cache, tables, lens).double().cpu()
+    ref, mag = attend_ref(q, cache, tables, lens, n_each=n)
+    fine = ref.isfinite()
+    assert bool(((got == ref) | (got.isnan() & ref.isnan()))[~fine].all())
+    c = 2.0 ** -13 + (2.02 * 2.0 ** -8 if 4 * n > 16 else 0.0)
+    assert bool(((got - ref).abs() <= 2.0 ** -8 * (ref.abs() + c * mag) + c * mag)[fine].all())
